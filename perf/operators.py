@@ -193,14 +193,15 @@ def _to_int4(w, group, zero_points):
     k, n = w.shape
     kp, np_ = -(-k // 128) * 128, -(-n // 16) * 16
     w = _pad(w.float(), kp, np_).view(kp // group, group, np_)
+    steps = torch.full((1,), 15.0 if zero_points else 7.0, device=w.device)          # a tensor: torch multiplies by a number's reciprocal instead of dividing
     if zero_points:
         low, high = w.amin(1, keepdim=True).clamp(max=0.0), w.amax(1, keepdim=True).clamp(min=0.0)
-        s = ((high - low) / 15.0).to(torch.bfloat16).float()
+        s = ((high - low) / steps).to(torch.bfloat16).float()
         some = s > 0
         z = torch.where(some, torch.round(-low / s).clamp(0.0, 15.0), 0.0)
         u = torch.where(some, (torch.round(w / s) + z).clamp(0.0, 15.0), 0.0)
     else:
-        s = (w.abs().amax(1, keepdim=True) / 7.0).to(torch.bfloat16).float()
+        s = (w.abs().amax(1, keepdim=True) / steps).to(torch.bfloat16).float()
         z = torch.full_like(s, 8.0)
         u = torch.where(s > 0, torch.round(w / s).clamp(-8.0, 7.0), 0.0) + 8.0
     values = ((u - z) * s).view(kp, np_)[:k, :n]
