@@ -396,6 +396,34 @@ PB_API size_t pb_dense_dot_workspace_best(int tokens, int64_t rows, int64_t cols
 PB_API int pb_dense_dot(int tokens, const uint8_t* q, const uint8_t* sc8, const float* sc32, int64_t rows, int64_t cols, int a, int b,
                  const void* g, int g_dtype, int64_t g_free, float* out, void* workspace, size_t workspace_bytes, void* stream);
 
+/* From logits to scores and answers: for every row of logits z [vocab] (f32 or bf16), row (o, i) at o * stride_outer + i * stride_inner elements,
+ *   logprobs [rows][n_tokens]  log softmax(z) at the given tokens (at most 128 of a row); a negative token is none and gives 0, one beyond the vocabulary NaN
+ *   entropy [rows]             -sum p log p of p = softmax(z), natural logarithm
+ *   top_tokens, top_logprobs [rows][top]  the `top` (at most 128) largest logits, equal ones in the order of their indices (-0 is 0, NaN ranks with -inf)
+ * all in f32.  A row of nothing but -inf has log probabilities of -inf and an entropy of 0; a row with a NaN or +inf has NaN.  entropy and stats may be null.
+ * stats [rows][2] is for the backward call, which writes dlogits [rows][vocab] (the logits' type, contiguous) from the cotangents of logprobs, entropy and
+ * top_logprobs (each may be null):  dz_j = sum g_i [j == token_i] + sum h_i [j == top_i] - p_j (sum g_i + sum h_i + g_entropy (log p_j + entropy)). */
+PB_API int pb_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t stride_outer, int64_t stride_inner, int64_t vocab,
+                      const int64_t* tokens, int n_tokens, int top, float* logprobs, float* entropy, float* top_logprobs, int64_t* top_tokens,
+                      float* stats, void* stream);
+PB_API int pb_token_logprobs_bwd(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t stride_outer, int64_t stride_inner, int64_t vocab,
+                          const int64_t* tokens, int n_tokens, const int64_t* top_tokens, int top, const float* stats, const float* entropy,
+                          const float* g_logprobs, const float* g_entropy, const float* g_top, void* dlogits, void* stream);
+
+/* Weights in 4 bits: w[k][n] = scale[n][k / group] * (u[k][n] - zero[n][k / group]), group 32, 64 or 128, u and zero in 0..15 (zero 8 where the array is null).
+ * With A = ceil(cols / 16) and B = ceil(depth / 128):
+ *   q     uint8 [A][B][1024]: byte half * 512 + (g * 4 + t) * 16 + c * 4 + b belongs to column 16 a + 8 half + g; the word of bytes b = 0..3 holds
+ *         k = 128 kb + 32 c + 8 t + i, i = 0..7, at nibbles 0, 4, 1, 5, 2, 6, 3, 7 (a byte's lower nibble first)
+ *   scale bf16 [A][B][16][128 / group], zero uint8 the same.
+ * pb_quantize_int4 takes w [depth, cols] (f32 or bf16): scale = bf16(max|w| / 7), u = rint(w / scale) + 8; with zero points scale = bf16((max(w, 0) - min(w, 0)) / 15),
+ * zero = rint(-min / scale), u = rint(w / scale) + zero; codes and zero points within 0..15.  pb_dequantize_int4 is the inverse.
+ * pb_int4_product: out[rows, cols] = x[rows, depth] w, x's rows `stride` elements apart; sums in f32 of x as it is (an f32 x is not rounded).  Made for few rows:
+ * the weight is read once for every 32 rows of a bf16 x and every ten of an f32 one. */
+PB_API int pb_quantize_int4(const void* w, int dtype, int64_t depth, int64_t cols, int group, uint8_t* q, void* scale, uint8_t* zero, void* stream);
+PB_API int pb_dequantize_int4(const uint8_t* q, const void* scale, const uint8_t* zero, int64_t depth, int64_t cols, int group, void* out, int dtype, void* stream);
+PB_API int pb_int4_product(const void* x, int x_dtype, int64_t rows, int64_t depth, int64_t stride, const uint8_t* q, const void* scale, const uint8_t* zero, int group,
+                    int64_t cols, void* out, int out_dtype, void* stream);
+
 /* byte transpose [rows, cols] -> [cols, rows] of an fp8 matrix (weight prepared for the forward GEMM) */
 PB_API int pb_transpose_bytes(const void* src, int64_t rows, int64_t cols, void* dst, void* stream);
 

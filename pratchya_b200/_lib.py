@@ -95,6 +95,11 @@ _SIGNATURES = {
     "pb_wkv7_forward": (_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _int, _ptr, _ptr, _ptr, _ptr, _ptr]),
     "pb_wkv7_checkpoint_floats": (_sz, [_i64, _i64, _i64, _int]),
     "pb_wkv7_backward": (_int, [_ptr] * 10 + [_i64, _i64, _i64, _int] + [_ptr] * 8),
+    "pb_token_logprobs": (_int, [_ptr, _int] + [_i64] * 5 + [_ptr, _int, _int] + [_ptr] * 6),
+    "pb_token_logprobs_bwd": (_int, [_ptr, _int] + [_i64] * 5 + [_ptr, _int, _ptr, _int] + [_ptr] * 7),
+    "pb_quantize_int4": (_int, [_ptr, _int, _i64, _i64, _int, _ptr, _ptr, _ptr, _ptr]),
+    "pb_dequantize_int4": (_int, [_ptr, _ptr, _ptr, _i64, _i64, _int, _ptr, _int, _ptr]),
+    "pb_int4_product": (_int, [_ptr, _int, _i64, _i64, _i64, _ptr, _ptr, _ptr, _int, _i64, _ptr, _int, _ptr]),
 }
 # extra exports of the diagnostics build (libpratchya_b200_diag.so): test hooks, not part of the C ABI
 _DIAG_SIGNATURES = {

@@ -5,4 +5,5 @@ from ._ops import (quantize_impl, dequantize_impl, dequantize_impl_bwd, quantize
                    quantize_impl_bwd, matmul_impl_bwd, matmul_mixed_impl_bwd, rmatmul_mixed_impl_bwd, make_elementwise_impl_bwd,
                    add_impl_bwd, mul_impl_bwd, sub_impl_bwd, truediv_impl_bwd, floordiv_impl_bwd, mod_impl_bwd, pow_impl_bwd,
                    reduce_broadcast, set_literal_dot_precision)
+from ._int4 import quantize_int4_impl, dequantize_int4_impl, int4_matmul_impl
 from . import _qual as qx

@@ -635,6 +635,167 @@ OP(dense_dot) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- from logits to scores and answers ----
+// a strided CUDA tensor of f32 or bf16 whose last dimension lies together: its rows as (outer, inner) with a stride each
+struct StridedRows { int64_t outer = 1, inner = 1, stride_outer = 0, stride_inner = 0; };
+bool strided_rows(const at::Tensor& x, StridedRows* r) {
+  if (x.dim() < 1 || (x.size(-1) > 1 && x.stride(-1) != 1)) return false;
+  int found = 0;
+  for (int64_t d = x.dim() - 2; d >= 0; --d) {      // from the innermost: dimensions that continue one another are one
+    const int64_t n = x.size(d), s = x.stride(d);
+    if (n == 1) continue;
+    if (s < 0) return false;
+    if (found == 0) { r->inner = n; r->stride_inner = s; found = 1; }
+    else if (found == 1 && s == r->stride_inner * r->inner) r->inner *= n;
+    else if (found == 1) { r->outer = n; r->stride_outer = s; found = 2; }
+    else if (s == r->stride_outer * r->outer) r->outer *= n;
+    else return false;
+  }
+  return true;
+}
+const at::Tensor* plain_rows(PyObject* o, StridedRows* r) {
+  if (!THPVariable_CheckExact(o)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_cuda() || t.layout() != at::kStrided || at::isTensorSubclassLike(t) || t.is_neg() || t._is_zerotensor() || !dense(t.scalar_type()) || !strided_rows(t, r)) return nullptr;
+  return &t;
+}
+
+// token_logprobs(logits, tokens or None, top) -> (logprobs or None, entropy, top_logprobs, top_tokens, stats)
+OP(token_logprobs) {
+  HANDLE_TH_ERRORS
+  NARGS(3);
+  StridedRows r;
+  const at::Tensor *z = plain_rows(args[0], &r), *tokens = args[1] == Py_None ? nullptr : plain(args[1]);
+  const long long top = PyLong_AsLongLong(args[2]);
+  if (top == -1 && PyErr_Occurred()) return nullptr;
+  if (!z || watched() || (args[1] != Py_None && (!tokens || tokens->scalar_type() != at::kLong || tokens->device() != z->device())) || top < 0 || top > 0x7fffffff) return none();
+  const at::IntArrayRef lead = z->sizes().slice(0, z->dim() - 1);
+  int64_t n = 0;
+  if (tokens) {
+    const bool one = tokens->sizes() == lead;
+    if (!one && (tokens->dim() != z->dim() || tokens->sizes().slice(0, z->dim() - 1) != lead)) return none();
+    n = one ? 1 : tokens->size(-1);
+    if (n > 0x7fffffff) return none();
+  }
+  const c10::cuda::CUDAGuard guard(z->device());
+  c10::SmallVector<int64_t, 8> with_top(lead.begin(), lead.end()), with_two(lead.begin(), lead.end());
+  with_top.push_back(top); with_two.push_back(2);
+  at::Tensor logprobs, entropy = empty(lead, at::kFloat, *z), top_logprobs = empty(with_top, at::kFloat, *z), top_tokens = empty(with_top, at::kLong, *z), stats = empty(with_two, at::kFloat, *z);
+  if (tokens) logprobs = empty(tokens->sizes(), at::kFloat, *z);
+  RUN(pb_token_logprobs(z->data_ptr(), code(z->scalar_type()), r.outer, z->numel() ? r.inner : 0, r.stride_outer, r.stride_inner, z->size(-1), n ? tokens->data_ptr<int64_t>() : nullptr, (int)n,
+                        (int)top, n ? logprobs.data_ptr<float>() : nullptr, entropy.data_ptr<float>(), top ? top_logprobs.data_ptr<float>() : nullptr,
+                        top ? top_tokens.data_ptr<int64_t>() : nullptr, stats.data_ptr<float>(), current_stream(z->device())));
+  PyObject* out = wrap({entropy, entropy, top_logprobs, top_tokens, stats});
+  PyObject* first = tokens ? wrap(logprobs) : none();
+  PyTuple_SetItem(out, 0, first);
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
+// token_logprobs_backward(logits, tokens or None, top_tokens, stats, entropy, g_logprobs or None, g_entropy or None, g_top or None) -> dlogits
+OP(token_logprobs_backward) {
+  HANDLE_TH_ERRORS
+  NARGS(8);
+  StridedRows r;
+  const at::Tensor* z = plain_rows(args[0], &r);
+  const at::Tensor* in[7];
+  for (int i = 0; i < 7; ++i) {
+    const bool may_miss = i == 0 || i >= 4;
+    if (may_miss && args[1 + i] == Py_None) { in[i] = nullptr; continue; }
+    if (!(in[i] = plain(args[1 + i]))) return none();
+  }
+  if (!z || watched()) return none();
+  const int64_t rows = z->numel() ? r.outer * r.inner : 0, top = in[1]->size(-1), n = in[0] && rows ? in[0]->numel() / rows : 0;
+  for (int i = 2; i < 7; ++i)
+    if (in[i] && (in[i]->scalar_type() != at::kFloat || in[i]->numel() != (i == 2 ? 2 * rows : i == 3 || i == 5 ? rows : i == 4 ? n * rows : top * rows))) return none();
+  const c10::cuda::CUDAGuard guard(z->device());
+  at::Tensor dz = empty(z->sizes(), z->scalar_type(), *z);
+  auto data = [&](int i) { return in[i] && in[i]->numel() ? in[i]->data_ptr<float>() : nullptr; };
+  RUN(pb_token_logprobs_bwd(z->data_ptr(), code(z->scalar_type()), r.outer, z->numel() ? r.inner : 0, r.stride_outer, r.stride_inner, z->size(-1),
+                            n ? in[0]->data_ptr<int64_t>() : nullptr, (int)n, top ? in[1]->data_ptr<int64_t>() : nullptr, (int)top, data(2), data(3), data(4), data(5), data(6), dz.data_ptr(),
+                            current_stream(z->device())));
+  return wrap(dz);
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- weights in 4 bits ----
+// quantize_int4(w [depth, cols], group, zero_points) -> (q, scale, zero or None)
+OP(quantize_int4) {
+  HANDLE_TH_ERRORS
+  NARGS(3);
+  const at::Tensor* w = plain(args[0]);
+  const int group = small(args[1]);
+  const bool zeros = PyObject_IsTrue(args[2]) == 1;
+  if (!w || watched() || !dense(w->scalar_type()) || w->dim() != 2 || w->numel() == 0 || (group != 32 && group != 64 && group != 128)) return none();
+  const c10::cuda::CUDAGuard guard(w->device());
+  const int64_t depth = w->size(0), cols = w->size(1), a = (cols + 15) / 16, b = (depth + 127) / 128;
+  at::Tensor q = empty({a, b, 1024}, at::kByte, *w), scale = empty({a, b, 16, 128 / group}, at::kBFloat16, *w), zero;
+  if (zeros) zero = empty({a, b, 16, 128 / group}, at::kByte, *w);
+  RUN(pb_quantize_int4(w->data_ptr(), code(w->scalar_type()), depth, cols, group, (uint8_t*)q.data_ptr(), scale.data_ptr(), zeros ? (uint8_t*)zero.data_ptr() : nullptr,
+                       current_stream(w->device())));
+  PyObject* out = wrap({q, scale, scale});
+  PyObject* last = zeros ? wrap(zero) : none();
+  PyTuple_SetItem(out, 2, last);
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
+// the parts of a 4-bit weight of [depth, cols]
+struct Int4 {
+  const at::Tensor *q, *scale, *zero = nullptr;
+  int group = 0;
+  bool take(PyObject* const* args, int64_t depth, int64_t cols) {
+    q = plain(args[0]); scale = plain(args[1]);
+    if (args[2] != Py_None && !(zero = plain(args[2]))) return false;
+    const int64_t a = (cols + 15) / 16, b = (depth + 127) / 128;
+    if (!q || !scale || depth <= 0 || cols <= 0 || q->scalar_type() != at::kByte || scale->scalar_type() != at::kBFloat16 || q->sizes() != at::IntArrayRef({a, b, 1024}) || scale->dim() != 4 ||
+        scale->size(0) != a || scale->size(1) != b || scale->size(2) != 16 || scale->device() != q->device())
+      return false;
+    const int64_t groups = scale->size(3);
+    if (groups != 1 && groups != 2 && groups != 4) return false;
+    group = (int)(128 / groups);
+    return !zero || (zero->scalar_type() == at::kByte && zero->sizes() == scale->sizes() && zero->device() == q->device());
+  }
+  uint8_t* zeros() const { return zero ? (uint8_t*)zero->data_ptr() : nullptr; }
+};
+
+// dequantize_int4(q, scale, zero or None, depth, cols, dtype) -> [depth, cols]
+OP(dequantize_int4) {
+  HANDLE_TH_ERRORS
+  NARGS(6);
+  const int64_t depth = integer(args[3]), cols = integer(args[4]);
+  Int4 w;
+  if (watched() || !THPDtype_Check(args[5]) || !w.take(args, depth, cols)) return none();
+  const at::ScalarType type = reinterpret_cast<THPDtype*>(args[5])->scalar_type;
+  if (!dense(type)) return none();
+  const c10::cuda::CUDAGuard guard(w.q->device());
+  at::Tensor out = empty({depth, cols}, type, *w.q);
+  RUN(pb_dequantize_int4((const uint8_t*)w.q->data_ptr(), w.scale->data_ptr(), w.zeros(), depth, cols, w.group, out.data_ptr(), code(type), current_stream(w.q->device())));
+  return wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// int4_product(x [.., depth], q, scale, zero or None, cols, dtype or None) -> [.., cols]
+OP(int4_product) {
+  HANDLE_TH_ERRORS
+  NARGS(6);
+  StridedRows r;
+  const at::Tensor* x = plain_rows(args[0], &r);
+  const int64_t cols = integer(args[4]);
+  Int4 w;
+  if (!x || watched() || r.outer != 1 || (args[5] != Py_None && !THPDtype_Check(args[5])) || !w.take(args + 1, x->size(-1), cols) || x->device() != w.q->device()) return none();
+  const at::ScalarType type = args[5] == Py_None ? x->scalar_type() : reinterpret_cast<THPDtype*>(args[5])->scalar_type;
+  if (!dense(type)) return none();
+  const c10::cuda::CUDAGuard guard(x->device());
+  c10::SmallVector<int64_t, 8> shape(x->sizes().begin(), x->sizes().end());
+  shape.back() = cols;
+  at::Tensor out = empty(shape, type, *x);
+  RUN(pb_int4_product(x->data_ptr(), code(x->scalar_type()), x->numel() ? r.inner : 0, x->size(-1), r.stride_inner, (const uint8_t*)w.q->data_ptr(), w.scale->data_ptr(), w.zeros(), w.group, cols,
+                      out.data_ptr(), code(type), current_stream(x->device())));
+  return wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
 // empty(shape, dtype, like) -> a tensor on the device of `like`; empties(like, count) -> a list of them, contiguous, of its shape and type
 OP(empty_on) {
   HANDLE_TH_ERRORS
@@ -678,6 +839,8 @@ PyMethodDef methods[] = {
     METHOD("quantize", quantize), METHOD("quantize_transposed", quantize_transposed), METHOD("dequantize", dequantize), METHOD("dequantize_bwd", dequantize_bwd),
     METHOD("fake_quantize", fake_quantize), METHOD("transpose_bytes", transpose_bytes), METHOD("gemm", gemm), METHOD("linear_step", linear_step), METHOD("linear", linear), METHOD("linear_takes", linear_takes),
     METHOD("linear_forward", linear_forward), METHOD("linear_backward", linear_backward),
+    METHOD("token_logprobs", token_logprobs), METHOD("token_logprobs_backward", token_logprobs_backward), METHOD("quantize_int4", quantize_int4),
+    METHOD("dequantize_int4", dequantize_int4), METHOD("int4_product", int4_product),
     METHOD("dense_dot", dense_dot), METHOD("empty", empty_on), METHOD("empties", empties),
     ENTRY(pb_quantize_dual), ENTRY(pb_dequantize_bwd_quantize_dual), ENTRY(pb_relu2_requantize), ENTRY(pb_quantize_transposed_workspace_size),
     ENTRY(pb_wkv7_forward), ENTRY(pb_wkv7_backward), ENTRY(pb_wkv7_checkpoint_floats),
@@ -686,6 +849,7 @@ PyMethodDef methods[] = {
     ENTRY(pb_rms_norm), ENTRY(pb_rms_norm_bwd), ENTRY(pb_rms_norm_bwd_workspace_size), ENTRY(pb_relu2), ENTRY(pb_relu2_bwd),
     ENTRY(pb_wkv_finish), ENTRY(pb_wkv_finish_workspace_size), ENTRY(pb_wkv_finish_bwd), ENTRY(pb_wkv_finish_bwd_workspace_size),
     ENTRY(pb_smoothed_xent), ENTRY(pb_smoothed_xent_bwd),
+    ENTRY(pb_token_logprobs), ENTRY(pb_token_logprobs_bwd), ENTRY(pb_quantize_int4), ENTRY(pb_dequantize_int4), ENTRY(pb_int4_product),
     {"set_error", set_error, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
