@@ -13,6 +13,8 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <cstring>
+#include <type_traits>
 
 namespace pb {
 namespace {
@@ -119,9 +121,11 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_int4_kernel(const ui
 // 128 + zero, both exact; sums over a group are f32, and meet the group's scale in f32.  An f32 x goes as three bf16 terms, 8 bits of its 24 each, in
 // three columns of the instruction whose sums meet at the end: for one or two rows they cost nothing.
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kStages = 4;             // tiles that a warp has on the way
 constexpr int kPad = 32;               // values behind a row of x in shared memory: neighbouring rows' 64 bytes then lie in other banks
 constexpr int kMaxCluster = 8;
+constexpr int kMaxChunk = 16;
+// tiles of a chunk that one warp's run can touch
+__host__ __device__ constexpr uint32_t segments_of(uint32_t chunk) { return (chunk + kWarps - 1) / kWarps + 1; }
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -133,10 +137,11 @@ __device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
 }
 // two codes of a word, less 128 + zero of `bias`
 template <int SHIFT> __device__ __forceinline__ uint32_t pair_of(uint32_t word, uint32_t bias) {
-  return sub_bf16x2((word >> SHIFT & 0x000f000fu) | 0x43004300u, bias);
+  uint32_t r;      // (word >> SHIFT & mask) | 128s in one operation behind the shift
+  asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xea;" : "=r"(r) : "r"(word >> SHIFT), "r"(0x43004300u));
+  return sub_bf16x2(r, bias);
 }
 __device__ __forceinline__ void copy16(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
-__device__ __forceinline__ void copy4(uint32_t to, const void* from) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory"); }
 __device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 // 8 bits of an f32 after another: x = hi + mid + lo (but for the last bits of numbers below 2^-110); an infinity or a NaN is hi alone
@@ -159,179 +164,289 @@ struct Product {
   uint32_t rows, depth, cols;
   uint32_t kblocks, tiles;               // of the weight
   uint32_t rows_per_pass;                // rows of x that one pass over the weight serves (blockIdx.y)
+  uint32_t chunk;                        // tiles between two barriers
+  uint32_t per_cta;                      // blocks of k of a CTA of a cluster
+  uint32_t tiles_each, tiles_over;       // tiles of a cluster; the first tiles_over clusters have one more
   int out_f32;
 };
 
-// A warp's ring of tiles: codes, scales and zero points of PER_GROUP groups
-template <int PER_GROUP, bool ZERO> struct Stage {
-  static constexpr int kScales = 1024, kZeros = kScales + 32 * PER_GROUP, kBytes = kZeros + (ZERO ? 16 * PER_GROUP : 0);
+// 128 values of k of 16 columns as a lane has them: the codes of two columns (g and g + 8 of the tile), 32 values of k each, and these columns' scales and
+// zero points
+template <int PER_GROUP, bool ZERO> struct Block {
+  uint4 lower, upper;
+  uint16_t scale[2][PER_GROUP];
+  uint8_t zero[2][PER_GROUP];
+  __device__ __forceinline__ void load(const Product& p, uint32_t unit, uint32_t lane) {
+    const uint4* codes = reinterpret_cast<const uint4*>(p.q + (uint64_t)unit * 1024) + lane;
+    lower = __ldg(codes);
+    upper = __ldg(codes + 32);
+    const uint16_t* s = reinterpret_cast<const uint16_t*>(p.scale) + (uint64_t)unit * (16 * PER_GROUP) + (lane >> 2) * PER_GROUP;
+    vector(scale[0], s);
+    vector(scale[1], s + 8 * PER_GROUP);
+    if (ZERO) {
+      const uint8_t* z = p.zero + (uint64_t)unit * (16 * PER_GROUP) + (lane >> 2) * PER_GROUP;
+      vector(zero[0], z);
+      vector(zero[1], z + 8 * PER_GROUP);
+    }
+  }
+  template <typename E> static __device__ __forceinline__ void vector(E (&to)[PER_GROUP], const E* from) {      // one load of 1 to 8 bytes
+    constexpr int kBytes = PER_GROUP * sizeof(E);
+    using W = std::conditional_t<kBytes == 1, uint8_t, std::conditional_t<kBytes == 2, uint16_t, std::conditional_t<kBytes == 4, uint32_t, uint2>>>;
+    const W w = __ldg(reinterpret_cast<const W*>(from));
+    memcpy(to, &w, kBytes);
+  }
 };
 
-// MT: sets of 8 columns.  A CTA's warps share a tile's 16 columns n and split its 128-blocks of k; the CTAs of a cluster split k before that.
-// Each warp copies its tiles ahead into a ring of its own.
+// MT: sets of 8 columns of the instruction.  The CTAs of a cluster split k; a cluster has a run of the weight's tiles, `chunk` of them at a time.  A CTA's
+// blocks of a chunk, tile after tile, are cut evenly over its eight warps wherever the cut falls: a warp reads one run of memory, a block ahead of the one
+// that it computes, and leaves its sum of each tile (or part of one) in shared memory.  They meet behind one barrier a chunk.
 template <typename TX, int MT, int PER_GROUP, bool ZERO>
 __global__ void __launch_bounds__(kThreads) int4_product_kernel(const Product p) {
   grid_wait();
-  using S = Stage<PER_GROUP, ZERO>;
   constexpr int kTerms = sizeof(TX) == 4 ? 3 : 1;
   extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ uint32_t starts[kWarps + 1], tiles_at[kWarps];      // of the warps' runs in a chunk: their first blocks, and the tiles these are in
   cg::cluster_group cluster = cg::this_cluster();
-  const uint32_t ctas = cluster.num_blocks(), rank = cluster.block_rank();
-  const uint32_t per = (p.kblocks + ctas - 1) / ctas, kb0 = min(rank * per, p.kblocks), kbn = min(per, p.kblocks - kb0);
+  const uint32_t ctas = cluster.num_blocks(), rank = cluster.block_rank(), id = blockIdx.x / ctas;
+  const uint32_t kb0 = min(rank * p.per_cta, p.kblocks), kbn = min(p.per_cta, p.kblocks - kb0);
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const uint32_t row0 = blockIdx.y * p.rows_per_pass, rows = min(p.rows_per_pass, p.rows - row0), columns = rows * kTerms;
-  uint8_t* ring = smem + warp * (kStages * S::kBytes);
-  float* sums = reinterpret_cast<float*>(smem + kWarps * kStages * S::kBytes);      // [warps][16][8 MT]; the CTA's at its beginning
-  uint16_t* xs = reinterpret_cast<uint16_t*>(sums + kWarps * 16 * 8 * MT);
-  const uint32_t pitch = per * 128 + kPad;
+  const uint32_t first = id * p.tiles_each + min(id, p.tiles_over), last = first + p.tiles_each + (id < p.tiles_over ? 1 : 0);
+  const uint32_t sum_floats = columns * 16, segments = segments_of(p.chunk);
+  float* sums = reinterpret_cast<float*>(smem);                                     // [warp][segment][column][16 n]
+  float* joined = sums + kWarps * segments * sum_floats;                            // a cluster's: [tile][column][16 n]
+  uint16_t* xs = reinterpret_cast<uint16_t*>(joined + (ctas > 1 ? p.chunk * sum_floats : 0));
+  const uint32_t pitch = p.per_cta * 128 + kPad;
 
-  // the tiles of this warp: tile after tile of the grid's stride, in each its blocks of k
-  uint32_t ahead_tile = blockIdx.x / ctas, ahead_kb = warp;
-  const uint32_t tile_step = gridDim.x / ctas;
-  const uint32_t ring_at = shared_address(ring);
-  auto ask = [&](uint32_t stage) {
-    while (ahead_kb >= kbn && ahead_tile < p.tiles) { ahead_kb = warp; ahead_tile += tile_step; if (warp >= kbn) ahead_tile = p.tiles; }
-    if (ahead_tile < p.tiles) {
-      const uint64_t unit = (uint64_t)ahead_tile * p.kblocks + kb0 + ahead_kb;
-      const uint32_t to = ring_at + stage * S::kBytes;
-      copy16(to + lane * 16, p.q + unit * 1024 + lane * 16);
-      copy16(to + 512 + lane * 16, p.q + unit * 1024 + 512 + lane * 16);
-      if (lane < 8 * PER_GROUP) copy4(to + S::kScales + lane * 4, reinterpret_cast<const uint8_t*>(p.scale) + unit * (32 * PER_GROUP) + lane * 4);
-      if (ZERO && lane < 4 * PER_GROUP) copy4(to + S::kZeros + lane * 4, p.zero + unit * (16 * PER_GROUP) + lane * 4);
-      ahead_kb += kWarps;
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
+  uint32_t unit = 0, run = 0, kb = 0;      // of this warp: the next block's number in the weight, blocks of the chunk, and where the first one is in its tile
+  auto start_chunk = [&](uint32_t tile0, uint32_t count) {
+    const uint32_t all = count * kbn, begin = all * warp / kWarps;
+    run = all * (warp + 1) / kWarps - begin;
+    const uint32_t tile = kbn ? begin / kbn : 0;
+    kb = begin - tile * kbn;
+    if (lane == 0) { starts[warp] = begin; tiles_at[warp] = tile; }
+    if (tid == 0) starts[kWarps] = all;
+    unit = (tile0 + tile) * p.kblocks + kb0 + kb;
   };
-#pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) ask(s);
+  start_chunk(first, min(p.chunk, last - first));
+  Block<PER_GROUP, ZERO> one, two;
+  uint32_t asked = kb;      // the place in its tile of the block to be loaded next
+  auto load = [&](Block<PER_GROUP, ZERO>& to) {
+    to.load(p, unit, lane);
+    ++unit;
+    if (++asked == kbn) { asked = 0; unit += p.kblocks - kbn; }
+  };
+  if (run > 0) load(one);
+  if (run > 1) load(two);
 
-  // this CTA's part of x, as bf16
-  const TX* x = static_cast<const TX*>(p.x) + (int64_t)row0 * p.stride;
-  for (uint32_t m = 0; m < rows; ++m)
-    for (uint32_t k = tid; k < kbn * 128; k += kThreads) {
-      const uint32_t at = kb0 * 128 + k;
+  // this CTA's part of x, as bf16, eight values at a time; where they are bf16 and lie at 16 bytes they are copied while the first tiles are
+  const TX* x = static_cast<const TX*>(p.x) + (int64_t)row0 * p.stride + kb0 * 128;
+  const uint32_t eights = kbn * 16, depth = p.depth - min(p.depth, kb0 * 128);
+  const bool whole = ((reinterpret_cast<uintptr_t>(x) | (uint64_t)p.stride * sizeof(TX)) & 15) == 0;
+  if (kTerms == 1 && whole) {
+    for (uint32_t i = tid; i < rows * eights; i += kThreads) {
+      const uint32_t m = i / eights, k = (i - m * eights) * 8;
+      const TX* from = x + (int64_t)m * p.stride + k;
+      uint16_t* to = xs + m * pitch + k;
+      if (k + 8 <= depth) copy16(shared_address(to), from);
+      else
+        for (uint32_t e = 0; e < 8; ++e) to[e] = k + e < depth ? reinterpret_cast<const uint16_t*>(from)[e] : (uint16_t)0;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else {
+#pragma unroll 4
+    for (uint32_t i = tid; i < rows * eights; i += kThreads) {
+      const uint32_t m = i / eights, k = (i - m * eights) * 8;
+      const TX* from = x + (int64_t)m * p.stride + k;
       if constexpr (kTerms == 3) {
-        uint16_t* to = xs + (uint64_t)(m * 3) * pitch + k;
-        three_terms(at < p.depth ? x[m * p.stride + at] : 0.0f, to[0], to[pitch], to[2 * pitch]);
+        float v[8];
+        if (whole && k + 8 <= depth) {
+          const float4 a = *reinterpret_cast<const float4*>(from), b = *reinterpret_cast<const float4*>(from + 4);
+          v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
+#pragma unroll
+          for (uint32_t e = 0; e < 8; ++e) v[e] = k + e < depth ? from[e] : 0.0f;
+        }
+        uint32_t t[3][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint16_t lo[3], hi[3];
+          three_terms(v[2 * e], lo[0], lo[1], lo[2]);
+          three_terms(v[2 * e + 1], hi[0], hi[1], hi[2]);
+#pragma unroll
+          for (int j = 0; j < 3; ++j) t[j][e] = lo[j] | (uint32_t)hi[j] << 16;
+        }
+#pragma unroll
+        for (int j = 0; j < 3; ++j) *reinterpret_cast<uint4*>(xs + (m * 3 + j) * pitch + k) = make_uint4(t[j][0], t[j][1], t[j][2], t[j][3]);
       } else {
-        xs[(uint64_t)m * pitch + k] = at < p.depth ? reinterpret_cast<const uint16_t*>(x)[m * p.stride + at] : (uint16_t)0;
+        uint32_t t[4];
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) {
+          const uint16_t* h = reinterpret_cast<const uint16_t*>(from) + 2 * e;
+          t[e] = (k + 2 * e < depth ? h[0] : 0u) | (k + 2 * e + 1 < depth ? (uint32_t)h[1] << 16 : 0u);
+        }
+        *reinterpret_cast<uint4*>(xs + m * pitch + k) = make_uint4(t[0], t[1], t[2], t[3]);
       }
     }
+  }
   __syncthreads();
 
-  uint32_t stage = 0;
-  for (uint32_t tile = blockIdx.x / ctas; tile < p.tiles; tile += tile_step) {
+  // a column of the instruction that is none of x's has another's values: nobody reads its sums
+  const uint16_t* mine[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) mine[i] = xs + min(i * 8 + g, columns - 1) * pitch + t * 8;
+  for (uint32_t tile0 = first; tile0 < last; tile0 += p.chunk) {
+    const uint32_t count = min(p.chunk, last - tile0);
     float total[MT][4];
 #pragma unroll
     for (int i = 0; i < MT; ++i) total[i][0] = total[i][1] = total[i][2] = total[i][3] = 0.0f;
-    for (uint32_t kb = warp; kb < kbn; kb += kWarps) {
-      ask((stage + kStages - 1) % kStages);
-      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
-      __syncwarp();
-      const uint8_t* in = ring + stage * S::kBytes;
-      const uint4 lower = *reinterpret_cast<const uint4*>(in + lane * 16), upper = *reinterpret_cast<const uint4*>(in + 512 + lane * 16);
-      const uint16_t* scales = reinterpret_cast<const uint16_t*>(in + S::kScales);
-      const uint32_t lo[4] = {lower.x, lower.y, lower.z, lower.w}, up[4] = {upper.x, upper.y, upper.z, upper.w};
-      float sum[MT][4];
+    float* own = sums + warp * segments * sum_floats;
+    auto multiply = [&](const Block<PER_GROUP, ZERO>& w, bool ends) {
+      const uint32_t lo[4] = {w.lower.x, w.lower.y, w.lower.z, w.lower.w}, up[4] = {w.upper.x, w.upper.y, w.upper.z, w.upper.w};
+      constexpr int kRun = 4 / PER_GROUP;                                   // 32-value runs of a group
+      constexpr int kChains = MT == 1 && PER_GROUP == 1 ? 2 : 1;            // sums under way at once where one would wait for itself
+      float sum[MT][kChains][4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        constexpr int kRun = 4 / PER_GROUP;      // 32-value runs of a group
-        const int of = c / kRun;
+        const int of = c / kRun, chain = c % kChains;
         uint32_t bias_lo = 0x43084308u, bias_up = 0x43084308u;
         if (ZERO) {
-          bias_lo = (0x4300u | in[S::kZeros + g * PER_GROUP + of]) * 0x10001u;
-          bias_up = (0x4300u | in[S::kZeros + (g + 8) * PER_GROUP + of]) * 0x10001u;
+          bias_lo = (0x4300u | w.zero[0][of]) * 0x10001u;
+          bias_up = (0x4300u | w.zero[1][of]) * 0x10001u;
         }
         if (c % kRun == 0)
 #pragma unroll
-          for (int i = 0; i < MT; ++i) sum[i][0] = sum[i][1] = sum[i][2] = sum[i][3] = 0.0f;
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int h = 0; h < kChains; ++h) sum[i][h][0] = sum[i][h][1] = sum[i][h][2] = sum[i][h][3] = 0.0f;
         const uint32_t a[8] = {pair_of<0>(lo[c], bias_lo), pair_of<0>(up[c], bias_up), pair_of<4>(lo[c], bias_lo), pair_of<4>(up[c], bias_up),
                                pair_of<8>(lo[c], bias_lo), pair_of<8>(up[c], bias_up), pair_of<12>(lo[c], bias_lo), pair_of<12>(up[c], bias_up)};
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-          uint4 b = make_uint4(0, 0, 0, 0);
-          if (i * 8 + g < columns) b = *reinterpret_cast<const uint4*>(xs + (uint64_t)(i * 8 + g) * pitch + kb * 128 + c * 32 + t * 8);
-          mma(sum[i], a[0], a[1], a[2], a[3], b.x, b.y);
-          mma(sum[i], a[4], a[5], a[6], a[7], b.z, b.w);
+          const uint4 x4 = *reinterpret_cast<const uint4*>(mine[i] + kb * 128 + c * 32);
+          mma(sum[i][chain], a[0], a[1], a[2], a[3], x4.x, x4.y);
+          mma(sum[i][chain], a[4], a[5], a[6], a[7], x4.z, x4.w);
         }
         if (c % kRun == kRun - 1) {
-          const float s_lo = __uint_as_float((uint32_t)scales[g * PER_GROUP + of] << 16), s_up = __uint_as_float((uint32_t)scales[(g + 8) * PER_GROUP + of] << 16);
+          const float s_lo = __uint_as_float((uint32_t)w.scale[0][of] << 16), s_up = __uint_as_float((uint32_t)w.scale[1][of] << 16);
 #pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            total[i][0] = fmaf(s_lo, sum[i][0], total[i][0]);
-            total[i][1] = fmaf(s_lo, sum[i][1], total[i][1]);
-            total[i][2] = fmaf(s_up, sum[i][2], total[i][2]);
-            total[i][3] = fmaf(s_up, sum[i][3], total[i][3]);
-          }
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) total[i][e] = fmaf(e < 2 ? s_lo : s_up, kChains == 2 ? sum[i][0][e] + sum[i][kChains - 1][e] : sum[i][0][e], total[i][e]);
         }
       }
-      __syncwarp();      // the stage is free for the next copy
-      stage = (stage + 1) % kStages;
-    }
-    // the warps' sums, column by column of the instruction: [column][16 n]
+      if (++kb == kbn || ends) {      // a tile's end, or the run's
+        kb = 0;
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t column = i * 8 + t * 2 + (e & 1);
-        if (column < columns) sums[warp * (128 * MT) + column * 16 + g + (e & 2) * 4] = total[i][e];
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t column = i * 8 + t * 2 + (e & 1);
+            if (column < columns) own[column * 16 + g + (e & 2) * 4] = total[i][e];
+            total[i][e] = 0.0f;
+          }
+        own += sum_floats;
       }
-    __syncthreads();
-    for (uint32_t i = tid; i < columns * 16; i += kThreads) {
-      float s = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) s += sums[w * (128 * MT) + i];
-      sums[i] = s;
+    };
+    for (uint32_t b = run; b > 0;) {
+      multiply(one, b == 1);
+      if (b > 2) load(one);
+      if (--b == 0) break;
+      multiply(two, b == 1);
+      if (b > 2) load(two);
+      --b;
     }
-    if (ctas > 1) cluster.sync(); else __syncthreads();
-    // the ranks' sums: each rank finishes a part of the rows
-    for (uint32_t i = rank * kThreads + tid; i < rows * 16; i += ctas * kThreads) {
-      const uint32_t m = i / 16, n = i % 16;
+    __syncthreads();
+    // the sum of a tile's entry over the warps that have a part of it
+    auto over_warps = [&](uint32_t j, uint32_t at) {
       float y = 0.0f;
 #pragma unroll
-      for (int term = kTerms - 1; term >= 0; --term) {      // the small ones first
-        const uint32_t at = (m * kTerms + term) * 16 + n;
-        if (ctas == 1) y += sums[at];
-        else for (uint32_t r = 0; r < ctas; ++r) y += *cluster.map_shared_rank(sums + at, r);
+      for (int w = 0; w < kWarps; ++w) {
+        const uint32_t lo = starts[w], hi = starts[w + 1];
+        const bool has = lo < hi && lo < (j + 1) * kbn && hi > j * kbn;
+        const float s = sums[(w * segments + (has ? j - tiles_at[w] : 0)) * sum_floats + at];
+        y += has ? s : 0.0f;
       }
-      const uint32_t col = tile * 16 + n;
-      if (col < p.cols) {
-        const int64_t at = (int64_t)(row0 + m) * p.cols + col;
-        if (p.out_f32) static_cast<float*>(p.out)[at] = y;
-        else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(y);
+      return y;
+    };
+    auto write = [&](uint32_t j, uint32_t m, uint32_t n, float y) {
+      const uint32_t col = (tile0 + j) * 16 + n;
+      if (col >= p.cols) return;
+      const int64_t at = (int64_t)(row0 + m) * p.cols + col;
+      if (p.out_f32) static_cast<float*>(p.out)[at] = y;
+      else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(y);
+    };
+    const uint32_t outputs = rows * 16;      // of a tile; a term's and a row's sums lie 16 apart
+    if (ctas == 1) {
+      for (uint32_t i = tid; i < count * outputs; i += kThreads) {
+        const uint32_t j = i / outputs, m = (i - j * outputs) / 16, n = i % 16;
+        float y = 0.0f;
+#pragma unroll
+        for (int term = kTerms - 1; term >= 0; --term) y += over_warps(j, (m * kTerms + term) * 16 + n);      // the small ones first
+        write(j, m, n, y);
+      }
+    } else {
+      for (uint32_t i = tid; i < count * sum_floats; i += kThreads) {
+        const uint32_t j = i / sum_floats;
+        joined[i] = over_warps(j, i - j * sum_floats);
+      }
+      cluster.sync();
+      for (uint32_t i = rank * kThreads + tid; i < count * outputs; i += ctas * kThreads) {      // each rank finishes a part
+        const uint32_t j = i / outputs, m = (i - j * outputs) / 16, n = i % 16;
+        float y = 0.0f;
+#pragma unroll
+        for (int term = kTerms - 1; term >= 0; --term)
+          for (uint32_t r = 0; r < ctas; ++r) y += *cluster.map_shared_rank(joined + j * sum_floats + (m * kTerms + term) * 16 + n, r);
+        write(j, m, n, y);
       }
     }
-    if (ctas > 1) cluster.sync(); else __syncthreads();      // the sums' memory is free, and nobody leaves while it is read
+    const uint32_t next = tile0 + p.chunk;
+    if (ctas > 1) cluster.sync();                 // nobody leaves or writes its sums again while they are read
+    else if (next < last) __syncthreads();
+    if (next < last) {
+      start_chunk(next, min(p.chunk, last - next));
+      asked = kb;
+      if (run > 0) load(one);
+      if (run > 1) load(two);
+    }
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-template <typename TX, int MT, int PER_GROUP, bool ZERO> size_t shared_bytes(uint32_t columns, uint32_t kblocks_of_cta) {
-  return kWarps * kStages * Stage<PER_GROUP, ZERO>::kBytes + kWarps * 16 * 8 * MT * 4 + (size_t)columns * (kblocks_of_cta * 128 + kPad) * 2;
+template <int MT> size_t shared_bytes(uint32_t columns, uint32_t kblocks_of_cta, uint32_t chunk, uint32_t ctas) {
+  return (size_t)columns * 64 * (kWarps * segments_of(chunk) + (ctas > 1 ? chunk : 0)) + (size_t)columns * (kblocks_of_cta * 128 + kPad) * 2;
 }
 
-constexpr size_t kMaxShared = 227 * 1024;
+constexpr size_t kMaxShared = 226 * 1024;      // of 227 KB, beside the kernel's own few bytes
 
 template <typename TX, int MT, int PER_GROUP, bool ZERO> int launch_product(Product p, cudaStream_t st) {
   constexpr uint32_t kTerms = sizeof(TX) == 4 ? 3 : 1;
   auto kernel = int4_product_kernel<TX, MT, PER_GROUP, ZERO>;
-  uint32_t ctas = 1, per_pass = p.rows < 8 * MT / kTerms ? p.rows : 8 * MT / kTerms;
+  uint32_t ctas = 1, per_pass = p.rows < 8 * MT / kTerms ? p.rows : 8 * MT / kTerms, per_sm = 2, clusters = 1;
   size_t bytes;
+  const uint32_t wanted = env_switch("PB_INT4_PERSM", 2), force = env_switch("PB_INT4_CTAS", 0);
   while (true) {      // x in shared memory: split k over a cluster, and where that is not enough serve fewer rows with a pass
-    bytes = shared_bytes<TX, MT, PER_GROUP, ZERO>(per_pass * kTerms, (p.kblocks + ctas - 1) / ctas);
-    if (bytes <= kMaxShared) break;
+    const uint32_t per = (p.kblocks + ctas - 1) / ctas;
+    for (per_sm = wanted; per_sm > 0; --per_sm) {
+      clusters = std::max<uint32_t>(1, std::min<uint32_t>(p.tiles, sm_count() * per_sm / ctas));
+      p.chunk = std::min<uint32_t>(kMaxChunk, (p.tiles + clusters - 1) / clusters);
+      bytes = shared_bytes<MT>(per_pass * kTerms, per, p.chunk, ctas);
+      if (bytes <= kMaxShared && (per_sm == 1 || per_sm * (bytes + 1024) <= 228 * 1024)) break;
+    }
+    const bool fits = per_sm > 0;
+    if (fits && (force ? ctas == force : ctas == kMaxCluster || (per_sm == wanted && (p.tiles * ctas >= (uint32_t)sm_count() || p.kblocks <= ctas * kWarps * 4)))) break;
     if (ctas < kMaxCluster) ctas *= 2;
     else if (per_pass > 1) { per_pass /= 2; ctas = 1; }
     else return fail(PB_ERR_UNSUPPORTED, "pb_int4_product: a contraction of %u does not fit", p.depth);
   }
   p.rows_per_pass = per_pass;
+  p.per_cta = (p.kblocks + ctas - 1) / ctas;
+  p.tiles_each = p.tiles / clusters;
+  p.tiles_over = p.tiles % clusters;
   PB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxShared));
-  const uint32_t per_sm = (uint32_t)std::max<size_t>(1, std::min<size_t>(4, (size_t)(228 * 1024) / (bytes + 1024)));
-  const uint32_t room = std::max<uint32_t>(1, sm_count() * per_sm / ctas);
   const uint32_t passes = (p.rows + per_pass - 1) / per_pass;
   if (passes > 65535) return fail(PB_ERR_UNSUPPORTED, "pb_int4_product: %u rows", p.rows);
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(std::min(p.tiles, room) * ctas, passes);
+  config.gridDim = dim3(clusters * ctas, passes);
   config.blockDim = dim3(kThreads);
   config.dynamicSmemBytes = bytes;
   config.stream = st;
@@ -416,7 +531,7 @@ extern "C" int pb_int4_product(const void* x, int x_dtype, int64_t rows, int64_t
       (reinterpret_cast<uintptr_t>(x) % (x_dtype == PB_F32 ? 4 : 2)) || (reinterpret_cast<uintptr_t>(out) % (out_dtype == PB_F32 ? 4 : 2)))
     return fail(PB_ERR_MISALIGNED, "pb_int4_product: q 16, scale and zero 4 bytes, x and out their types");
   Product p{x, stride, q, static_cast<const __nv_bfloat16*>(scale), zero, out, (uint32_t)rows, (uint32_t)depth, (uint32_t)cols, (uint32_t)((depth + 127) / 128),
-            (uint32_t)((cols + 15) / 16), 0, out_dtype == PB_F32};
+            (uint32_t)((cols + 15) / 16), 0, 0, 0, 0, 0, out_dtype == PB_F32};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int64_t columns = rows * (x_dtype == PB_F32 ? 3 : 1);
   if (x_dtype == PB_F32) return columns <= 8 ? launch_of<float, 1>(p, 128 / group, st) : columns <= 16 ? launch_of<float, 2>(p, 128 / group, st) : launch_of<float, 4>(p, 128 / group, st);
