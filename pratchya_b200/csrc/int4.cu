@@ -122,8 +122,10 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_int4_kernel(const ui
 // three columns of the instruction whose sums meet at the end: for one or two rows they cost nothing.
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kPad = 32;               // values behind a row of x in shared memory: neighbouring rows' 64 bytes then lie in other banks
+constexpr int kPadDigits = 16;         // the same for digits: neighbouring rows' sixteen bytes of four lanes in turn
 constexpr int kMaxCluster = 8;
 constexpr int kMaxChunk = 16;
+constexpr uint32_t kNoTile = 0xffffffffu;
 // tiles of a chunk that one warp's run can touch
 __host__ __device__ constexpr uint32_t segments_of(uint32_t chunk) { return (chunk + kWarps - 1) / kWarps + 1; }
 
@@ -144,15 +146,35 @@ template <int SHIFT> __device__ __forceinline__ uint32_t pair_of(uint32_t word, 
 __device__ __forceinline__ void copy16(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
 __device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
-// 8 bits of an f32 after another: x = hi + mid + lo (but for the last bits of numbers below 2^-110); an infinity or a NaN is hi alone
-__device__ __forceinline__ void three_terms(float x, uint16_t& hi, uint16_t& mid, uint16_t& lo) {
-  const uint32_t h = __float_as_uint(x) & 0xffff0000u;
-  hi = x != x ? 0x7fc0 : (uint16_t)(h >> 16);
-  const float r = (h & 0x7f800000u) == 0x7f800000u ? 0.0f : x - __uint_as_float(h);
-  const uint32_t m = __float_as_uint(r) & 0xffff0000u;
-  mid = (uint16_t)(m >> 16);
-  lo = (uint16_t)(__float_as_uint(r - __uint_as_float(m)) >> 16);
+__device__ __forceinline__ void mma_from_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
+__device__ __forceinline__ void mma(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// A whole number below 2^22 in size as the low bits of an f32: kWhole + i, whose value less kWholeValue is i
+constexpr int kWhole = 0x4b400000;
+constexpr float kWholeValue = 12582912.0f;
+
+// The whole numbers that a block of 128 values of x becomes: x = scale * t in DIGITS digits of eight bits with a sign each.  The scale is a power of two, and
+// |t| < 2^22 or 2^30: a bf16 within 2^-14 of its block's largest and an f32 within 2^-7 are exact, smaller ones to 2^-22 and 2^-30 of the largest.
+template <int DIGITS> struct Whole {
+  static constexpr uint32_t kBits = 8 * DIGITS - 3;
+  float up, scale;
+  __device__ __forceinline__ explicit Whole(uint32_t largest) {      // the bits of the block's largest |x|
+    const uint32_t e = max(largest >> 23, 30u);                      // below 2^-97 digits of 2^-126 and more are left
+    const bool finite = largest < 0x7f800000u;                       // with an infinity or a NaN every product of the row is NaN
+    up = finite ? __uint_as_float((254u + kBits - e) << 23) : 0.0f;
+    scale = __uint_as_float(finite ? (e - kBits) << 23 : 0x7fc00000u);
+  }
+  // the digits of x as bytes, each with its sign, the lowest first: halves of their range are added, so that none borrows, and turned into signs
+  __device__ __forceinline__ uint32_t digits(float x) const {
+    constexpr uint32_t kHalves = DIGITS == 4 ? 0x00808080u : 0x00008080u;
+    return ((uint32_t)(up == 0.0f ? 0 : __float2int_rn(x * up)) + kHalves) ^ kHalves;
+  }
+};
 
 struct Product {
   const void* x;
@@ -197,26 +219,32 @@ template <int PER_GROUP, bool ZERO> struct Block {
   }
 };
 
-// MT: sets of 8 columns of the instruction.  The CTAs of a cluster split k; a cluster has a run of the weight's tiles, `chunk` of them at a time.  A CTA's
-// blocks of a chunk, tile after tile, are cut evenly over its eight warps wherever the cut falls: a warp reads one run of memory, a block ahead of the one
-// that it computes, and leaves its sum of each tile (or part of one) in shared memory.  They meet behind one barrier a chunk.
-template <typename TX, int MT, int PER_GROUP, bool ZERO>
-__global__ void __launch_bounds__(kThreads) int4_product_kernel(const Product p) {
+// DIGITS: 0 takes a bf16 x as it is, 3 and 4 take x as whole numbers; MT: sets of 8 columns of the instruction.  The CTAs of a cluster split k; a cluster has a
+// run of the weight's tiles, `chunk` of them at a time.  A CTA's blocks of a chunk, tile after tile, are cut evenly over its eight warps wherever the cut
+// falls: a warp reads one run of memory, blocks ahead of the one that it computes, and leaves its sum of each tile (or part of one) in shared
+// memory.  They meet behind one barrier a chunk.
+template <typename TX, int DIGITS, int MT, int PER_GROUP, bool ZERO>
+__global__ void __launch_bounds__(kThreads, MT <= 2 ? 2 : 1) int4_product_kernel(const Product p) {
   grid_wait();
-  constexpr int kTerms = sizeof(TX) == 4 ? 3 : 1;
+  constexpr int kParts = DIGITS ? DIGITS : 1;      // columns of the instruction that a row of x takes, the first with its uppermost digits
+  constexpr int kAhead = MT <= 2 ? 4 : 2;          // blocks that a warp has on the way or in hand
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ uint32_t starts[kWarps + 1], tiles_at[kWarps];      // of the warps' runs in a chunk: their first blocks, and the tiles these are in
+  // of a chunk: the tile that a warp's run begins in (none: kNoTile), and the warps that have a tile's first and last block
+  __shared__ uint32_t tiles_at[kWarps], first_warp[kMaxChunk], last_warp[kMaxChunk];
   cg::cluster_group cluster = cg::this_cluster();
   const uint32_t ctas = cluster.num_blocks(), rank = cluster.block_rank(), id = blockIdx.x / ctas;
   const uint32_t kb0 = min(rank * p.per_cta, p.kblocks), kbn = min(p.per_cta, p.kblocks - kb0);
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const uint32_t row0 = blockIdx.y * p.rows_per_pass, rows = min(p.rows_per_pass, p.rows - row0), columns = rows * kTerms;
+  const uint32_t row0 = blockIdx.y * p.rows_per_pass, rows = min(p.rows_per_pass, p.rows - row0), columns = rows * kParts;
   const uint32_t first = id * p.tiles_each + min(id, p.tiles_over), last = first + p.tiles_each + (id < p.tiles_over ? 1 : 0);
   const uint32_t sum_floats = columns * 16, segments = segments_of(p.chunk);
   float* sums = reinterpret_cast<float*>(smem);                                     // [warp][segment][column][16 n]
   float* joined = sums + kWarps * segments * sum_floats;                            // a cluster's: [tile][column][16 n]
-  uint16_t* xs = reinterpret_cast<uint16_t*>(joined + (ctas > 1 ? p.chunk * sum_floats : 0));
-  const uint32_t pitch = p.per_cta * 128 + kPad;
+  // x: a column's bf16 values or digits, [column][k]; of the digits also, of every column, the scale of each block, and of each group the sum, for the weight's zero points
+  uint8_t* xs = reinterpret_cast<uint8_t*>(joined + (ctas > 1 ? p.chunk * sum_floats : 0));
+  const uint32_t pitch = DIGITS ? p.per_cta * 128 + kPadDigits : (p.per_cta * 128 + kPad) * 2;
+  float* x_scales = reinterpret_cast<float*>(xs + columns * pitch);                 // [block][8 MT]
+  int* x_sums = reinterpret_cast<int*>(x_scales + p.per_cta * 8 * MT);              // [block][group][8 MT]
 
   uint32_t unit = 0, run = 0, kb = 0;      // of this warp: the next block's number in the weight, blocks of the chunk, and where the first one is in its tile
   auto start_chunk = [&](uint32_t tile0, uint32_t count) {
@@ -224,115 +252,193 @@ __global__ void __launch_bounds__(kThreads) int4_product_kernel(const Product p)
     run = all * (warp + 1) / kWarps - begin;
     const uint32_t tile = kbn ? begin / kbn : 0;
     kb = begin - tile * kbn;
-    if (lane == 0) { starts[warp] = begin; tiles_at[warp] = tile; }
-    if (tid == 0) starts[kWarps] = all;
+    if (lane == 0) tiles_at[warp] = run ? tile : kNoTile;
+    if (tid < count && kbn) {      // block b is of the last warp w whose run begins, at all * w / kWarps, no later
+      first_warp[tid] = ((tid * kbn + 1) * kWarps + all - 1) / all - 1;
+      last_warp[tid] = ((tid + 1) * kbn * kWarps + all - 1) / all - 1;
+    }
     unit = (tile0 + tile) * p.kblocks + kb0 + kb;
   };
   start_chunk(first, min(p.chunk, last - first));
-  Block<PER_GROUP, ZERO> one, two;
+  Block<PER_GROUP, ZERO> ahead[kAhead];
   uint32_t asked = kb;      // the place in its tile of the block to be loaded next
   auto load = [&](Block<PER_GROUP, ZERO>& to) {
     to.load(p, unit, lane);
     ++unit;
     if (++asked == kbn) { asked = 0; unit += p.kblocks - kbn; }
   };
-  if (run > 0) load(one);
-  if (run > 1) load(two);
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+    if (run > (uint32_t)i) load(ahead[i]);
 
-  // this CTA's part of x, as bf16, eight values at a time; where they are bf16 and lie at 16 bytes they are copied while the first tiles are
+  // this CTA's part of x
   const TX* x = static_cast<const TX*>(p.x) + (int64_t)row0 * p.stride + kb0 * 128;
-  const uint32_t eights = kbn * 16, depth = p.depth - min(p.depth, kb0 * 128);
-  const bool whole = ((reinterpret_cast<uintptr_t>(x) | (uint64_t)p.stride * sizeof(TX)) & 15) == 0;
-  if (kTerms == 1 && whole) {
-    for (uint32_t i = tid; i < rows * eights; i += kThreads) {
-      const uint32_t m = i / eights, k = (i - m * eights) * 8;
-      const TX* from = x + (int64_t)m * p.stride + k;
-      uint16_t* to = xs + m * pitch + k;
-      if (k + 8 <= depth) copy16(shared_address(to), from);
-      else
-        for (uint32_t e = 0; e < 8; ++e) to[e] = k + e < depth ? reinterpret_cast<const uint16_t*>(from)[e] : (uint16_t)0;
-    }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-  } else {
-#pragma unroll 4
-    for (uint32_t i = tid; i < rows * eights; i += kThreads) {
-      const uint32_t m = i / eights, k = (i - m * eights) * 8;
-      const TX* from = x + (int64_t)m * p.stride + k;
-      if constexpr (kTerms == 3) {
-        float v[8];
-        if (whole && k + 8 <= depth) {
-          const float4 a = *reinterpret_cast<const float4*>(from), b = *reinterpret_cast<const float4*>(from + 4);
-          v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
+  const uint32_t depth = p.depth - min(p.depth, kb0 * 128);
+  if constexpr (DIGITS != 0) {      // a warp takes a row's block at a time, a lane four values of it: two pairs of the eight that a word of codes meets
+    const uint32_t word = lane / 2, at = word * 8 + (lane & 1) * 2;
+    const bool pairs = ((reinterpret_cast<uintptr_t>(x) | (uint64_t)p.stride * sizeof(TX)) & (2 * sizeof(TX) - 1)) == 0;
+    constexpr int kBatch = MT == 1 ? 2 : 4;      // row blocks on the way
+    for (uint32_t i0 = warp; i0 < rows * kbn; i0 += kWarps * kBatch) {
+      float batch[kBatch][4];
 #pragma unroll
-          for (uint32_t e = 0; e < 8; ++e) v[e] = k + e < depth ? from[e] : 0.0f;
+      for (int q = 0; q < kBatch; ++q) {
+        const uint32_t i = min(i0 + q * kWarps, rows * kbn - 1), m = i / kbn, k = (i - m * kbn) * 128 + at;      // the last one again where there is none
+        const TX* from = x + (int64_t)m * p.stride + k;
+        float (&v)[4] = batch[q];
+#pragma unroll
+        for (uint32_t j = 0; j < 2; ++j) {
+          const TX* pair = from + j * 4;
+          if (pairs && k + j * 4 + 1 < depth) {
+            if constexpr (sizeof(TX) == 4) {
+              const float2 w = *reinterpret_cast<const float2*>(pair);
+              v[2 * j] = w.x; v[2 * j + 1] = w.y;
+            } else {
+              const uint32_t w = *reinterpret_cast<const uint32_t*>(pair);
+              v[2 * j] = __uint_as_float(w << 16); v[2 * j + 1] = __uint_as_float(w & 0xffff0000u);
+            }
+          } else {
+            v[2 * j] = k + j * 4 < depth ? Elem<TX>::to_f32(pair[0]) : 0.0f;
+            v[2 * j + 1] = k + j * 4 + 1 < depth ? Elem<TX>::to_f32(pair[1]) : 0.0f;
+          }
         }
-        uint32_t t[3][4];
+      }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint16_t lo[3], hi[3];
-          three_terms(v[2 * e], lo[0], lo[1], lo[2]);
-          three_terms(v[2 * e + 1], hi[0], hi[1], hi[2]);
+      for (int q = 0; q < kBatch; ++q) {
+      const uint32_t i = min(i0 + q * kWarps, rows * kbn - 1), m = i / kbn, b = i - m * kbn;
+      float (&v)[4] = batch[q];
+      uint32_t size = 0;
 #pragma unroll
-          for (int j = 0; j < 3; ++j) t[j][e] = lo[j] | (uint32_t)hi[j] << 16;
-        }
+      for (int e = 0; e < 4; ++e) size = max(size, __float_as_uint(v[e]) & 0x7fffffffu);
+      const Whole<kParts> whole(__reduce_max_sync(0xffffffffu, size));
+      uint32_t d[4];
 #pragma unroll
-        for (int j = 0; j < 3; ++j) *reinterpret_cast<uint4*>(xs + (m * 3 + j) * pitch + k) = make_uint4(t[j][0], t[j][1], t[j][2], t[j][3]);
-      } else {
-        uint32_t t[4];
+      for (int e = 0; e < 4; ++e) d[e] = whole.digits(v[e]);
+      // the j-th digits of k = 0, 4, 1, 5 of the word or of 2, 6, 3, 7: as a byte's lower and upper nibbles have the codes
+      uint32_t part[4];
+      const uint32_t l02 = __byte_perm(d[0], d[2], 0x5140), l13 = __byte_perm(d[1], d[3], 0x5140), u02 = __byte_perm(d[0], d[2], 0x7362), u13 = __byte_perm(d[1], d[3], 0x7362);
+      part[0] = __byte_perm(l02, l13, 0x5410); part[1] = __byte_perm(l02, l13, 0x7632); part[2] = __byte_perm(u02, u13, 0x5410); part[3] = __byte_perm(u02, u13, 0x7632);
+      uint32_t two[2];      // sums of two digits each, of 16 bits with their signs
 #pragma unroll
-        for (uint32_t e = 0; e < 4; ++e) {
-          const uint16_t* h = reinterpret_cast<const uint16_t*>(from) + 2 * e;
-          t[e] = (k + 2 * e < depth ? h[0] : 0u) | (k + 2 * e + 1 < depth ? (uint32_t)h[1] << 16 : 0u);
-        }
-        *reinterpret_cast<uint4*>(xs + m * pitch + k) = make_uint4(t[0], t[1], t[2], t[3]);
+      for (int j = 0; j < 2; ++j) two[j] = (uint32_t)__dp4a((int)part[2 * j], 0x01010101, 0) + ((uint32_t)__dp4a((int)part[2 * j + 1], 0x01010101, 0) << 16);
+      constexpr int kLanes = 32 / PER_GROUP;
+#pragma unroll
+      for (int o = 1; o < kLanes; o <<= 1)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) two[j] += __shfl_xor_sync(0xffffffffu, two[j], o);
+#pragma unroll
+      for (int j = 0; j < kParts; ++j) {
+        const uint32_t column = m * kParts + kParts - 1 - j;
+        *reinterpret_cast<uint32_t*>(xs + column * pitch + b * 128 + (word % 4) * 32 + (word / 4) * 8 + (lane & 1) * 4) = part[j];
+        const int lower = (int)(int16_t)two[j / 2], sum = j % 2 ? (int)(two[j / 2] - (uint32_t)lower) >> 16 : lower;
+        if (lane % kLanes == 0) x_sums[(b * PER_GROUP + lane / kLanes) * (8 * MT) + column] = ZERO ? sum : kWhole - 8 * sum;
+        if (lane == 0) x_scales[b * (8 * MT) + column] = whole.scale * (float)(1u << 8 * j);
+      }
       }
     }
+  } else {      // bf16, eight values at a time
+    const bool whole = ((reinterpret_cast<uintptr_t>(x) | (uint64_t)p.stride * 2) & 15) == 0;
+    // rows over the warps, and where there are fewer of them a row over several
+    const uint32_t over = rows >= (uint32_t)kWarps ? 1 : rows > kWarps / 2 ? 1 : rows > kWarps / 4 ? 2 : rows > kWarps / 8 ? 4 : 8;
+    for (uint32_t m = warp / over; m < rows; m += kWarps / over) {
+      const uint16_t* row = reinterpret_cast<const uint16_t*>(x) + (int64_t)m * p.stride;
+      uint8_t* to = xs + m * pitch;
+#pragma unroll 4
+      for (uint32_t k = (warp % over * 32 + lane) * 8; k < kbn * 128; k += over * 256) {
+        if (whole && k + 8 <= depth) {
+          copy16(shared_address(to + k * 2), row + k);
+        } else {
+          uint32_t w[4];
+#pragma unroll
+          for (uint32_t e = 0; e < 4; ++e) w[e] = (k + 2 * e < depth ? row[k + 2 * e] : 0u) | (k + 2 * e + 1 < depth ? (uint32_t)row[k + 2 * e + 1] << 16 : 0u);
+          *reinterpret_cast<uint4*>(to + k * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
   __syncthreads();
 
   // a column of the instruction that is none of x's has another's values: nobody reads its sums
-  const uint16_t* mine[MT];
+  const uint8_t* mine[MT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) mine[i] = xs + min(i * 8 + g, columns - 1) * pitch + t * 8;
+  for (int i = 0; i < MT; ++i) mine[i] = xs + min(i * 8 + g, columns - 1) * pitch + t * (DIGITS ? 32 : 16);
   for (uint32_t tile0 = first; tile0 < last; tile0 += p.chunk) {
     const uint32_t count = min(p.chunk, last - tile0);
     float total[MT][4];
 #pragma unroll
     for (int i = 0; i < MT; ++i) total[i][0] = total[i][1] = total[i][2] = total[i][3] = 0.0f;
-    float* own = sums + warp * segments * sum_floats;
+    float* own = sums + warp * segments * sum_floats + t * 32 + g;
     auto multiply = [&](const Block<PER_GROUP, ZERO>& w, bool ends) {
       const uint32_t lo[4] = {w.lower.x, w.lower.y, w.lower.z, w.lower.w}, up[4] = {w.upper.x, w.upper.y, w.upper.z, w.upper.w};
       constexpr int kRun = 4 / PER_GROUP;                                   // 32-value runs of a group
-      constexpr int kChains = MT == 1 && PER_GROUP == 1 ? 2 : 1;            // sums under way at once where one would wait for itself
-      float sum[MT][kChains][4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int of = c / kRun, chain = c % kChains;
-        uint32_t bias_lo = 0x43084308u, bias_up = 0x43084308u;
-        if (ZERO) {
-          bias_lo = (0x4300u | w.zero[0][of]) * 0x10001u;
-          bias_up = (0x4300u | w.zero[1][of]) * 0x10001u;
-        }
-        if (c % kRun == 0)
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int h = 0; h < kChains; ++h) sum[i][h][0] = sum[i][h][1] = sum[i][h][2] = sum[i][h][3] = 0.0f;
-        const uint32_t a[8] = {pair_of<0>(lo[c], bias_lo), pair_of<0>(up[c], bias_up), pair_of<4>(lo[c], bias_lo), pair_of<4>(up[c], bias_up),
-                               pair_of<8>(lo[c], bias_lo), pair_of<8>(up[c], bias_up), pair_of<12>(lo[c], bias_lo), pair_of<12>(up[c], bias_up)};
+      if constexpr (DIGITS != 0) {
+        int sum[MT][4];
+        float of_block[MT][4];
+        uint4 x4[MT][2];
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-          const uint4 x4 = *reinterpret_cast<const uint4*>(mine[i] + kb * 128 + c * 32);
-          mma(sum[i][chain], a[0], a[1], a[2], a[3], x4.x, x4.y);
-          mma(sum[i][chain], a[4], a[5], a[6], a[7], x4.z, x4.w);
+          x4[i][0] = *reinterpret_cast<const uint4*>(mine[i] + kb * 128);
+          x4[i][1] = *reinterpret_cast<const uint4*>(mine[i] + kb * 128 + 16);
         }
-        if (c % kRun == kRun - 1) {
-          const float s_lo = __uint_as_float((uint32_t)w.scale[0][of] << 16), s_up = __uint_as_float((uint32_t)w.scale[1][of] << 16);
 #pragma unroll
-          for (int i = 0; i < MT; ++i)
+        for (int c = 0; c < 4; ++c) {
+          const int of = c / kRun;
+          if (c % kRun == 0)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) total[i][e] = fmaf(e < 2 ? s_lo : s_up, kChains == 2 ? sum[i][0][e] + sum[i][kChains - 1][e] : sum[i][0][e], total[i][e]);
+            for (int i = 0; i < MT; ++i) {      // what the zero points take off, in the sum from its start
+              const int2 s = *reinterpret_cast<const int2*>(x_sums + (kb * PER_GROUP + of) * (8 * MT) + i * 8 + t * 2);
+              sum[i][0] = ZERO ? kWhole - (int)w.zero[0][of] * s.x : s.x;
+              sum[i][1] = ZERO ? kWhole - (int)w.zero[0][of] * s.y : s.y;
+              sum[i][2] = ZERO ? kWhole - (int)w.zero[1][of] * s.x : s.x;
+              sum[i][3] = ZERO ? kWhole - (int)w.zero[1][of] * s.y : s.y;
+            }
+          const uint32_t a0 = lo[c] & 0x0f0f0f0fu, a1 = up[c] & 0x0f0f0f0fu, a2 = lo[c] >> 4 & 0x0f0f0f0fu, a3 = up[c] >> 4 & 0x0f0f0f0fu;
+#pragma unroll
+          for (int i = 0; i < MT; ++i) mma(sum[i], a0, a1, a2, a3, c % 2 ? x4[i][c / 2].z : x4[i][c / 2].x, c % 2 ? x4[i][c / 2].w : x4[i][c / 2].y);
+          if (c % kRun == kRun - 1) {
+            const float s_lo = __uint_as_float((uint32_t)w.scale[0][of] << 16), s_up = __uint_as_float((uint32_t)w.scale[1][of] << 16);
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {      // exact until it meets the scale
+                const float whole = __int_as_float(sum[i][e]) - kWholeValue, s = e < 2 ? s_lo : s_up;
+                of_block[i][e] = of == 0 ? s * whole : fmaf(s, whole, of_block[i][e]);
+              }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const float2 s = *reinterpret_cast<const float2*>(x_scales + kb * (8 * MT) + i * 8 + t * 2);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) total[i][e] = fmaf(e & 1 ? s.y : s.x, of_block[i][e], total[i][e]);
+        }
+      } else {
+        constexpr int kChains = MT == 1 && PER_GROUP == 1 ? 2 : 1;            // sums under way at once where one would wait for itself
+        float sum[MT][kChains][4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int of = c / kRun, chain = c % kChains;
+          uint32_t bias_lo = 0x43084308u, bias_up = 0x43084308u;
+          if (ZERO) {
+            bias_lo = (0x4300u | w.zero[0][of]) * 0x10001u;
+            bias_up = (0x4300u | w.zero[1][of]) * 0x10001u;
+          }
+          const uint32_t a[8] = {pair_of<0>(lo[c], bias_lo), pair_of<0>(up[c], bias_up), pair_of<4>(lo[c], bias_lo), pair_of<4>(up[c], bias_up),
+                                 pair_of<8>(lo[c], bias_lo), pair_of<8>(up[c], bias_up), pair_of<12>(lo[c], bias_lo), pair_of<12>(up[c], bias_up)};
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            const uint4 x4 = *reinterpret_cast<const uint4*>(mine[i] + kb * 256 + c * 64);
+            if (c % kRun < kChains) mma_from_zero(sum[i][chain], a[0], a[1], a[2], a[3], x4.x, x4.y);
+            else mma(sum[i][chain], a[0], a[1], a[2], a[3], x4.x, x4.y);
+            mma(sum[i][chain], a[4], a[5], a[6], a[7], x4.z, x4.w);
+          }
+          if (c % kRun == kRun - 1) {
+            const float s_lo = __uint_as_float((uint32_t)w.scale[0][of] << 16), s_up = __uint_as_float((uint32_t)w.scale[1][of] << 16);
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) total[i][e] = fmaf(e < 2 ? s_lo : s_up, kChains == 2 ? sum[i][0][e] + sum[i][kChains - 1][e] : sum[i][0][e], total[i][e]);
+          }
         }
       }
       if (++kb == kbn || ends) {      // a tile's end, or the run's
@@ -341,33 +447,40 @@ __global__ void __launch_bounds__(kThreads) int4_product_kernel(const Product p)
         for (int i = 0; i < MT; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const uint32_t column = i * 8 + t * 2 + (e & 1);
-            if (column < columns) own[column * 16 + g + (e & 2) * 4] = total[i][e];
+            if (i * 8 + (e & 1) + t * 2 < columns) own[i * 128 + (e & 1) * 16 + (e & 2) * 4] = total[i][e];
             total[i][e] = 0.0f;
           }
         own += sum_floats;
       }
     };
     for (uint32_t b = run; b > 0;) {
-      multiply(one, b == 1);
-      if (b > 2) load(one);
-      if (--b == 0) break;
-      multiply(two, b == 1);
-      if (b > 2) load(two);
-      --b;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (b > 0) {
+          multiply(ahead[i], b == 1);
+          if (b > (uint32_t)kAhead) load(ahead[i]);
+          --b;
+        }
     }
     __syncthreads();
-    // the sum of a tile's entry over the warps that have a part of it
-    auto over_warps = [&](uint32_t j, uint32_t at) {
-      float y = 0.0f;
+    // the sums of a tile's entries over the warps that have a part of it: ENTRIES of them, 16 apart
+    auto over_warps = [&](uint32_t j, uint32_t at, auto& y) {
+      constexpr int kEntries = sizeof(y) / sizeof(float);
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const uint32_t lo = starts[w], hi = starts[w + 1];
-        const bool has = lo < hi && lo < (j + 1) * kbn && hi > j * kbn;
-        const float s = sums[(w * segments + (has ? j - tiles_at[w] : 0)) * sum_floats + at];
-        y += has ? s : 0.0f;
+      for (int e = 0; e < kEntries; ++e) y[e] = 0.0f;
+      if (kbn) {
+        const uint32_t end = last_warp[j];
+#pragma unroll 2
+        for (uint32_t w = first_warp[j]; w <= end; ++w) {
+          const uint32_t tile = tiles_at[w];
+          const float* from = sums + (w * segments + (tile == kNoTile ? 0 : j - tile)) * sum_floats + at;
+#pragma unroll
+          for (int e = 0; e < kEntries; ++e) {
+            const float s = from[e * 16];
+            y[e] += tile == kNoTile ? 0.0f : s;
+          }
+        }
       }
-      return y;
     };
     auto write = [&](uint32_t j, uint32_t m, uint32_t n, float y) {
       const uint32_t col = (tile0 + j) * 16 + n;
@@ -380,23 +493,31 @@ __global__ void __launch_bounds__(kThreads) int4_product_kernel(const Product p)
     if (ctas == 1) {
       for (uint32_t i = tid; i < count * outputs; i += kThreads) {
         const uint32_t j = i / outputs, m = (i - j * outputs) / 16, n = i % 16;
-        float y = 0.0f;
+        float of[kParts], y = 0.0f;
+        over_warps(j, m * (kParts * 16) + n, of);
 #pragma unroll
-        for (int term = kTerms - 1; term >= 0; --term) y += over_warps(j, (m * kTerms + term) * 16 + n);      // the small ones first
+        for (int part = kParts - 1; part >= 0; --part) y += of[part];      // the small ones first
         write(j, m, n, y);
       }
     } else {
       for (uint32_t i = tid; i < count * sum_floats; i += kThreads) {
         const uint32_t j = i / sum_floats;
-        joined[i] = over_warps(j, i - j * sum_floats);
+        float of[1];
+        over_warps(j, i - j * sum_floats, of);
+        joined[i] = of[0];
       }
       cluster.sync();
       for (uint32_t i = rank * kThreads + tid; i < count * outputs; i += ctas * kThreads) {      // each rank finishes a part
         const uint32_t j = i / outputs, m = (i - j * outputs) / 16, n = i % 16;
         float y = 0.0f;
 #pragma unroll
-        for (int term = kTerms - 1; term >= 0; --term)
-          for (uint32_t r = 0; r < ctas; ++r) y += *cluster.map_shared_rank(joined + j * sum_floats + (m * kTerms + term) * 16 + n, r);
+        for (int term = kParts - 1; term >= 0; --term) {
+          float of[kMaxCluster];
+#pragma unroll
+          for (uint32_t r = 0; r < kMaxCluster; ++r) of[r] = r < ctas ? *cluster.map_shared_rank(joined + j * sum_floats + (m * kParts + term) * 16 + n, r) : 0.0f;
+#pragma unroll
+          for (uint32_t r = 0; r < kMaxCluster; ++r) y += of[r];
+        }
         write(j, m, n, y);
       }
     }
@@ -406,34 +527,44 @@ __global__ void __launch_bounds__(kThreads) int4_product_kernel(const Product p)
     if (next < last) {
       start_chunk(next, min(p.chunk, last - next));
       asked = kb;
-      if (run > 0) load(one);
-      if (run > 1) load(two);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (run > (uint32_t)i) load(ahead[i]);
     }
   }
 }
 
-template <int MT> size_t shared_bytes(uint32_t columns, uint32_t kblocks_of_cta, uint32_t chunk, uint32_t ctas) {
-  return (size_t)columns * 64 * (kWarps * segments_of(chunk) + (ctas > 1 ? chunk : 0)) + (size_t)columns * (kblocks_of_cta * 128 + kPad) * 2;
+template <int DIGITS, int MT, int PER_GROUP> size_t shared_bytes(uint32_t columns, uint32_t kblocks_of_cta, uint32_t chunk, uint32_t ctas) {
+  const size_t sums = (size_t)columns * 64 * (kWarps * segments_of(chunk) + (ctas > 1 ? chunk : 0));
+  return sums + (DIGITS ? (size_t)columns * (kblocks_of_cta * 128 + kPadDigits) + (size_t)kblocks_of_cta * 32 * MT * (1 + PER_GROUP) : (size_t)columns * (kblocks_of_cta * 128 + kPad) * 2);
 }
 
 constexpr size_t kMaxShared = 226 * 1024;      // of 227 KB, beside the kernel's own few bytes
 
-template <typename TX, int MT, int PER_GROUP, bool ZERO> int launch_product(Product p, cudaStream_t st) {
-  constexpr uint32_t kTerms = sizeof(TX) == 4 ? 3 : 1;
-  auto kernel = int4_product_kernel<TX, MT, PER_GROUP, ZERO>;
-  uint32_t ctas = 1, per_pass = p.rows < 8 * MT / kTerms ? p.rows : 8 * MT / kTerms, per_sm = 2, clusters = 1;
-  size_t bytes;
-  const uint32_t wanted = env_switch("PB_INT4_PERSM", 2), force = env_switch("PB_INT4_CTAS", 0);
-  while (true) {      // x in shared memory: split k over a cluster, and where that is not enough serve fewer rows with a pass
+template <typename TX, int DIGITS, int MT, int PER_GROUP, bool ZERO> int launch_product(Product p, cudaStream_t st) {
+  constexpr uint32_t kParts = DIGITS ? DIGITS : 1;
+  auto kernel = int4_product_kernel<TX, DIGITS, MT, PER_GROUP, ZERO>;
+  uint32_t ctas = 1, per_pass = std::min<uint32_t>(p.rows, 8 * MT / kParts), clusters, bytes;
+  const uint32_t sms = sm_count(), force = env_switch("PB_INT4_CTAS", 0), force_sm = env_switch("PB_INT4_PERSM", 0);
+  // x in shared memory: split k over a cluster, and where that is not enough serve fewer rows with a pass.  Few tiles of a long contraction are split, too
+  while (true) {
     const uint32_t per = (p.kblocks + ctas - 1) / ctas;
-    for (per_sm = wanted; per_sm > 0; --per_sm) {
-      clusters = std::max<uint32_t>(1, std::min<uint32_t>(p.tiles, sm_count() * per_sm / ctas));
+    uint32_t room = sms / ctas;      // clusters that are resident at once with a CTA an SM; 33 of four and 15 of eight CTAs on 148 SMs
+    if (ctas >= 4) room -= room / (ctas == 4 ? 9 : 6);
+    const uint64_t x_bytes = (uint64_t)per_pass * kParts * per * (DIGITS ? 128 : 256);
+    // two CTAs on an SM where one of them has more to read of the weight than of x
+    uint32_t per_sm = force_sm ? force_sm : (uint64_t)p.tiles * p.kblocks * 1024 / (2 * sms) >= 2 * x_bytes ? 2 : 1;
+    size_t need;
+    while (true) {
+      clusters = std::max<uint32_t>(1, std::min<uint32_t>(p.tiles, room * per_sm));
       p.chunk = std::min<uint32_t>(kMaxChunk, (p.tiles + clusters - 1) / clusters);
-      bytes = shared_bytes<MT>(per_pass * kTerms, per, p.chunk, ctas);
-      if (bytes <= kMaxShared && (per_sm == 1 || per_sm * (bytes + 1024) <= 228 * 1024)) break;
+      need = shared_bytes<DIGITS, MT, PER_GROUP>(per_pass * kParts, per, p.chunk, ctas);
+      if (per_sm == 1 || per_sm * (need + 1024) <= 228 * 1024) break;
+      --per_sm;
     }
-    const bool fits = per_sm > 0;
-    if (fits && (force ? ctas == force : ctas == kMaxCluster || (per_sm == wanted && (p.tiles * ctas >= (uint32_t)sm_count() || p.kblocks <= ctas * kWarps * 4)))) break;
+    bytes = (uint32_t)std::min<size_t>(need, kMaxShared + 1);
+    const bool few = p.tiles * ctas < 4 * sms && p.kblocks > ctas * kWarps * 2;
+    if (bytes <= kMaxShared && (force ? ctas == force : ctas == kMaxCluster || !few)) break;
     if (ctas < kMaxCluster) ctas *= 2;
     else if (per_pass > 1) { per_pass /= 2; ctas = 1; }
     else return fail(PB_ERR_UNSUPPORTED, "pb_int4_product: a contraction of %u does not fit", p.depth);
@@ -462,9 +593,10 @@ template <typename TX, int MT, int PER_GROUP, bool ZERO> int launch_product(Prod
   return PB_OK;
 }
 
-template <typename TX, int MT> int launch_of(const Product& p, int per_group, cudaStream_t st) {
-  if (p.zero) return per_group == 1 ? launch_product<TX, MT, 1, true>(p, st) : per_group == 2 ? launch_product<TX, MT, 2, true>(p, st) : launch_product<TX, MT, 4, true>(p, st);
-  return per_group == 1 ? launch_product<TX, MT, 1, false>(p, st) : per_group == 2 ? launch_product<TX, MT, 2, false>(p, st) : launch_product<TX, MT, 4, false>(p, st);
+template <typename TX, int DIGITS, int MT> int launch_of(const Product& p, int per_group, cudaStream_t st) {
+  if (p.zero)
+    return per_group == 1 ? launch_product<TX, DIGITS, MT, 1, true>(p, st) : per_group == 2 ? launch_product<TX, DIGITS, MT, 2, true>(p, st) : launch_product<TX, DIGITS, MT, 4, true>(p, st);
+  return per_group == 1 ? launch_product<TX, DIGITS, MT, 1, false>(p, st) : per_group == 2 ? launch_product<TX, DIGITS, MT, 2, false>(p, st) : launch_product<TX, DIGITS, MT, 4, false>(p, st);
 }
 
 int check_int4(const char* who, int64_t depth, int64_t cols, int group) {
@@ -533,7 +665,9 @@ extern "C" int pb_int4_product(const void* x, int x_dtype, int64_t rows, int64_t
   Product p{x, stride, q, static_cast<const __nv_bfloat16*>(scale), zero, out, (uint32_t)rows, (uint32_t)depth, (uint32_t)cols, (uint32_t)((depth + 127) / 128),
             (uint32_t)((cols + 15) / 16), 0, 0, 0, 0, 0, out_dtype == PB_F32};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int64_t columns = rows * (x_dtype == PB_F32 ? 3 : 1);
-  if (x_dtype == PB_F32) return columns <= 8 ? launch_of<float, 1>(p, 128 / group, st) : columns <= 16 ? launch_of<float, 2>(p, 128 / group, st) : launch_of<float, 4>(p, 128 / group, st);
-  return columns <= 8 ? launch_of<__nv_bfloat16, 1>(p, 128 / group, st) : columns <= 16 ? launch_of<__nv_bfloat16, 2>(p, 128 / group, st) : launch_of<__nv_bfloat16, 4>(p, 128 / group, st);
+  const int per_group = 128 / group;
+  if (x_dtype == PB_F32) return rows <= 2 ? launch_of<float, 4, 1>(p, per_group, st) : rows <= 4 ? launch_of<float, 4, 2>(p, per_group, st) : launch_of<float, 4, 4>(p, per_group, st);
+  if (rows <= env_switch("PB_INT4_DIGITS", 5))
+    return rows <= 2 ? launch_of<__nv_bfloat16, 3, 1>(p, per_group, st) : launch_of<__nv_bfloat16, 3, 2>(p, per_group, st);
+  return rows <= 8 ? launch_of<__nv_bfloat16, 0, 1>(p, per_group, st) : rows <= 16 ? launch_of<__nv_bfloat16, 0, 2>(p, per_group, st) : launch_of<__nv_bfloat16, 0, 4>(p, per_group, st);
 }
