@@ -151,7 +151,7 @@ __device__ __forceinline__ void mma_from_zero(float (&d)[4], uint32_t a0, uint32
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ void mma(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // A whole number below 2^22 in size as the low bits of an f32: kWhole + i, whose value less kWholeValue is i
@@ -188,6 +188,7 @@ struct Product {
   uint32_t rows_per_pass;                // rows of x that one pass over the weight serves (blockIdx.y)
   uint32_t chunk;                        // tiles between two barriers
   uint32_t per_cta;                      // blocks of k of a CTA of a cluster
+  FastDiv by_per_cta;
   uint32_t tiles_each, tiles_over;       // tiles of a cluster; the first tiles_over clusters have one more
   int out_f32;
 };
@@ -224,7 +225,7 @@ template <int PER_GROUP, bool ZERO> struct Block {
 // falls: a warp reads one run of memory, blocks ahead of the one that it computes, and leaves its sum of each tile (or part of one) in shared
 // memory.  They meet behind one barrier a chunk.
 template <typename TX, int DIGITS, int MT, int PER_GROUP, bool ZERO>
-__global__ void __launch_bounds__(kThreads, MT <= 2 ? 2 : 1) int4_product_kernel(const Product p) {
+__global__ void __launch_bounds__(kThreads, DIGITS == 0 && MT == 4 ? 1 : 2) int4_product_kernel(const Product p) {
   grid_wait();
   constexpr int kParts = DIGITS ? DIGITS : 1;      // columns of the instruction that a row of x takes, the first with its uppermost digits
   constexpr int kAhead = MT <= 2 ? 4 : 2;          // blocks that a warp has on the way or in hand
@@ -277,12 +278,13 @@ __global__ void __launch_bounds__(kThreads, MT <= 2 ? 2 : 1) int4_product_kernel
   if constexpr (DIGITS != 0) {      // a warp takes a row's block at a time, a lane four values of it: two pairs of the eight that a word of codes meets
     const uint32_t word = lane / 2, at = word * 8 + (lane & 1) * 2;
     const bool pairs = ((reinterpret_cast<uintptr_t>(x) | (uint64_t)p.stride * sizeof(TX)) & (2 * sizeof(TX) - 1)) == 0;
-    constexpr int kBatch = MT == 1 ? 2 : 4;      // row blocks on the way
-    for (uint32_t i0 = warp; i0 < rows * kbn; i0 += kWarps * kBatch) {
+    constexpr int kBatch = MT == 1 ? 2 : 4;      // row blocks on the way; the last one again where there is none
+    const uint32_t all = rows * p.per_cta;
+    for (uint32_t i0 = warp; i0 < all; i0 += kWarps * kBatch) {
       float batch[kBatch][4];
 #pragma unroll
       for (int q = 0; q < kBatch; ++q) {
-        const uint32_t i = min(i0 + q * kWarps, rows * kbn - 1), m = i / kbn, k = (i - m * kbn) * 128 + at;      // the last one again where there is none
+        const uint32_t i = min(i0 + q * kWarps, all - 1), m = p.by_per_cta.div(i), k = (i - m * p.per_cta) * 128 + at;
         const TX* from = x + (int64_t)m * p.stride + k;
         float (&v)[4] = batch[q];
 #pragma unroll
@@ -304,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, MT <= 2 ? 2 : 1) int4_product_kernel
       }
 #pragma unroll
       for (int q = 0; q < kBatch; ++q) {
-      const uint32_t i = min(i0 + q * kWarps, rows * kbn - 1), m = i / kbn, b = i - m * kbn;
+      const uint32_t i = min(i0 + q * kWarps, all - 1), m = p.by_per_cta.div(i), b = i - m * p.per_cta;
       float (&v)[4] = batch[q];
       uint32_t size = 0;
 #pragma unroll
@@ -317,21 +319,25 @@ __global__ void __launch_bounds__(kThreads, MT <= 2 ? 2 : 1) int4_product_kernel
       uint32_t part[4];
       const uint32_t l02 = __byte_perm(d[0], d[2], 0x5140), l13 = __byte_perm(d[1], d[3], 0x5140), u02 = __byte_perm(d[0], d[2], 0x7362), u13 = __byte_perm(d[1], d[3], 0x7362);
       part[0] = __byte_perm(l02, l13, 0x5410); part[1] = __byte_perm(l02, l13, 0x7632); part[2] = __byte_perm(u02, u13, 0x5410); part[3] = __byte_perm(u02, u13, 0x7632);
-      uint32_t two[2];      // sums of two digits each, of 16 bits with their signs
-#pragma unroll
-      for (int j = 0; j < 2; ++j) two[j] = (uint32_t)__dp4a((int)part[2 * j], 0x01010101, 0) + ((uint32_t)__dp4a((int)part[2 * j + 1], 0x01010101, 0) << 16);
       constexpr int kLanes = 32 / PER_GROUP;
+      uint32_t two[2] = {0, 0};      // a group's sums of two digits each, of 16 bits with their signs
+      if constexpr (ZERO) {
 #pragma unroll
-      for (int o = 1; o < kLanes; o <<= 1)
+        for (int j = 0; j < 2; ++j) two[j] = (uint32_t)__dp4a((int)part[2 * j], 0x01010101, 0) + ((uint32_t)__dp4a((int)part[2 * j + 1], 0x01010101, 0) << 16);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) two[j] += __shfl_xor_sync(0xffffffffu, two[j], o);
+        for (int o = 1; o < kLanes; o <<= 1)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) two[j] += __shfl_xor_sync(0xffffffffu, two[j], o);
+      }
 #pragma unroll
       for (int j = 0; j < kParts; ++j) {
         const uint32_t column = m * kParts + kParts - 1 - j;
         *reinterpret_cast<uint32_t*>(xs + column * pitch + b * 128 + (word % 4) * 32 + (word / 4) * 8 + (lane & 1) * 4) = part[j];
-        const int lower = (int)(int16_t)two[j / 2], sum = j % 2 ? (int)(two[j / 2] - (uint32_t)lower) >> 16 : lower;
-        if (lane % kLanes == 0) x_sums[(b * PER_GROUP + lane / kLanes) * (8 * MT) + column] = ZERO ? sum : kWhole - 8 * sum;
-        if (lane == 0) x_scales[b * (8 * MT) + column] = whole.scale * (float)(1u << 8 * j);
+        if constexpr (ZERO) {
+          const int lower = (int)(int16_t)two[j / 2], sum = j % 2 ? (int)(two[j / 2] - (uint32_t)lower) >> 16 : lower;
+          if (lane % kLanes == 0) x_sums[(b * PER_GROUP + lane / kLanes) * (8 * MT) + column] = 16 * sum;
+        }
+        if (lane == 0) x_scales[b * (8 * MT) + column] = whole.scale * ((float)(1u << 8 * j) * 0.0625f);      // the codes are sixteen times theirs
       }
       }
     }
@@ -385,14 +391,17 @@ __global__ void __launch_bounds__(kThreads, MT <= 2 ? 2 : 1) int4_product_kernel
           const int of = c / kRun;
           if (c % kRun == 0)
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {      // what the zero points take off, in the sum from its start
-              const int2 s = *reinterpret_cast<const int2*>(x_sums + (kb * PER_GROUP + of) * (8 * MT) + i * 8 + t * 2);
-              sum[i][0] = ZERO ? kWhole - (int)w.zero[0][of] * s.x : s.x;
-              sum[i][1] = ZERO ? kWhole - (int)w.zero[0][of] * s.y : s.y;
-              sum[i][2] = ZERO ? kWhole - (int)w.zero[1][of] * s.x : s.x;
-              sum[i][3] = ZERO ? kWhole - (int)w.zero[1][of] * s.y : s.y;
+            for (int i = 0; i < MT; ++i) {
+              sum[i][0] = sum[i][1] = sum[i][2] = sum[i][3] = kWhole;
+              if (ZERO) {      // what the zero points take off beside the eight that the codes are less, in the sum from its start
+                const int2 s = *reinterpret_cast<const int2*>(x_sums + (kb * PER_GROUP + of) * (8 * MT) + i * 8 + t * 2);
+                const int z_lo = 8 - (int)w.zero[0][of], z_up = 8 - (int)w.zero[1][of];
+                sum[i][0] += z_lo * s.x; sum[i][1] += z_lo * s.y; sum[i][2] += z_up * s.x; sum[i][3] += z_up * s.y;
+              }
             }
-          const uint32_t a0 = lo[c] & 0x0f0f0f0fu, a1 = up[c] & 0x0f0f0f0fu, a2 = lo[c] >> 4 & 0x0f0f0f0fu, a3 = up[c] >> 4 & 0x0f0f0f0fu;
+          // codes u as bytes of 16 (u - 8): a nibble in the upper half of its byte with its highest bit turned
+          const uint32_t a0 = (lo[c] << 4 & 0xf0f0f0f0u) ^ 0x80808080u, a1 = (up[c] << 4 & 0xf0f0f0f0u) ^ 0x80808080u;
+          const uint32_t a2 = (lo[c] & 0xf0f0f0f0u) ^ 0x80808080u, a3 = (up[c] & 0xf0f0f0f0u) ^ 0x80808080u;
 #pragma unroll
           for (int i = 0; i < MT; ++i) mma(sum[i], a0, a1, a2, a3, c % 2 ? x4[i][c / 2].z : x4[i][c / 2].x, c % 2 ? x4[i][c / 2].w : x4[i][c / 2].y);
           if (c % kRun == kRun - 1) {
@@ -564,13 +573,15 @@ template <typename TX, int DIGITS, int MT, int PER_GROUP, bool ZERO> int launch_
     }
     bytes = (uint32_t)std::min<size_t>(need, kMaxShared + 1);
     const bool few = p.tiles * ctas < 4 * sms && p.kblocks > ctas * kWarps * 2;
-    if (bytes <= kMaxShared && (force ? ctas == force : ctas == kMaxCluster || !few)) break;
+    const bool heavy = DIGITS && per_pass >= 4 && per_pass > MT * ((p.tiles + clusters - 1) / clusters);      // more digits to make than products
+    if (bytes <= kMaxShared && (force ? ctas == force : ctas == kMaxCluster || !(few || heavy))) break;
     if (ctas < kMaxCluster) ctas *= 2;
     else if (per_pass > 1) { per_pass /= 2; ctas = 1; }
     else return fail(PB_ERR_UNSUPPORTED, "pb_int4_product: a contraction of %u does not fit", p.depth);
   }
   p.rows_per_pass = per_pass;
   p.per_cta = (p.kblocks + ctas - 1) / ctas;
+  p.by_per_cta = FastDiv(p.per_cta);
   p.tiles_each = p.tiles / clusters;
   p.tiles_over = p.tiles % clusters;
   PB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxShared));
@@ -663,11 +674,12 @@ extern "C" int pb_int4_product(const void* x, int x_dtype, int64_t rows, int64_t
       (reinterpret_cast<uintptr_t>(x) % (x_dtype == PB_F32 ? 4 : 2)) || (reinterpret_cast<uintptr_t>(out) % (out_dtype == PB_F32 ? 4 : 2)))
     return fail(PB_ERR_MISALIGNED, "pb_int4_product: q 16, scale and zero 4 bytes, x and out their types");
   Product p{x, stride, q, static_cast<const __nv_bfloat16*>(scale), zero, out, (uint32_t)rows, (uint32_t)depth, (uint32_t)cols, (uint32_t)((depth + 127) / 128),
-            (uint32_t)((cols + 15) / 16), 0, 0, 0, 0, 0, out_dtype == PB_F32};
+            (uint32_t)((cols + 15) / 16), 0, 0, 0, FastDiv(), 0, 0, out_dtype == PB_F32};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int per_group = 128 / group;
   if (x_dtype == PB_F32) return rows <= 2 ? launch_of<float, 4, 1>(p, per_group, st) : rows <= 4 ? launch_of<float, 4, 2>(p, per_group, st) : launch_of<float, 4, 4>(p, per_group, st);
-  if (rows <= env_switch("PB_INT4_DIGITS", 5))
-    return rows <= 2 ? launch_of<__nv_bfloat16, 3, 1>(p, per_group, st) : launch_of<__nv_bfloat16, 3, 2>(p, per_group, st);
+  // A bf16 x as it is or in digits, us, 2048 values deep: 2048 columns 2.97 | 3.22 (one row) and 3.06 | 3.98 (two), 8192 columns 4.80 | 4.38 and 5.43 | 5.26 (with zero
+  // points, 8192 deep and 2048 columns, 5.70 | 6.44), 65536 columns 18.8 | 15.6 and 19.4 | 17.0, four rows 20.1 | 21.7: making digits is made good by many columns
+  if (rows <= 2 && (int64_t)p.tiles * p.kblocks >= 16384) return launch_of<__nv_bfloat16, 3, 1>(p, per_group, st);
   return rows <= 8 ? launch_of<__nv_bfloat16, 0, 1>(p, per_group, st) : rows <= 16 ? launch_of<__nv_bfloat16, 0, 2>(p, per_group, st) : launch_of<__nv_bfloat16, 0, 4>(p, per_group, st);
 }
