@@ -14,13 +14,16 @@
 
 #include <cooperative_groups.h>
 
+#ifndef LPMIN
+#define LPMIN 1024
+#endif
 namespace pb {
 namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kLoads = 4;                  // 16-byte loads that a thread has in flight
+constexpr int kBackThreads = 256;
 constexpr int kMaxTop = 128, kMaxTokens = 128;
 constexpr int kCandidates = 1024;          // keys of a row that are ranked against one another
 constexpr int kMaxCluster = 8;             // CTAs that share a row; kMaxCluster * kMaxTop <= kCandidates
@@ -39,34 +42,36 @@ __device__ __forceinline__ float max_nan(float a, float b) {      // unlike fmax
 }
 constexpr float kFar = -1e30f;             // a difference below it weighs nothing, and times a weight of zero it is zero where -inf is NaN
 
-// 16 bytes of logits as numbers
+// 16 bytes of logits as numbers, two at a time, and their largest
 template <typename T> struct Vec;
 template <> struct Vec<float> {
   static constexpr int kSize = 4;
-  static __device__ __forceinline__ void unpack(const uint4& r, float (&v)[4]) {
-    v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
+  static __device__ __forceinline__ void unpack(const uint4& r, float2 (&v)[2]) {
+    v[0] = make_float2(__uint_as_float(r.x), __uint_as_float(r.y)); v[1] = make_float2(__uint_as_float(r.z), __uint_as_float(r.w));
   }
-  static __device__ __forceinline__ uint4 pack(const float (&v)[4]) {
-    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  static __device__ __forceinline__ uint4 pack(const float2 (&v)[2]) {
+    return make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
+  }
+  static __device__ __forceinline__ float top(const uint4& r) {
+    return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
   }
 };
 template <> struct Vec<__nv_bfloat16> {
   static constexpr int kSize = 8;
-  static __device__ __forceinline__ void unpack(const uint4& r, float (&v)[8]) {
+  static __device__ __forceinline__ void unpack(const uint4& r, float2 (&v)[4]) {
     const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    for (int i = 0; i < 4; ++i) v[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
   }
-  static __device__ __forceinline__ uint4 pack(const float (&v)[8]) {
-    return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+  static __device__ __forceinline__ uint4 pack(const float2 (&v)[4]) {
+    return make_uint4(pack_bf16x2(v[0].x, v[0].y), pack_bf16x2(v[1].x, v[1].y), pack_bf16x2(v[2].x, v[2].y), pack_bf16x2(v[3].x, v[3].y));
+  }
+  static __device__ __forceinline__ float top(const uint4& r) {
+    auto both = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
+    const __nv_bfloat162 m = __hmax2(__hmax2(both(r.x), both(r.y)), __hmax2(both(r.z), both(r.w)));      // of a number and a NaN the number
+    return fmaxf(__low2float(m), __high2float(m));
   }
 };
-template <int N> __device__ __forceinline__ float top_of(const float (&v)[N]) {
-  float t = v[0];
-#pragma unroll
-  for (int i = 1; i < N; ++i) t = fmaxf(t, v[i]);
-  return t;
-}
 
 // A maximum, the sum of exp(z - maximum) and the sum of exp(z - maximum) (z - maximum).  While the maximum is -inf (nothing but -inf seen) the
 // differences are taken from 0, so that -inf - -inf does not make a NaN of a logit that only weighs nothing.
@@ -86,20 +91,19 @@ struct Terms : Sums {
     s += e;
     w += e * d;
   }
-  __device__ __forceinline__ void join(const Terms& o) {      // o's maximum and this one's may be -inf: sums of zero then
-    const float top = fmaxf(m, o.m), from = top == -INFINITY ? 0.0f : top;
-    const float a = max_nan(m - from, kFar), b = max_nan(o.m - from, kFar);
-    const float ca = exp2_fast(a * kLog2e), cb = exp2_fast(b * kLog2e);
-    w = ca * (w + s * a) + cb * (o.w + o.s * b);
-    s = ca * s + cb * o.s;
-    m = top;
-  }
+  // the terms of LANES lanes of a warp together, in each of them
   template <int LANES> __device__ __forceinline__ void over_lanes() {
+    float top = m;
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float by = max_nan(m - (top == -INFINITY ? 0.0f : top), kFar), c = exp2_fast(by * kLog2e);      // m = -inf: sums of zero
+    w = c * (w + s * by);
+    s *= c;
+    m = top;
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) {
-      Terms t;
-      t.m = __shfl_xor_sync(0xffffffffu, m, o); t.s = __shfl_xor_sync(0xffffffffu, s, o); t.w = __shfl_xor_sync(0xffffffffu, w, o);
-      join(t);
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      w += __shfl_xor_sync(0xffffffffu, w, o);
     }
   }
 };
@@ -113,9 +117,13 @@ __device__ __forceinline__ uint32_t order_of(float z) {
 __device__ __forceinline__ float value_of(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o); }
 __device__ __forceinline__ uint64_t key_of(float z, uint32_t index) { return (uint64_t)order_of(z) << 32 | (uint32_t)~index; }
 
-struct Rows {
-  int64_t inner, stride_outer, stride_inner;      // row r at (r / inner) * stride_outer + (r % inner) * stride_inner
-  __device__ __forceinline__ int64_t at(int64_t r) const { return (r / inner) * stride_outer + (r % inner) * stride_inner; }
+struct Rows {      // row r at (r / inner) * stride_outer + (r % inner) * stride_inner
+  FastDiv by_inner;
+  int64_t stride_outer, stride_inner;
+  __device__ __forceinline__ int64_t at(uint32_t r) const {
+    const uint32_t o = by_inner.div(r);
+    return o * stride_outer + (r - o * by_inner.d) * stride_inner;
+  }
 };
 
 // A row as elements up to the first 16-byte boundary, whole 16-byte vectors and the rest; CTA `rank` of `ctas` has every vector of its slice, the
@@ -126,7 +134,7 @@ template <typename T> struct Slice {
   uint32_t head, tail, tail_at, first, count;      // count vectors from vector `first` on
   __device__ __forceinline__ Slice(const T* row, uint32_t vocab, uint32_t rank, uint32_t ctas) : z(row) {
     head = min((uint32_t)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (uint32_t)sizeof(T), vocab);
-    const uint32_t vecs = (vocab - head) / kVec, per = (vecs + ctas - 1) / ctas;
+    const uint32_t vecs = (vocab - head) / kVec, per = ctas == 1 ? vecs : (vecs + ctas - 1) / ctas;
     tail_at = head + vecs * kVec;
     tail = vocab - tail_at;
     first = min(rank * per, vecs);
@@ -139,96 +147,123 @@ template <typename T> struct Slice {
   __device__ __forceinline__ uint32_t elements() const { return head + tail + count * kVec; }
 };
 
-struct Shared {
+template <int THREADS> struct Shared {
   uint64_t cand[kCandidates];
-  uint64_t lists[kThreads];             // the threads' best keys, 32 of a warp in order
+  uint64_t groups[THREADS];             // the best keys of groups of threads
   uint64_t sorted[kMaxTop];
-  Sums terms[kWarps], cta;
-  uint64_t threshold;
+  uint64_t bound;
+  Sums terms[THREADS / 32], cta;
   uint32_t n_cand, n_hot;
-  uint16_t hot[kThreads];
+  uint16_t hot[THREADS];
 };
 
-// The keys in[0, n) that are among the k largest, in order
-__device__ __forceinline__ void rank_keys(const uint64_t* in, uint32_t n, uint32_t k, uint64_t* out) {
-  for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+// How many of the keys in[0, n) are above `key`; `in` lies at 16 bytes
+__device__ __forceinline__ uint32_t keys_above(const uint64_t* in, uint32_t n, uint64_t key) {
+  uint32_t above = 0;
+#pragma unroll 4
+  for (uint32_t j = 0; j + 1 < n; j += 2) {
+    const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(in + j);
+    above += (two.x > key) + (two.y > key);
+  }
+  if (n & 1) above += in[n - 1] > key;
+  return above;
+}
+// Those of the keys in[0, n) that are among the k largest, in order; no two are equal
+template <int THREADS> __device__ __forceinline__ void rank_keys(const uint64_t* in, uint32_t n, uint32_t k, uint64_t* out) {
+  for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
     const uint64_t key = in[i];
-    uint32_t above = 0;
-    for (uint32_t j = 0; j < n; ++j) above += in[j] > key;
+    const uint32_t above = keys_above(in, n, key);
     if (above < k) out[above] = key;
   }
 }
 
-// sorted[0, k) of the slice's k best logits.  Every thread brings the best of its own: `mine` is that logit's value with the last index of the vector
-// that it first came in.  Of these keys, the k-th largest is a bound that at least k logits of the slice reach, and they all belong to
-// the k threads whose keys reach it: vectors do not overlap, so another thread's logit of the same value lies behind.  Those threads' logits
-// (k / 256 of the slice) are read again, from L2, and the ones that reach the bound are ranked.
-template <typename T>
-__device__ void best_of_slice(Shared& sh, const Slice<T>& sl, uint64_t mine, uint32_t k) {
+// What a thread knows of its logits: the largest, the last index of the vector that it first came in (its own index before and behind the vectors), and the largest
+// of its other vectors' largest.
+struct Best {
+  float top = -INFINITY, second = -INFINITY;
+  uint32_t at;
+  __device__ __forceinline__ void meet(float t, uint32_t index) {
+    second = fmaxf(second, fminf(top, t));
+    if (t > top) { top = t; at = index; }
+  }
+};
+
+// sorted[0, k) of the slice's k best logits; sh.bound = 1 and sh.n_cand = sh.n_hot = 0 behind a barrier.  Every thread brings the best of its own as a key, `mine`,
+// 0 where it has none.  The k-th largest of the keys of groups of threads, of twice k groups or more, is a bound that at least k and as a rule not
+// half as many more of the threads' keys reach.  So at least k logits of the slice reach it, and they all belong to those threads: vectors do
+// not overlap, so another thread's logit of the same value lies behind.  Such a thread looks at its best vector again, which is in `raw` or else is read
+// again; where its second one reaches the bound, too, the CTA reads all of that thread's.  The logits that reach the bound are ranked.
+template <typename T, int THREADS>
+__device__ void best_of_slice(Shared<THREADS>& sh, const Slice<T>& sl, const Best& best, uint64_t mine, const uint4 (&raw)[kLoads], uint32_t k) {
   constexpr int kVec = Vec<T>::kSize;
-  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // 32 keys of a warp in falling order
+  const uint32_t tid = threadIdx.x;
+  const uint32_t groups = k <= 4 ? 8 : k <= 16 ? 32 : k <= 64 ? 128 : THREADS, lanes = THREADS / groups;
   uint64_t key = mine;
-#pragma unroll
-  for (uint32_t size = 2; size <= 32; size <<= 1)
-#pragma unroll
-    for (uint32_t step = size >> 1; step > 0; step >>= 1) {
-      const uint64_t other = __shfl_xor_sync(0xffffffffu, key, step);
-      const bool larger = ((lane & step) == 0) == ((lane & size) == 0);      // of the two, whether this lane takes the larger
-      key = (key > other) == larger ? key : other;
-    }
-  sh.lists[tid] = key;
-  if (tid == 0) { sh.threshold = 1; sh.n_hot = 0; }
+  for (uint32_t o = 1; o < min(lanes, 32u); o <<= 1) {
+    const uint64_t other = __shfl_xor_sync(0xffffffffu, key, o);
+    key = other > key ? other : key;
+  }
+  const uint32_t held = max(groups, (uint32_t)THREADS / 32);      // a group is a warp at most
+  if (tid % (THREADS / held) == 0) sh.groups[tid / (THREADS / held)] = key;
   __syncthreads();
-  if (key != 0) {      // no two of the others are equal
-    uint32_t above = lane;
-    for (uint32_t l = 1; l < kWarps; ++l) {
-      const uint64_t* list = sh.lists + ((warp + l) % kWarps) * 32;
-      uint32_t at = 0;
-#pragma unroll
-      for (uint32_t step = 16; step > 0; step >>= 1)
-        if (list[at + step - 1] > key) at += step;
-      above += at + (list[at] > key);
-    }
-    if (above == k - 1) sh.threshold = key;
+  if (tid < held) {
+    const uint64_t own = sh.groups[tid];
+    if (own != 0 && keys_above(sh.groups, held, own) == k - 1) sh.bound = own;      // no two of the others are equal
   }
   __syncthreads();
-  const uint32_t rounds = (sl.count + kThreads - 1) / kThreads;
+  const uint32_t rounds = (sl.count + THREADS - 1) / THREADS, at0 = sl.at0();
   while (true) {      // once, but for rows whose best logits crowd into a few threads: the bound rises until what reaches it has room
-    const uint64_t bound = sh.threshold;
-    if (tid == 0) sh.n_cand = 0;
-    __syncthreads();
+    const uint64_t bound = sh.bound;
+    const float bound_z = value_of((uint32_t)(bound >> 32));
     auto offer = [&](float z, uint32_t index) {
+      if (z < bound_z) return;      // a NaN is not: it ranks with -inf
       const uint64_t c = key_of(z, index);
       if (c >= bound) {
         const uint32_t at = atomicAdd(&sh.n_cand, 1u);
         if (at < kCandidates) sh.cand[at] = c;
       }
     };
+    auto offer_all = [&](const uint4& r, uint32_t at) {
+      float2 v[kVec / 2];
+      Vec<T>::unpack(r, v);
+#pragma unroll
+      for (int e = 0; e < kVec / 2; ++e) { offer(v[e].x, at + 2 * e); offer(v[e].y, at + 2 * e + 1); }
+    };
     if (mine >= bound) {
-      sh.hot[atomicAdd(&sh.n_hot, 1u)] = (uint16_t)tid;
       if (tid < sl.head) offer(Elem<T>::to_f32(sl.z[tid]), tid);
       if (tid < sl.tail) offer(Elem<T>::to_f32(sl.z[sl.tail_at + tid]), sl.tail_at + tid);
-    }
-    __syncthreads();
-    const uint32_t items = sh.n_hot * rounds;
-    const uint32_t at0 = sl.at0();
-    for (uint32_t i = tid; i < items; i += kThreads) {
-      const uint32_t h = i / rounds, vec = (i - h * rounds) * kThreads + sh.hot[h];
-      if (vec < sl.count) {
-        const uint32_t at = at0 + vec * kVec;
-        float v[kVec];
-        Vec<T>::unpack(*reinterpret_cast<const uint4*>(sl.z + at), v);
+      const bool several = !(best.second < bound_z);
+      if (rounds <= kLoads) {
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) offer(v[e], at + e);
+        for (int l = 0; l < kLoads; ++l) {
+          const uint32_t at = at0 + (tid + l * THREADS) * kVec;
+          if (tid + l * THREADS < sl.count && (several || best.at == at + kVec - 1)) offer_all(raw[l], at);
+        }
+      } else if (several) {
+        sh.hot[atomicAdd(&sh.n_hot, 1u)] = (uint16_t)tid;
+      } else if (best.at >= at0 && best.at < sl.tail_at) {
+        const uint32_t at = best.at - (kVec - 1);
+        offer_all(*reinterpret_cast<const uint4*>(sl.z + at), at);
       }
     }
     __syncthreads();
+    if (sh.n_hot != 0) {
+      const uint32_t items = sh.n_hot * rounds;
+      for (uint32_t i = tid; i < items; i += THREADS) {
+        const uint32_t h = i / rounds, vec = (i - h * rounds) * THREADS + sh.hot[h];
+        if (vec < sl.count) {
+          const uint32_t at = at0 + vec * kVec;
+          const uint4 r = *reinterpret_cast<const uint4*>(sl.z + at);
+          if (!(Vec<T>::top(r) < bound_z)) offer_all(r, at);      // of nothing but NaN the top is one
+        }
+      }
+      __syncthreads();
+    }
     const uint32_t n = sh.n_cand, kept = min(n, (uint32_t)kCandidates);
-    rank_keys(sh.cand, kept, k, sh.sorted);
+    rank_keys<THREADS>(sh.cand, kept, k, sh.sorted);
     __syncthreads();
     if (n <= kCandidates) break;
-    if (tid == 0) { sh.threshold = sh.sorted[k - 1]; sh.n_hot = 0; }
+    if (tid == 0) { sh.bound = sh.sorted[k - 1]; sh.n_cand = 0; sh.n_hot = 0; }
     __syncthreads();
   }
 }
@@ -244,108 +279,128 @@ struct Forward {
 };
 
 // One row per cluster of CTAs (of one CTA where there are rows enough to fill the chip); its CTAs' terms and best logits meet in the first one.
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Forward p) {
+template <typename T, int THREADS, bool TOP>
+__global__ void __launch_bounds__(THREADS, LPMIN / THREADS) token_logprobs_kernel(const Forward p) {
   grid_wait();
-  __shared__ Shared sh;
-  constexpr int kVec = Vec<T>::kSize;
+  __shared__ __align__(16) Shared<THREADS> sh;
+  constexpr int kVec = Vec<T>::kSize, kWarps = THREADS / 32;
   cg::cluster_group cluster = cg::this_cluster();
   const uint32_t ctas = cluster.num_blocks(), rank = cluster.block_rank(), tid = threadIdx.x;
-  const int64_t row = blockIdx.x / ctas;
+  const uint32_t row = ctas == 1 ? blockIdx.x : blockIdx.x / ctas;
   const T* z = static_cast<const T*>(p.logits) + p.rows.at(row);
   const Slice<T> sl(z, p.vocab, rank, ctas);
-  const uint4* vecs = reinterpret_cast<const uint4*>(z + sl.at0());
+  const uint32_t at0 = sl.at0();
+  const uint4* vecs = reinterpret_cast<const uint4*>(z + at0);
 
   // a given token's logit, asked for ahead of the row
   int64_t token = -1;
   float token_z = 0.0f;
   if (rank == 0 && tid < p.n_tokens) {
-    token = p.tokens[row * p.n_tokens + tid];
+    token = p.tokens[(int64_t)row * p.n_tokens + tid];
     if (token >= 0) token_z = token < p.vocab ? Elem<T>::to_f32(z[token]) : NAN;
   }
 
   Terms t;
-  const uint32_t at0 = sl.at0();
-  // where the thread's best logit is: the last index of its vector
-  uint32_t best = tid < sl.head ? tid : tid < sl.count ? at0 + tid * kVec + kVec - 1 : sl.tail_at + tid;
+  Best best;
+  best.at = tid < sl.head ? tid : tid < sl.count ? at0 + tid * kVec + kVec - 1 : sl.tail_at + tid;      // of its first logit, while there are none but -inf
   const bool any = tid < sl.head || tid < sl.count || tid < sl.tail;
+  bool masked = false;      // this thread has met a logit that is no number
   if (tid < sl.head) {
     const float v = Elem<T>::to_f32(sl.z[tid]);
     if (v > t.m) t.m = v;
+    best.meet(v, tid);
     t.add(v, t.base());
   }
-  uint32_t j = tid;
-  for (; j + (kLoads - 1) * kThreads < sl.count; j += kLoads * kThreads) {
-    uint4 raw[kLoads];
+  // Four vectors at a time; each is asked for while the ones before it are added up.
+  uint4 raw[kLoads];
 #pragma unroll
-    for (int l = 0; l < kLoads; ++l) raw[l] = __ldg(vecs + j + l * kThreads);
+  for (int l = 0; l < kLoads; ++l)
+    if (tid + l * THREADS < sl.count) raw[l] = __ldg(vecs + tid + l * THREADS);
+  for (uint32_t j0 = 0; j0 < sl.count; j0 += kLoads * THREADS) {
+    const uint32_t j = j0 + tid;
+    const bool full = j0 + kLoads * THREADS <= sl.count;
     float tops[kLoads];
 #pragma unroll
     for (int l = 0; l < kLoads; ++l) {
-      float v[kVec];
-      Vec<T>::unpack(raw[l], v);
-      tops[l] = top_of(v);
+      tops[l] = full || j + l * THREADS < sl.count ? Vec<T>::top(raw[l]) : -INFINITY;
+      if constexpr (TOP) best.meet(tops[l], at0 + (j + l * THREADS) * kVec + kVec - 1);
     }
-    const float top = top_of(tops);
-    if (top > t.m) {
-      t.raise(top);
-      if constexpr (TOP) {
-        uint32_t l = kLoads - 1;
+    static_assert(kLoads == 4, "the largest of four");
+    const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    if (top > t.m) t.raise(top);
+    const float from = t.base();
+    float2 v[kVec / 2];
+    if (full && !masked) {
+      const float2 minus = make_float2(-from, -from), scale = make_float2(kLog2e, kLog2e);
+      float2 sum = make_float2(t.s, 0.0f), weighted = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int i = kLoads - 2; i >= 0; --i) l = tops[i] == top ? i : l;
-        best = at0 + (j + l * kThreads) * kVec + kVec - 1;
+      for (int l = 0; l < kLoads; ++l) {
+        Vec<T>::unpack(raw[l], v);
+        const uint32_t next = j + (kLoads + l) * THREADS;
+        if (next < sl.count) raw[l] = __ldg(vecs + next);
+#pragma unroll
+        for (int i = 0; i < kVec / 2; ++i) {
+          const float2 d = __fadd2_rn(v[i], minus), a = __fmul2_rn(d, scale), e = make_float2(exp2_fast(a.x), exp2_fast(a.y));
+          sum = __fadd2_rn(sum, e);
+          weighted = __ffma2_rn(e, d, weighted);
+        }
+      }
+      t.s = sum.x + sum.y;
+      float w = weighted.x + weighted.y;
+      if (w != w) {      // 0 * -inf: from here on with differences that are kept finite, and for these logits once more
+        masked = true;
+        Terms again;
+#pragma unroll 1
+        for (int l = 0; l < kLoads; ++l) {
+          Vec<T>::unpack(__ldg(vecs + j + l * THREADS), v);
+#pragma unroll
+          for (int i = 0; i < kVec / 2; ++i) { again.add(v[i].x, from); again.add(v[i].y, from); }
+        }
+        w = again.w;
+      }
+      t.w += w;
+    } else {
+#pragma unroll
+      for (int l = 0; l < kLoads; ++l) {
+        const bool has = full || j + l * THREADS < sl.count;
+        if (has) Vec<T>::unpack(raw[l], v);
+        const uint32_t next = j + (kLoads + l) * THREADS;
+        if (next < sl.count) raw[l] = __ldg(vecs + next);
+        if (has)
+#pragma unroll
+          for (int i = 0; i < kVec / 2; ++i) { t.add(v[i].x, from); t.add(v[i].y, from); }
       }
     }
-    const float from = t.base();
-#pragma unroll
-    for (int l = 0; l < kLoads; ++l) {
-      float v[kVec];
-      Vec<T>::unpack(raw[l], v);
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) t.add(v[e], from);
-    }
-  }
-  for (; j < sl.count; j += kThreads) {
-    float v[kVec];
-    Vec<T>::unpack(__ldg(vecs + j), v);
-    const float top = top_of(v);
-    if (top > t.m) {
-      t.raise(top);
-      best = at0 + j * kVec + kVec - 1;
-    }
-    const float from = t.base();
-#pragma unroll
-    for (int e = 0; e < kVec; ++e) t.add(v[e], from);
   }
   if (tid < sl.tail) {
     const float v = Elem<T>::to_f32(sl.z[sl.tail_at + tid]);
-    if (v > t.m) {
-      t.raise(v);
-      best = sl.tail_at + tid;
-    }
+    if (v > t.m) t.raise(v);
+    best.meet(v, sl.tail_at + tid);
     t.add(v, t.base());
   }
-  const uint64_t mine = any ? key_of(t.m, best) : 0;
+  const uint64_t mine = any ? key_of(best.top, best.at) : 0;
 
-  t.over_lanes<32>();
+  t.template over_lanes<32>();
   if ((tid & 31) == 0) sh.terms[tid >> 5] = t;
+  if (TOP && tid == 0) { sh.bound = 1; sh.n_cand = 0; sh.n_hot = 0; }
   __syncthreads();
-  if (tid < 32) {
+  if (tid / 32 == kWarps - 1) {      // the last warp: the first ones have a bound to find
+    const uint32_t lane = tid & 31;
     Terms r;
-    if (tid < kWarps) r = sh.terms[tid];
-    r.over_lanes<kWarps>();
-    if (tid == 0) sh.cta = r;
+    if (lane < kWarps) r = sh.terms[lane];
+    r.template over_lanes<kWarps>();
+    if (lane == 0) sh.cta = r;
   }
   const uint32_t own = TOP ? min(p.top, sl.elements()) : 0;
-  if (TOP && own) best_of_slice(sh, sl, mine, own);
-  __syncthreads();
+  if (TOP && own) best_of_slice<T, THREADS>(sh, sl, best, mine, raw, own);
+  else __syncthreads();
   if (ctas > 1) {
     cluster.sync();
     if (rank == 0) {
       if (tid < 32) {
         Terms r;
         if (tid < ctas) r = cluster.map_shared_rank(&sh, tid)->cta;
-        r.over_lanes<kMaxCluster>();
+        r.template over_lanes<kMaxCluster>();
         __syncwarp();
         if (tid == 0) sh.cta = r;      // every lane has read its CTA's, this one's among them
       }
@@ -357,7 +412,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Forward 
           n += of;
         }
         __syncthreads();
-        rank_keys(sh.cand, n, p.top, sh.sorted);
+        rank_keys<THREADS>(sh.cand, n, p.top, sh.sorted);
       }
     }
     cluster.sync();      // nobody leaves while its memory is read
@@ -370,11 +425,11 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Forward 
     if (p.entropy) p.entropy[row] = dead ? 0.0f : log_s - r.w / r.s;
     if (p.stats) p.stats[row] = make_float2(from, log_s);
   }
-  if (tid < p.n_tokens) p.logprobs[row * p.n_tokens + tid] = token < 0 ? 0.0f : (token_z - from) - log_s;
+  if (tid < p.n_tokens) p.logprobs[(int64_t)row * p.n_tokens + tid] = token < 0 ? 0.0f : (token_z - from) - log_s;
   if (TOP && tid < p.top) {
     const uint64_t key = sh.sorted[tid];
-    p.top_tokens[row * p.top + tid] = (int64_t)(uint32_t)~(uint32_t)key;
-    p.top_logprobs[row * p.top + tid] = (value_of((uint32_t)(key >> 32)) - from) - log_s;
+    p.top_tokens[(int64_t)row * p.top + tid] = (int64_t)(uint32_t)~(uint32_t)key;
+    p.top_logprobs[(int64_t)row * p.top + tid] = (value_of((uint32_t)(key >> 32)) - from) - log_s;
   }
 }
 
@@ -390,26 +445,26 @@ struct Backward {
 
 // A row's slice per CTA (gridDim.y slices of a row).  Few logits have a cotangent of their own: they are written again behind the slice's.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(const Backward p) {
+__global__ void __launch_bounds__(kBackThreads) token_logprobs_bwd_kernel(const Backward p) {
   grid_wait();
   constexpr int kVec = Vec<T>::kSize;
   __shared__ int64_t at[kMaxTokens + kMaxTop];
   __shared__ float own[kMaxTokens + kMaxTop];
   __shared__ float total;
   const uint32_t tid = threadIdx.x;
-  const int64_t row = blockIdx.x;
+  const uint32_t row = blockIdx.x;
   const T* z = static_cast<const T*>(p.logits) + p.rows.at(row);
-  T* dz = static_cast<T*>(p.dlogits) + row * p.vocab;
+  T* dz = static_cast<T*>(p.dlogits) + (int64_t)row * p.vocab;
   const uint32_t n = p.n_tokens + p.top;
   const float2 st = p.stats[row];
   const float g_entropy = p.g_entropy ? p.g_entropy[row] : 0.0f, entropy = p.g_entropy ? p.entropy[row] : 0.0f;
-  for (uint32_t i = tid; i < n; i += kThreads) {
+  for (uint32_t i = tid; i < n; i += kBackThreads) {
     const bool given = i < p.n_tokens;
-    int64_t j = given ? p.tokens[row * p.n_tokens + i] : p.top_tokens[row * p.top + i - p.n_tokens];
+    int64_t j = given ? p.tokens[(int64_t)row * p.n_tokens + i] : p.top_tokens[(int64_t)row * p.top + i - p.n_tokens];
     const float* g = given ? p.g_logprobs : p.g_top;
     const bool counts = j >= 0 && j < p.vocab && g != nullptr;
     at[i] = counts ? j : -1;
-    own[i] = counts ? (given ? g[row * p.n_tokens + i] : g[row * p.top + i - p.n_tokens]) : 0.0f;
+    own[i] = counts ? (given ? g[(int64_t)row * p.n_tokens + i] : g[(int64_t)row * p.top + i - p.n_tokens]) : 0.0f;
   }
   __syncthreads();
   if (tid < 32) {
@@ -435,22 +490,22 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(const Back
     if (tid < sl.tail) dz[sl.tail_at + tid] = Elem<T>::from_f32(gradient(Elem<T>::to_f32(z[sl.tail_at + tid])));
     const uint4* in = reinterpret_cast<const uint4*>(z + at0);
     uint4* out = reinterpret_cast<uint4*>(dz + at0);
-    for (uint32_t j = tid; j < sl.count; j += kThreads) {
-      float v[kVec];
+    for (uint32_t j = tid; j < sl.count; j += kBackThreads) {
+      float2 v[kVec / 2];
       Vec<T>::unpack(__ldg(in + j), v);
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) v[e] = gradient(v[e]);
+      for (int e = 0; e < kVec / 2; ++e) v[e] = make_float2(gradient(v[e].x), gradient(v[e].y));
       out[j] = Vec<T>::pack(v);
     }
   } else {      // rows of logits and of dz that start at other places of 16 bytes
     const uint32_t per = (p.vocab + gridDim.y - 1) / gridDim.y;
     lo = min(blockIdx.y * per, p.vocab);
     hi = min(lo + per, p.vocab);
-    for (uint32_t j = lo + tid; j < hi; j += kThreads) dz[j] = Elem<T>::from_f32(gradient(Elem<T>::to_f32(z[j])));
+    for (uint32_t j = lo + tid; j < hi; j += kBackThreads) dz[j] = Elem<T>::from_f32(gradient(Elem<T>::to_f32(z[j])));
   }
   if (n == 0 || st.y == INFINITY) return;      // a row without any logit has no gradient
   __syncthreads();
-  for (uint32_t i = tid; i < n; i += kThreads) {
+  for (uint32_t i = tid; i < n; i += kBackThreads) {
     const int64_t j = at[i];
     if (j < (int64_t)lo || j >= (int64_t)hi) continue;
     float g = 0.0f;
@@ -471,18 +526,26 @@ int ctas_of_row(int64_t rows, int64_t bytes) {
   return c;
 }
 
-template <typename T, bool TOP> cudaError_t launch_forward(const Forward& p, int64_t rows, cudaStream_t st) {
-  const int ctas = ctas_of_row(rows, (int64_t)p.vocab * sizeof(T));
+template <typename T, int THREADS, bool TOP> cudaError_t launch_forward(const Forward& p, int64_t rows, int ctas, cudaStream_t st) {
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3((unsigned)(rows * ctas)); config.blockDim = dim3(kThreads); config.stream = st;
+  config.gridDim = dim3((unsigned)(rows * ctas)); config.blockDim = dim3(THREADS); config.stream = st;
   cudaLaunchAttribute attrs[2];
   attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attrs[0].val.programmaticStreamSerializationAllowed = 1;
   attrs[1].id = cudaLaunchAttributeClusterDimension;
   attrs[1].val.clusterDim.x = ctas; attrs[1].val.clusterDim.y = 1; attrs[1].val.clusterDim.z = 1;
   config.attrs = attrs;
-  config.numAttrs = 2;
-  return cudaLaunchKernelEx(&config, token_logprobs_kernel<T, TOP>, p);
+  config.numAttrs = ctas > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&config, token_logprobs_kernel<T, THREADS, TOP>, p);
+}
+template <typename T> cudaError_t forward_of(const Forward& p, int64_t rows, cudaStream_t st) {
+  const int64_t bytes = (int64_t)p.vocab * sizeof(T);
+  int ctas = ctas_of_row(rows, bytes);
+  bool wide = false;
+  if (int v = env_switch("PB_LP_CTAS", 0)) ctas = v;
+  if (int v = env_switch("PB_LP_WIDE", 0)) wide = v == 2;
+  if (wide) return p.top ? launch_forward<T, 512, true>(p, rows, ctas, st) : launch_forward<T, 512, false>(p, rows, ctas, st);
+  return p.top ? launch_forward<T, 256, true>(p, rows, ctas, st) : launch_forward<T, 256, false>(p, rows, ctas, st);
 }
 
 int check_rows(const char* who, const void* logits, int dtype, int64_t outer, int64_t inner, int64_t stride_outer, int64_t stride_inner, int64_t vocab,
@@ -511,11 +574,11 @@ extern "C" int pb_token_logprobs(const void* logits, int dtype, int64_t outer, i
   if (rows == 0) return PB_OK;
   if ((n_tokens && !logprobs) || (top && (!top_logprobs || !top_tokens))) return fail(PB_ERR_NULL_POINTER, "pb_token_logprobs: null argument");
   if (reinterpret_cast<uintptr_t>(stats) & 7) return fail(PB_ERR_MISALIGNED, "pb_token_logprobs: stats must be 8-byte aligned");
-  const Forward p{logits, {inner, stride_outer, stride_inner}, (uint32_t)vocab, (uint32_t)n_tokens, (uint32_t)top, tokens, logprobs, entropy, top_logprobs, top_tokens,
+  const Forward p{logits, {FastDiv((uint32_t)inner), stride_outer, stride_inner}, (uint32_t)vocab, (uint32_t)n_tokens, (uint32_t)top, tokens, logprobs, entropy, top_logprobs, top_tokens,
                   reinterpret_cast<float2*>(stats)};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == PB_F32) top ? launch_forward<float, true>(p, rows, st) : launch_forward<float, false>(p, rows, st);
-  else top ? launch_forward<__nv_bfloat16, true>(p, rows, st) : launch_forward<__nv_bfloat16, false>(p, rows, st);
+  if (dtype == PB_F32) forward_of<float>(p, rows, st);
+  else forward_of<__nv_bfloat16>(p, rows, st);
   PB_LAUNCH_CHECK("token_logprobs_kernel");
   return PB_OK;
 }
@@ -528,12 +591,12 @@ extern "C" int pb_token_logprobs_bwd(const void* logits, int dtype, int64_t oute
   if (rows == 0) return PB_OK;
   if (!stats || !dlogits || (top && !top_tokens) || (g_entropy && !entropy)) return fail(PB_ERR_NULL_POINTER, "pb_token_logprobs_bwd: null argument");
   if ((reinterpret_cast<uintptr_t>(stats) & 7) || (reinterpret_cast<uintptr_t>(dlogits) & 15)) return fail(PB_ERR_MISALIGNED, "pb_token_logprobs_bwd: stats 8 and dlogits 16 bytes");
-  const Backward p{logits, {inner, stride_outer, stride_inner}, (uint32_t)vocab, (uint32_t)n_tokens, (uint32_t)top, tokens, top_tokens,
+  const Backward p{logits, {FastDiv((uint32_t)inner), stride_outer, stride_inner}, (uint32_t)vocab, (uint32_t)n_tokens, (uint32_t)top, tokens, top_tokens,
                    reinterpret_cast<const float2*>(stats), entropy, g_logprobs, g_entropy, g_top, dlogits};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const dim3 grid((unsigned)rows, (unsigned)ctas_of_row(rows, vocab * (dtype == PB_F32 ? 4 : 2)));
-  if (dtype == PB_F32) launch_behind(token_logprobs_bwd_kernel<float>, grid, kThreads, 0, st, p);
-  else launch_behind(token_logprobs_bwd_kernel<__nv_bfloat16>, grid, kThreads, 0, st, p);
+  if (dtype == PB_F32) launch_behind(token_logprobs_bwd_kernel<float>, grid, kBackThreads, 0, st, p);
+  else launch_behind(token_logprobs_bwd_kernel<__nv_bfloat16>, grid, kBackThreads, 0, st, p);
   PB_LAUNCH_CHECK("token_logprobs_bwd_kernel");
   return PB_OK;
 }
