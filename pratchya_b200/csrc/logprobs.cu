@@ -14,9 +14,6 @@
 
 #include <cooperative_groups.h>
 
-#ifndef LPMIN
-#define LPMIN 1024
-#endif
 namespace pb {
 namespace {
 
@@ -52,6 +49,7 @@ template <> struct Vec<float> {
   static __device__ __forceinline__ uint4 pack(const float2 (&v)[2]) {
     return make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
   }
+  static __device__ __forceinline__ float at(const uint4& r, uint32_t i) { return __uint_as_float(i < 2 ? i == 0 ? r.x : r.y : i == 2 ? r.z : r.w); }
   static __device__ __forceinline__ float top(const uint4& r) {
     return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
   }
@@ -65,6 +63,10 @@ template <> struct Vec<__nv_bfloat16> {
   }
   static __device__ __forceinline__ uint4 pack(const float2 (&v)[4]) {
     return make_uint4(pack_bf16x2(v[0].x, v[0].y), pack_bf16x2(v[1].x, v[1].y), pack_bf16x2(v[2].x, v[2].y), pack_bf16x2(v[3].x, v[3].y));
+  }
+  static __device__ __forceinline__ float at(const uint4& r, uint32_t i) {
+    const uint32_t w = i < 4 ? i < 2 ? r.x : r.y : i < 6 ? r.z : r.w;
+    return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
   }
   static __device__ __forceinline__ float top(const uint4& r) {
     auto both = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
@@ -151,33 +153,33 @@ template <int THREADS> struct Shared {
   uint64_t cand[kCandidates];
   uint64_t groups[THREADS];             // the best keys of groups of threads
   uint64_t sorted[kMaxTop];
+  uint64_t gathered[kMaxCluster * kMaxTop];      // of a cluster's CTAs, in its first one
   uint64_t bound;
-  Sums terms[THREADS / 32], cta;
+  Sums terms[THREADS / 32], cta, of_cta[kMaxCluster];
   uint32_t n_cand, n_hot;
   uint16_t hot[THREADS];
 };
 
-// How many of the keys in[0, n) are above `key`; `in` lies at 16 bytes
-__device__ __forceinline__ uint32_t keys_above(const uint64_t* in, uint32_t n, uint64_t key) {
-  uint32_t above = 0;
+// For every key in[0, n), which lie at 16 bytes, how many are above it, as done(index, key, above) in one thread.  Where there are fewer keys than threads, neighbouring threads share one.
+template <int THREADS, typename Done> __device__ __forceinline__ void rank_keys(const uint64_t* in, uint32_t n, Done done) {
+  const uint32_t tid = threadIdx.x, share = n <= THREADS / 8 ? 8 : n <= THREADS / 4 ? 4 : n <= THREADS / 2 ? 2 : 1;
+  const uint32_t part = tid % share, step = THREADS / share;
+  for (uint32_t i0 = 0; i0 < n; i0 += step) {      // a warp's threads go round together
+    const uint32_t i = i0 + tid / share;
+    const uint64_t key = i < n ? in[i] : ~0ull;
+    uint32_t above = 0;
 #pragma unroll 4
-  for (uint32_t j = 0; j + 1 < n; j += 2) {
-    const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(in + j);
-    above += (two.x > key) + (two.y > key);
-  }
-  if (n & 1) above += in[n - 1] > key;
-  return above;
-}
-// Those of the keys in[0, n) that are among the k largest, in order; no two are equal
-template <int THREADS> __device__ __forceinline__ void rank_keys(const uint64_t* in, uint32_t n, uint32_t k, uint64_t* out) {
-  for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-    const uint64_t key = in[i];
-    const uint32_t above = keys_above(in, n, key);
-    if (above < k) out[above] = key;
+    for (uint32_t j = part * 2; j + 1 < n; j += share * 2) {
+      const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(in + j);
+      above += (two.x > key) + (two.y > key);
+    }
+    if ((n & 1) && part == 0) above += in[n - 1] > key;
+    for (uint32_t o = 1; o < share; o <<= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+    if (i < n && part == 0) done(i, key, above);
   }
 }
 
-// What a thread knows of its logits: the largest, the last index of the vector that it first came in (its own index before and behind the vectors), and the largest
+// What a thread knows of its logits: the largest and the last index of the vector that it first came in (its own index before and behind the vectors), and the largest
 // of its other vectors' largest.
 struct Best {
   float top = -INFINITY, second = -INFINITY;
@@ -197,7 +199,11 @@ template <typename T, int THREADS>
 __device__ void best_of_slice(Shared<THREADS>& sh, const Slice<T>& sl, const Best& best, uint64_t mine, const uint4 (&raw)[kLoads], uint32_t k) {
   constexpr int kVec = Vec<T>::kSize;
   const uint32_t tid = threadIdx.x;
+  const uint32_t rounds = (sl.count + THREADS - 1) / THREADS, at0 = sl.at0();
   const uint32_t groups = k <= 4 ? 8 : k <= 16 ? 32 : k <= 64 ? 128 : THREADS, lanes = THREADS / groups;
+  uint4 best_vector;      // asked for before it is known whether it is wanted: most of the time that takes is then over
+  const bool vector = rounds > kLoads && best.at >= at0 && best.at < sl.tail_at;
+  if (vector) best_vector = *reinterpret_cast<const uint4*>(sl.z + best.at - (kVec - 1));
   uint64_t key = mine;
   for (uint32_t o = 1; o < min(lanes, 32u); o <<= 1) {
     const uint64_t other = __shfl_xor_sync(0xffffffffu, key, o);
@@ -206,12 +212,10 @@ __device__ void best_of_slice(Shared<THREADS>& sh, const Slice<T>& sl, const Bes
   const uint32_t held = max(groups, (uint32_t)THREADS / 32);      // a group is a warp at most
   if (tid % (THREADS / held) == 0) sh.groups[tid / (THREADS / held)] = key;
   __syncthreads();
-  if (tid < held) {
-    const uint64_t own = sh.groups[tid];
-    if (own != 0 && keys_above(sh.groups, held, own) == k - 1) sh.bound = own;      // no two of the others are equal
-  }
+  rank_keys<THREADS>(sh.groups, held, [&](uint32_t, uint64_t own, uint32_t above) {
+    if (own != 0 && above == k - 1) sh.bound = own;      // no two of the others are equal
+  });
   __syncthreads();
-  const uint32_t rounds = (sl.count + THREADS - 1) / THREADS, at0 = sl.at0();
   while (true) {      // once, but for rows whose best logits crowd into a few threads: the bound rises until what reaches it has room
     const uint64_t bound = sh.bound;
     const float bound_z = value_of((uint32_t)(bound >> 32));
@@ -223,44 +227,51 @@ __device__ void best_of_slice(Shared<THREADS>& sh, const Slice<T>& sl, const Bes
         if (at < kCandidates) sh.cand[at] = c;
       }
     };
-    auto offer_all = [&](const uint4& r, uint32_t at) {
+    auto offer_all = [&](const uint4& r, uint32_t at) {      // few reach it, in most vectors one
       float2 v[kVec / 2];
       Vec<T>::unpack(r, v);
+      uint32_t reach = 0;
 #pragma unroll
-      for (int e = 0; e < kVec / 2; ++e) { offer(v[e].x, at + 2 * e); offer(v[e].y, at + 2 * e + 1); }
+      for (int e = 0; e < kVec / 2; ++e) reach |= (v[e].x < bound_z ? 0u : 1u << (2 * e)) | (v[e].y < bound_z ? 0u : 2u << (2 * e));
+      for (; reach; reach &= reach - 1) {
+        const uint32_t e = __ffs(reach) - 1;
+        offer(Vec<T>::at(r, e), at + e);
+      }
     };
     if (mine >= bound) {
       if (tid < sl.head) offer(Elem<T>::to_f32(sl.z[tid]), tid);
       if (tid < sl.tail) offer(Elem<T>::to_f32(sl.z[sl.tail_at + tid]), sl.tail_at + tid);
-      const bool several = !(best.second < bound_z);
+      // a bound of -inf has the index of a thread's first vector: of other -inf only those of first vectors reach it
+      const bool nothing = bound_z == -INFINITY, several = nothing ? best.second > -INFINITY : !(best.second < bound_z);
       if (rounds <= kLoads) {
 #pragma unroll
         for (int l = 0; l < kLoads; ++l) {
           const uint32_t at = at0 + (tid + l * THREADS) * kVec;
-          if (tid + l * THREADS < sl.count && (several || best.at == at + kVec - 1)) offer_all(raw[l], at);
+          if (tid + l * THREADS < sl.count && (several || best.at == at + kVec - 1 || (nothing && l == 0))) offer_all(raw[l], at);
         }
       } else if (several) {
         sh.hot[atomicAdd(&sh.n_hot, 1u)] = (uint16_t)tid;
-      } else if (best.at >= at0 && best.at < sl.tail_at) {
-        const uint32_t at = best.at - (kVec - 1);
-        offer_all(*reinterpret_cast<const uint4*>(sl.z + at), at);
+      } else {
+        if (vector) offer_all(best_vector, best.at - (kVec - 1));
+        const uint32_t first = at0 + tid * kVec;
+        if (nothing && tid < sl.count && !(vector && best.at == first + kVec - 1)) offer_all(*reinterpret_cast<const uint4*>(sl.z + first), first);
       }
     }
     __syncthreads();
     if (sh.n_hot != 0) {
-      const uint32_t items = sh.n_hot * rounds;
-      for (uint32_t i = tid; i < items; i += THREADS) {
-        const uint32_t h = i / rounds, vec = (i - h * rounds) * THREADS + sh.hot[h];
-        if (vec < sl.count) {
+      const uint32_t bits = rounds >= 32 ? 5 : 32 - __clz(rounds - 1), lane = tid & ((1u << bits) - 1);      // a warp or a part of it for each
+      for (uint32_t h = tid >> bits; h < sh.n_hot; h += THREADS >> bits)
+        for (uint32_t vec = lane * THREADS + sh.hot[h]; vec < sl.count; vec += THREADS << bits) {
           const uint32_t at = at0 + vec * kVec;
           const uint4 r = *reinterpret_cast<const uint4*>(sl.z + at);
           if (!(Vec<T>::top(r) < bound_z)) offer_all(r, at);      // of nothing but NaN the top is one
         }
-      }
       __syncthreads();
     }
     const uint32_t n = sh.n_cand, kept = min(n, (uint32_t)kCandidates);
-    rank_keys<THREADS>(sh.cand, kept, k, sh.sorted);
+    rank_keys<THREADS>(sh.cand, kept, [&](uint32_t, uint64_t key, uint32_t above) {
+      if (above < k) sh.sorted[above] = key;
+    });
     __syncthreads();
     if (n <= kCandidates) break;
     if (tid == 0) { sh.bound = sh.sorted[k - 1]; sh.n_cand = 0; sh.n_hot = 0; }
@@ -280,7 +291,7 @@ struct Forward {
 
 // One row per cluster of CTAs (of one CTA where there are rows enough to fill the chip); its CTAs' terms and best logits meet in the first one.
 template <typename T, int THREADS, bool TOP>
-__global__ void __launch_bounds__(THREADS, LPMIN / THREADS) token_logprobs_kernel(const Forward p) {
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel(const Forward p) {
   grid_wait();
   __shared__ __align__(16) Shared<THREADS> sh;
   constexpr int kVec = Vec<T>::kSize, kWarps = THREADS / 32;
@@ -302,9 +313,9 @@ __global__ void __launch_bounds__(THREADS, LPMIN / THREADS) token_logprobs_kerne
 
   Terms t;
   Best best;
-  best.at = tid < sl.head ? tid : tid < sl.count ? at0 + tid * kVec + kVec - 1 : sl.tail_at + tid;      // of its first logit, while there are none but -inf
+  best.at = tid < sl.head ? tid : tid < sl.count ? at0 + tid * kVec + kVec - 1 : sl.tail_at + tid;
   const bool any = tid < sl.head || tid < sl.count || tid < sl.tail;
-  bool masked = false;      // this thread has met a logit that is no number
+  bool masked = false;      // this warp has met a logit that is no number
   if (tid < sl.head) {
     const float v = Elem<T>::to_f32(sl.z[tid]);
     if (v > t.m) t.m = v;
@@ -347,7 +358,7 @@ __global__ void __launch_bounds__(THREADS, LPMIN / THREADS) token_logprobs_kerne
       }
       t.s = sum.x + sum.y;
       float w = weighted.x + weighted.y;
-      if (w != w) {      // 0 * -inf: from here on with differences that are kept finite, and for these logits once more
+      if (__any_sync(0xffffffffu, w != w)) {      // 0 * -inf: the warp goes on with differences that are kept finite, and adds these logits up once more
         masked = true;
         Terms again;
 #pragma unroll 1
@@ -394,30 +405,26 @@ __global__ void __launch_bounds__(THREADS, LPMIN / THREADS) token_logprobs_kerne
   const uint32_t own = TOP ? min(p.top, sl.elements()) : 0;
   if (TOP && own) best_of_slice<T, THREADS>(sh, sl, best, mine, raw, own);
   else __syncthreads();
-  if (ctas > 1) {
+  if (ctas > 1) {      // everyone hands what it has to the first CTA
+    Shared<THREADS>* to = cluster.map_shared_rank(&sh, 0);
+    if (TOP)
+      for (uint32_t i = tid; i < p.top; i += THREADS) to->gathered[rank * p.top + i] = i < own ? sh.sorted[i] : 0;
+    if (tid == 0) to->of_cta[rank] = sh.cta;
     cluster.sync();
-    if (rank == 0) {
-      if (tid < 32) {
-        Terms r;
-        if (tid < ctas) r = cluster.map_shared_rank(&sh, tid)->cta;
-        r.template over_lanes<kMaxCluster>();
-        __syncwarp();
-        if (tid == 0) sh.cta = r;      // every lane has read its CTA's, this one's among them
-      }
-      if (TOP) {
-        uint32_t n = 0;
-        for (uint32_t r = 0; r < ctas; ++r) {
-          const uint32_t of = min(p.top, Slice<T>(z, p.vocab, r, ctas).elements());
-          if (tid < of) sh.cand[n + tid] = cluster.map_shared_rank(&sh, r)->sorted[tid];
-          n += of;
-        }
-        __syncthreads();
-        rank_keys<THREADS>(sh.cand, n, p.top, sh.sorted);
-      }
-    }
-    cluster.sync();      // nobody leaves while its memory is read
     if (rank != 0) return;
+    if (tid < 32) {
+      Terms r;
+      if (tid < ctas) r = sh.of_cta[tid];
+      r.template over_lanes<kMaxCluster>();
+      if (tid == 0) sh.cta = r;
+    }
+    if (TOP)
+      rank_keys<THREADS>(sh.gathered, ctas * p.top, [&](uint32_t, uint64_t key, uint32_t above) {
+        if (above < p.top && key != 0) sh.sorted[above] = key;
+      });
+    __syncthreads();
   }
+  if (tid >= max(max(p.n_tokens, p.top), 1u)) return;
   const Sums r = sh.cta;
   const bool dead = r.s == 0.0f;      // nothing but -inf: every token's log probability is -inf
   const float log_s = dead ? INFINITY : logf(r.s), from = dead ? 0.0f : r.m;
@@ -443,7 +450,17 @@ struct Backward {
   void* dlogits;
 };
 
-// A row's slice per CTA (gridDim.y slices of a row).  Few logits have a cotangent of their own: they are written again behind the slice's.
+// sizeof(T) * kVec bytes of logits from an address that is a multiple of sizeof(T) only
+template <typename T> __device__ __forceinline__ uint4 load_anywhere(const T* from) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(from);
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(at & ~(uintptr_t)3);
+  const uint32_t a = __ldg(w), b = __ldg(w + 1), c = __ldg(w + 2), d = __ldg(w + 3);
+  if ((at & 3) == 0) return make_uint4(a, b, c, d);
+  const uint32_t e = __ldg(w + 4);      // holds the last one
+  return make_uint4(__funnelshift_r(a, b, 16), __funnelshift_r(b, c, 16), __funnelshift_r(c, d, 16), __funnelshift_r(d, e, 16));
+}
+
+// A row's slice per CTA (gridDim.y slices of a row), in vectors of dz.  Few logits have a cotangent of their own: they are written again behind the slice's.
 template <typename T>
 __global__ void __launch_bounds__(kBackThreads) token_logprobs_bwd_kernel(const Backward p) {
   grid_wait();
@@ -475,33 +492,30 @@ __global__ void __launch_bounds__(kBackThreads) token_logprobs_bwd_kernel(const 
     if (tid == 0) total = sum;
   }
   __syncthreads();
-  const float all = total;
-  auto gradient = [&](float v) {
-    const float x = max_nan((v - st.x) - st.y, kFar), pr = exp2_fast(x * kLog2e);
-    return -pr * (all + g_entropy * (x + entropy));
+  // p_j (c - g_entropy log p_j), with everything that a row has one of in c
+  const float c = fmaf(-g_entropy, entropy, -total);
+  const float2 minus_m = make_float2(-st.x, -st.x), minus_s = make_float2(-st.y, -st.y), scale = make_float2(kLog2e, kLog2e), minus_g = make_float2(-g_entropy, -g_entropy), c2 = make_float2(c, c);
+  auto gradient = [&](const float2& v) {
+    float2 x = __fadd2_rn(__fadd2_rn(v, minus_m), minus_s);
+    x = make_float2(max_nan(x.x, kFar), max_nan(x.y, kFar));
+    const float2 a = __fmul2_rn(x, scale);
+    return __fmul2_rn(make_float2(exp2_fast(a.x), exp2_fast(a.y)), __ffma2_rn(minus_g, x, c2));
   };
-  uint32_t lo, hi;      // elements of this CTA
-  if (((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15) == 0) {
-    const Slice<T> sl(z, p.vocab, blockIdx.y, gridDim.y);
-    const uint32_t at0 = sl.at0();
-    lo = blockIdx.y == 0 ? 0 : at0;
-    hi = at0 + sl.count * kVec + sl.tail;
-    if (tid < sl.head) dz[tid] = Elem<T>::from_f32(gradient(Elem<T>::to_f32(z[tid])));
-    if (tid < sl.tail) dz[sl.tail_at + tid] = Elem<T>::from_f32(gradient(Elem<T>::to_f32(z[sl.tail_at + tid])));
-    const uint4* in = reinterpret_cast<const uint4*>(z + at0);
-    uint4* out = reinterpret_cast<uint4*>(dz + at0);
-    for (uint32_t j = tid; j < sl.count; j += kBackThreads) {
-      float2 v[kVec / 2];
-      Vec<T>::unpack(__ldg(in + j), v);
+  auto one = [&](uint32_t j) { return gradient(make_float2(Elem<T>::to_f32(z[j]), 0.0f)).x; };
+  const Slice<T> sl(dz, p.vocab, blockIdx.y, gridDim.y);
+  const uint32_t at0 = sl.at0(), lo = blockIdx.y == 0 ? 0 : at0, hi = at0 + sl.count * kVec + sl.tail;      // elements of this CTA
+  const bool same = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15) == 0;
+  if (tid < sl.head) dz[tid] = Elem<T>::from_f32(one(tid));
+  if (tid < sl.tail) dz[sl.tail_at + tid] = Elem<T>::from_f32(one(sl.tail_at + tid));
+  uint4* out = reinterpret_cast<uint4*>(dz + at0);
+#pragma unroll 2
+  for (uint32_t j = tid; j < sl.count; j += kBackThreads) {
+    const uint4 r = same ? __ldg(reinterpret_cast<const uint4*>(z + at0) + j) : load_anywhere(z + at0 + j * kVec);
+    float2 v[kVec / 2];
+    Vec<T>::unpack(r, v);
 #pragma unroll
-      for (int e = 0; e < kVec / 2; ++e) v[e] = make_float2(gradient(v[e].x), gradient(v[e].y));
-      out[j] = Vec<T>::pack(v);
-    }
-  } else {      // rows of logits and of dz that start at other places of 16 bytes
-    const uint32_t per = (p.vocab + gridDim.y - 1) / gridDim.y;
-    lo = min(blockIdx.y * per, p.vocab);
-    hi = min(lo + per, p.vocab);
-    for (uint32_t j = lo + tid; j < hi; j += kBackThreads) dz[j] = Elem<T>::from_f32(gradient(Elem<T>::to_f32(z[j])));
+    for (int e = 0; e < kVec / 2; ++e) v[e] = gradient(v[e]);
+    out[j] = Vec<T>::pack(v);
   }
   if (n == 0 || st.y == INFINITY) return;      // a row without any logit has no gradient
   __syncthreads();
@@ -515,7 +529,7 @@ __global__ void __launch_bounds__(kBackThreads) token_logprobs_bwd_kernel(const 
         first = first && o >= i;
         g += own[o];
       }
-    if (first) dz[j] = Elem<T>::from_f32(gradient(Elem<T>::to_f32(z[j])) + g);
+    if (first) dz[j] = Elem<T>::from_f32(one((uint32_t)j) + g);
   }
 }
 
@@ -540,11 +554,18 @@ template <typename T, int THREADS, bool TOP> cudaError_t launch_forward(const Fo
 }
 template <typename T> cudaError_t forward_of(const Forward& p, int64_t rows, cudaStream_t st) {
   const int64_t bytes = (int64_t)p.vocab * sizeof(T);
-  int ctas = ctas_of_row(rows, bytes);
-  bool wide = false;
+  const int64_t sms = sm_count();
+  int ctas = 1;
+  while (ctas < kMaxCluster && rows * ctas * 2 <= sms && bytes / (ctas * 2) >= 32768) ctas *= 2;
+  // us, 128 | 256 | 512 threads a row: 4096 rows of 16 KB 25 | 38 | 71 (five alternatives), 17.5 | 21.5 | 38 (none), 51 | 65 | 98 (64); 2000 rows of 128 KB 55 | 57 | 69
+  // (five), 50 | 48 | 52 (none), 90 | 74 | 85 (64); 148 rows of 256 KB 20.9 | 19.7 | 13.8 (20); one such row over eight CTAs 6.6 | 6.0 | 6.4
+  int threads;
+  if (rows * ctas <= sms) threads = bytes / ctas > 32768 ? 512 : bytes / ctas > 8192 ? 256 : 128;
+  else threads = bytes <= 32768 || (bytes <= 131072 && p.top > 0 && p.top <= 32) ? 128 : 256;
   if (int v = env_switch("PB_LP_CTAS", 0)) ctas = v;
-  if (int v = env_switch("PB_LP_WIDE", 0)) wide = v == 2;
-  if (wide) return p.top ? launch_forward<T, 512, true>(p, rows, ctas, st) : launch_forward<T, 512, false>(p, rows, ctas, st);
+  if (int v = env_switch("PB_LP_WIDE", 0)) threads = v;
+  if (threads == 128) return p.top ? launch_forward<T, 128, true>(p, rows, ctas, st) : launch_forward<T, 128, false>(p, rows, ctas, st);
+  if (threads == 512) return p.top ? launch_forward<T, 512, true>(p, rows, ctas, st) : launch_forward<T, 512, false>(p, rows, ctas, st);
   return p.top ? launch_forward<T, 256, true>(p, rows, ctas, st) : launch_forward<T, 256, false>(p, rows, ctas, st);
 }
 
