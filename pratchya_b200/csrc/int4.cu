@@ -22,97 +22,163 @@ namespace {
 namespace cg = cooperative_groups;
 
 // ---- the quantizer -----------------------------------------------------------------------------------------------------
-constexpr int kQuantThreads = 256, kQuantCols = 64;      // 128 x 64 weights a CTA, 32 values of one column a thread
+constexpr int kQuantThreads = 256, kQuantCols = 64;      // 128 x 64 weights a CTA
+constexpr int kHalf = 160;             // words of eight columns in shared memory, 20 a column; a word's place among four goes by the eight: a warp's columns meet no bank twice
 
-// the word that holds eight codes, the i-th of them k = i
-__device__ __forceinline__ uint32_t pack_codes(const uint32_t (&u)[8]) {
-  return u[0] | u[2] << 4 | u[4] << 8 | u[6] << 12 | u[1] << 16 | u[3] << 20 | u[5] << 24 | u[7] << 28;
-}
 __device__ __forceinline__ uint32_t code_at(uint32_t word, int i) { return word >> (4 * (i / 2 + 4 * (i % 2))) & 15u; }
 __device__ __forceinline__ float max_nan(float a, float b) {
   float y;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
 }
+// where word (t, quarter) of a CTA's column is in shared memory, and a tile's sixteen bytes `slot` there
+__device__ __forceinline__ uint32_t staged_at(uint32_t col, uint32_t t, uint32_t quarter) { return col / 8 * kHalf + col % 8 * 20 + t * 4 + (quarter ^ (col / 8 & 3)); }
+__device__ __forceinline__ uint4* staged_slot(uint32_t* staged, uint32_t eight, uint32_t slot) { return reinterpret_cast<uint4*>(staged + eight * kHalf + slot / 4 * 20 + slot % 4 * 4); }
+__device__ __forceinline__ uint4 turned(uint4 o, uint32_t eight) {      // its words to their places, and back
+  if (eight & 1) o = make_uint4(o.y, o.x, o.w, o.z);
+  if (eight & 2) o = make_uint4(o.z, o.w, o.x, o.y);
+  return o;
+}
+constexpr float kRound = 12582912.0f;      // added to a number below 2^22 in size, it leaves that number's nearest integer (of two the even one) in the last bits
+constexpr uint32_t kRoundBits = 0x4b400000u;
 
 // ZERO: scale = bf16((max(w, 0) - min(w, 0)) / 15), zero = rint(-min / scale), u = rint(w / scale) + zero, both within 0..15;
-// otherwise scale = bf16(max|w| / 7), u = rint(w / scale) within -8..7, plus 8.  A group of nothing but zeros has scale 0.
-// The scale is rounded before the codes are taken: they are the nearest ones for the scale that is stored.
+// otherwise scale = bf16(max|w| / 7), u = rint(w / scale) + 8: the scale is 2^-9 of itself too small at most, and u within 1..15 by itself.
+// A group of nothing but zeros has scale 0.  The scale is rounded before the codes are taken: they are the nearest ones for the scale that is stored.
 // A group that holds a NaN or an infinity has a scale that is no finite number.
-template <typename T, bool ZERO>
+// A thread has COLS neighbouring columns (two where one load brings two bf16) and 32 / COLS values of k of each.  Bound by HBM: f32 [2048, 8192] in
+// 13.7 us (5.5 TB/s); with a division per weight, __fdiv_rn, it was bound by instructions (22 us).
+template <typename T, bool ZERO, int COLS>
 __global__ void __launch_bounds__(kQuantThreads) quantize_int4_kernel(const T* __restrict__ w, int64_t depth, int64_t cols, int per_group, uint32_t kblocks,
                                                                       uint32_t* __restrict__ q, __nv_bfloat16* __restrict__ scale, uint8_t* __restrict__ zero) {
   grid_wait();
-  __shared__ float lows[4][kQuantCols], highs[4][kQuantCols];
-  __shared__ __align__(16) uint32_t staged[4 * 256];
-  const uint32_t col = threadIdx.x % kQuantCols, c = threadIdx.x / kQuantCols;      // a warp has 32 neighbouring columns
+  constexpr int kRows = 32 / COLS, kRuns = 4 * COLS, kWords = kRows / 8;      // of a thread; threads along k
+  __shared__ float lows[ZERO ? kRuns : 1][kQuantCols], highs[kRuns][kQuantCols];
+  __shared__ __align__(16) uint32_t staged[8 * kHalf];
+  const uint32_t pair = threadIdx.x % (kQuantCols / COLS), run = threadIdx.x / (kQuantCols / COLS);      // a warp has neighbouring columns
   const uint32_t kb = blockIdx.x;
-  const int64_t n = (int64_t)blockIdx.y * kQuantCols + col, k0 = (int64_t)kb * 128 + c * 32;
-  float v[32];
-  float low = 0.0f, high = 0.0f;
+  const int64_t n0 = (int64_t)blockIdx.y * kQuantCols + pair * COLS, k0 = (int64_t)kb * 128 + run * kRows;
+  float v[COLS][kRows], low[COLS], high[COLS];
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    v[i] = n < cols && k0 + i < depth ? Elem<T>::to_f32(w[(k0 + i) * cols + n]) : 0.0f;
-    if (ZERO) {
-      low = -max_nan(-low, -v[i]);
-      high = max_nan(high, v[i]);
+  for (int i = 0; i < kRows; ++i) {
+    const T* from = w + (k0 + i) * cols + n0;
+    const bool in = k0 + i < depth;
+    if constexpr (COLS == 2) {      // of an even number of columns, two bf16 at four bytes
+      const uint32_t two = in && n0 < cols ? __ldg(reinterpret_cast<const uint32_t*>(from)) : 0u;
+      v[0][i] = __uint_as_float(two << 16);
+      v[1][i] = __uint_as_float(two & 0xffff0000u);
     } else {
-      high = max_nan(high, fabsf(v[i]));
+      v[0][i] = in && n0 < cols ? Elem<T>::to_f32(from[0]) : 0.0f;
     }
   }
-  lows[c][col] = low;
-  highs[c][col] = high;
+#pragma unroll
+  for (int c = 0; c < COLS; ++c) {
+    low[c] = high[c] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      if (ZERO) {
+        low[c] = -max_nan(-low[c], -v[c][i]);
+        high[c] = max_nan(high[c], v[c][i]);
+      } else {
+        high[c] = max_nan(high[c], fabsf(v[c][i]));
+      }
+    }
+    if (ZERO) lows[run][pair * COLS + c] = low[c];
+    highs[run][pair * COLS + c] = high[c];
+  }
   __syncthreads();
-  const int quarters = 4 / per_group;      // 32-value runs of a group
-  const int first = (int)c / quarters * quarters;
-  for (int o = 0; o < quarters; ++o) {
-    if (ZERO) low = -max_nan(-low, -lows[first + o][col]);
-    high = max_nan(high, highs[first + o][col]);
-  }
-  const float s = __bfloat162float(__float2bfloat16_rn(ZERO ? __fdiv_rn(__fsub_rn(high, low), 15.0f) : __fdiv_rn(high, 7.0f)));
-  const bool some = s != 0.0f;
-  const float z = !ZERO ? 8.0f : some ? fminf(fmaxf(rintf(__fdiv_rn(-low, s)), 0.0f), 15.0f) : 0.0f;
-  const uint32_t half = col % 16 / 8, g = col % 8, tile = col / 16;
+  const int runs = kRuns / per_group, first = (int)run / runs * runs;      // of a group
+  const int64_t tiles = (cols + 15) / 16;
 #pragma unroll
-  for (uint32_t t = 0; t < 4; ++t) {
-    uint32_t u[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float r = some ? rintf(__fdiv_rn(v[t * 8 + i], s)) : 0.0f;
-      u[i] = (uint32_t)(int)(ZERO ? fminf(fmaxf(r + z, 0.0f), 15.0f) : fminf(fmaxf(r, -8.0f), 7.0f) + 8.0f);
+  for (int c = 0; c < COLS; ++c) {
+    const uint32_t col = pair * COLS + c;
+    for (int o = 0; o < runs; ++o) {
+      if (ZERO) low[c] = -max_nan(-low[c], -lows[first + o][col]);
+      high[c] = max_nan(high[c], highs[first + o][col]);
     }
-    staged[tile * 256 + half * 128 + (g * 4 + t) * 4 + c] = pack_codes(u);
-  }
-  const int64_t tiles = (cols + 15) / 16, at = (int64_t)blockIdx.y * 4 + tile;
-  if (at < tiles && (int)c == first) {
-    const int64_t i = ((at * kblocks + kb) * 16 + col % 16) * per_group + c / quarters;
-    scale[i] = __float2bfloat16_rn(s);
-    if (ZERO) zero[i] = (uint8_t)z;
+    const float s = __bfloat162float(__float2bfloat16_rn(ZERO ? __fdiv_rn(__fsub_rn(high[c], low[c]), 15.0f) : __fdiv_rn(high[c], 7.0f)));
+    const float z = !ZERO ? 8.0f : s != 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(-low[c], s)), 0.0f), 15.0f) : 0.0f;
+    // Correctly rounded quotients by a reciprocal and two corrections, of numbers that a power of two has taken from the ends of the range (what it loses of a
+    // number below 2^-62 is nothing beside a scale above 2^90).  A scale of zero or no number: codes of 0, or any.
+    const float f = s < 0x1p-90f ? 0x1p64f : s > 0x1p90f ? 0x1p-64f : 1.0f, d = s * f, r = s > 0.0f && s < INFINITY ? __frcp_rn(d) : 0.0f;
+    const float2 f2 = make_float2(f, f), r2 = make_float2(r, r), nd2 = make_float2(-d, -d), round2 = make_float2(kRound, kRound), z2 = make_float2(z, z);
+#pragma unroll
+    for (int word = 0; word < kWords; ++word) {
+      float2 u[4];      // of k = 2 i and 2 i + 1
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 x = __fmul2_rn(make_float2(v[c][word * 8 + 2 * i], v[c][word * 8 + 2 * i + 1]), f2);
+        u[i] = __fadd2_rn(__fadd2_rn(div_hoisted_unsigned2(x, nd2, r2), round2), z2);
+        if (ZERO) u[i] = make_float2(fminf(fmaxf(u[i].x, kRound), kRound + 15.0f), fminf(fmaxf(u[i].y, kRound), kRound + 15.0f));
+      }
+      // nibbles 7..0 hold k = 7, 5, 3, 1, 6, 4, 2, 0; the bits of kRound come out of all eight together
+      uint32_t packed = __float_as_uint(u[3].y);
+      packed = packed * 16 + __float_as_uint(u[2].y);
+      packed = packed * 16 + __float_as_uint(u[1].y);
+      packed = packed * 16 + __float_as_uint(u[0].y);
+      packed = packed * 16 + __float_as_uint(u[3].x);
+      packed = packed * 16 + __float_as_uint(u[2].x);
+      packed = packed * 16 + __float_as_uint(u[1].x);
+      packed = packed * 16 + __float_as_uint(u[0].x);
+      const uint32_t k8 = run * kWords + word, t = k8 % 4, quarter = k8 / 4;      // k = 32 quarter + 8 t + ..
+      staged[staged_at(col, t, quarter)] = packed - kRoundBits * 0x11111111u;
+    }
+    const int64_t at = (int64_t)blockIdx.y * 4 + col / 16;
+    if (at < tiles && (int)run == first) {
+      const int64_t i = ((at * kblocks + kb) * 16 + col % 16) * per_group + run / runs;
+      scale[i] = __float2bfloat16_rn(s);
+      if (ZERO) zero[i] = (uint8_t)z;
+    }
   }
   __syncthreads();
   const uint32_t part = threadIdx.x / 64;      // a tile's 1024 bytes, 16 a thread
   const int64_t a = (int64_t)blockIdx.y * 4 + part;
-  if (a < tiles)
-    reinterpret_cast<uint4*>(q + (a * kblocks + kb) * 256)[threadIdx.x % 64] = reinterpret_cast<const uint4*>(staged + part * 256)[threadIdx.x % 64];
+  if (a < tiles) {
+    const uint32_t slot = threadIdx.x % 64, eight = threadIdx.x / 32;
+    reinterpret_cast<uint4*>(q + (a * kblocks + kb) * 256)[slot] = turned(*staged_slot(staged, eight, slot % 32), eight);
+  }
 }
 
-template <typename T>
+// A thread has COLS neighbouring columns (two of bf16, which one store takes) and 32 / COLS values of k of each.
+template <typename T, int COLS>
 __global__ void __launch_bounds__(kQuantThreads) dequantize_int4_kernel(const uint32_t* __restrict__ q, const __nv_bfloat16* __restrict__ scale, const uint8_t* __restrict__ zero,
                                                                         int64_t depth, int64_t cols, int per_group, uint32_t kblocks, T* __restrict__ w) {
   grid_wait();
-  const uint32_t col = threadIdx.x % kQuantCols, c = threadIdx.x / kQuantCols, kb = blockIdx.x;
-  const int64_t n = (int64_t)blockIdx.y * kQuantCols + col, k0 = (int64_t)kb * 128 + c * 32;
+  constexpr int kRows = 32 / COLS, kWords = kRows / 8;
+  __shared__ __align__(16) uint32_t staged[8 * kHalf];
+  const uint32_t pair = threadIdx.x % (kQuantCols / COLS), run = threadIdx.x / (kQuantCols / COLS), kb = blockIdx.x, quarter = run * kWords / 4;
+  const int64_t n = (int64_t)blockIdx.y * kQuantCols + pair * COLS, k0 = (int64_t)kb * 128 + run * kRows, tiles = (cols + 15) / 16;
+  float s[COLS], z[COLS];
+  if (n < cols)
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) {
+      const int64_t i = (((n / 16 * kblocks + kb) * 16) + (n + c) % 16) * per_group + quarter * per_group / 4;
+      s[c] = __bfloat162float(scale[i]);
+      z[c] = kRound + (zero ? (float)zero[i] : 8.0f);
+    }
+  const int64_t a = (int64_t)blockIdx.y * 4 + threadIdx.x / 64;
+  const uint32_t eight = threadIdx.x / 32;
+  if (a < tiles) *staged_slot(staged, eight, threadIdx.x % 32) = turned(__ldg(reinterpret_cast<const uint4*>(q + (a * kblocks + kb) * 256) + threadIdx.x % 64), eight);
+  __syncthreads();
   if (n >= cols) return;
-  const int64_t tile = n / 16 * kblocks + kb, i = (tile * 16 + n % 16) * per_group + c * per_group / 4;
-  const float s = __bfloat162float(scale[i]), z = zero ? (float)zero[i] : 8.0f;
-  const uint32_t* words = q + tile * 256 + (n % 16 / 8) * 128 + (n % 8) * 16 + c;
+  uint32_t word[COLS][kWords];
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const uint32_t word = words[t * 4];
+  for (int c = 0; c < COLS; ++c)
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (k0 + t * 8 + j < depth) w[(k0 + t * 8 + j) * cols + n] = Elem<T>::from_f32(s * ((float)code_at(word, j) - z));
-  }
+    for (int t = 0; t < kWords; ++t) word[c][t] = staged[staged_at(pair * COLS + c, (run * kWords + t) % 4, quarter)];
+  T* to = w + k0 * cols + n;
+  const bool whole = k0 + kRows <= depth;
+#pragma unroll
+  for (int t = 0; t < kWords; ++t)
+#pragma unroll
+    for (int j = 0; j < 8; ++j, to += cols) {
+      if (!whole && k0 + t * 8 + j >= depth) continue;
+      float v[COLS];
+#pragma unroll
+      for (int c = 0; c < COLS; ++c) v[c] = s[c] * (__uint_as_float(kRoundBits | code_at(word[c][t], j)) - z[c]);
+      if constexpr (COLS == 2) *reinterpret_cast<uint32_t*>(to) = pack_bf16x2(v[0], v[1]);
+      else *to = Elem<T>::from_f32(v[0]);
+    }
 }
 
 // ---- products of few rows ------------------------------------------------------------------------------------------------
@@ -633,15 +699,16 @@ extern "C" int pb_quantize_int4(const void* w, int dtype, int64_t depth, int64_t
   auto* words = reinterpret_cast<uint32_t*>(q);
   auto* s = static_cast<__nv_bfloat16*>(scale);
   const int per_group = 128 / group;
-  if (dtype == PB_F32) {
-    const float* in = static_cast<const float*>(w);
-    if (zero) launch_behind(quantize_int4_kernel<float, true>, grid, kQuantThreads, 0, st, in, depth, cols, per_group, kblocks, words, s, zero);
-    else launch_behind(quantize_int4_kernel<float, false>, grid, kQuantThreads, 0, st, in, depth, cols, per_group, kblocks, words, s, zero);
-  } else {
-    const __nv_bfloat16* in = static_cast<const __nv_bfloat16*>(w);
-    if (zero) launch_behind(quantize_int4_kernel<__nv_bfloat16, true>, grid, kQuantThreads, 0, st, in, depth, cols, per_group, kblocks, words, s, zero);
-    else launch_behind(quantize_int4_kernel<__nv_bfloat16, false>, grid, kQuantThreads, 0, st, in, depth, cols, per_group, kblocks, words, s, zero);
-  }
+  auto launch = [&](auto* in, auto cols_of_thread) {
+    using T = std::remove_const_t<std::remove_pointer_t<decltype(in)>>;
+    constexpr int kCols = decltype(cols_of_thread)::value;
+    if (zero) launch_behind(quantize_int4_kernel<T, true, kCols>, grid, kQuantThreads, 0, st, in, depth, cols, per_group, kblocks, words, s, zero);
+    else launch_behind(quantize_int4_kernel<T, false, kCols>, grid, kQuantThreads, 0, st, in, depth, cols, per_group, kblocks, words, s, zero);
+  };
+  const bool pairs = cols % 2 == 0 && (reinterpret_cast<uintptr_t>(w) & 3) == 0;
+  if (dtype == PB_F32) launch(static_cast<const float*>(w), std::integral_constant<int, 1>());
+  else if (pairs) launch(static_cast<const __nv_bfloat16*>(w), std::integral_constant<int, 2>());
+  else launch(static_cast<const __nv_bfloat16*>(w), std::integral_constant<int, 1>());
   PB_LAUNCH_CHECK("quantize_int4_kernel");
   return PB_OK;
 }
@@ -657,8 +724,10 @@ extern "C" int pb_dequantize_int4(const uint8_t* q, const void* scale, const uin
   const dim3 grid(kblocks, col_blocks);
   const auto* words = reinterpret_cast<const uint32_t*>(q);
   const auto* s = static_cast<const __nv_bfloat16*>(scale);
-  if (dtype == PB_F32) launch_behind(dequantize_int4_kernel<float>, grid, kQuantThreads, 0, st, words, s, zero, depth, cols, 128 / group, kblocks, static_cast<float*>(out));
-  else launch_behind(dequantize_int4_kernel<__nv_bfloat16>, grid, kQuantThreads, 0, st, words, s, zero, depth, cols, 128 / group, kblocks, static_cast<__nv_bfloat16*>(out));
+  auto launch = [&](auto kernel, auto* to) { launch_behind(kernel, grid, kQuantThreads, 0, st, words, s, zero, depth, cols, 128 / group, kblocks, to); };
+  if (dtype == PB_F32) launch(dequantize_int4_kernel<float, 1>, static_cast<float*>(out));
+  else if (cols % 2 == 0 && (reinterpret_cast<uintptr_t>(out) & 3) == 0) launch(dequantize_int4_kernel<__nv_bfloat16, 2>, static_cast<__nv_bfloat16*>(out));
+  else launch(dequantize_int4_kernel<__nv_bfloat16, 1>, static_cast<__nv_bfloat16*>(out));
   PB_LAUNCH_CHECK("dequantize_int4_kernel");
   return PB_OK;
 }
