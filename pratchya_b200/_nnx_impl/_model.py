@@ -21,6 +21,7 @@ import torch
 from .._qualia import _ops
 from ._glue import QuantizedMix, can_quantize_mixes, can_quantize_relu2, relu2, relu2_quantized, rms_norm, token_shift_lerp, token_shift_lerp_quantized, wkv_finish, wkv_prepare
 from ._glue import smoothed_cross_entropy as fused_cross_entropy
+from ._int4 import Int4Linear
 from ._module import linear_fp8
 from ._nograph import no_graph
 from ._wkv7 import wkv_state_scan
@@ -174,7 +175,7 @@ class TimeMix(torch.nn.Module):                      # _module.py:92-225
         bsz, steps, c = x.shape
         n, h, blk = self.n_head, self.head_dim, self.cfg.blksize
         mu = read_param(self.mu, (1, blk))
-        if self.cfg.fused_glue and can_quantize_mixes(x, torch.is_grad_enabled()):
+        if self.cfg.fused_glue and isinstance(self.w_key, Linear) and can_quantize_mixes(x, torch.is_grad_enabled()):
             # every mix only feeds linears: they leave the lerp kernel as fp8 triples (the three that feed a (128,128)
             # kernel also in the token-major form its wgrad wants) and are never written as f32
             x_r, x_d, x_k, x_v, x_i, x_g = token_shift_lerp_quantized(x, tm_state, mu, (0, 2, 3) if torch.is_grad_enabled() else ())
@@ -235,7 +236,8 @@ class ChannelMix(torch.nn.Module):                   # _module.py:228-258
 
     def forward(self, x, cm_state):
         mu_x = read_param(self.mu_x, (1, self.blk))
-        if self.fused_glue and can_quantize_mixes(x, torch.is_grad_enabled()):
+        fp8 = isinstance(self.w_k, Linear)          # not the weights in 4 bits of a model that answers
+        if self.fused_glue and fp8 and can_quantize_mixes(x, torch.is_grad_enabled()):
             x_k = token_shift_lerp_quantized(x, cm_state, mu_x, (0,) if torch.is_grad_enabled() else ())[0]
         elif self.fused_glue:
             x_k = token_shift_lerp(x, cm_state, mu_x)[0]
@@ -243,14 +245,14 @@ class ChannelMix(torch.nn.Module):                   # _module.py:228-258
             x_shifted = torch.cat([cm_state, x[:, :-1, :]], dim=1)
             x_k = lerp(x.to(torch.float32), x_shifted.to(torch.float32), mu_x)
         cm_state = x[:, -1:, :]
-        if self.fused_glue and not torch.is_grad_enabled() and x.is_cuda and self.w_k.kernel.shape[1] % 1024 == 0 and self.w_k.tgrid[1] == 128:
+        if self.fused_glue and fp8 and not torch.is_grad_enabled() and x.is_cuda and self.w_k.kernel.shape[1] % 1024 == 0 and self.w_k.tgrid[1] == 128:
             # no backward pass follows (the first pass of a recomputed block): the first product's re-quantization, relu^2 and
             # the second Linear's input quantization are one pass over the f32 product, and k is never written
             y = self.w_k(x_k, raw=True)
             k = QuantizedMix(y.new_zeros(1).expand(y.shape), _ops.relu2_requantize_impl(y), None)
             return self.w_v(k), cm_state
         k = self.w_k(x_k).to(torch.float32)
-        if self.fused_glue and torch.is_grad_enabled() and can_quantize_relu2(k) and self.w_v.tgrid == (128, 128):
+        if self.fused_glue and fp8 and torch.is_grad_enabled() and can_quantize_relu2(k) and self.w_v.tgrid == (128, 128):
             k = relu2_quantized(k)       # relu^2 as the prologue of w_v's two input quantizers
         else:
             k = relu2(k) if self.fused_glue else torch.relu(k) ** 2
@@ -348,6 +350,37 @@ class PratchyaCausalLM(torch.nn.Module):
             else:
                 loss = smoothed_cross_entropy(logits, label)
         return logits, loss
+
+    def init_state(self, batch: int):
+        """The zero state of `batch` sequences (`init_state`, _config.py:41-52): (position, [(tm_state, cm_state, wkv_state) of each block])."""
+        cfg, dev = self.cfg, self.embedding.device
+        zeros = torch.zeros(batch, 1, cfg.hidden_size, device=dev)
+        heads = cfg.hidden_size // cfg.head_dim
+        wkv = torch.zeros(batch, heads, cfg.head_dim, cfg.head_dim, device=dev)
+        return 0, [(zeros, zeros, wkv) for _ in self.blocks]
+
+    @torch.no_grad()
+    def advance(self, input_ids, state=None):
+        """(logits [B, T, V], the state behind the T tokens) of input_ids [B, T] read from `state` on (None: from the beginning): a prompt, or one token at
+        a time.  The norm over a block's heads runs over the T tokens of a call, as the reference's does (_module.py:118-123), so that a text read in pieces
+        has other logits than the same text at once."""
+        bsz, steps = input_ids.shape
+        position, layers = self.init_state(bsz) if state is None else state
+        t_positions = torch.arange(position, position + steps, device=input_ids.device, dtype=torch.int32)
+        x, v, behind = self.pre_rmsnorm(self.embed(input_ids)), None, []
+        for blk, (tm_state, cm_state, wkv_state) in zip(self.blocks, layers):
+            x, v, tm_state, cm_state, wkv_state = blk(x, v, t_positions, tm_state, cm_state, wkv_state)
+            behind.append((tm_state.contiguous(), cm_state.contiguous(), wkv_state))
+        return self.lm_head(self.final_rmsnorm(x)), (position + steps, behind)
+
+    def to_int4(self, group: int = 128, zero_points: bool = False):
+        """Turns every Linear's weight into 4 bits, in place, and lets go of the dense ones: for a model that answers (`advance`, `score` without gradients).
+        Returns the model."""
+        for module in list(self.modules()):
+            for name, child in list(module.named_children()):
+                if isinstance(child, Linear):
+                    setattr(module, name, Int4Linear(child.kernel, group, zero_points))
+        return self
 
 
 def smoothed_cross_entropy(logits, labels, alpha: float = 0.1):

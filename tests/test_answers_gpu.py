@@ -1,0 +1,138 @@
+"""A model that answers: Linears in 4 bits in every layer, a state carried from call to call, tokens with their scores."""
+import copy
+import subprocess
+import sys
+from pathlib import Path
+
+import pytest
+import torch
+
+from pratchya_b200._nnx_impl import Int4Linear, generate, score, token_logprobs
+from pratchya_b200._nnx_impl._model import Linear, PratchyaCausalLM, PratchyaConfig
+
+pytestmark = pytest.mark.gpu
+
+SMALL = dict(vocab_size=640, hidden_size=256, intermediate_size=512, lora_rank=128, n_layers=2)
+
+
+class _Dense(torch.nn.Module):
+    """The product with the values that an Int4Linear stands for, as plain torch computes it."""
+    def __init__(self, layer):
+        super().__init__()
+        self.w = layer.weight()
+
+    def forward(self, x, raw=False):
+        return torch.matmul(x, self.w)
+
+
+def _plain(model):
+    """The same model without this package's products and fused kernels (but for the scan)."""
+    plain = PratchyaCausalLM(PratchyaConfig(**{**SMALL, "fused_glue": False}), seed=1)
+    plain.load_state_dict(model.state_dict())
+    plain.to_int4(64, True)
+    for module in list(plain.modules()):
+        for name, child in list(module.named_children()):
+            if isinstance(child, Int4Linear):
+                setattr(module, name, _Dense(child))
+    return plain
+
+
+def _model():
+    torch.manual_seed(0)
+    model = PratchyaCausalLM(PratchyaConfig(**SMALL), seed=1)
+    plain = _plain(model)
+    return model.to_int4(64, True), plain
+
+
+def test_every_linear_is_taken(built_lib):
+    model, _ = _model()
+    assert not any(isinstance(m, Linear) for m in model.modules())
+    assert sum(isinstance(m, Int4Linear) for m in model.modules()) == 2 * (4 + 2 * 4 + 2) - 2 + 1          # the first layer has no nu_lora
+    assert not any(name.endswith("kernel") for name, _ in model.named_parameters())
+
+
+def test_a_prompt_and_single_tokens_against_the_plain_model(built_lib):
+    """The two differ by f32 rounding alone.  Behind two layers of some thirty operations each, at 2^-24 apiece and grown by norms of a random model by
+    ten or so, 1e-4 of the logits' size leaves room for two orders of magnitude."""
+    model, plain = _model()
+    ids = torch.randint(0, 640, (3, 9), device="cuda")
+    states = [None, None]
+    for part in (ids[:, :6], ids[:, 6:7], ids[:, 7:8], ids[:, 8:]):
+        got, states[0] = model.advance(part, states[0])
+        want, states[1] = plain.advance(part, states[1])
+        assert got.shape == (3, part.shape[1], 640)
+        assert float((got - want).norm() / want.norm()) <= 1e-4
+    assert states[0][0] == 9
+    for (a, b) in zip(states[0][1], states[1][1]):
+        for x, y in zip(a, b):
+            assert float((x - y).norm()) <= 1e-4 * float(y.norm())
+
+
+def test_a_state_of_zeros_is_the_beginning(built_lib):
+    model, _ = _model()
+    ids = torch.randint(0, 640, (2, 5), device="cuda")
+    with torch.no_grad():
+        assert torch.equal(model.advance(ids)[0], model.advance(ids, model.init_state(2))[0]) and torch.equal(model.advance(ids)[0], model(ids)[0])
+
+
+def test_generate_takes_the_best_or_by_the_numbers_given(built_lib):
+    model, _ = _model()
+    prompt = torch.randint(0, 640, (2, 4), device="cuda")
+    answer = generate(model, prompt, 5, top=3)
+    assert answer.tokens.shape == (2, 5) and answer.top_tokens.shape == (2, 5, 3) and torch.equal(answer.tokens, answer.top_tokens[..., 0])
+    state, ids = None, prompt
+    for i in range(5):          # the same by hand
+        logits, state = model.advance(ids, state)
+        logp = torch.log_softmax(logits[:, -1].double(), -1)
+        ids = logits[:, -1].argmax(-1, keepdim=True)
+        assert torch.equal(answer.tokens[:, i], ids[:, 0])
+        assert (answer.logprobs[:, i].double() - logp.gather(1, ids)[:, 0]).abs().max() <= 1e-5
+        assert (answer.entropy[:, i].double() + (logp.exp() * logp).sum(-1)).abs().max() <= 1e-5
+    u = torch.tensor([[0.0, 0.999999], [0.4, 0.6]], device="cuda")
+    sampled = generate(model, prompt, 2, top=4, uniform=u)
+    first = torch.softmax(answer.top_logprobs[:, 0].double(), -1)
+    assert sampled.tokens[0, 0] == answer.tokens[0, 0] and sampled.tokens[0, 1] == sampled.top_tokens[0, 1, 3]
+    assert all(t in row for t, row in zip(sampled.tokens[:, 1].tolist(), sampled.top_tokens[:, 1].tolist())) and first.shape == (2, 3)
+    for bad in (dict(steps=0), dict(steps=1, top=0), dict(steps=3, uniform=u)):
+        with pytest.raises(ValueError):
+            generate(model, prompt, **bad)
+
+
+def test_score_trains_a_model_of_fp8_linears(built_lib):
+    """A policy's loss through the whole model: the gradient of its lm_head is what the log probabilities' own gradient gives."""
+    model = PratchyaCausalLM(PratchyaConfig(**SMALL), seed=1, remat=False)
+    ids = torch.randint(0, 640, (2, 8), device="cuda")
+    out = score(model, ids, top=2)
+    assert out.logprobs.shape == (2, 7) and out.top_tokens.shape == (2, 7, 2)
+    loss = -out.logprobs.mean() - 0.01 * out.entropy.mean()
+    loss.backward()
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in (model.lm_head.kernel, model.embedding, model.blocks[0].tm.w_key.kernel))
+    again = copy.deepcopy(model)
+    again.zero_grad()
+    logits, _ = again(ids)
+    logp = torch.log_softmax(logits[:, :-1], -1)
+    plain = -logp.gather(-1, ids[:, 1:, None]).mean() + 0.01 * (logp.exp() * logp).sum(-1).mean()
+    plain.backward()
+    # the cotangents of the logits agree to 2^-20 or so; an fp8 step here and there behind them is what the Linear's backward pass makes of that
+    a, b = model.lm_head.kernel.grad, again.lm_head.kernel.grad
+    assert float((a - b).norm() / b.norm()) <= 1e-2
+
+
+def test_a_model_in_4_bits_refuses_gradients(built_lib):
+    model, _ = _model()
+    with pytest.raises(RuntimeError, match="backward"):
+        model(torch.randint(0, 640, (1, 4), device="cuda"))
+
+
+def test_token_logprobs_of_one_step(built_lib):
+    model, _ = _model()
+    logits, _ = model.advance(torch.randint(0, 640, (1, 3), device="cuda"))
+    one = token_logprobs(logits[0, -1], top=640 if 640 <= 128 else 128)
+    assert one.entropy.shape == () and one.top_tokens.shape == (128,)
+
+
+def test_the_example_runs(built_lib):
+    root = Path(__file__).resolve().parent.parent
+    r = subprocess.run([sys.executable, str(root / "examples" / "answer.py"), "--layers", "1", "--vocab", "1024", "--tokens", "3", "--batch", "2"], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+    assert "log probability of the whole text" in r.stdout
