@@ -6,6 +6,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 from ._nograph import no_graph
@@ -22,35 +23,6 @@ class TokenLogprobs(NamedTuple):
     top_tokens: torch.Tensor
 
 
-class _TokenLogprobsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tokens, top):
-        logprobs, entropy, top_logprobs, top_tokens, stats = _forward(logits, tokens, top)
-        ctx.save_for_backward(logits, tokens, top_tokens, stats, entropy)
-        ctx.mark_non_differentiable(top_tokens)
-        ctx.set_materialize_grads(False)
-        return logprobs, entropy, top_logprobs, top_tokens
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_logprobs, g_entropy, g_top, _):
-        logits, tokens, top_tokens, stats, entropy = ctx.saved_tensors
-        gs = [g if g is None else g.to(torch.float32).contiguous() for g in (g_logprobs, g_entropy, g_top)]
-        if all(g is None for g in gs):
-            return None, None, None
-        dlogits = _lib.native().token_logprobs_backward(logits, tokens, top_tokens, stats, entropy, *gs)
-        if dlogits is None:
-            raise RuntimeError("token_logprobs: the backward pass takes plain CUDA tensors only")
-        return dlogits, None, None
-
-
-def _forward(logits, tokens, top):
-    out = _lib.native().token_logprobs(logits, tokens, top)
-    if out is None:
-        raise RuntimeError("token_logprobs takes plain CUDA tensors only")
-    return out
-
-
 def token_logprobs(logits, tokens=None, top: int = 0) -> TokenLogprobs:
     """Scores of f32 or bf16 `logits` [..., V], in one pass over them:
 
@@ -62,6 +34,25 @@ def token_logprobs(logits, tokens=None, top: int = 0) -> TokenLogprobs:
     -inf masks a token out.  A position where nothing is left has log probabilities of -inf, an entropy of 0 and no gradient; one with a
     NaN or +inf has NaN throughout (its top_tokens are valid indices).  Logits may be a strided view such as logits[:, :-1]: it is read in place.
     Differentiable in the logits through all three; the gradient has the logits' type."""
+    derivative = wants_derivative(logits)
+    out = _lib.native().token_logprobs(logits, tokens, top, derivative)
+    if out is None:          # what has to be converted first, or refused
+        logits, tokens, top = _checked(logits, tokens, top)
+        out = _lib.native().token_logprobs(logits, tokens, top, derivative)
+        if out is None:
+            raise RuntimeError("token_logprobs takes plain CUDA tensors only")
+    return TokenLogprobs(*out)
+
+
+def wants_derivative(x) -> bool:
+    """Whether anything can ask for a derivative of an op on x: a graph that x is in, or forward-mode differentiation or a function transform under way (which the
+    op's autograd.Function then refuses)."""
+    if torch.is_grad_enabled():
+        return (isinstance(x, torch.Tensor) and x.requires_grad) or forward_ad._current_level >= 0
+    return not no_graph()
+
+
+def _checked(logits, tokens, top):
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
         raise RuntimeError("token_logprobs needs CUDA tensors: pratchya_b200 has no CPU path")
     if logits.dtype not in (torch.float32, torch.bfloat16):
@@ -83,25 +74,4 @@ def token_logprobs(logits, tokens=None, top: int = 0) -> TokenLogprobs:
         if tokens.shape != lead and tokens.shape[-1] > MAX_TOKENS:
             raise ValueError(f"token_logprobs: {tokens.shape[-1]} tokens of a position (at most {MAX_TOKENS})")
         tokens = tokens.contiguous()
-    if no_graph() or not (torch.is_grad_enabled() and logits.requires_grad):
-        out = _lib.native().token_logprobs(logits, tokens, top)
-        if out is None:          # strides that are no two-level rows, a subclass, a mode that watches
-            out = _forward(logits.contiguous(), tokens, top)
-        return TokenLogprobs(*out[:4])
-    return TokenLogprobs(*_TokenLogprobsFn.apply(_readable(logits), tokens, top))
-
-
-def _readable(x):
-    """x itself where its rows lie at one or two strides, a contiguous copy otherwise."""
-    if x.is_contiguous():
-        return x
-    if x.shape[-1] > 1 and x.stride(-1) != 1:
-        return x.contiguous()
-    steps, expected = 0, None
-    for n, s in zip(reversed(x.shape[:-1]), reversed(x.stride()[:-1])):
-        if n == 1:
-            continue
-        if expected is None or s != expected:
-            steps += 1
-        expected = s * n
-    return x if steps <= 2 else x.contiguous()
+    return logits if _lib.native().rows_at_two_strides(logits) else logits.contiguous(), tokens, top

@@ -21,6 +21,8 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/DynamicTypes.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <initializer_list>
@@ -660,61 +662,111 @@ const at::Tensor* plain_rows(PyObject* o, StridedRows* r) {
   return &t;
 }
 
-// token_logprobs(logits, tokens or None, top) -> (logprobs or None, entropy, top_logprobs, top_tokens, stats)
-OP(token_logprobs) {
+// rows_at_two_strides(x): whether an op that takes strided rows reads x in place
+OP(rows_at_two_strides) {
   HANDLE_TH_ERRORS
-  NARGS(3);
+  NARGS(1);
   StridedRows r;
-  const at::Tensor *z = plain_rows(args[0], &r), *tokens = args[1] == Py_None ? nullptr : plain(args[1]);
-  const long long top = PyLong_AsLongLong(args[2]);
-  if (top == -1 && PyErr_Occurred()) return nullptr;
-  if (!z || watched() || (args[1] != Py_None && (!tokens || tokens->scalar_type() != at::kLong || tokens->device() != z->device())) || top < 0 || top > 0x7fffffff) return none();
-  const at::IntArrayRef lead = z->sizes().slice(0, z->dim() - 1);
-  int64_t n = 0;
-  if (tokens) {
-    const bool one = tokens->sizes() == lead;
-    if (!one && (tokens->dim() != z->dim() || tokens->sizes().slice(0, z->dim() - 1) != lead)) return none();
-    n = one ? 1 : tokens->size(-1);
-    if (n > 0x7fffffff) return none();
-  }
-  const c10::cuda::CUDAGuard guard(z->device());
-  c10::SmallVector<int64_t, 8> with_top(lead.begin(), lead.end()), with_two(lead.begin(), lead.end());
-  with_top.push_back(top); with_two.push_back(2);
-  at::Tensor logprobs, entropy = empty(lead, at::kFloat, *z), top_logprobs = empty(with_top, at::kFloat, *z), top_tokens = empty(with_top, at::kLong, *z), stats = empty(with_two, at::kFloat, *z);
-  if (tokens) logprobs = empty(tokens->sizes(), at::kFloat, *z);
-  RUN(pb_token_logprobs(z->data_ptr(), code(z->scalar_type()), r.outer, z->numel() ? r.inner : 0, r.stride_outer, r.stride_inner, z->size(-1), n ? tokens->data_ptr<int64_t>() : nullptr, (int)n,
-                        (int)top, n ? logprobs.data_ptr<float>() : nullptr, entropy.data_ptr<float>(), top ? top_logprobs.data_ptr<float>() : nullptr,
-                        top ? top_tokens.data_ptr<int64_t>() : nullptr, stats.data_ptr<float>(), current_stream(z->device())));
-  PyObject* out = wrap({entropy, entropy, top_logprobs, top_tokens, stats});
-  PyObject* first = tokens ? wrap(logprobs) : none();
-  PyTuple_SetItem(out, 0, first);
-  return out;
+  return PyBool_FromLong(THPVariable_Check(args[0]) && strided_rows(THPVariable_Unpack(args[0]), &r));
   END_HANDLE_TH_ERRORS
 }
 
-// token_logprobs_backward(logits, tokens or None, top_tokens, stats, entropy, g_logprobs or None, g_entropy or None, g_top or None) -> dlogits
-OP(token_logprobs_backward) {
-  HANDLE_TH_ERRORS
-  NARGS(8);
-  StridedRows r;
-  const at::Tensor* z = plain_rows(args[0], &r);
-  const at::Tensor* in[7];
-  for (int i = 0; i < 7; ++i) {
-    const bool may_miss = i == 0 || i >= 4;
-    if (may_miss && args[1 + i] == Py_None) { in[i] = nullptr; continue; }
-    if (!(in[i] = plain(args[1 + i]))) return none();
+struct Scores { at::Tensor logprobs, entropy, top_logprobs, top_tokens, stats; };
+// of rows that plain_rows has found, n tokens of each (as tokens' shape has them); stats only for a backward pass
+int scores_of(const at::Tensor& z, const StridedRows& r, const at::Tensor* tokens, int64_t n, int64_t top, bool backward, Scores* out) {
+  const at::IntArrayRef lead = z.sizes().slice(0, z.dim() - 1);
+  c10::SmallVector<int64_t, 8> with_top(lead.begin(), lead.end());
+  with_top.push_back(top);
+  out->entropy = empty(lead, at::kFloat, z); out->top_logprobs = empty(with_top, at::kFloat, z); out->top_tokens = empty(with_top, at::kLong, z);
+  if (backward) out->stats = empty({z.numel() / z.size(-1), 2}, at::kFloat, z);
+  if (tokens) out->logprobs = empty(tokens->sizes(), at::kFloat, z);
+  auto floats = [](const at::Tensor& t) { return t.defined() && t.numel() ? t.data_ptr<float>() : nullptr; };
+  return without_gil([&] {
+    return pb_token_logprobs(z.data_ptr(), code(z.scalar_type()), r.outer, z.numel() ? r.inner : 0, r.stride_outer, r.stride_inner, z.size(-1), n ? tokens->data_ptr<int64_t>() : nullptr, (int)n,
+                             (int)top, floats(out->logprobs), floats(out->entropy), floats(out->top_logprobs), top ? out->top_tokens.data_ptr<int64_t>() : nullptr, floats(out->stats),
+                             current_stream(z.device()));
+  });
+}
+
+// The scores with their derivative, once.  What cannot fail by its arguments is left to fail by CUDA, as a c10::Error.
+struct ScoresFunction : torch::autograd::Function<ScoresFunction> {
+  using List = torch::autograd::variable_list;
+  static List forward(torch::autograd::AutogradContext* ctx, const at::Tensor& z, const std::optional<at::Tensor>& given, int64_t n, int64_t top) {
+    const at::Tensor tokens = given.value_or(at::Tensor());
+    StridedRows r;
+    TORCH_CHECK(strided_rows(z, &r), "token_logprobs: rows at no two strides");
+    Scores s;
+    const c10::cuda::CUDAGuard guard(z.device());
+    const int status = scores_of(z, r, tokens.defined() ? &tokens : nullptr, n, top, true, &s);
+    TORCH_CHECK(status == PB_OK, "pratchya_b200 status ", status, ": ", pb_last_error());
+    if (!s.logprobs.defined()) s.logprobs = at::empty({0}, s.entropy.options());      // nobody is given it
+    ctx->save_for_backward({z, tokens, s.top_tokens, s.stats, s.entropy});
+    ctx->saved_data["n"] = n;
+    ctx->mark_non_differentiable({s.top_tokens});
+    ctx->set_materialize_grads(false);
+    return {s.logprobs, s.entropy, s.top_logprobs, s.top_tokens};
   }
-  if (!z || watched()) return none();
-  const int64_t rows = z->numel() ? r.outer * r.inner : 0, top = in[1]->size(-1), n = in[0] && rows ? in[0]->numel() / rows : 0;
-  for (int i = 2; i < 7; ++i)
-    if (in[i] && (in[i]->scalar_type() != at::kFloat || in[i]->numel() != (i == 2 ? 2 * rows : i == 3 || i == 5 ? rows : i == 4 ? n * rows : top * rows))) return none();
+  static List backward(torch::autograd::AutogradContext* ctx, List g) {
+    const List saved = ctx->get_saved_variables();
+    const at::Tensor &z = saved[0], &tokens = saved[1], &top_tokens = saved[2], &stats = saved[3], &entropy = saved[4];
+    const int64_t n = ctx->saved_data["n"].toInt(), top = top_tokens.size(-1);
+    bool again = false;      // a derivative of this one is asked for
+    for (const at::Tensor& x : g) again = again || (x.defined() && x.requires_grad());
+    again = (again || z.requires_grad()) && at::GradMode::is_enabled();
+    at::Tensor dz;
+    if (g[0].defined() || g[1].defined() || g[2].defined()) {
+      at::AutoDispatchBelowADInplaceOrView below;
+      StridedRows r;
+      TORCH_CHECK(strided_rows(z, &r), "token_logprobs: rows at no two strides");
+      const c10::cuda::CUDAGuard guard(z.device());
+      for (int i = 0; i < 3; ++i)
+        if (g[i].defined()) g[i] = g[i].to(at::kFloat).contiguous();
+      dz = empty(z.sizes(), z.scalar_type(), z);
+      auto floats = [](const at::Tensor& t) { return t.defined() && t.numel() ? t.data_ptr<float>() : nullptr; };
+      const int status = pb_token_logprobs_bwd(z.data_ptr(), code(z.scalar_type()), r.outer, z.numel() ? r.inner : 0, r.stride_outer, r.stride_inner, z.size(-1),
+                                               n && z.numel() ? tokens.data_ptr<int64_t>() : nullptr, (int)n, top && z.numel() ? top_tokens.data_ptr<int64_t>() : nullptr, (int)top, floats(stats),
+                                               floats(entropy), n ? floats(g[0]) : nullptr, floats(g[1]), floats(g[2]), dz.data_ptr(), current_stream(z.device()));
+      TORCH_CHECK(status == PB_OK, "pratchya_b200 status ", status, ": ", pb_last_error());
+    }
+    if (again && dz.defined()) {
+      dz.requires_grad_(true);      // an input of a node that fails when its own derivative is asked for
+      auto refuse = std::make_shared<torch::autograd::DelayedError>("token_logprobs has no second derivative", 1);
+      dz = (*refuse)({std::move(dz)})[0];
+    }
+    return {dz, at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+// token_logprobs(logits, tokens or None, top, derivative) -> (logprobs or None, entropy, top_logprobs, top_tokens); with derivative it is differentiable in the logits
+OP(token_logprobs) {
+  HANDLE_TH_ERRORS
+  NARGS(4);
+  StridedRows r;
+  const at::Tensor *z = plain_rows(args[0], &r), *tokens = args[1] == Py_None ? nullptr : plain(args[1]);
+  const long long top = integer(args[2]);
+  if (!z || watched() || (args[1] != Py_None && (!tokens || tokens->scalar_type() != at::kLong || tokens->device() != z->device())) || !PyLong_Check(args[2]) || top < 0 || top > 128 ||
+      z->size(-1) == 0 || top > z->size(-1))
+    return none();
+  int64_t n = 0;
+  if (tokens) {
+    const at::IntArrayRef lead = z->sizes().slice(0, z->dim() - 1);
+    const bool one = tokens->sizes() == lead;
+    if (!one && (tokens->dim() != z->dim() || tokens->sizes().slice(0, z->dim() - 1) != lead)) return none();
+    n = one ? 1 : tokens->size(-1);
+    if (n > 128) return none();
+  }
   const c10::cuda::CUDAGuard guard(z->device());
-  at::Tensor dz = empty(z->sizes(), z->scalar_type(), *z);
-  auto data = [&](int i) { return in[i] && in[i]->numel() ? in[i]->data_ptr<float>() : nullptr; };
-  RUN(pb_token_logprobs_bwd(z->data_ptr(), code(z->scalar_type()), r.outer, z->numel() ? r.inner : 0, r.stride_outer, r.stride_inner, z->size(-1),
-                            n ? in[0]->data_ptr<int64_t>() : nullptr, (int)n, top ? in[1]->data_ptr<int64_t>() : nullptr, (int)top, data(2), data(3), data(4), data(5), data(6), dz.data_ptr(),
-                            current_stream(z->device())));
-  return wrap(dz);
+  Scores s;
+  if (PyObject_IsTrue(args[3]) == 1) {
+    const auto out = ScoresFunction::apply(*z, tokens ? std::optional<at::Tensor>(*tokens) : std::nullopt, n, top);
+    s = {out[0], out[1], out[2], out[3], {}};
+  } else if (const int status = scores_of(*z, r, tokens, n, top, false, &s)) {
+    return raise_status(status);
+  }
+  PyObject* out = wrap({s.entropy, s.entropy, s.top_logprobs, s.top_tokens});
+  PyObject* first = tokens ? wrap(s.logprobs) : none();
+  PyTuple_SetItem(out, 0, first);
+  return out;
   END_HANDLE_TH_ERRORS
 }
 
@@ -839,7 +891,7 @@ PyMethodDef methods[] = {
     METHOD("quantize", quantize), METHOD("quantize_transposed", quantize_transposed), METHOD("dequantize", dequantize), METHOD("dequantize_bwd", dequantize_bwd),
     METHOD("fake_quantize", fake_quantize), METHOD("transpose_bytes", transpose_bytes), METHOD("gemm", gemm), METHOD("linear_step", linear_step), METHOD("linear", linear), METHOD("linear_takes", linear_takes),
     METHOD("linear_forward", linear_forward), METHOD("linear_backward", linear_backward),
-    METHOD("token_logprobs", token_logprobs), METHOD("token_logprobs_backward", token_logprobs_backward), METHOD("quantize_int4", quantize_int4),
+    METHOD("token_logprobs", token_logprobs), METHOD("rows_at_two_strides", rows_at_two_strides), METHOD("quantize_int4", quantize_int4),
     METHOD("dequantize_int4", dequantize_int4), METHOD("int4_product", int4_product),
     METHOD("dense_dot", dense_dot), METHOD("empty", empty_on), METHOD("empties", empties),
     ENTRY(pb_quantize_dual), ENTRY(pb_dequantize_bwd_quantize_dual), ENTRY(pb_relu2_requantize), ENTRY(pb_quantize_transposed_workspace_size),

@@ -278,6 +278,24 @@ def test_gradient_of_a_shared_row(built_lib):
     assert (z.grad[0].double() - want).abs().max() <= 5 * 2.0 ** -20
 
 
+def test_gradient_without_tokens_and_without_use(built_lib):
+    z, _ = _case(3, 1001, "f32", 31)
+    z.requires_grad_(True)
+    out = token_logprobs(z)
+    assert out.logprobs is None and out.top_logprobs.shape == (3, 0)
+    out.entropy.sum().backward()
+    z64 = z.detach().double().requires_grad_(True)
+    logp = torch.log_softmax(z64, -1)
+    (-(logp.exp() * logp).sum()).backward()
+    assert (z.grad.double() - z64.grad).abs().max() <= 2.0 ** -19
+    with torch.no_grad():
+        assert not token_logprobs(z).entropy.requires_grad
+    assert not token_logprobs(z, None, 3).top_tokens.requires_grad
+    best = token_logprobs(z, None, 2)
+    (g,) = torch.autograd.grad(best.top_logprobs[:, 0].sum(), z)
+    assert (g.sum(-1).abs() <= 2.0 ** -18).all() and (g.gather(1, best.top_tokens[:, :1]) > 0).all()
+
+
 def test_gradient_against_differences(built_lib):
     """A step h along a direction v of unit size: (f(z + h v) - f(z - h v)) / 2h is v . grad f up to h^2 / 6 of a third derivative and 2^-22 of |f| / h.  f is a sum
     of log probabilities and entropies of three rows; a third derivative of either along a unit vector is below 8 (1 + entropy)."""
