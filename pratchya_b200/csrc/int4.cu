@@ -13,6 +13,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstring>
 #include <type_traits>
 
@@ -650,7 +651,13 @@ template <typename TX, int DIGITS, int MT, int PER_GROUP, bool ZERO> int launch_
   p.by_per_cta = FastDiv(p.per_cta);
   p.tiles_each = p.tiles / clusters;
   p.tiles_over = p.tiles % clusters;
-  PB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxShared));
+  static std::atomic<uint64_t> allowed{0};      // devices on which this kernel may have so much
+  int device = 0;
+  PB_CUDA_TRY(cudaGetDevice(&device));
+  if (device >= 64 || !(allowed.load(std::memory_order_relaxed) >> device & 1)) {
+    PB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxShared));
+    if (device < 64) allowed.fetch_or(1ull << device, std::memory_order_relaxed);
+  }
   const uint32_t passes = (p.rows + per_pass - 1) / per_pass;
   if (passes > 65535) return fail(PB_ERR_UNSUPPORTED, "pb_int4_product: %u rows", p.rows);
   cudaLaunchConfig_t config{};

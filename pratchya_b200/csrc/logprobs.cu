@@ -217,7 +217,12 @@ __device__ void best_of_slice(Shared<THREADS>& sh, const Slice<T>& sl, const Bes
   });
   __syncthreads();
   while (true) {      // once, but for rows whose best logits crowd into a few threads: the bound rises until what reaches it has room
-    const uint64_t bound = sh.bound;
+    uint64_t bound = sh.bound;
+    if (bound >> 32 == order_of(-INFINITY)) {      // -inf is wanted only where fewer than k are more: those that are lie before 2 k - 1 others
+      uint32_t last = at0 - sl.head + 2 * k - 2;
+      if (last >= at0) last += kVec - 1 - (last - at0) % kVec;
+      if (last < sl.tail_at) bound = max(bound, key_of(-INFINITY, last));
+    }
     const float bound_z = value_of((uint32_t)(bound >> 32));
     auto offer = [&](float z, uint32_t index) {
       if (z < bound_z) return;      // a NaN is not: it ranks with -inf

@@ -13,9 +13,11 @@
 
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/TensorSubclassLikeUtils.h>
+#include <ATen/EmptyTensor.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -168,6 +170,10 @@ int format(const at::Tensor& t) { return t.scalar_type() == kE4M3 ? PB_E4M3 : PB
 bool dense(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16; }
 int code(at::ScalarType t) { return t == at::kBFloat16 ? PB_BF16 : PB_F32; }
 at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, const at::Tensor& like) { return at::empty(shape, at::TensorOptions().device(like.device()).dtype(type)); }
+// the same from the allocator itself, on the current device, for calls that no mode watches: half of what at::empty costs a call of a few microseconds
+at::Tensor fresh(at::IntArrayRef shape, at::ScalarType type) {
+  return at::detail::empty_generic(shape, c10::cuda::CUDACachingAllocator::get(), c10::DispatchKeySet(c10::DispatchKey::CUDA), type, std::nullopt);
+}
 at::Tensor scratch(size_t bytes, const at::Tensor& like) { return empty({(int64_t)bytes}, at::kByte, like); }
 
 struct Grid {
@@ -677,9 +683,9 @@ int scores_of(const at::Tensor& z, const StridedRows& r, const at::Tensor* token
   const at::IntArrayRef lead = z.sizes().slice(0, z.dim() - 1);
   c10::SmallVector<int64_t, 8> with_top(lead.begin(), lead.end());
   with_top.push_back(top);
-  out->entropy = empty(lead, at::kFloat, z); out->top_logprobs = empty(with_top, at::kFloat, z); out->top_tokens = empty(with_top, at::kLong, z);
-  if (backward) out->stats = empty({z.numel() / z.size(-1), 2}, at::kFloat, z);
-  if (tokens) out->logprobs = empty(tokens->sizes(), at::kFloat, z);
+  out->entropy = fresh(lead, at::kFloat); out->top_logprobs = fresh(with_top, at::kFloat); out->top_tokens = fresh(with_top, at::kLong);
+  if (backward) out->stats = fresh({z.numel() / z.size(-1), 2}, at::kFloat);
+  if (tokens) out->logprobs = fresh(tokens->sizes(), at::kFloat);
   auto floats = [](const at::Tensor& t) { return t.defined() && t.numel() ? t.data_ptr<float>() : nullptr; };
   return without_gil([&] {
     return pb_token_logprobs(z.data_ptr(), code(z.scalar_type()), r.outer, z.numel() ? r.inner : 0, r.stride_outer, r.stride_inner, z.size(-1), n ? tokens->data_ptr<int64_t>() : nullptr, (int)n,
@@ -721,7 +727,7 @@ struct ScoresFunction : torch::autograd::Function<ScoresFunction> {
       const c10::cuda::CUDAGuard guard(z.device());
       for (int i = 0; i < 3; ++i)
         if (g[i].defined()) g[i] = g[i].to(at::kFloat).contiguous();
-      dz = empty(z.sizes(), z.scalar_type(), z);
+      dz = fresh(z.sizes(), z.scalar_type());
       auto floats = [](const at::Tensor& t) { return t.defined() && t.numel() ? t.data_ptr<float>() : nullptr; };
       const int status = pb_token_logprobs_bwd(z.data_ptr(), code(z.scalar_type()), r.outer, z.numel() ? r.inner : 0, r.stride_outer, r.stride_inner, z.size(-1),
                                                n && z.numel() ? tokens.data_ptr<int64_t>() : nullptr, (int)n, top && z.numel() ? top_tokens.data_ptr<int64_t>() : nullptr, (int)top, floats(stats),
@@ -781,8 +787,8 @@ OP(quantize_int4) {
   if (!w || watched() || !dense(w->scalar_type()) || w->dim() != 2 || w->numel() == 0 || (group != 32 && group != 64 && group != 128)) return none();
   const c10::cuda::CUDAGuard guard(w->device());
   const int64_t depth = w->size(0), cols = w->size(1), a = (cols + 15) / 16, b = (depth + 127) / 128;
-  at::Tensor q = empty({a, b, 1024}, at::kByte, *w), scale = empty({a, b, 16, 128 / group}, at::kBFloat16, *w), zero;
-  if (zeros) zero = empty({a, b, 16, 128 / group}, at::kByte, *w);
+  at::Tensor q = fresh({a, b, 1024}, at::kByte), scale = fresh({a, b, 16, 128 / group}, at::kBFloat16), zero;
+  if (zeros) zero = fresh({a, b, 16, 128 / group}, at::kByte);
   RUN(pb_quantize_int4(w->data_ptr(), code(w->scalar_type()), depth, cols, group, (uint8_t*)q.data_ptr(), scale.data_ptr(), zeros ? (uint8_t*)zero.data_ptr() : nullptr,
                        current_stream(w->device())));
   PyObject* out = wrap({q, scale, scale});
@@ -821,7 +827,7 @@ OP(dequantize_int4) {
   const at::ScalarType type = reinterpret_cast<THPDtype*>(args[5])->scalar_type;
   if (!dense(type)) return none();
   const c10::cuda::CUDAGuard guard(w.q->device());
-  at::Tensor out = empty({depth, cols}, type, *w.q);
+  at::Tensor out = fresh({depth, cols}, type);
   RUN(pb_dequantize_int4((const uint8_t*)w.q->data_ptr(), w.scale->data_ptr(), w.zeros(), depth, cols, w.group, out.data_ptr(), code(type), current_stream(w.q->device())));
   return wrap(out);
   END_HANDLE_TH_ERRORS
@@ -841,7 +847,7 @@ OP(int4_product) {
   const c10::cuda::CUDAGuard guard(x->device());
   c10::SmallVector<int64_t, 8> shape(x->sizes().begin(), x->sizes().end());
   shape.back() = cols;
-  at::Tensor out = empty(shape, type, *x);
+  at::Tensor out = fresh(shape, type);
   RUN(pb_int4_product(x->data_ptr(), code(x->scalar_type()), x->numel() ? r.inner : 0, x->size(-1), r.stride_inner, (const uint8_t*)w.q->data_ptr(), w.scale->data_ptr(), w.zeros(), w.group, cols,
                       out.data_ptr(), code(type), current_stream(x->device())));
   return wrap(out);
