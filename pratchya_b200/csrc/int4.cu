@@ -335,11 +335,13 @@ __global__ void __launch_bounds__(kThreads, DIGITS == 0 && MT == 4 ? 1 : 2) int4
     ++unit;
     if (++asked == kbn) { asked = 0; unit += p.kblocks - kbn; }
   };
+  auto load_ahead = [&] {
 #pragma unroll
-  for (int i = 0; i < kAhead; ++i)
-    if (run > (uint32_t)i) load(ahead[i]);
+    for (int i = 0; i < kAhead; ++i)
+      if (run > (uint32_t)i) load(ahead[i]);
+  };
 
-  // this CTA's part of x
+  // This CTA's part of x.  It is asked for before the weight: behind four blocks of every warp's it would come 3000 cycles later.
   const TX* x = static_cast<const TX*>(p.x) + (int64_t)row0 * p.stride + kb0 * 128;
   const uint32_t depth = p.depth - min(p.depth, kb0 * 128);
   if constexpr (DIGITS != 0) {      // a warp takes a row's block at a time, a lane four values of it: two pairs of the eight that a word of codes meets
@@ -347,8 +349,8 @@ __global__ void __launch_bounds__(kThreads, DIGITS == 0 && MT == 4 ? 1 : 2) int4
     const bool pairs = ((reinterpret_cast<uintptr_t>(x) | (uint64_t)p.stride * sizeof(TX)) & (2 * sizeof(TX) - 1)) == 0;
     constexpr int kBatch = MT == 1 ? 2 : 4;      // row blocks on the way; the last one again where there is none
     const uint32_t all = rows * p.per_cta;
-    for (uint32_t i0 = warp; i0 < all; i0 += kWarps * kBatch) {
-      float batch[kBatch][4];
+    float batch[kBatch][4];
+    auto load_batch = [&](uint32_t i0) {
 #pragma unroll
       for (int q = 0; q < kBatch; ++q) {
         const uint32_t i = min(i0 + q * kWarps, all - 1), m = p.by_per_cta.div(i), k = (i - m * p.per_cta) * 128 + at;
@@ -371,41 +373,46 @@ __global__ void __launch_bounds__(kThreads, DIGITS == 0 && MT == 4 ? 1 : 2) int4
           }
         }
       }
+    };
+    load_batch(warp);
+    load_ahead();
+    for (uint32_t i0 = warp; i0 < all; i0 += kWarps * kBatch) {
+      if (i0 != warp) load_batch(i0);
 #pragma unroll
       for (int q = 0; q < kBatch; ++q) {
-      const uint32_t i = min(i0 + q * kWarps, all - 1), m = p.by_per_cta.div(i), b = i - m * p.per_cta;
-      float (&v)[4] = batch[q];
-      uint32_t size = 0;
+        const uint32_t i = min(i0 + q * kWarps, all - 1), m = p.by_per_cta.div(i), b = i - m * p.per_cta;
+        float (&v)[4] = batch[q];
+        uint32_t size = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) size = max(size, __float_as_uint(v[e]) & 0x7fffffffu);
-      const Whole<kParts> whole(__reduce_max_sync(0xffffffffu, size));
-      uint32_t d[4];
+        for (int e = 0; e < 4; ++e) size = max(size, __float_as_uint(v[e]) & 0x7fffffffu);
+        const Whole<kParts> whole(__reduce_max_sync(0xffffffffu, size));
+        uint32_t d[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) d[e] = whole.digits(v[e]);
-      // the j-th digits of k = 0, 4, 1, 5 of the word or of 2, 6, 3, 7: as a byte's lower and upper nibbles have the codes
-      uint32_t part[4];
-      const uint32_t l02 = __byte_perm(d[0], d[2], 0x5140), l13 = __byte_perm(d[1], d[3], 0x5140), u02 = __byte_perm(d[0], d[2], 0x7362), u13 = __byte_perm(d[1], d[3], 0x7362);
-      part[0] = __byte_perm(l02, l13, 0x5410); part[1] = __byte_perm(l02, l13, 0x7632); part[2] = __byte_perm(u02, u13, 0x5410); part[3] = __byte_perm(u02, u13, 0x7632);
-      constexpr int kLanes = 32 / PER_GROUP;
-      uint32_t two[2] = {0, 0};      // a group's sums of two digits each, of 16 bits with their signs
-      if constexpr (ZERO) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) two[j] = (uint32_t)__dp4a((int)part[2 * j], 0x01010101, 0) + ((uint32_t)__dp4a((int)part[2 * j + 1], 0x01010101, 0) << 16);
-#pragma unroll
-        for (int o = 1; o < kLanes; o <<= 1)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) two[j] += __shfl_xor_sync(0xffffffffu, two[j], o);
-      }
-#pragma unroll
-      for (int j = 0; j < kParts; ++j) {
-        const uint32_t column = m * kParts + kParts - 1 - j;
-        *reinterpret_cast<uint32_t*>(xs + column * pitch + b * 128 + (word % 4) * 32 + (word / 4) * 8 + (lane & 1) * 4) = part[j];
+        for (int e = 0; e < 4; ++e) d[e] = whole.digits(v[e]);
+        // the j-th digits of k = 0, 4, 1, 5 of the word or of 2, 6, 3, 7: as a byte's lower and upper nibbles have the codes
+        uint32_t part[4];
+        const uint32_t l02 = __byte_perm(d[0], d[2], 0x5140), l13 = __byte_perm(d[1], d[3], 0x5140), u02 = __byte_perm(d[0], d[2], 0x7362), u13 = __byte_perm(d[1], d[3], 0x7362);
+        part[0] = __byte_perm(l02, l13, 0x5410); part[1] = __byte_perm(l02, l13, 0x7632); part[2] = __byte_perm(u02, u13, 0x5410); part[3] = __byte_perm(u02, u13, 0x7632);
+        constexpr int kLanes = 32 / PER_GROUP;
+        uint32_t two[2] = {0, 0};      // a group's sums of two digits each, of 16 bits with their signs
         if constexpr (ZERO) {
-          const int lower = (int)(int16_t)two[j / 2], sum = j % 2 ? (int)(two[j / 2] - (uint32_t)lower) >> 16 : lower;
-          if (lane % kLanes == 0) x_sums[(b * PER_GROUP + lane / kLanes) * (8 * MT) + column] = 16 * sum;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) two[j] = (uint32_t)__dp4a((int)part[2 * j], 0x01010101, 0) + ((uint32_t)__dp4a((int)part[2 * j + 1], 0x01010101, 0) << 16);
+#pragma unroll
+          for (int o = 1; o < kLanes; o <<= 1)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) two[j] += __shfl_xor_sync(0xffffffffu, two[j], o);
         }
-        if (lane == 0) x_scales[b * (8 * MT) + column] = whole.scale * ((float)(1u << 8 * j) * 0.0625f);      // the codes are sixteen times theirs
-      }
+#pragma unroll
+        for (int j = 0; j < kParts; ++j) {
+          const uint32_t column = m * kParts + kParts - 1 - j;
+          *reinterpret_cast<uint32_t*>(xs + column * pitch + b * 128 + (word % 4) * 32 + (word / 4) * 8 + (lane & 1) * 4) = part[j];
+          if constexpr (ZERO) {
+            const int lower = (int)(int16_t)two[j / 2], sum = j % 2 ? (int)(two[j / 2] - (uint32_t)lower) >> 16 : lower;
+            if (lane % kLanes == 0) x_sums[(b * PER_GROUP + lane / kLanes) * (8 * MT) + column] = 16 * sum;
+          }
+          if (lane == 0) x_scales[b * (8 * MT) + column] = whole.scale * ((float)(1u << 8 * j) * 0.0625f);      // the codes are sixteen times theirs
+        }
       }
     }
   } else {      // bf16, eight values at a time
@@ -427,6 +434,7 @@ __global__ void __launch_bounds__(kThreads, DIGITS == 0 && MT == 4 ? 1 : 2) int4
         }
       }
     }
+    load_ahead();
     asm volatile("cp.async.wait_all;" ::: "memory");
   }
   __syncthreads();
@@ -576,11 +584,14 @@ __global__ void __launch_bounds__(kThreads, DIGITS == 0 && MT == 4 ? 1 : 2) int4
         write(j, m, n, y);
       }
     } else {
-      for (uint32_t i = tid; i < count * sum_floats; i += kThreads) {
-        const uint32_t j = i / sum_floats;
-        float of[1];
-        over_warps(j, i - j * sum_floats, of);
-        joined[i] = of[0];
+      const uint32_t fours = (columns + 3) / 4 * 16;      // of a tile, four columns' sums at a time
+      for (uint32_t i = tid; i < count * fours; i += kThreads) {
+        const uint32_t j = i / fours, column = (i - j * fours) / 16 * 4, at = column * 16 + i % 16;
+        float of[4];
+        over_warps(j, at, of);
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e)
+          if (column + e < columns) joined[j * sum_floats + at + e * 16] = of[e];
       }
       cluster.sync();
       for (uint32_t i = rank * kThreads + tid; i < count * outputs; i += ctas * kThreads) {      // each rank finishes a part
@@ -603,9 +614,7 @@ __global__ void __launch_bounds__(kThreads, DIGITS == 0 && MT == 4 ? 1 : 2) int4
     if (next < last) {
       start_chunk(next, min(p.chunk, last - next));
       asked = kb;
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i)
-        if (run > (uint32_t)i) load(ahead[i]);
+      load_ahead();
     }
   }
 }
@@ -749,6 +758,7 @@ extern "C" int pb_int4_product(const void* x, int x_dtype, int64_t rows, int64_t
   if ((reinterpret_cast<uintptr_t>(q) & 15) || ((reinterpret_cast<uintptr_t>(scale) | reinterpret_cast<uintptr_t>(zero)) & 3) ||
       (reinterpret_cast<uintptr_t>(x) % (x_dtype == PB_F32 ? 4 : 2)) || (reinterpret_cast<uintptr_t>(out) % (out_dtype == PB_F32 ? 4 : 2)))
     return fail(PB_ERR_MISALIGNED, "pb_int4_product: q 16, scale and zero 4 bytes, x and out their types");
+  if ((uint64_t)((cols + 15) / 16) * ((depth + 127) / 128) > 0x7fffffffull) return fail(PB_ERR_BAD_SHAPE, "pb_int4_product: depth=%lld cols=%lld", (long long)depth, (long long)cols);
   Product p{x, stride, q, static_cast<const __nv_bfloat16*>(scale), zero, out, (uint32_t)rows, (uint32_t)depth, (uint32_t)cols, (uint32_t)((depth + 127) / 128),
             (uint32_t)((cols + 15) / 16), 0, 0, 0, FastDiv(), 0, 0, out_dtype == PB_F32};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
