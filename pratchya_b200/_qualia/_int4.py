@@ -62,9 +62,10 @@ def dequantize_int4_impl(q, scale, zero, shape, dtype=torch.float32):
 
 
 def int4_matmul_impl(x, q, scale, zero, cols: int, dtype=None):
-    """x [..., K] times a weight of [K, cols] in its parts, in x's type or `dtype`: f32 products and sums of x as it is.  Made for few rows: the
-    weight is read once for every 32 of a bf16 x and every ten of an f32 one.  Not differentiable: an x that asks for a
-    gradient is refused."""
+    """x [..., K] times a weight of [K, cols] in its parts, in x's type or `dtype`.  Sums are f32; x keeps its bits but for what is far below its
+    neighbours (of 128 the largest has 2^30 steps above zero where x is f32, 2^22 at least where it is bf16, and the others the same steps).  A row of x with an
+    infinity or a NaN has no finite products.  Made for few rows: the weight is read once for every 32 of a bf16 x and every eight of an f32 one.
+    Not differentiable: an x that asks for a gradient is refused."""
     if isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("int4_matmul_impl has no backward pass: call it under torch.no_grad(), or with x.detach()")
     out = _lib.native().int4_product(x, q, scale, zero, cols, dtype)

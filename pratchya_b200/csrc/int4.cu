@@ -26,7 +26,6 @@ namespace cg = cooperative_groups;
 constexpr int kQuantThreads = 256, kQuantCols = 64;      // 128 x 64 weights a CTA
 constexpr int kHalf = 160;             // words of eight columns in shared memory, 20 a column; a word's place among four goes by the eight: a warp's columns meet no bank twice
 
-__device__ __forceinline__ uint32_t code_at(uint32_t word, int i) { return word >> (4 * (i / 2 + 4 * (i % 2))) & 15u; }
 __device__ __forceinline__ float max_nan(float a, float b) {
   float y;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
@@ -47,8 +46,8 @@ constexpr uint32_t kRoundBits = 0x4b400000u;
 // otherwise scale = bf16(max|w| / 7), u = rint(w / scale) + 8: the scale is 2^-9 of itself too small at most, and u within 1..15 by itself.
 // A group of nothing but zeros has scale 0.  The scale is rounded before the codes are taken: they are the nearest ones for the scale that is stored.
 // A group that holds a NaN or an infinity has a scale that is no finite number.
-// A thread has COLS neighbouring columns (two where one load brings two bf16) and 32 / COLS values of k of each.  Bound by HBM: f32 [2048, 8192] in
-// 13.7 us (5.5 TB/s); with a division per weight, __fdiv_rn, it was bound by instructions (22 us).
+// A thread has COLS neighbouring columns (two where one load brings two bf16) and 32 / COLS values of k of each.  f32 [2048, 8192] in 16.1 us (floor 11.6), [2048, 65536]
+// in 105 (92, HBM); bf16 [2048, 8192] in 15.3.  With a division per weight, __fdiv_rn, and words staged without regard to banks 22.
 template <typename T, bool ZERO, int COLS>
 __global__ void __launch_bounds__(kQuantThreads) quantize_int4_kernel(const T* __restrict__ w, int64_t depth, int64_t cols, int per_group, uint32_t kblocks,
                                                                       uint32_t* __restrict__ q, __nv_bfloat16* __restrict__ scale, uint8_t* __restrict__ zero) {
@@ -60,16 +59,17 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_int4_kernel(const T* _
   const uint32_t kb = blockIdx.x;
   const int64_t n0 = (int64_t)blockIdx.y * kQuantCols + pair * COLS, k0 = (int64_t)kb * 128 + run * kRows;
   float v[COLS][kRows], low[COLS], high[COLS];
+  const T* from = w + k0 * cols + n0;
+  const int rows = n0 >= cols ? 0 : (int)min((int64_t)kRows, depth - k0);
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
-    const T* from = w + (k0 + i) * cols + n0;
-    const bool in = k0 + i < depth;
+    const T* at = from + i * cols;
     if constexpr (COLS == 2) {      // of an even number of columns, two bf16 at four bytes
-      const uint32_t two = in && n0 < cols ? __ldg(reinterpret_cast<const uint32_t*>(from)) : 0u;
+      const uint32_t two = i < rows ? __ldg(reinterpret_cast<const uint32_t*>(at)) : 0u;
       v[0][i] = __uint_as_float(two << 16);
       v[1][i] = __uint_as_float(two & 0xffff0000u);
     } else {
-      v[0][i] = in && n0 < cols ? Elem<T>::to_f32(from[0]) : 0.0f;
+      v[0][i] = i < rows ? Elem<T>::to_f32(*at) : 0.0f;
     }
   }
 #pragma unroll
@@ -140,7 +140,8 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_int4_kernel(const T* _
   }
 }
 
-// A thread has COLS neighbouring columns (two of bf16, which one store takes) and 32 / COLS values of k of each.
+// A thread has COLS neighbouring columns (two of bf16, which one store takes) and 32 / COLS values of k of each.  f32 [2048, 8192] in 12.6 us, [2048, 65536] in 101
+// (floor 92); bf16 [2048, 8192] in 9.7.  With the words straight from global memory, 64 bytes apart, bf16 took 13.8; with every code shifted to the bottom of its word 11.1.
 template <typename T, int COLS>
 __global__ void __launch_bounds__(kQuantThreads) dequantize_int4_kernel(const uint32_t* __restrict__ q, const __nv_bfloat16* __restrict__ scale, const uint8_t* __restrict__ zero,
                                                                         int64_t depth, int64_t cols, int per_group, uint32_t kblocks, T* __restrict__ w) {
@@ -155,7 +156,7 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_int4_kernel(const ui
     for (int c = 0; c < COLS; ++c) {
       const int64_t i = (((n / 16 * kblocks + kb) * 16) + (n + c) % 16) * per_group + quarter * per_group / 4;
       s[c] = __bfloat162float(scale[i]);
-      z[c] = kRound + (zero ? (float)zero[i] : 8.0f);
+      z[c] = zero ? (float)zero[i] : 8.0f;
     }
   const int64_t a = (int64_t)blockIdx.y * 4 + threadIdx.x / 64;
   const uint32_t eight = threadIdx.x / 32;
@@ -167,26 +168,47 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_int4_kernel(const ui
   for (int c = 0; c < COLS; ++c)
 #pragma unroll
     for (int t = 0; t < kWords; ++t) word[c][t] = staged[staged_at(pair * COLS + c, (run * kWords + t) % 4, quarter)];
+  // A code at nibble p of a word (or, p > 4, of its upper half) is 16^p times itself there: it is taken as that, and the scale is so much smaller.
+  float scales[COLS][5], zeros[COLS][5];
+#pragma unroll
+  for (int c = 0; c < COLS; ++c)
+#pragma unroll
+    for (int p = 0; p < 5; ++p) {
+      scales[c][p] = s[c] * (1.0f / (1 << 4 * p));
+      zeros[c][p] = kRound + z[c] * (1 << 4 * p);
+    }
   T* to = w + k0 * cols + n;
-  const bool whole = k0 + kRows <= depth;
+  const uint32_t pitch = (uint32_t)cols;      // columns are fewer than 2^22 (the grid's second dimension): offsets within a run of k take 32 bits, one operation
+  const int rows = (int)min((int64_t)kRows, depth - k0);
 #pragma unroll
   for (int t = 0; t < kWords; ++t)
 #pragma unroll
-    for (int j = 0; j < 8; ++j, to += cols) {
-      if (!whole && k0 + t * 8 + j >= depth) continue;
+    for (int j = 0; j < 8; ++j) {
+      const int nibble = j / 2 + 4 * (j % 2), p = nibble > 4 ? nibble - 4 : nibble;
       float v[COLS];
 #pragma unroll
-      for (int c = 0; c < COLS; ++c) v[c] = s[c] * (__uint_as_float(kRoundBits | code_at(word[c][t], j)) - z[c]);
-      if constexpr (COLS == 2) *reinterpret_cast<uint32_t*>(to) = pack_bf16x2(v[0], v[1]);
-      else *to = Elem<T>::from_f32(v[0]);
+      for (int c = 0; c < COLS; ++c) v[c] = scales[c][p] * (__uint_as_float(((nibble > 4 ? word[c][t] >> 16 : word[c][t]) & (15u << 4 * p)) | kRoundBits) - zeros[c][p]);
+      if (t * 8 + j < rows) {
+        T* at = to + (uint32_t)(t * 8 + j) * pitch;
+        if constexpr (COLS == 2) *reinterpret_cast<uint32_t*>(at) = pack_bf16x2(v[0], v[1]);
+        else *at = Elem<T>::from_f32(v[0]);
+      }
     }
 }
 
 // ---- products of few rows ------------------------------------------------------------------------------------------------
-// A warp's matrix instruction m16n8k16 takes 16 columns n of the weight as its rows and 8 rows of x as its columns: the weight, of which there is much,
-// fills it, and x, of which there is little, is what may be padded.  Codes become bf16 by their bits (0x4300 | u is 128 + u) and are taken less
-// 128 + zero, both exact; sums over a group are f32, and meet the group's scale in f32.  An f32 x goes as three bf16 terms, 8 bits of its 24 each, in
-// three columns of the instruction whose sums meet at the end: for one or two rows they cost nothing.
+// A warp's matrix instruction takes 16 columns n of the weight as its rows and 8 rows of x as its columns: the weight, of which there is much, fills it, and
+// x, of which there is little, is what may be padded.  (tcgen05's tiles of 64 rows and more would want codes unpacked into shared memory for one to thirty-two
+// columns; the tensor core is busy a fifth of the time here.)  Two forms of x:
+//  - whole numbers: every block of 128 values of a row gets a scale, a power of two, and its values become whole numbers of three (bf16) or four (f32) digits of
+//    eight bits with a sign, each digit a column of its own.  Codes become bytes of 16 (u - 8) by one operation on four of them, products and sums of a group
+//    are exact in int32 (m16n8k32), and meet the scales in f32.  24 operations unpack a kilobyte of codes.
+//  - bf16 as it is (m16n8k16): codes become bf16 by their bits (0x4300 | u is 128 + u) less 128 + zero, both exact, 88 operations a kilobyte; a row of x is one column.
+// Sums over a group meet the group's scale in f32, groups and warps add in f32.
+// Floor: the weight's bytes from HBM, 10.6 us for 2048 x 65536.  On one B200, us:
+//   one row, f32: 2048 x 65536 15.6 (68 %), 2048 x 8192 4.2, 2048 x 2048 3.0, 2048 x 128 2.9 (a launch, x's way to the digits and one barrier)
+//   bf16 rows x depth x columns: 8 x 2048 x 8192 5.8, 32 x 8192 x 2048 11.0, 32 x 2048 x 65536 58 (32 columns keep the tensor core's old instructions, 8 cycles each, busy)
+// What a row of 65536 columns takes beside the stream of codes (9.4 us at 7.3 TB/s): 2.7 until x is in digits, 0.9 for the sums of the warps, a launch.
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kPad = 32;               // values behind a row of x in shared memory: neighbouring rows' 64 bytes then lie in other banks
 constexpr int kPadDigits = 16;         // the same for digits: neighbouring rows' sixteen bytes of four lanes in turn
@@ -226,7 +248,7 @@ constexpr int kWhole = 0x4b400000;
 constexpr float kWholeValue = 12582912.0f;
 
 // The whole numbers that a block of 128 values of x becomes: x = scale * t in DIGITS digits of eight bits with a sign each.  The scale is a power of two, and
-// |t| < 2^22 or 2^30: a bf16 within 2^-14 of its block's largest and an f32 within 2^-7 are exact, smaller ones to 2^-22 and 2^-30 of the largest.
+// |t| < 2^22 or 2^30: a bf16 within 2^-14 of its block's largest and an f32 within 2^-6 are exact, smaller ones to 2^-22 and 2^-30 of the largest.
 template <int DIGITS> struct Whole {
   static constexpr uint32_t kBits = 8 * DIGITS - 3;
   float up, scale;
@@ -290,7 +312,8 @@ template <int PER_GROUP, bool ZERO> struct Block {
 // DIGITS: 0 takes a bf16 x as it is, 3 and 4 take x as whole numbers; MT: sets of 8 columns of the instruction.  The CTAs of a cluster split k; a cluster has a
 // run of the weight's tiles, `chunk` of them at a time.  A CTA's blocks of a chunk, tile after tile, are cut evenly over its eight warps wherever the cut
 // falls: a warp reads one run of memory, blocks ahead of the one that it computes, and leaves its sum of each tile (or part of one) in shared
-// memory.  They meet behind one barrier a chunk.
+// memory.  They meet behind one barrier a chunk.  (A tile per warp leaves SMs with four CTAs beside others with three; a tile split over a CTA's warps has a
+// barrier for every 16 columns: 2048 x 65536 20.1 and 23.6 us where this took 19.8.  Sixteen warps a CTA repeat more of what every warp does once: 20.7.)
 template <typename TX, int DIGITS, int MT, int PER_GROUP, bool ZERO>
 __global__ void __launch_bounds__(kThreads, DIGITS == 0 && MT == 4 ? 1 : 2) int4_product_kernel(const Product p) {
   grid_wait();

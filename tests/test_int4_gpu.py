@@ -96,6 +96,22 @@ def test_quantizer_of_groups_that_are_no_numbers(built_lib):
             assert torch.equal(back[~bad], clean[~bad])
 
 
+@pytest.mark.parametrize("zero_points", [False, True])
+def test_every_scale(built_lib, zero_points):
+    """scale * (code - zero) to the bit for all 65536 bit patterns of a scale, the smallest and those that are no numbers among them."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+    depth, cols = 128, 65536
+    q = torch.randint(0, 256, (cols // 16, 1, 1024), generator=g, device="cuda", dtype=torch.uint8)
+    scale = torch.arange(cols, device="cuda").to(torch.int16).view(torch.bfloat16).view(cols // 16, 1, 16, 1)
+    zero = torch.randint(0, 16, (cols // 16, 1, 16, 1), generator=g, device="cuda", dtype=torch.uint8) if zero_points else None
+    less = zero.view(1, cols).float() if zero_points else 8.0
+    want = (_codes(q, depth, cols).float() - less) * scale.view(1, cols).float()
+    got = dequantize_int4_impl(q, scale, zero, (depth, cols))
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0.0, math.inf, -math.inf), want.nan_to_num(0.0, math.inf, -math.inf))
+    low = dequantize_int4_impl(q, scale, zero, (depth, cols), torch.bfloat16)
+    assert torch.equal(low.float().nan_to_num(0.0, math.inf, -math.inf), want.bfloat16().float().nan_to_num(0.0, math.inf, -math.inf))
+
+
 def _check_product(x, parts, depth, cols, dtype=None, warps=8):
     y = int4_matmul_impl(x, *parts, cols, dtype)
     assert y.shape == (*x.shape[:-1], cols) and y.dtype is (dtype or x.dtype)
