@@ -169,8 +169,8 @@ template <int THREADS> struct Shared {
 template <int THREADS, typename Done> __device__ __forceinline__ void rank_keys(const uint64_t* in, uint32_t n, Done done) {
   const uint32_t tid = threadIdx.x, share = n <= THREADS / 8 ? 8 : n <= THREADS / 4 ? 4 : n <= THREADS / 2 ? 2 : 1;
   const uint32_t part = tid % share, step = THREADS / share;
-  for (uint32_t i0 = 0; i0 < n; i0 += step) {      // a warp's threads go round together
-    const uint32_t i = i0 + tid / share;
+  for (uint32_t i0 = tid / 32 * 32 / share; i0 < n; i0 += step) {      // a warp's threads go round together
+    const uint32_t i = i0 + tid % 32 / share;
     const uint64_t key = i < n ? in[i] : ~0ull;
     uint32_t above = 0;
 #pragma unroll 4
@@ -337,12 +337,16 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
   }
   // Four vectors at a time; each is asked for while the ones before it are added up.
   uint4 raw[kLoads];
+  const uint4* ahead = vecs + tid;      // of the next four, and how many vectors are left from there on
+  int left = (int)(sl.count - tid);
 #pragma unroll
   for (int l = 0; l < kLoads; ++l)
-    if (tid + l * THREADS < sl.count) raw[l] = __ldg(vecs + tid + l * THREADS);
+    if (l * THREADS < left) raw[l] = __ldg(ahead + l * THREADS);
   for (uint32_t j0 = 0; j0 < sl.count; j0 += kLoads * THREADS) {
     const uint32_t j = j0 + tid;
     const bool full = j0 + kLoads * THREADS <= sl.count;
+    ahead += kLoads * THREADS;
+    left -= kLoads * THREADS;
     float tops[kLoads];
 #pragma unroll
     for (int l = 0; l < kLoads; ++l) {
@@ -360,8 +364,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
 #pragma unroll
       for (int l = 0; l < kLoads; ++l) {
         Vec<T>::unpack(raw[l], v);
-        const uint32_t next = j + (kLoads + l) * THREADS;
-        if (next < sl.count) raw[l] = __ldg(vecs + next);
+        if (l * THREADS < left) raw[l] = __ldg(ahead + l * THREADS);
 #pragma unroll
         for (int i = 0; i < kVec / 2; ++i) {
           const float2 d = __fadd2_rn(v[i], minus), a = __fmul2_rn(d, scale), e = make_float2(exp2_fast(a.x), exp2_fast(a.y));
@@ -388,8 +391,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
       for (int l = 0; l < kLoads; ++l) {
         const bool has = full || j + l * THREADS < sl.count;
         if (has) Vec<T>::unpack(raw[l], v);
-        const uint32_t next = j + (kLoads + l) * THREADS;
-        if (next < sl.count) raw[l] = __ldg(vecs + next);
+        if (l * THREADS < left) raw[l] = __ldg(ahead + l * THREADS);
         if (has)
 #pragma unroll
           for (int i = 0; i < kVec / 2; ++i) { t.add(v[i].x, from); t.add(v[i].y, from); }
