@@ -12,8 +12,8 @@
 // Floor: HBM.  The forward pass reads the logits once (4 or 2 bytes each), the backward pass once more and writes dz.  What it takes beside that is an
 // exponential per logit (16 a cycle and SM: 73 % of a bf16 logit's time at 6.5 TB/s) and six to seven instructions, so packed f32x2 arithmetic, and for the
 // alternatives no more than a thread's two best vectors while the row goes by.  On one B200, us (and of the measured 6.53 TB/s):
-//   2000 x 65536 bf16     48 (84 %) without alternatives, 55 with five, 74 with 64
-//   1000 x 65536 f32      43.5 (92 %), 64 with 64;  4096 x 65536 f32, forward and gradient 509 (97 %)
+//   2000 x 65536 bf16     48 (84 %) without alternatives, 55 with five, 68 with 64
+//   1000 x 65536 f32      43.5 (92 %), 60 with 64;  4096 x 65536 f32, forward and gradient 509 (97 %)
 //   one row of 65536 f32, five alternatives: 5.7, a launch and some ten dependent steps of 0.2 to 0.8 each
 #include "common.cuh"
 
@@ -27,7 +27,9 @@ namespace cg = cooperative_groups;
 constexpr int kLoads = 4;                  // 16-byte loads that a thread has in flight
 constexpr int kBackThreads = 256;
 constexpr int kMaxTop = 128, kMaxTokens = 128;
-constexpr int kCandidates = 1024;          // keys of a row that are ranked against one another
+constexpr int kCandidates = 1024;          // keys of a row that are looked at together
+constexpr uint32_t kHalve = 16;            // alternatives up to which the bound is a group's key
+constexpr uint32_t kNarrow = 256;          // more keys than this become fewer before they are ranked
 constexpr int kMaxCluster = 8;             // CTAs that share a row; kMaxCluster * kMaxTop <= kCandidates
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -154,14 +156,17 @@ template <typename T> struct Slice {
   __device__ __forceinline__ uint32_t elements() const { return head + tail + count * kVec; }
 };
 
+struct Halving { uint32_t counts[3], lowest, highest; };      // `lowest` ~0, the others 0 behind a barrier
+
 template <int THREADS> struct Shared {
   uint64_t cand[kCandidates];
-  uint64_t groups[THREADS];             // the best keys of groups of threads
+  uint64_t groups[32];             // the best keys of groups of threads
   uint64_t sorted[kMaxTop];
   uint64_t gathered[kMaxCluster * kMaxTop];      // of a cluster's CTAs, in its first one
   uint64_t bound;
   Sums terms[THREADS / 32], cta, of_cta[kMaxCluster];
   uint32_t n_cand, n_hot;
+  Halving halving;
   uint16_t hot[THREADS];
 };
 
@@ -184,6 +189,44 @@ template <int THREADS, typename Done> __device__ __forceinline__ void rank_keys(
   }
 }
 
+__device__ __forceinline__ void reset(Halving& h) {
+  if (threadIdx.x < 3) h.counts[threadIdx.x] = 0;
+  if (threadIdx.x == 0) { h.lowest = ~0u; h.highest = 0; }
+}
+
+// A bound that at least k and at most `most` of the threads' keys reach, found by halving.  k of the keys are not 0, and none of those is another's like; every(f) is f(key) for all of a
+// thread's.
+template <typename Every> __device__ __forceinline__ uint64_t bound_by_halving(Halving& h, uint32_t k, uint32_t most, Every every) {
+  const uint32_t tid = threadIdx.x;
+  uint32_t lowest = ~0u, highest = 0;
+  every([&](uint64_t key) {
+    const uint32_t order = (uint32_t)(key >> 32);
+    if (key) lowest = min(lowest, order);
+    highest = max(highest, order);
+  });
+  lowest = __reduce_min_sync(0xffffffffu, lowest);
+  highest = __reduce_max_sync(0xffffffffu, highest);
+  if (tid % 32 == 0) { atomicMin(&h.lowest, lowest); atomicMax(&h.highest, highest); }
+  __syncthreads();
+  uint64_t low = (uint64_t)h.lowest << 32 | 1, high = ((uint64_t)h.highest + 1) << 32;      // at least k reach low, none high (an order is below 2^32 - 1)
+  for (uint32_t slot = 0; high - low > 1;) {
+    const uint64_t middle = low + (high - low) / 2;
+    uint32_t reach = 0;
+    every([&](uint64_t key) { reach += key >= middle; });
+    reach = __reduce_add_sync(0xffffffffu, reach);
+    if (tid % 32 == 0 && reach) atomicAdd(&h.counts[slot], reach);
+    const uint32_t next = slot == 2 ? 0 : slot + 1;
+    if (tid == 0) h.counts[next] = 0;      // those who read it are past the barrier before
+    __syncthreads();
+    const uint32_t all = h.counts[slot];
+    slot = next;
+    if (all < k) { high = middle; continue; }
+    low = middle;
+    if (all <= most) break;
+  }
+  return low;
+}
+
 // What a thread knows of its logits: the largest and the last index of the vector that it first came in (its own index before and behind the vectors), and the largest
 // of its other vectors' largest.
 struct Best {
@@ -195,32 +238,44 @@ struct Best {
   }
 };
 
-// sorted[0, k) of the slice's k best logits; sh.bound = 1 and sh.n_cand = sh.n_hot = 0 behind a barrier.  Every thread brings the best of its own as a key, `mine`,
-// 0 where it has none.  The k-th largest of the keys of groups of threads, of twice k groups or more, is a bound that at least k and as a rule not
-// half as many more of the threads' keys reach.  So at least k logits of the slice reach it, and they all belong to those threads: vectors do
-// not overlap, so another thread's logit of the same value lies behind.  Such a thread looks at its best vector again, which is in `raw` or else is read
-// again; where its second one reaches the bound, too, the CTA reads all of that thread's.  The logits that reach the bound are ranked.
+// sorted[0, k) of the slice's k best logits; sh.bound = 1, sh.n_cand = sh.n_hot = 0 and sh.halving reset behind a barrier.  Every thread brings the best of its own as a
+// key, `mine`, 0 where it has none.  A bound that at least k of the threads' keys reach and few more: for small k the k-th largest of the keys of groups of threads,
+// of twice k groups or more, else one found by halving (2000 rows of 65536 bf16, us, ranked groups | halving: 64 of them 75 | 68, 20 69 | 61, five 55 | 59).  So at
+// least k logits of the slice reach it, and all of the k best are those threads': vectors do not overlap, so another thread's logit of the same value lies
+// behind.  Such a thread looks at its best vector again, which is in `raw` or else is read again; where its second one reaches the bound, too, the CTA reads all of
+// that thread's.  The logits that reach the bound are ranked, unless they are so many (rows of few vectors, ties, best logits that crowd into a few threads) that
+// it is better raised first: eight rows of 1000, 128 of them, 148 -> 14 us.
 template <typename T, int THREADS>
 __device__ void best_of_slice(Shared<THREADS>& sh, const Slice<T>& sl, const Best& best, uint64_t mine, const uint4 (&raw)[kLoads], uint32_t k) {
   constexpr int kVec = Vec<T>::kSize;
   const uint32_t tid = threadIdx.x;
   const uint32_t rounds = (sl.count + THREADS - 1) / THREADS, at0 = sl.at0();
-  const uint32_t groups = k <= 4 ? 8 : k <= 16 ? 32 : k <= 64 ? 128 : THREADS, lanes = THREADS / groups;
+  const uint32_t groups = k <= 4 ? 8 : 32, lanes = THREADS / groups;
   uint4 best_vector;      // asked for before it is known whether it is wanted: most of the time that takes is then over
   const bool vector = rounds > kLoads && best.at >= at0 && best.at < sl.tail_at;
+  // the key of the first logit that `mine` may stand for: an index of a vector is its last one's
+  const uint64_t reach = mine + (mine != 0 && best.at >= at0 && best.at < sl.tail_at ? kVec - 1 : 0);
   if (vector) best_vector = *reinterpret_cast<const uint4*>(sl.z + best.at - (kVec - 1));
-  uint64_t key = mine;
-  for (uint32_t o = 1; o < min(lanes, 32u); o <<= 1) {
-    const uint64_t other = __shfl_xor_sync(0xffffffffu, key, o);
-    key = other > key ? other : key;
+  if (k > kHalve) {
+    if (min(max(max(sl.head, sl.tail), sl.count), (uint32_t)THREADS) >= k) {      // as many threads have a key
+      const uint64_t bound = bound_by_halving(sh.halving, k, k + 8, [&](auto f) { f(mine); });
+      if (tid == 0) sh.bound = bound;
+    }
+    __syncthreads();
+  } else {
+    uint64_t key = mine;
+    for (uint32_t o = 1; o < min(lanes, 32u); o <<= 1) {
+      const uint64_t other = __shfl_xor_sync(0xffffffffu, key, o);
+      key = other > key ? other : key;
+    }
+    const uint32_t held = max(groups, (uint32_t)THREADS / 32);      // a group is a warp at most
+    if (tid % (THREADS / held) == 0) sh.groups[tid / (THREADS / held)] = key;
+    __syncthreads();
+    rank_keys<THREADS>(sh.groups, held, [&](uint32_t, uint64_t own, uint32_t above) {
+      if (own != 0 && above == k - 1) sh.bound = own;      // no two of the others are equal
+    });
+    __syncthreads();
   }
-  const uint32_t held = max(groups, (uint32_t)THREADS / 32);      // a group is a warp at most
-  if (tid % (THREADS / held) == 0) sh.groups[tid / (THREADS / held)] = key;
-  __syncthreads();
-  rank_keys<THREADS>(sh.groups, held, [&](uint32_t, uint64_t own, uint32_t above) {
-    if (own != 0 && above == k - 1) sh.bound = own;      // no two of the others are equal
-  });
-  __syncthreads();
   while (true) {      // once, but for rows whose best logits crowd into a few threads: the bound rises until what reaches it has room
     uint64_t bound = sh.bound;
     if (bound >> 32 == order_of(-INFINITY)) {      // -inf is wanted only where fewer than k are more: those that are lie before 2 k - 1 others
@@ -248,7 +303,7 @@ __device__ void best_of_slice(Shared<THREADS>& sh, const Slice<T>& sl, const Bes
         offer(Vec<T>::at(r, e), at + e);
       }
     };
-    if (mine >= bound) {
+    if (reach >= bound) {
       if (tid < sl.head) offer(Elem<T>::to_f32(sl.z[tid]), tid);
       if (tid < sl.tail) offer(Elem<T>::to_f32(sl.z[sl.tail_at + tid]), sl.tail_at + tid);
       // a bound of -inf has the index of a thread's first vector: of other -inf only those of first vectors reach it
@@ -278,14 +333,22 @@ __device__ void best_of_slice(Shared<THREADS>& sh, const Slice<T>& sl, const Bes
         }
       __syncthreads();
     }
-    const uint32_t n = sh.n_cand, kept = min(n, (uint32_t)kCandidates);
-    rank_keys<THREADS>(sh.cand, kept, [&](uint32_t, uint64_t key, uint32_t above) {
+    const uint32_t n = sh.n_cand;
+    if (n > kNarrow) {
+      reset(sh.halving);
+      __syncthreads();
+      const uint64_t raised = bound_by_halving(sh.halving, k, k + 32, [&](auto f) {
+        for (uint32_t i = tid; i < min(n, (uint32_t)kCandidates); i += THREADS) f(sh.cand[i]);
+      });
+      if (tid == 0) { sh.bound = raised; sh.n_cand = 0; sh.n_hot = 0; }
+      __syncthreads();
+      continue;
+    }
+    rank_keys<THREADS>(sh.cand, n, [&](uint32_t, uint64_t key, uint32_t above) {
       if (above < k) sh.sorted[above] = key;
     });
     __syncthreads();
-    if (n <= kCandidates) break;
-    if (tid == 0) { sh.bound = sh.sorted[k - 1]; sh.n_cand = 0; sh.n_hot = 0; }
-    __syncthreads();
+    break;
   }
 }
 
@@ -301,8 +364,8 @@ struct Forward {
 
 // One row per cluster of CTAs (of one CTA where there are rows enough to fill the chip); its CTAs' terms and best logits meet in the first one, which the
 // others write to: behind the one barrier that this takes they are done (reading from the first CTA took two, and 1.2 us more for a single row).
-// With alternatives a row is two phases, the stream (22000 cycles of a 128 KB row among three others on the SM) and the selection (15000 for 64 of them, 6000
-// for five), which other rows' streams hide in part: more, smaller CTAs are better until the selection is longer than they can hide.
+// With alternatives a row is two phases, the stream (22000 cycles of a 128 KB row among three others on the SM) and the selection (half as many for 64 of them, a
+// quarter for five), which other rows' streams hide in part: more, smaller CTAs are better until the selection is longer than they can hide.
 template <typename T, int THREADS, bool TOP>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel(const Forward p) {
   grid_wait();
@@ -409,6 +472,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
   t.template over_lanes<32>();
   if ((tid & 31) == 0) sh.terms[tid >> 5] = t;
   if (TOP && tid == 0) { sh.bound = 1; sh.n_cand = 0; sh.n_hot = 0; }
+  if (TOP) reset(sh.halving);
   __syncthreads();
   if (tid / 32 == kWarps - 1) {      // the last warp: the first ones have a bound to find
     const uint32_t lane = tid & 31;
@@ -433,10 +497,26 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
       r.template over_lanes<kMaxCluster>();
       if (tid == 0) sh.cta = r;
     }
-    if (TOP)
-      rank_keys<THREADS>(sh.gathered, ctas * p.top, [&](uint32_t, uint64_t key, uint32_t above) {
+    if (TOP) {
+      const uint64_t* all = sh.gathered;
+      uint32_t n = ctas * p.top;
+      if (n > kNarrow) {      // into cand, which is free again
+        if (tid == 0) sh.n_cand = 0;
+        reset(sh.halving);
+        __syncthreads();
+        const uint64_t bound = bound_by_halving(sh.halving, p.top, p.top + 32, [&](auto f) {
+          for (uint32_t i = tid; i < n; i += THREADS) f(sh.gathered[i]);
+        });
+        for (uint32_t i = tid; i < n; i += THREADS)
+          if (sh.gathered[i] >= bound) sh.cand[atomicAdd(&sh.n_cand, 1u)] = sh.gathered[i];
+        __syncthreads();
+        all = sh.cand;
+        n = sh.n_cand;
+      }
+      rank_keys<THREADS>(all, n, [&](uint32_t, uint64_t key, uint32_t above) {
         if (above < p.top && key != 0) sh.sorted[above] = key;
       });
+    }
     __syncthreads();
   }
   if (tid >= max(max(p.n_tokens, p.top), 1u)) return;
@@ -574,11 +654,11 @@ template <typename T> cudaError_t forward_of(const Forward& p, int64_t rows, cud
   const int64_t sms = sm_count();
   int ctas = 1;
   while (ctas < kMaxCluster && rows * ctas * 2 <= sms && bytes / (ctas * 2) >= 32768) ctas *= 2;
-  // us, 128 | 256 | 512 threads a row: 4096 rows of 16 KB 25 | 38 | 71 (five alternatives), 17.5 | 21.5 | 38 (none), 51 | 65 | 98 (64); 2000 rows of 128 KB 55 | 57 | 69
-  // (five), 50 | 48 | 52 (none), 90 | 74 | 85 (64); 148 rows of 256 KB 20.9 | 19.7 | 13.8 (20); one such row over eight CTAs 6.6 | 6.0 | 6.4
+  // us, 128 | 256 | 512 threads a row: 4096 rows of 16 KB 26 | 39 | 71 (five alternatives), 17.5 | 21.5 | 38 (none), 122 | 89 | 144 (128), of 8 KB 41 | 57 | 117 (64);
+  // 2000 rows of 128 KB 55 | 56 | 67 (five), 50 | 48 | 52 (none), 88 | 68 | 85 (64); 148 rows of 256 KB 20.2 | 18.2 | 13.5 (20); one such row over eight CTAs 6.6 | 5.7 | 6.1
   int threads;
-  if (rows * ctas <= sms) threads = bytes / ctas > 32768 ? 512 : bytes / ctas > 8192 ? 256 : 128;
-  else threads = bytes <= 32768 || (bytes <= 131072 && p.top > 0 && p.top <= 32) ? 128 : 256;
+  if (rows * ctas <= sms) threads = bytes / ctas > 32768 ? 512 : bytes / ctas > 8192 || p.top > 64 ? 256 : 128;
+  else threads = p.top <= 64 && (bytes <= 32768 || (bytes <= 131072 && p.top > 0 && p.top <= 32)) ? 128 : 256;
   if (int v = env_switch("PB_LP_CTAS", 0)) ctas = v;
   if (int v = env_switch("PB_LP_WIDE", 0)) threads = v;
   if (threads == 128) return p.top ? launch_forward<T, 128, true>(p, rows, ctas, st) : launch_forward<T, 128, false>(p, rows, ctas, st);

@@ -177,6 +177,22 @@ def test_best_logits_that_crowd_together(built_lib, rows, period):
     _check(z.flip(-1).contiguous(), None, 128)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("top", [3, 17, 60, 128])
+@pytest.mark.parametrize("rows,vocab", [(2, 300), (3, 1000), (160, 1001), (2, 2051), (300, 4096), (2, 9001), (310, 9001), (2, 65536), (160, 65535)])
+def test_few_values(built_lib, rows, vocab, top, dtype):
+    """Rows of one, two, five, fifty and some thousand different values, a row of which two thirds are -inf, and one of -inf but for five: the bound's value is
+    many logits', and the number of alternatives ends inside a vector."""
+    g = _gen(vocab + top)
+    levels = torch.tensor([1, 2, 5, 50, 5000], device="cuda")[torch.arange(rows, device="cuda") % 5].unsqueeze(1)
+    z = ((torch.rand(rows, vocab, generator=g, device="cuda") * levels).floor() * 0.125 - 3.0).to(DTYPES[dtype])
+    z[1, torch.rand(vocab, generator=g, device="cuda") < 0.67] = -math.inf
+    if rows > 2:
+        z[2, 5:] = -math.inf
+    _check(z, None, top)
+    _check(z[:, 1:], None, min(top, vocab - 1))        # off 16 bytes
+
+
 def test_another_stream_and_a_graph(built_lib):
     z, tokens = _case(3, 32003, "bf16", 4)
     want = token_logprobs(z, tokens, 5)
