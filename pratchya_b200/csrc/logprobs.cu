@@ -194,25 +194,27 @@ __device__ __forceinline__ void reset(Halving& h) {
   if (threadIdx.x == 0) { h.lowest = ~0u; h.highest = 0; }
 }
 
-// A bound that at least k and at most `most` of the threads' keys reach, found by halving.  k of the keys are not 0, and none of those is another's like; every(f) is f(key) for all of a
-// thread's.
-template <typename Every> __device__ __forceinline__ uint64_t bound_by_halving(Halving& h, uint32_t k, uint32_t most, Every every) {
-  const uint32_t tid = threadIdx.x;
+// A bound that at least k and, where it is above -inf, at most `most` of the threads' keys reach, found by halving between the lowest and the highest of them.  Where those are far apart (masks
+// of the type's lowest value, -inf), thirty halvings would only come to where the others are: there it goes down from the highest, four times as far each time, until k reach it, and halves
+// then (48 rows of 65536 under such masks, 20 alternatives, us: 13.9 | 9.8; without masks going down takes more steps, 9.1 | 9.6).  k of the keys are not 0, none of those is another's like, and their
+// indices are below vocab; every(f) is f(key) for all of a thread's.
+template <typename Every> __device__ __forceinline__ uint64_t bound_by_halving(Halving& h, uint32_t k, uint32_t most, uint32_t vocab, Every every) {
+  const uint32_t tid = threadIdx.x, nothing = order_of(-INFINITY);
+  const uint64_t something = (uint64_t)(nothing + 1) << 32;
   uint32_t lowest = ~0u, highest = 0;
   every([&](uint64_t key) {
-    const uint32_t order = (uint32_t)(key >> 32);
-    if (key) lowest = min(lowest, order);
-    highest = max(highest, order);
+    if (key) lowest = min(lowest, (uint32_t)(key >> 32));
+    highest = max(highest, (uint32_t)(key >> 32));
   });
   lowest = __reduce_min_sync(0xffffffffu, lowest);
   highest = __reduce_max_sync(0xffffffffu, highest);
   if (tid % 32 == 0) { atomicMin(&h.lowest, lowest); atomicMax(&h.highest, highest); }
   __syncthreads();
-  uint64_t low = (uint64_t)h.lowest << 32 | 1, high = ((uint64_t)h.highest + 1) << 32;      // at least k reach low, none high (an order is below 2^32 - 1)
-  for (uint32_t slot = 0; high - low > 1;) {
-    const uint64_t middle = low + (high - low) / 2;
+  uint64_t low = (uint64_t)h.lowest << 32 | ~(vocab - 1), high = ((uint64_t)h.highest + 1) << 32;      // none reach high (an order is below 2^32 - 1)
+  uint32_t slot = 0;
+  auto reached = [&](uint64_t bound) {
     uint32_t reach = 0;
-    every([&](uint64_t key) { reach += key >= middle; });
+    every([&](uint64_t key) { reach += key >= bound; });
     reach = __reduce_add_sync(0xffffffffu, reach);
     if (tid % 32 == 0 && reach) atomicAdd(&h.counts[slot], reach);
     const uint32_t next = slot == 2 ? 0 : slot + 1;
@@ -220,8 +222,25 @@ template <typename Every> __device__ __forceinline__ uint64_t bound_by_halving(H
     __syncthreads();
     const uint32_t all = h.counts[slot];
     slot = next;
+    return all;
+  };
+  if (high - low >= 1ull << 58 || low < something) {
+    for (uint64_t step = 1ull << 52;; step = step < 1ull << 62 ? step << 2 : ~0ull) {
+      low = high - something > step ? high - step : something;
+      const uint32_t all = reached(low);
+      if (all >= k) {
+        if (all <= most) return low;
+        break;
+      }
+      if (low == something) return (uint64_t)nothing << 32;      // fewer than k are more than -inf
+      high = low;
+    }
+  }
+  while (high - low > 1) {
+    const uint64_t middle = low + (high - low) / 2;
+    const uint32_t all = reached(middle);
     if (all < k) { high = middle; continue; }
-    low = middle;
+    low = max(middle, middle >> 32 << 32 | ~(vocab - 1));      // as many reach the last index's key
     if (all <= most) break;
   }
   return low;
@@ -245,8 +264,8 @@ struct Best {
 // behind.  Such a thread looks at its best vector again, which is in `raw` or else is read again; where its second one reaches the bound, too, the CTA reads all of
 // that thread's.  The logits that reach the bound are ranked, unless they are so many (rows of few vectors, ties, best logits that crowd into a few threads) that
 // it is better raised first: eight rows of 1000, 128 of them, 148 -> 14 us.
-template <typename T, int THREADS>
-__device__ void best_of_slice(Shared<THREADS>& sh, const Slice<T>& sl, const Best& best, uint64_t mine, const uint4 (&raw)[kLoads], uint32_t k) {
+template <typename T, int THREADS, bool MANY>
+__device__ void best_of_slice(Shared<THREADS>& sh, const Slice<T>& sl, const Best& best, uint64_t mine, const uint4 (&raw)[kLoads], uint32_t k, uint32_t vocab) {
   constexpr int kVec = Vec<T>::kSize;
   const uint32_t tid = threadIdx.x;
   const uint32_t rounds = (sl.count + THREADS - 1) / THREADS, at0 = sl.at0();
@@ -256,9 +275,9 @@ __device__ void best_of_slice(Shared<THREADS>& sh, const Slice<T>& sl, const Bes
   // the key of the first logit that `mine` may stand for: an index of a vector is its last one's
   const uint64_t reach = mine + (mine != 0 && best.at >= at0 && best.at < sl.tail_at ? kVec - 1 : 0);
   if (vector) best_vector = *reinterpret_cast<const uint4*>(sl.z + best.at - (kVec - 1));
-  if (k > kHalve) {
+  if constexpr (MANY) {
     if (min(max(max(sl.head, sl.tail), sl.count), (uint32_t)THREADS) >= k) {      // as many threads have a key
-      const uint64_t bound = bound_by_halving(sh.halving, k, k + 8, [&](auto f) { f(mine); });
+      const uint64_t bound = bound_by_halving(sh.halving, k, k + 8, vocab, [&](auto f) { f(mine); });
       if (tid == 0) sh.bound = bound;
     }
     __syncthreads();
@@ -337,14 +356,16 @@ __device__ void best_of_slice(Shared<THREADS>& sh, const Slice<T>& sl, const Bes
     if (n > kNarrow) {
       reset(sh.halving);
       __syncthreads();
-      const uint64_t raised = bound_by_halving(sh.halving, k, k + 32, [&](auto f) {
+      const uint64_t raised = bound_by_halving(sh.halving, k, k + 32, vocab, [&](auto f) {
         for (uint32_t i = tid; i < min(n, (uint32_t)kCandidates); i += THREADS) f(sh.cand[i]);
       });
-      if (tid == 0) { sh.bound = raised; sh.n_cand = 0; sh.n_hot = 0; }
-      __syncthreads();
-      continue;
+      if (raised > bound) {      // fewer reach it: `most` of those looked at.  Else fewer than k are more than -inf, and there is room for as many of those as may be wanted
+        if (tid == 0) { sh.bound = raised; sh.n_cand = 0; sh.n_hot = 0; }
+        __syncthreads();
+        continue;
+      }
     }
-    rank_keys<THREADS>(sh.cand, n, [&](uint32_t, uint64_t key, uint32_t above) {
+    rank_keys<THREADS>(sh.cand, min(n, (uint32_t)kCandidates), [&](uint32_t, uint64_t key, uint32_t above) {
       if (above < k) sh.sorted[above] = key;
     });
     __syncthreads();
@@ -366,7 +387,8 @@ struct Forward {
 // others write to: behind the one barrier that this takes they are done (reading from the first CTA took two, and 1.2 us more for a single row).
 // With alternatives a row is two phases, the stream (22000 cycles of a 128 KB row among three others on the SM) and the selection (half as many for 64 of them, a
 // quarter for five), which other rows' streams hide in part: more, smaller CTAs are better until the selection is longer than they can hide.
-template <typename T, int THREADS, bool TOP>
+// TOP: 0 for no alternatives, 1 for up to kHalve, 2 for more (in one kernel few of them took 1 to 3 % longer).
+template <typename T, int THREADS, int TOP>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel(const Forward p) {
   grid_wait();
   __shared__ __align__(16) Shared<THREADS> sh;
@@ -482,7 +504,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
     if (lane == 0) sh.cta = r;
   }
   const uint32_t own = TOP ? min(p.top, sl.elements()) : 0;
-  if (TOP && own) best_of_slice<T, THREADS>(sh, sl, best, mine, raw, own);
+  if (TOP && own) best_of_slice<T, THREADS, TOP == 2>(sh, sl, best, mine, raw, own, p.vocab);
   else __syncthreads();
   if (ctas > 1) {      // everyone hands what it has to the first CTA
     Shared<THREADS>* to = cluster.map_shared_rank(&sh, 0);
@@ -504,9 +526,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
         if (tid == 0) sh.n_cand = 0;
         reset(sh.halving);
         __syncthreads();
-        const uint64_t bound = bound_by_halving(sh.halving, p.top, p.top + 32, [&](auto f) {
+        uint64_t bound = bound_by_halving(sh.halving, p.top, p.top + 32, p.vocab, [&](auto f) {
           for (uint32_t i = tid; i < n; i += THREADS) f(sh.gathered[i]);
         });
+        bound = max(bound, key_of(-INFINITY, 2 * p.top - 2));      // where fewer than k are more than -inf, those that are wanted lie before 2 k - 1 others
         for (uint32_t i = tid; i < n; i += THREADS)
           if (sh.gathered[i] >= bound) sh.cand[atomicAdd(&sh.n_cand, 1u)] = sh.gathered[i];
         __syncthreads();
@@ -637,7 +660,7 @@ int ctas_of_row(int64_t rows, int64_t bytes) {
   return c;
 }
 
-template <typename T, int THREADS, bool TOP> cudaError_t launch_forward(const Forward& p, int64_t rows, int ctas, cudaStream_t st) {
+template <typename T, int THREADS, int TOP> cudaError_t launch_forward(const Forward& p, int64_t rows, int ctas, cudaStream_t st) {
   cudaLaunchConfig_t config{};
   config.gridDim = dim3((unsigned)(rows * ctas)); config.blockDim = dim3(THREADS); config.stream = st;
   cudaLaunchAttribute attrs[2];
@@ -661,9 +684,9 @@ template <typename T> cudaError_t forward_of(const Forward& p, int64_t rows, cud
   else threads = p.top <= 64 && (bytes <= 32768 || (bytes <= 131072 && p.top > 0 && p.top <= 32)) ? 128 : 256;
   if (int v = env_switch("PB_LP_CTAS", 0)) ctas = v;
   if (int v = env_switch("PB_LP_WIDE", 0)) threads = v;
-  if (threads == 128) return p.top ? launch_forward<T, 128, true>(p, rows, ctas, st) : launch_forward<T, 128, false>(p, rows, ctas, st);
-  if (threads == 512) return p.top ? launch_forward<T, 512, true>(p, rows, ctas, st) : launch_forward<T, 512, false>(p, rows, ctas, st);
-  return p.top ? launch_forward<T, 256, true>(p, rows, ctas, st) : launch_forward<T, 256, false>(p, rows, ctas, st);
+  if (threads == 128) return p.top > kHalve ? launch_forward<T, 128, 2>(p, rows, ctas, st) : p.top ? launch_forward<T, 128, 1>(p, rows, ctas, st) : launch_forward<T, 128, 0>(p, rows, ctas, st);
+  if (threads == 512) return p.top > kHalve ? launch_forward<T, 512, 2>(p, rows, ctas, st) : p.top ? launch_forward<T, 512, 1>(p, rows, ctas, st) : launch_forward<T, 512, 0>(p, rows, ctas, st);
+  return p.top > kHalve ? launch_forward<T, 256, 2>(p, rows, ctas, st) : p.top ? launch_forward<T, 256, 1>(p, rows, ctas, st) : launch_forward<T, 256, 0>(p, rows, ctas, st);
 }
 
 int check_rows(const char* who, const void* logits, int dtype, int64_t outer, int64_t inner, int64_t stride_outer, int64_t stride_inner, int64_t vocab,
