@@ -207,7 +207,8 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_int4_kernel(const ui
 // Sums over a group meet the group's scale in f32, groups and warps add in f32.
 // Floor: the weight's bytes from HBM, 10.6 us for 2048 x 65536.  On one B200, us:
 //   one row, f32: 2048 x 65536 15.6 (68 %), 2048 x 8192 4.2, 2048 x 2048 3.0, 2048 x 128 2.9 (a launch, x's way to the digits and one barrier)
-//   bf16 rows x depth x columns: 8 x 2048 x 8192 5.8, 32 x 8192 x 2048 11.0, 32 x 2048 x 65536 58 (32 columns keep the tensor core's old instructions, 8 cycles each, busy)
+//   bf16 rows x depth x columns: 8 x 2048 x 8192 5.8, 32 x 8192 x 2048 11.0, 32 x 2048 x 65536 53 (with so much of x in shared
+//   memory an SM has one CTA, two warps a scheduler: tensor pipe 30 %, issue slots 35 %; two blocks ahead instead of four 57)
 // What a row of 65536 columns takes beside the stream of codes (9.4 us at 7.3 TB/s): 2.7 until x is in digits, 0.9 for the sums of the warps, a launch.
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kPad = 32;               // values behind a row of x in shared memory: neighbouring rows' 64 bytes then lie in other banks
@@ -318,7 +319,7 @@ template <typename TX, int DIGITS, int MT, int PER_GROUP, bool ZERO>
 __global__ void __launch_bounds__(kThreads, DIGITS == 0 && MT == 4 ? 1 : 2) int4_product_kernel(const Product p) {
   grid_wait();
   constexpr int kParts = DIGITS ? DIGITS : 1;      // columns of the instruction that a row of x takes, the first with its uppermost digits
-  constexpr int kAhead = MT <= 2 ? 4 : 2;          // blocks that a warp has on the way or in hand
+  constexpr int kAhead = MT <= 2 || DIGITS == 0 ? 4 : 2;      // blocks that a warp has on the way or in hand
   extern __shared__ __align__(16) uint8_t smem[];
   // of a chunk: the tile that a warp's run begins in (none: kNoTile), and the warps that have a tile's first and last block
   __shared__ uint32_t tiles_at[kWarps], first_warp[kMaxChunk], last_warp[kMaxChunk];
