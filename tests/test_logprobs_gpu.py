@@ -193,6 +193,30 @@ def test_few_values(built_lib, rows, vocab, top, dtype):
     _check(z[:, 1:], None, min(top, vocab - 1))        # off 16 bytes
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("top", [5, 40, 128])
+@pytest.mark.parametrize("rows,vocab", [(6, 131073), (6, 3000), (300, 20000)])
+def test_rows_with_less_left_than_is_wanted(built_lib, rows, vocab, top, dtype):
+    """Nothing, five, a hundred and thirty-nine logits above -inf, at a row's start, end and all over it, and rows of the type's lowest value but for as many:
+    what fills the alternatives up are the first of the others, of a row's several CTAs, too."""
+    g = _gen(vocab + top)
+    z, _ = _case(rows, vocab, dtype, vocab)
+    low = torch.finfo(z.dtype).min
+    keep = torch.zeros(rows, vocab, dtype=torch.bool, device="cuda")
+    keep[1, -5:] = True
+    keep[2, torch.randperm(vocab, generator=g, device="cuda")[:100]] = True
+    keep[3, :39] = True
+    keep[4, torch.randperm(vocab, generator=g, device="cuda")[:39]] = True
+    keep[5, vocab // 2:vocab // 2 + 100] = True
+    z[:6] = torch.where(keep[:6], z[:6], -math.inf)
+    if rows > 12:
+        z[6:12] = torch.where(keep[:6], z[6:12], low)
+    _check(z, None, top)
+    z[:6] = torch.where(z[:6] == -math.inf, low, z[:6])
+    z[0, 7::9] = -math.inf
+    _check(z, None, top)
+
+
 def test_another_stream_and_a_graph(built_lib):
     z, tokens = _case(3, 32003, "bf16", 4)
     want = token_logprobs(z, tokens, 5)
