@@ -145,6 +145,23 @@ def test_not_a_number(built_lib):
         assert all(torch.equal(a[keep], b[keep]) for a, b in zip(out, clean))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,vocab", [(5, 2000), (5, 70001), (310, 9001)])
+def test_many_alternatives_where_logits_are_no_numbers(built_lib, rows, vocab, dtype):
+    z, tokens = _case(rows, vocab, dtype, 19)
+    tokens = tokens.clamp(min=0)
+    z[1, 5::3] = math.nan
+    z[2, 40:1900] = math.inf
+    z[3] = math.nan
+    z[4, 3:] = math.nan                                # three numbers, then the first of what is none
+    out = token_logprobs(z, tokens, 128)
+    want = torch.sort(torch.where(z.isnan(), -math.inf, z.float()) + 0.0, dim=-1, descending=True, stable=True).indices[:, :128]
+    assert torch.equal(out.top_tokens, want)
+    assert torch.isnan(out.top_logprobs[1:5]).all() and torch.isnan(out.entropy[1:5]).all()
+    keep = [i for i in range(rows) if not 1 <= i < 5]
+    _check(z[keep], tokens[keep], 128)
+
+
 def test_tokens_that_are_none_or_beyond(built_lib):
     z, _ = _case(5, 1000, "f32", 1)
     tokens = torch.tensor([0, -1, 999, 1000, -100], device="cuda")
