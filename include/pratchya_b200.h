@@ -420,7 +420,8 @@ PB_API int pb_token_logprobs_bwd(const void* logits, int dtype, int64_t outer, i
  * A group that holds a NaN or an infinity reads back as no finite numbers.
  * pb_int4_product: out[rows, cols] = x[rows, depth] w, x's rows `stride` elements apart, sums in f32.  x is not rounded to fewer bits than it has but for what is far below its
  * neighbours: of 128 that begin at a multiple of 128 the largest has 2^30 (f32) or 2^22 (bf16, one or two rows and many columns) steps above zero, the others the same steps.
- * A row of x with an infinity or a NaN has no finite products.  Made for few rows: the weight is read once for every 32 rows of a bf16 x and every eight of an f32 one. */
+ * A row of x with an infinity or a NaN has no finite products.  Made for few rows: the weight is read once for every 32 rows of a bf16 x and every eight of an f32 one.
+ * q is 16-byte aligned; the product wants scale at a multiple of 2 * 128 / group bytes and zero at one of 128 / group. */
 PB_API int pb_quantize_int4(const void* w, int dtype, int64_t depth, int64_t cols, int group, uint8_t* q, void* scale, uint8_t* zero, void* stream);
 PB_API int pb_dequantize_int4(const uint8_t* q, const void* scale, const uint8_t* zero, int64_t depth, int64_t cols, int group, void* out, int dtype, void* stream);
 PB_API int pb_int4_product(const void* x, int x_dtype, int64_t rows, int64_t depth, int64_t stride, const uint8_t* q, const void* scale, const uint8_t* zero, int group,

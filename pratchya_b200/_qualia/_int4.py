@@ -28,7 +28,14 @@ def _int4_parts(q, scale, zero, depth, cols, what):
         raise ValueError(f"{what}: scale {scale.dtype} {tuple(scale.shape)} for a weight of [{depth}, {cols}], which has bfloat16 {(*tiles, 16, '128 / group')}")
     if zero is not None and (zero.dtype is not torch.uint8 or zero.shape != scale.shape):
         raise ValueError(f"{what}: zero {zero.dtype} {tuple(zero.shape)} beside scale {tuple(scale.shape)}")
-    return q.contiguous(), scale.contiguous(), zero.contiguous() if zero is not None else None
+    groups = scale.shape[3]
+    return _at(q, 16), _at(scale, 2 * groups), _at(zero, groups) if zero is not None else None
+
+
+def _at(t, align):
+    """t as it is where the kernels can read it there, contiguous from a multiple of `align` bytes; else a copy."""
+    t = t.contiguous()
+    return t if t.data_ptr() % align == 0 else t.clone()
 
 
 def quantize_int4_impl(w: torch.Tensor, group: int = 128, zero_points: bool = False):

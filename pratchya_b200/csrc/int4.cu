@@ -779,14 +779,14 @@ extern "C" int pb_int4_product(const void* x, int x_dtype, int64_t rows, int64_t
   if ((x_dtype != PB_F32 && x_dtype != PB_BF16) || (out_dtype != PB_F32 && out_dtype != PB_BF16)) return fail(PB_ERR_BAD_DTYPE, "pb_int4_product: dtypes %d, %d", x_dtype, out_dtype);
   if (rows == 0) return PB_OK;
   if (!x || !q || !scale || !out) return fail(PB_ERR_NULL_POINTER, "pb_int4_product: null argument");
-  if ((reinterpret_cast<uintptr_t>(q) & 15) || ((reinterpret_cast<uintptr_t>(scale) | reinterpret_cast<uintptr_t>(zero)) & 3) ||
+  const int per_group = 128 / group;      // a lane loads as many scales, and zero points, at once
+  if ((reinterpret_cast<uintptr_t>(q) & 15) || reinterpret_cast<uintptr_t>(scale) % (2 * per_group) || reinterpret_cast<uintptr_t>(zero) % per_group ||
       (reinterpret_cast<uintptr_t>(x) % (x_dtype == PB_F32 ? 4 : 2)) || (reinterpret_cast<uintptr_t>(out) % (out_dtype == PB_F32 ? 4 : 2)))
-    return fail(PB_ERR_MISALIGNED, "pb_int4_product: q 16, scale and zero 4 bytes, x and out their types");
+    return fail(PB_ERR_MISALIGNED, "pb_int4_product: q 16, scale %d and zero %d bytes, x and out their types", 2 * per_group, per_group);
   if ((uint64_t)((cols + 15) / 16) * ((depth + 127) / 128) > 0x7fffffffull) return fail(PB_ERR_BAD_SHAPE, "pb_int4_product: depth=%lld cols=%lld", (long long)depth, (long long)cols);
   Product p{x, stride, q, static_cast<const __nv_bfloat16*>(scale), zero, out, (uint32_t)rows, (uint32_t)depth, (uint32_t)cols, (uint32_t)((depth + 127) / 128),
             (uint32_t)((cols + 15) / 16), 0, 0, 0, FastDiv(), 0, 0, out_dtype == PB_F32};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int per_group = 128 / group;
   if (x_dtype == PB_F32) return rows <= 2 ? launch_of<float, 4, 1>(p, per_group, st) : rows <= 4 ? launch_of<float, 4, 2>(p, per_group, st) : launch_of<float, 4, 4>(p, per_group, st);
   // A bf16 x as it is or in digits, us, 2048 values deep: 2048 columns 2.97 | 3.22 (one row) and 3.06 | 3.98 (two), 8192 columns 4.80 | 4.38 and 5.43 | 5.26 (with zero
   // points, 8192 deep and 2048 columns, 5.70 | 6.44), 65536 columns 18.8 | 15.6 and 19.4 | 17.0, four rows 20.1 | 21.7: making digits is made good by many columns

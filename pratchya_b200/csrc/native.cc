@@ -812,6 +812,8 @@ struct Int4 {
     const int64_t groups = scale->size(3);
     if (groups != 1 && groups != 2 && groups != 4) return false;
     group = (int)(128 / groups);
+    auto lies = [](const at::Tensor* t, int64_t bytes) { return !t || reinterpret_cast<uintptr_t>(t->data_ptr()) % bytes == 0; };      // where it does not, the Python text copies it
+    if (!lies(q, 16) || !lies(scale, 2 * groups) || !lies(zero, groups)) return false;
     return !zero || (zero->scalar_type() == at::kByte && zero->sizes() == scale->sizes() && zero->device() == q->device());
   }
   uint8_t* zeros() const { return zero ? (uint8_t*)zero->data_ptr() : nullptr; }

@@ -53,3 +53,14 @@ def test_product(built_lib):
     for bad in (dict(rows=-1), dict(depth=0), dict(cols=0), dict(stride=-1), dict(depth=1 << 31), dict(cols=1 << 30), dict(depth=1 << 30, cols=1 << 29)):
         assert _product(built_lib, **bad) == 2, bad
     assert _product(built_lib, rows=0, x=None) == 0
+
+
+def test_a_weights_parts_lie_where_a_lane_loads_them_from(built_lib):
+    """Four scales of a group of 32 come as eight bytes, two of a group of 64 as four; the zero points of each are half of that."""
+    at = lambda byte: C.c_void_p(4096 + byte)
+    for byte in (2, 4, 6):
+        assert _product(built_lib, scale=at(byte), group=32) == 9, byte
+    assert _product(built_lib, scale=at(2), group=64) == 9 and _product(built_lib, scale=at(1), group=128) == 9
+    for byte in (1, 2, 3):
+        assert _product(built_lib, zero=at(byte), group=32) == 9, byte
+    assert _product(built_lib, zero=at(1), group=64) == 9

@@ -260,3 +260,20 @@ def test_refusals(built_lib):
         dequantize_int4_impl(*parts, (256, 32), torch.float16)
     # the same parts, strided: taken by way of a copy
     assert torch.equal(int4_matmul_impl(x, q, scale.repeat(1, 1, 1, 2)[..., :2], zero, 32), int4_matmul_impl(x, *parts, 32))
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_parts_that_lie_anywhere_in_a_flat_buffer(built_lib, group, dtype):
+    """A model's buffers may be views of one: scales at any multiple of their two bytes, codes and zero points at any byte."""
+    g = torch.Generator(device="cuda").manual_seed(group)
+    w, x = torch.randn(260, 40, generator=g, device="cuda"), torch.randn(3, 260, generator=g, device="cuda").to(DTYPES[dtype])
+    parts = quantize_int4_impl(w, group, True)
+    want, back = int4_matmul_impl(x, *parts, 40), dequantize_int4_impl(*parts, (260, 40))
+    for ahead in (1, 2, 3, 4):
+        moved = []
+        for t in parts:
+            flat = torch.empty(t.numel() + ahead, dtype=t.dtype, device="cuda")
+            moved.append(flat[ahead:].view(t.shape).copy_(t))
+            assert moved[-1].is_contiguous() and moved[-1].data_ptr() % 512 == ahead * t.element_size()
+        assert torch.equal(int4_matmul_impl(x, *moved, 40), want) and torch.equal(dequantize_int4_impl(*moved, (260, 40)), back)
