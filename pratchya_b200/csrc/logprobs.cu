@@ -373,6 +373,11 @@ __device__ void best_of_slice(Shared<THREADS>& sh, const Slice<T>& sl, const Bes
   }
 }
 
+// A CTA's shared memory may be written from the others of its cluster once it runs: every thread says so at its kernel's start, and waits for the others' word where
+// they have long given it (none is late by more than the launch).  Between the two nothing is ordered, so the first is relaxed.
+__device__ __forceinline__ void cluster_here() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
+__device__ __forceinline__ void cluster_all_here() { asm volatile("barrier.cluster.wait;" ::: "memory"); }
+
 struct Forward {
   const void* logits;
   Rows rows;
@@ -384,7 +389,8 @@ struct Forward {
 };
 
 // One row per cluster of CTAs (of one CTA where there are rows enough to fill the chip); its CTAs' terms and best logits meet in the first one, which the
-// others write to: behind the one barrier that this takes they are done (reading from the first CTA took two, and 1.2 us more for a single row).
+// others write to: behind one barrier they are done (reading from the first CTA took two, and 1.2 us more for a single row).  That the first CTA runs
+// they know from a barrier that is begun at the kernel's start and ended in front of the writes, a whole stream later.
 // With alternatives a row is two phases, the stream (22000 cycles of a 128 KB row among three others on the SM) and the selection (half as many for 64 of them, a
 // quarter for five), which other rows' streams hide in part: more, smaller CTAs are better until the selection is longer than they can hide.
 // TOP: 0 for no alternatives, 1 for up to kHalve, 2 for more (in one kernel few of them took 1 to 3 % longer).
@@ -395,6 +401,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
   constexpr int kVec = Vec<T>::kSize, kWarps = THREADS / 32;
   cg::cluster_group cluster = cg::this_cluster();
   const uint32_t ctas = cluster.num_blocks(), rank = cluster.block_rank(), tid = threadIdx.x;
+  if (ctas > 1) cluster_here();
   const uint32_t row = ctas == 1 ? blockIdx.x : blockIdx.x / ctas;
   const T* z = static_cast<const T*>(p.logits) + p.rows.at(row);
   const Slice<T> sl(z, p.vocab, rank, ctas);
@@ -507,6 +514,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
   if (TOP && own) best_of_slice<T, THREADS, TOP == 2>(sh, sl, best, mine, raw, own, p.vocab);
   else __syncthreads();
   if (ctas > 1) {      // everyone hands what it has to the first CTA
+    cluster_all_here();
     Shared<THREADS>* to = cluster.map_shared_rank(&sh, 0);
     if (TOP)
       for (uint32_t i = tid; i < p.top; i += THREADS) to->gathered[rank * p.top + i] = i < own ? sh.sorted[i] : 0;

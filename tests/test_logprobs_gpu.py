@@ -406,3 +406,22 @@ def test_refusals(built_lib):
     empty = z[:0].clone().requires_grad_(True)
     token_logprobs(empty, tokens[:0], 3).entropy.sum().backward()
     assert empty.grad.shape == (0, 1000)
+
+
+@pytest.mark.parametrize("ctas", [2, 4, 8])
+@pytest.mark.parametrize("vocab,top", [(1, 1), (40, 20), (4099, 0), (4099, 5), (4099, 128)])
+def test_rows_so_short_that_a_cluster_has_hardly_begun(built_lib, diag_lib, monkeypatch, ctas, vocab, top):
+    """The diagnostics build gives a row to as many CTAs as it is told: of a short row most have nothing, and hand that to the first one at once."""
+    monkeypatch.setenv("PB_LP_CTAS", str(ctas))
+    rows = 301
+    z, tokens = _case(rows, vocab, "f32", ctas + vocab)
+    tokens = tokens.clamp(min=0)
+    f32 = lambda *shape: torch.full(shape, math.nan, device="cuda")
+    logprobs, entropy, tops, best = f32(rows), f32(rows), f32(rows, top), torch.full((rows, top), -1, device="cuda")
+    assert diag_lib.pb_token_logprobs(z.data_ptr(), 0, 1, rows, 0, vocab, vocab, tokens.data_ptr(), 1, top, logprobs.data_ptr(), entropy.data_ptr(), tops.data_ptr() if top else None,
+                                      best.data_ptr() if top else None, None, torch.cuda.current_stream().cuda_stream) == 0
+    picked, want, values, order, logp, p, dead = _definition(z, tokens, top)
+    log_s, e_log_s, e_entropy = _errors(z, logp, p, dead)
+    assert torch.equal(best, order) and ((entropy.double() - want).abs() <= e_entropy).all()
+    for got, exact in ((logprobs.unsqueeze(-1), picked.unsqueeze(-1)), (tops, values)):
+        assert ((got.double() - exact).abs() <= e_log_s.unsqueeze(-1) + 2.0 ** -23 * (exact.abs() + log_s.unsqueeze(-1))).all()
