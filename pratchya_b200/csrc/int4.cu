@@ -43,7 +43,8 @@ constexpr float kRound = 12582912.0f;      // added to a number below 2^22 in si
 constexpr uint32_t kRoundBits = 0x4b400000u;
 
 // ZERO: scale = bf16((max(w, 0) - min(w, 0)) / 15), zero = rint(-min / scale), u = rint(w / scale) + zero, both within 0..15;
-// otherwise scale = bf16(max|w| / 7), u = rint(w / scale) + 8: the scale is 2^-9 of itself too small at most, and u within 1..15 by itself.
+// otherwise scale = bf16(max|w| / 7), u = rint(w / scale) + 8 within 0..15: a normal scale is 2^-9 of itself too small at most, and u within 1..15 by itself; a subnormal
+// one may be a third too small, and there, alone, the values are brought to its reach first.
 // A group of nothing but zeros has scale 0.  The scale is rounded before the codes are taken: they are the nearest ones for the scale that is stored.
 // A group that holds a NaN or an infinity has a scale that is no finite number.
 // A thread has COLS neighbouring columns (two where one load brings two bf16) and 32 / COLS values of k of each.  f32 [2048, 8192] in 16.1 us (floor 11.6), [2048, 65536]
@@ -98,6 +99,9 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_int4_kernel(const T* _
       high[c] = max_nan(high[c], highs[first + o][col]);
     }
     const float s = __bfloat162float(__float2bfloat16_rn(ZERO ? __fdiv_rn(__fsub_rn(high[c], low[c]), 15.0f) : __fdiv_rn(high[c], 7.0f)));
+    if (!ZERO && s < 0x1p-126f && s > 0.0f)
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) v[c][i] = fminf(fmaxf(v[c][i], -8.0f * s), 7.0f * s);
     const float z = !ZERO ? 8.0f : s != 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(-low[c], s)), 0.0f), 15.0f) : 0.0f;
     // Correctly rounded quotients by a reciprocal and two corrections, of numbers that a power of two has taken from the ends of the range (what it loses of a
     // number below 2^-62 is nothing beside a scale above 2^90).  A scale of zero or no number: codes of 0, or any.

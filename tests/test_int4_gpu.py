@@ -277,3 +277,27 @@ def test_parts_that_lie_anywhere_in_a_flat_buffer(built_lib, group, dtype):
             moved.append(flat[ahead:].view(t.shape).copy_(t))
             assert moved[-1].is_contiguous() and moved[-1].data_ptr() % 512 == ahead * t.element_size()
         assert torch.equal(int4_matmul_impl(x, *moved, 40), want) and torch.equal(dequantize_int4_impl(*moved, (260, 40)), back)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("zero_points", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_quantizer_of_the_smallest_numbers(built_lib, group, zero_points, dtype):
+    """Groups whose largest value is 1 to 50 of bf16's smallest step: a scale is a few such steps there, up to a third off the quotient, and the codes of the ends lie beyond 0..15 but
+    for the clamp."""
+    g = torch.Generator(device="cuda").manual_seed(group)
+    depth, cols = 256, 50
+    most = torch.arange(1, cols + 1, device="cuda").float()
+    w = (torch.rand(depth, cols, generator=g, device="cuda") * (2 * most + 1)).floor() - most
+    w[::32], w[1::32] = most, -most                    # both ends in every group
+    w[:, 1::3] = w[:, 1::3].abs()
+    w[:, 2::3] = -w[:, 2::3].abs()
+    w = (w * 2.0 ** -133).to(DTYPES[dtype])
+    q, scale, zero = quantize_int4_impl(w, group, zero_points)
+    u, s, z = _rule(w, group, zero_points)
+    assert torch.equal(_codes(q, depth, cols), u.long())
+    assert torch.equal(_parts(scale, depth, cols, group).float(), s)
+    if zero_points:
+        assert torch.equal(_parts(zero, depth, cols, group).float(), z)
+    want = (u - z.repeat_interleave(group, 0)) * s.repeat_interleave(group, 0)
+    assert torch.equal(dequantize_int4_impl(q, scale, zero, (depth, cols)), want)
