@@ -98,7 +98,9 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_int4_kernel(const T* _
       if (ZERO) low[c] = -max_nan(-low[c], -lows[first + o][col]);
       high[c] = max_nan(high[c], highs[first + o][col]);
     }
-    const float s = __bfloat162float(__float2bfloat16_rn(ZERO ? __fdiv_rn(__fsub_rn(high[c], low[c]), 15.0f) : __fdiv_rn(high[c], 7.0f)));
+    float span = ZERO ? __fsub_rn(high[c], low[c]) : high[c], steps = ZERO ? 15.0f : 7.0f;
+    if (ZERO && span == INFINITY) { span = 0.5f * high[c] - 0.5f * low[c]; steps = 7.5f; }      // of finite weights, twice what the type holds
+    const float s = __bfloat162float(__float2bfloat16_rn(__fdiv_rn(span, steps)));
     if (!ZERO && s < 0x1p-126f && s > 0.0f)
 #pragma unroll
       for (int i = 0; i < kRows; ++i) v[c][i] = fminf(fmaxf(v[c][i], -8.0f * s), 7.0f * s);

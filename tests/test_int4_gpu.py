@@ -301,3 +301,23 @@ def test_quantizer_of_the_smallest_numbers(built_lib, group, zero_points, dtype)
         assert torch.equal(_parts(zero, depth, cols, group).float(), z)
     want = (u - z.repeat_interleave(group, 0)) * s.repeat_interleave(group, 0)
     assert torch.equal(dequantize_int4_impl(q, scale, zero, (depth, cols)), want)
+
+
+def test_quantizer_of_groups_whose_span_is_beyond_f32(built_lib):
+    """Finite weights of both signs whose largest less smallest is no f32: the scale is a fifteenth of it all the same, and the weights read back finite."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    w = (torch.randint(-12, 13, (256, 40), generator=g, device="cuda").double() * 2.0 ** 124).float()
+    w[::32], w[1::32] = -1.5 * 2.0 ** 127, 1.25 * 2.0 ** 127
+    w[:, 7] = -w[:, 7].abs()                           # of one sign: no more than the type holds
+    for dtype in (torch.float32, torch.bfloat16):
+        x = w.to(dtype)
+        q, scale, zero = quantize_int4_impl(x, 64, True)
+        v = x.double().view(4, 64, 40)
+        low, high = v.amin(1).clamp(max=0), v.amax(1).clamp(min=0)
+        s = ((high - low) / 15).float().bfloat16()
+        z = torch.round(-low / s.double()).clamp(0, 15)
+        u = (torch.round(v / s.double().unsqueeze(1)) + z.unsqueeze(1)).clamp(0, 15).view(256, 40)
+        assert torch.equal(_parts(scale, 256, 40, 64), s) and torch.isfinite(s).all()
+        assert torch.equal(_parts(zero, 256, 40, 64).double(), z) and torch.equal(_codes(q, 256, 40), u.long())
+        want = ((u - z.repeat_interleave(64, 0)) * s.double().repeat_interleave(64, 0)).float()
+        assert torch.equal(dequantize_int4_impl(q, scale, zero, (256, 40)), want) and torch.isfinite(want).all()
