@@ -37,6 +37,8 @@ def token_logprobs(logits, tokens=None, top: int = 0) -> TokenLogprobs:
     derivative = wants_derivative(logits)
     out = _lib.native().token_logprobs(logits, tokens, top, derivative)
     if out is None:          # what has to be converted first, or refused
+        if torch.jit.is_tracing():          # a trace would hold the results as constants
+            raise RuntimeError("token_logprobs cannot be traced")
         logits, tokens, top = _checked(logits, tokens, top)
         out = _lib.native().token_logprobs(logits, tokens, top, derivative)
         if out is None:
@@ -46,9 +48,9 @@ def token_logprobs(logits, tokens=None, top: int = 0) -> TokenLogprobs:
 
 def wants_derivative(x) -> bool:
     """Whether anything can ask for a derivative of an op on x: a graph that x is in, or forward-mode differentiation or a function transform under way (which the
-    op's autograd.Function then refuses)."""
+    op's autograd.Function then refuses).  Torch has no public name for the level of the former; where its own is gone, the answer is yes."""
     if torch.is_grad_enabled():
-        return (isinstance(x, torch.Tensor) and x.requires_grad) or forward_ad._current_level >= 0
+        return (isinstance(x, torch.Tensor) and x.requires_grad) or getattr(forward_ad, "_current_level", 0) >= 0
     return not no_graph()
 
 

@@ -9,11 +9,25 @@ With A = ceil(N / 16) and B = ceil(K / 128): q uint8 [A, B, 1024], scale bf16 [A
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 from ._ops import _require_cuda
 
 GROUPS = (32, 64, 128)
+
+
+def _no_derivative(what, *tensors):
+    """Refuses where a derivative could be asked for that the op does not have, or a trace would hold its result as a constant (the extension leaves such calls alone)."""
+    if torch.jit.is_tracing():
+        raise RuntimeError(f"{what} cannot be traced")
+    for t in tensors:
+        if not isinstance(t, torch.Tensor):
+            continue
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad(), or with detached tensors")
+        if getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what} has no forward-mode derivative")
 
 
 def _int4_parts(q, scale, zero, depth, cols, what):
@@ -41,7 +55,7 @@ def _at(t, align):
 def quantize_int4_impl(w: torch.Tensor, group: int = 128, zero_points: bool = False):
     """(q, scale, zero or None) of w [K, N]; K and N may be any sizes.  scale = bf16(max|w| / 7) of a group and u = rint(w / scale) + 8; with
     zero points scale = bf16((max(w, 0) - min(w, 0)) / 15), zero = rint(-min / scale) and u = rint(w / scale) + zero.  The codes are the nearest
-    ones for the scale as stored."""
+    ones for the scale as stored.  Like the other quantizers of this package it takes w's values: no graph leads back to w."""
     _require_cuda(w, "quantize_int4_impl input")
     if w.dim() != 2 or w.numel() == 0:
         raise ValueError(f"quantize_int4_impl: a weight of {tuple(w.shape)} is no [K, N]")
@@ -51,17 +65,19 @@ def quantize_int4_impl(w: torch.Tensor, group: int = 128, zero_points: bool = Fa
         w = w.to(torch.float32)
     out = _lib.native().quantize_int4(w.detach().contiguous(), group, bool(zero_points))
     if out is None:
+        _no_derivative("quantize_int4_impl")
         raise RuntimeError("quantize_int4_impl takes plain CUDA tensors only")
     return out
 
 
 def dequantize_int4_impl(q, scale, zero, shape, dtype=torch.float32):
-    """The values [K, N] that the parts of a weight of that shape stand for."""
+    """The values [K, N] that the parts of a weight of that shape stand for.  Not differentiable in the scale."""
     depth, cols = (int(n) for n in shape)
     if dtype not in (torch.float32, torch.bfloat16):
         raise TypeError(f"dequantize_int4_impl: {dtype}; float32 and bfloat16 are built")
     out = _lib.native().dequantize_int4(q, scale, zero, depth, cols, dtype)
     if out is None:
+        _no_derivative("dequantize_int4_impl", scale)
         out = _lib.native().dequantize_int4(*_int4_parts(q, scale, zero, depth, cols, "dequantize_int4_impl"), depth, cols, dtype)
         if out is None:
             raise RuntimeError("dequantize_int4_impl takes plain CUDA tensors only")
@@ -72,12 +88,11 @@ def int4_matmul_impl(x, q, scale, zero, cols: int, dtype=None):
     """x [..., K] times a weight of [K, cols] in its parts, in x's type or `dtype`.  Sums are f32; x keeps its bits but for what is far below its
     neighbours (of 128 the largest has 2^30 steps above zero where x is f32, 2^22 at least where it is bf16, and the others the same steps).  A row of x with an
     infinity or a NaN has no finite products.  Made for few rows: the weight is read once for every 32 of a bf16 x and every eight of an f32 one.
-    Not differentiable: an x that asks for a gradient is refused."""
-    if isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("int4_matmul_impl has no backward pass: call it under torch.no_grad(), or with x.detach()")
+    Not differentiable: an x or a scale that asks for a gradient or carries a tangent is refused, and so is tracing."""
     out = _lib.native().int4_product(x, q, scale, zero, cols, dtype)
     if out is not None:
         return out
+    _no_derivative("int4_matmul_impl", x, scale)
     _require_cuda(x, "int4_matmul_impl input")
     if x.dim() == 0:
         raise ValueError("int4_matmul_impl: x has no dimension")

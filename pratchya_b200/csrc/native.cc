@@ -26,6 +26,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <initializer_list>
 #include <numeric>
@@ -677,6 +678,11 @@ OP(rows_at_two_strides) {
   END_HANDLE_TH_ERRORS
 }
 
+// a call whose result a trace would hold as a constant: the Python text refuses it
+bool traced() { return torch::jit::tracer::isTracing(); }
+// a tensor that a derivative may be asked for, backward or forward: the Python text refuses it where the op has none
+bool differentiable(const at::Tensor& t) { return (t.requires_grad() && at::GradMode::is_enabled()) || t._fw_grad(0).defined(); }
+
 struct Scores { at::Tensor logprobs, entropy, top_logprobs, top_tokens, stats; };
 // of rows that plain_rows has found, n tokens of each (as tokens' shape has them); stats only for a backward pass
 int scores_of(const at::Tensor& z, const StridedRows& r, const at::Tensor* tokens, int64_t n, int64_t top, bool backward, Scores* out) {
@@ -750,7 +756,7 @@ OP(token_logprobs) {
   StridedRows r;
   const at::Tensor *z = plain_rows(args[0], &r), *tokens = args[1] == Py_None ? nullptr : plain(args[1]);
   const long long top = integer(args[2]);
-  if (!z || watched() || (args[1] != Py_None && (!tokens || tokens->scalar_type() != at::kLong || tokens->device() != z->device())) || !PyLong_Check(args[2]) || top < 0 || top > 128 ||
+  if (!z || watched() || traced() || (args[1] != Py_None && (!tokens || tokens->scalar_type() != at::kLong || tokens->device() != z->device())) || !PyLong_Check(args[2]) || top < 0 || top > 128 ||
       z->size(-1) == 0 || top > z->size(-1))
     return none();
   int64_t n = 0;
@@ -784,7 +790,7 @@ OP(quantize_int4) {
   const at::Tensor* w = plain(args[0]);
   const int group = small(args[1]);
   const bool zeros = PyObject_IsTrue(args[2]) == 1;
-  if (!w || watched() || !dense(w->scalar_type()) || w->dim() != 2 || w->numel() == 0 || (group != 32 && group != 64 && group != 128)) return none();
+  if (!w || watched() || traced() || !dense(w->scalar_type()) || w->dim() != 2 || w->numel() == 0 || (group != 32 && group != 64 && group != 128)) return none();
   const c10::cuda::CUDAGuard guard(w->device());
   const int64_t depth = w->size(0), cols = w->size(1), a = (cols + 15) / 16, b = (depth + 127) / 128;
   at::Tensor q = fresh({a, b, 1024}, at::kByte), scale = fresh({a, b, 16, 128 / group}, at::kBFloat16), zero;
@@ -825,7 +831,7 @@ OP(dequantize_int4) {
   NARGS(6);
   const int64_t depth = integer(args[3]), cols = integer(args[4]);
   Int4 w;
-  if (watched() || !THPDtype_Check(args[5]) || !w.take(args, depth, cols)) return none();
+  if (watched() || traced() || !THPDtype_Check(args[5]) || !w.take(args, depth, cols) || differentiable(*w.scale)) return none();
   const at::ScalarType type = reinterpret_cast<THPDtype*>(args[5])->scalar_type;
   if (!dense(type)) return none();
   const c10::cuda::CUDAGuard guard(w.q->device());
@@ -843,7 +849,9 @@ OP(int4_product) {
   const at::Tensor* x = plain_rows(args[0], &r);
   const int64_t cols = integer(args[4]);
   Int4 w;
-  if (!x || watched() || r.outer != 1 || (args[5] != Py_None && !THPDtype_Check(args[5])) || !w.take(args + 1, x->size(-1), cols) || x->device() != w.q->device()) return none();
+  if (!x || watched() || traced() || r.outer != 1 || (args[5] != Py_None && !THPDtype_Check(args[5])) || !w.take(args + 1, x->size(-1), cols) || x->device() != w.q->device() ||
+      differentiable(*x) || differentiable(*w.scale))
+    return none();
   const at::ScalarType type = args[5] == Py_None ? x->scalar_type() : reinterpret_cast<THPDtype*>(args[5])->scalar_type;
   if (!dense(type)) return none();
   const c10::cuda::CUDAGuard guard(x->device());

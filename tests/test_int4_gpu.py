@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from pratchya_b200._qualia import dequantize_int4_impl, int4_matmul_impl, quantize_int4_impl
 
@@ -321,3 +322,27 @@ def test_quantizer_of_groups_whose_span_is_beyond_f32(built_lib):
         assert torch.equal(_parts(zero, 256, 40, 64).double(), z) and torch.equal(_codes(q, 256, 40), u.long())
         want = ((u - z.repeat_interleave(64, 0)) * s.double().repeat_interleave(64, 0)).float()
         assert torch.equal(dequantize_int4_impl(q, scale, zero, (256, 40)), want) and torch.isfinite(want).all()
+
+
+def test_no_derivative_is_dropped_without_a_word(built_lib):
+    parts = q, scale, zero = quantize_int4_impl(_weight(256, 32, "f32", 1), 64, True)
+    x = torch.randn(2, 256, device="cuda")
+    want = int4_matmul_impl(x, *parts, 32)
+    learned = scale.clone().requires_grad_(True)
+    for f in (lambda: int4_matmul_impl(x.clone().requires_grad_(True), *parts, 32), lambda: int4_matmul_impl(x, q, learned, zero, 32),
+              lambda: dequantize_int4_impl(q, learned, zero, (256, 32))):
+        with pytest.raises(RuntimeError, match="backward"):
+            f()
+        with torch.no_grad():
+            f()
+    for grads in (True, False):
+        with torch.set_grad_enabled(grads), forward_ad.dual_level():
+            dual, scales = forward_ad.make_dual(x, torch.ones_like(x)), forward_ad.make_dual(scale, torch.ones_like(scale))
+            for f in (lambda: int4_matmul_impl(dual, *parts, 32), lambda: int4_matmul_impl(x, q, scales, zero, 32), lambda: dequantize_int4_impl(q, scales, zero, (256, 32))):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    f()
+            assert torch.equal(int4_matmul_impl(x, *parts, 32), want)          # nobody's tangent
+        with torch.set_grad_enabled(grads):
+            for f in (lambda t: int4_matmul_impl(t, *parts, 32), lambda t: quantize_int4_impl(t, 64)[0], lambda t: dequantize_int4_impl(*parts, (256, 32)) + t.sum()):
+                with pytest.raises(RuntimeError, match="traced"):
+                    torch.jit.trace(f, x, check_trace=False)

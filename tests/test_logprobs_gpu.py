@@ -5,6 +5,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from pratchya_b200._nnx_impl import token_logprobs
 
@@ -425,3 +426,17 @@ def test_rows_so_short_that_a_cluster_has_hardly_begun(built_lib, diag_lib, monk
     assert torch.equal(best, order) and ((entropy.double() - want).abs() <= e_entropy).all()
     for got, exact in ((logprobs.unsqueeze(-1), picked.unsqueeze(-1)), (tops, values)):
         assert ((got.double() - exact).abs() <= e_log_s.unsqueeze(-1) + 2.0 ** -23 * (exact.abs() + log_s.unsqueeze(-1))).all()
+
+
+def test_no_derivative_is_dropped_without_a_word(built_lib, monkeypatch):
+    z, tokens = _case(3, 1000, "f32", 23)
+    for grads in (True, False):
+        with torch.set_grad_enabled(grads):
+            with forward_ad.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
+                token_logprobs(forward_ad.make_dual(z, torch.ones_like(z)), tokens, 2)
+            with pytest.raises(RuntimeError, match="traced"):
+                torch.jit.trace(lambda t: token_logprobs(t, tokens, 2).entropy, z, check_trace=False)
+    monkeypatch.delattr(forward_ad, "_current_level")          # a torch without its own name for it
+    for grads in (True, False):
+        with torch.set_grad_enabled(grads):
+            assert torch.equal(token_logprobs(z, tokens, 2).entropy, token_logprobs(z.clone().requires_grad_(True), tokens, 2).entropy.detach())
