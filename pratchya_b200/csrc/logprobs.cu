@@ -566,6 +566,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
   }
 }
 
+constexpr float kNothing = -1000.0f;       // a log probability below it is a probability of 0, and times an entropy's cotangent of up to 2^117 it is finite
+
 struct Backward {
   const void* logits;
   Rows rows;
@@ -602,7 +604,8 @@ __global__ void __launch_bounds__(kBackThreads) token_logprobs_bwd_kernel(const 
   T* dz = static_cast<T*>(p.dlogits) + (int64_t)row * p.vocab;
   const uint32_t n = p.n_tokens + p.top;
   const float2 st = p.stats[row];
-  const float g_entropy = p.g_entropy ? p.g_entropy[row] : 0.0f, entropy = p.g_entropy ? p.entropy[row] : 0.0f;
+  const bool dead = st.y == INFINITY;
+  const float g_entropy = p.g_entropy && !dead ? p.g_entropy[row] : 0.0f, entropy = p.g_entropy ? p.entropy[row] : 0.0f;
   for (uint32_t i = tid; i < n; i += kBackThreads) {
     const bool given = i < p.n_tokens;
     int64_t j = given ? p.tokens[(int64_t)row * p.n_tokens + i] : p.top_tokens[(int64_t)row * p.top + i - p.n_tokens];
@@ -620,12 +623,12 @@ __global__ void __launch_bounds__(kBackThreads) token_logprobs_bwd_kernel(const 
     if (tid == 0) total = sum;
   }
   __syncthreads();
-  // p_j (c - g_entropy log p_j), with everything that a row has one of in c
-  const float c = fmaf(-g_entropy, entropy, -total);
+  // p_j (c - g_entropy log p_j), with everything that a row has one of in c.  A row without any logit has no gradient, whatever its cotangents.
+  const float c = dead ? 0.0f : fmaf(-g_entropy, entropy, -total);
   const float2 minus_m = make_float2(-st.x, -st.x), minus_s = make_float2(-st.y, -st.y), scale = make_float2(kLog2e, kLog2e), minus_g = make_float2(-g_entropy, -g_entropy), c2 = make_float2(c, c);
   auto gradient = [&](const float2& v) {
     float2 x = __fadd2_rn(__fadd2_rn(v, minus_m), minus_s);
-    x = make_float2(max_nan(x.x, kFar), max_nan(x.y, kFar));
+    x = make_float2(max_nan(x.x, kNothing), max_nan(x.y, kNothing));
     const float2 a = __fmul2_rn(x, scale);
     return __fmul2_rn(make_float2(exp2_fast(a.x), exp2_fast(a.y)), __ffma2_rn(minus_g, x, c2));
   };
@@ -645,7 +648,7 @@ __global__ void __launch_bounds__(kBackThreads) token_logprobs_bwd_kernel(const 
     for (int e = 0; e < kVec / 2; ++e) v[e] = gradient(v[e]);
     out[j] = Vec<T>::pack(v);
   }
-  if (n == 0 || st.y == INFINITY) return;      // a row without any logit has no gradient
+  if (n == 0 || dead) return;
   __syncthreads();
   for (uint32_t i = tid; i < n; i += kBackThreads) {
     const int64_t j = at[i];

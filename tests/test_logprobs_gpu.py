@@ -440,3 +440,38 @@ def test_no_derivative_is_dropped_without_a_word(built_lib, monkeypatch):
     for grads in (True, False):
         with torch.set_grad_enabled(grads):
             assert torch.equal(token_logprobs(z, tokens, 2).entropy, token_logprobs(z.clone().requires_grad_(True), tokens, 2).entropy.detach())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_gradient_of_rows_without_a_logit_whatever_their_cotangents(built_lib, dtype):
+    """A loss that divides or takes an exponential of the -inf of such a row hands back what is no number: the row has no gradient all the same, nor do the others lose theirs."""
+    z, tokens = _case(4, 3001, dtype, 41, n=2)
+    tokens = tokens.clamp(min=0)
+    z[1] = -math.inf
+    z.requires_grad_(True)
+    out = token_logprobs(z, tokens, 3)
+    cotangents = [torch.ones_like(t) for t in (out.logprobs, out.entropy, out.top_logprobs)]
+    (want,) = torch.autograd.grad(out[:3], z, cotangents, retain_graph=True)
+    for bad in (math.nan, math.inf, -math.inf):
+        for which in range(3):
+            g = [c.clone() for c in cotangents]
+            g[which][1] = bad
+            (got,) = torch.autograd.grad(out[:3], z, g, retain_graph=True)
+            assert torch.equal(got, want) and (got[1] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_gradient_of_masked_logits_under_large_cotangents(built_lib, dtype):
+    """What has no probability has no gradient, however large the entropy's cotangent is; the others' is that many times the one of a cotangent of 1."""
+    z, _ = _case(3, 2003, dtype, 43, sharp=1.0)
+    z[0, 5:1000] = -math.inf
+    z[1, 7:] = torch.finfo(z.dtype).min
+    z.requires_grad_(True)
+    entropy = token_logprobs(z).entropy
+    (one,) = torch.autograd.grad(entropy.sum(), z, retain_graph=True)
+    for power in (29, 60, 90, 110):
+        (got,) = torch.autograd.grad(entropy, z, torch.full_like(entropy, 2.0 ** power), retain_graph=True)
+        assert (got[0, 5:1000] == 0).all() and (got[1, 7:] == 0).all()
+        # what is below the type's normal numbers for a cotangent of 1 has fewer bits there
+        fine = one.abs() >= 2.0 ** -100
+        assert torch.equal(got[fine], (one.double() * 2.0 ** power).to(z.dtype)[fine]) and torch.isfinite(got).all()
