@@ -402,7 +402,8 @@ PB_API int pb_dense_dot(int tokens, const uint8_t* q, const uint8_t* sc8, const 
  *   top_tokens, top_logprobs [rows][top]  the `top` (at most 128) largest logits, equal ones in the order of their indices (-0 is 0, NaN ranks with -inf)
  * all in f32.  A row of nothing but -inf has log probabilities of -inf and an entropy of 0; a row with a NaN or +inf has NaN.  entropy and stats may be null.
  * stats [rows][2] is for the backward call, which writes dlogits [rows][vocab] (the logits' type, contiguous) from the cotangents of logprobs, entropy and
- * top_logprobs (each may be null):  dz_j = sum g_i [j == token_i] + sum h_i [j == top_i] - p_j (sum g_i + sum h_i + g_entropy (log p_j + entropy)). */
+ * top_logprobs (each may be null):  dz_j = sum g_i [j == token_i] + sum h_i [j == top_i] - p_j (sum g_i + sum h_i + g_entropy (log p_j + entropy)).
+ * stats is 8-byte and dlogits 16-byte aligned, every other array as its type is. */
 PB_API int pb_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t stride_outer, int64_t stride_inner, int64_t vocab,
                       const int64_t* tokens, int n_tokens, int top, float* logprobs, float* entropy, float* top_logprobs, int64_t* top_tokens,
                       float* stats, void* stream);
@@ -421,7 +422,7 @@ PB_API int pb_token_logprobs_bwd(const void* logits, int dtype, int64_t outer, i
  * pb_int4_product: out[rows, cols] = x[rows, depth] w, x's rows `stride` elements apart, sums in f32.  x is not rounded to fewer bits than it has but for what is far below its
  * neighbours: of 128 that begin at a multiple of 128 the largest has 2^30 (f32) or 2^22 (bf16, one or two rows and many columns) steps above zero, the others the same steps.
  * A row of x with an infinity or a NaN has no finite products.  Made for few rows: the weight is read once for every 32 rows of a bf16 x and every eight of an f32 one.
- * q is 16-byte aligned; the product wants scale at a multiple of 2 * 128 / group bytes and zero at one of 128 / group. */
+ * q is 16-byte aligned and every other array as its type is, but that the product wants scale at a multiple of 2 * 128 / group bytes and zero at one of 128 / group. */
 PB_API int pb_quantize_int4(const void* w, int dtype, int64_t depth, int64_t cols, int group, uint8_t* q, void* scale, uint8_t* zero, void* stream);
 PB_API int pb_dequantize_int4(const uint8_t* q, const void* scale, const uint8_t* zero, int64_t depth, int64_t cols, int group, void* out, int dtype, void* stream);
 PB_API int pb_int4_product(const void* x, int x_dtype, int64_t rows, int64_t depth, int64_t stride, const uint8_t* q, const void* scale, const uint8_t* zero, int group,

@@ -44,6 +44,8 @@ cudaError_t launch_behind(void (*kernel)(Params...), dim3 grid, dim3 block, size
 }
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+inline bool off_by(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
+
 #define PB_LAUNCH_CHECK(name)                                                      \
   do {                                                                             \
     cudaError_t _e = cudaGetLastError();                                           \

@@ -737,7 +737,7 @@ extern "C" int pb_quantize_int4(const void* w, int dtype, int64_t depth, int64_t
   if (!w || !q || !scale) return fail(PB_ERR_NULL_POINTER, "pb_quantize_int4: null argument");
   if (dtype != PB_F32 && dtype != PB_BF16) return fail(PB_ERR_BAD_DTYPE, "pb_quantize_int4: dtype %d", dtype);
   if (int s = check_int4("pb_quantize_int4", depth, cols, group)) return s;
-  if (reinterpret_cast<uintptr_t>(q) & 15) return fail(PB_ERR_MISALIGNED, "pb_quantize_int4: q must be 16-byte aligned");
+  if (off_by(q, 16) || off_by(w, dtype == PB_F32 ? 4 : 2) || off_by(scale, 2)) return fail(PB_ERR_MISALIGNED, "pb_quantize_int4: q 16 bytes, w and scale their types");
   const uint32_t kblocks = (uint32_t)((depth + 127) / 128), col_blocks = (uint32_t)((cols + kQuantCols - 1) / kQuantCols);
   if (col_blocks > 65535) return fail(PB_ERR_UNSUPPORTED, "pb_quantize_int4: %lld columns", (long long)cols);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -763,7 +763,7 @@ extern "C" int pb_dequantize_int4(const uint8_t* q, const void* scale, const uin
   if (!q || !scale || !out) return fail(PB_ERR_NULL_POINTER, "pb_dequantize_int4: null argument");
   if (dtype != PB_F32 && dtype != PB_BF16) return fail(PB_ERR_BAD_DTYPE, "pb_dequantize_int4: dtype %d", dtype);
   if (int s = check_int4("pb_dequantize_int4", depth, cols, group)) return s;
-  if (reinterpret_cast<uintptr_t>(q) & 15) return fail(PB_ERR_MISALIGNED, "pb_dequantize_int4: q must be 16-byte aligned");
+  if (off_by(q, 16) || off_by(out, dtype == PB_F32 ? 4 : 2) || off_by(scale, 2)) return fail(PB_ERR_MISALIGNED, "pb_dequantize_int4: q 16 bytes, scale and out their types");
   const uint32_t kblocks = (uint32_t)((depth + 127) / 128), col_blocks = (uint32_t)((cols + kQuantCols - 1) / kQuantCols);
   if (col_blocks > 65535) return fail(PB_ERR_UNSUPPORTED, "pb_dequantize_int4: %lld columns", (long long)cols);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -786,8 +786,7 @@ extern "C" int pb_int4_product(const void* x, int x_dtype, int64_t rows, int64_t
   if (rows == 0) return PB_OK;
   if (!x || !q || !scale || !out) return fail(PB_ERR_NULL_POINTER, "pb_int4_product: null argument");
   const int per_group = 128 / group;      // a lane loads as many scales, and zero points, at once
-  if ((reinterpret_cast<uintptr_t>(q) & 15) || reinterpret_cast<uintptr_t>(scale) % (2 * per_group) || reinterpret_cast<uintptr_t>(zero) % per_group ||
-      (reinterpret_cast<uintptr_t>(x) % (x_dtype == PB_F32 ? 4 : 2)) || (reinterpret_cast<uintptr_t>(out) % (out_dtype == PB_F32 ? 4 : 2)))
+  if (off_by(q, 16) || off_by(scale, 2 * per_group) || off_by(zero, per_group) || off_by(x, x_dtype == PB_F32 ? 4 : 2) || off_by(out, out_dtype == PB_F32 ? 4 : 2))
     return fail(PB_ERR_MISALIGNED, "pb_int4_product: q 16, scale %d and zero %d bytes, x and out their types", 2 * per_group, per_group);
   if ((uint64_t)((cols + 15) / 16) * ((depth + 127) / 128) > 0x7fffffffull) return fail(PB_ERR_BAD_SHAPE, "pb_int4_product: depth=%lld cols=%lld", (long long)depth, (long long)cols);
   Product p{x, stride, q, static_cast<const __nv_bfloat16*>(scale), zero, out, (uint32_t)rows, (uint32_t)depth, (uint32_t)cols, (uint32_t)((depth + 127) / 128),

@@ -709,7 +709,7 @@ int check_rows(const char* who, const void* logits, int dtype, int64_t outer, in
     return fail(PB_ERR_BAD_SHAPE, "%s: %d tokens and %d alternatives of %lld (at most %d and %d)", who, n_tokens, top, (long long)vocab, kMaxTokens, kMaxTop);
   if (inner > 0 && outer > 0x7fffffffll / kMaxCluster / inner) return fail(PB_ERR_BAD_SHAPE, "%s: too many rows (%lld x %lld)", who, (long long)outer, (long long)inner);
   if (outer * inner > 0 && (!logits || (n_tokens && !tokens))) return fail(PB_ERR_NULL_POINTER, "%s: null argument", who);
-  if (reinterpret_cast<uintptr_t>(logits) % (dtype == PB_F32 ? 4 : 2)) return fail(PB_ERR_MISALIGNED, "%s: logits are not aligned to their type", who);
+  if (off_by(logits, dtype == PB_F32 ? 4 : 2) || off_by(tokens, 8)) return fail(PB_ERR_MISALIGNED, "%s: logits and tokens lie at their types' bytes", who);
   return PB_OK;
 }
 
@@ -725,7 +725,8 @@ extern "C" int pb_token_logprobs(const void* logits, int dtype, int64_t outer, i
   const int64_t rows = outer * inner;
   if (rows == 0) return PB_OK;
   if ((n_tokens && !logprobs) || (top && (!top_logprobs || !top_tokens))) return fail(PB_ERR_NULL_POINTER, "pb_token_logprobs: null argument");
-  if (reinterpret_cast<uintptr_t>(stats) & 7) return fail(PB_ERR_MISALIGNED, "pb_token_logprobs: stats must be 8-byte aligned");
+  if (off_by(stats, 8) || off_by(top_tokens, 8) || off_by(logprobs, 4) || off_by(entropy, 4) || off_by(top_logprobs, 4))
+    return fail(PB_ERR_MISALIGNED, "pb_token_logprobs: stats 8 bytes, the others their types");
   const Forward p{logits, {FastDiv((uint32_t)inner), stride_outer, stride_inner}, (uint32_t)vocab, (uint32_t)n_tokens, (uint32_t)top, tokens, logprobs, entropy, top_logprobs, top_tokens,
                   reinterpret_cast<float2*>(stats)};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -742,7 +743,8 @@ extern "C" int pb_token_logprobs_bwd(const void* logits, int dtype, int64_t oute
   const int64_t rows = outer * inner;
   if (rows == 0) return PB_OK;
   if (!stats || !dlogits || (top && !top_tokens) || (g_entropy && !entropy)) return fail(PB_ERR_NULL_POINTER, "pb_token_logprobs_bwd: null argument");
-  if ((reinterpret_cast<uintptr_t>(stats) & 7) || (reinterpret_cast<uintptr_t>(dlogits) & 15)) return fail(PB_ERR_MISALIGNED, "pb_token_logprobs_bwd: stats 8 and dlogits 16 bytes");
+  if (off_by(stats, 8) || off_by(dlogits, 16) || off_by(top_tokens, 8) || off_by(entropy, 4) || off_by(g_logprobs, 4) || off_by(g_entropy, 4) || off_by(g_top, 4))
+    return fail(PB_ERR_MISALIGNED, "pb_token_logprobs_bwd: stats 8 and dlogits 16 bytes, the others their types");
   const Backward p{logits, {FastDiv((uint32_t)inner), stride_outer, stride_inner}, (uint32_t)vocab, (uint32_t)n_tokens, (uint32_t)top, tokens, top_tokens,
                    reinterpret_cast<const float2*>(stats), entropy, g_logprobs, g_entropy, g_top, dlogits};
   cudaStream_t st = static_cast<cudaStream_t>(stream);

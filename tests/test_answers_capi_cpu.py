@@ -64,3 +64,18 @@ def test_a_weights_parts_lie_where_a_lane_loads_them_from(built_lib):
     for byte in (1, 2, 3):
         assert _product(built_lib, zero=at(byte), group=32) == 9, byte
     assert _product(built_lib, zero=at(1), group=64) == 9
+
+
+def test_every_array_lies_at_its_types_bytes(built_lib):
+    """Nothing reaches a kernel that would load or store across an element."""
+    at = lambda byte: C.c_void_p(4096 + byte)
+    f, b = built_lib.pb_quantize_int4, built_lib.pb_dequantize_int4
+    assert f(at(2), 0, 128, 16, 128, ONE, ONE, None, None) == 9 and f(at(1), 1, 128, 16, 128, ONE, ONE, None, None) == 9 and f(ONE, 0, 128, 16, 128, ONE, at(1), None, None) == 9
+    assert b(ONE, at(1), None, 128, 16, 128, ONE, 0, None) == 9 and b(ONE, ONE, None, 128, 16, 128, at(2), 0, None) == 9 and b(ONE, ONE, None, 128, 16, 128, at(1), 1, None) == 9
+    for name, byte in (("z", 2), ("tokens", 4), ("lp", 2), ("tl", 2), ("tt", 4), ("stats", 4)):
+        assert _scores(built_lib, **{name: at(byte)}) == 9, name
+    assert built_lib.pb_token_logprobs(ONE, 0, 1, 4, 0, 8, 8, ONE, 1, 2, ONE, at(2), ONE, ONE, None, None) == 9          # the entropy
+    arrays = dict(z=ONE, tokens=ONE, tt=ONE, stats=ONE, entropy=ONE, g_logprobs=ONE, g_entropy=ONE, g_top=ONE, dz=ONE)
+    for name, byte in (("z", 1), ("tokens", 4), ("tt", 4), ("stats", 4), ("entropy", 2), ("g_logprobs", 2), ("g_entropy", 2), ("g_top", 2), ("dz", 8)):
+        a = {**arrays, name: at(byte)}
+        assert built_lib.pb_token_logprobs_bwd(a["z"], 1, 1, 4, 0, 8, 8, a["tokens"], 1, a["tt"], 2, a["stats"], a["entropy"], a["g_logprobs"], a["g_entropy"], a["g_top"], a["dz"], None) == 9, name
