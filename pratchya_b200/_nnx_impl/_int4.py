@@ -19,6 +19,15 @@ class Int4Linear(torch.nn.Module):
         self.register_buffer("scale", scale)
         self.register_buffer("zero", zero)
 
+    def _apply(self, fn, recurse=True):
+        """Moves the weight's parts with the module, but a cast of the module is none of theirs."""
+        parts = {name: self._buffers[name] for name in ("q", "scale", "zero")}
+        super()._apply(fn, recurse)
+        for name, t in parts.items():
+            if t is not None and self._buffers[name].dtype is not t.dtype:
+                self._buffers[name] = t.to(self._buffers[name].device)
+        return self
+
     def forward(self, x, raw=False):
         """`raw` is for callers of a Linear that re-quantizes its product: this one never does."""
         return int4_matmul_impl(x, self.q, self.scale, self.zero, self.fan_out)

@@ -136,3 +136,20 @@ def test_the_example_runs(built_lib):
     r = subprocess.run([sys.executable, str(root / "examples" / "answer.py"), "--layers", "1", "--vocab", "1024", "--tokens", "3", "--batch", "2"], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
     assert "log probability of the whole text" in r.stdout
+
+
+def test_casts_leave_the_weights_parts_as_they_are(built_lib):
+    """Module.float(), .half() and the like are about parameters; a scale in another type would be no weight of 4 bits."""
+    model, _ = _model()
+    ids = torch.randint(0, 640, (1, 5), device="cuda")
+    want, _ = model.advance(ids)
+    assert torch.equal(model.float().advance(ids)[0], want)
+    layer = Int4Linear(torch.randn(300, 70, device="cuda"), 64, True)
+    x = torch.randn(2, 300, device="cuda")
+    parts, y = [t.clone() for t in (layer.q, layer.scale, layer.zero)], layer(x)
+    for cast in (lambda m: m.half(), lambda m: m.double(), lambda m: m.float(), lambda m: m.bfloat16(), lambda m: m.to(torch.float16), lambda m: m.type(torch.float32), lambda m: m.to("cuda:0", torch.float32)):
+        layer = cast(layer)
+        assert all(a.dtype is b.dtype and torch.equal(a, b) for a, b in zip((layer.q, layer.scale, layer.zero), parts)) and torch.equal(layer(x), y)
+    moved = copy.deepcopy(layer).cpu().half()
+    assert moved.scale.device.type == "cpu" and moved.scale.dtype is torch.bfloat16 and torch.equal(moved.cuda()(x), y)
+    assert layer.half().state_dict()["scale"].dtype is torch.bfloat16 and Int4Linear(torch.randn(128, 16, device="cuda")).float().zero is None
