@@ -32,7 +32,8 @@ def generate(model, prompt, steps: int, top: int = 1, uniform: Optional[torch.Te
         pick = torch.zeros_like(scores.top_tokens[:, :1])
         if uniform is not None:
             share = torch.softmax(scores.top_logprobs, -1).cumsum(-1)
-            pick = (share <= uniform[:, i:i + 1]).sum(-1, keepdim=True).clamp(max=top - 1)
+            last = (share < share[:, -1:]).sum(-1, keepdim=True)          # behind it is what has no probability; a sum of shares may round to less than the number
+            pick = torch.minimum((share <= uniform[:, i:i + 1]).sum(-1, keepdim=True), last)
         ids = scores.top_tokens.gather(-1, pick)
         taken.append((ids[:, 0], scores.top_logprobs.gather(-1, pick)[:, 0], scores.entropy, scores.top_logprobs, scores.top_tokens))
     return Answer(*(torch.stack(part, dim=1) for part in zip(*taken)))

@@ -1,5 +1,6 @@
 """A model that answers: Linears in 4 bits in every layer, a state carried from call to call, tokens with their scores."""
 import copy
+import math
 import subprocess
 import sys
 from pathlib import Path
@@ -153,3 +154,39 @@ def test_casts_leave_the_weights_parts_as_they_are(built_lib):
     moved = copy.deepcopy(layer).cpu().half()
     assert moved.scale.device.type == "cpu" and moved.scale.dtype is torch.bfloat16 and torch.equal(moved.cuda()(x), y)
     assert layer.half().state_dict()["scale"].dtype is torch.bfloat16 and Int4Linear(torch.randn(128, 16, device="cuda")).float().zero is None
+
+
+class _Fixed:
+    """A model whose next-token logits [B, V] are given, the same at every step."""
+    def __init__(self, logits):
+        self.logits = logits
+
+    def advance(self, ids, state=None, **_):
+        return self.logits.unsqueeze(1), state
+
+
+def test_the_number_given_decides_among_the_alternatives(built_lib):
+    """The expected pick in 64 bits from the alternatives' own log probabilities, for numbers a thousandth away from where it changes."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    logits = torch.randn(2000, 50, generator=g, device="cuda") * 2
+    u = torch.rand(2000, 2, generator=g, device="cuda")
+    answer = generate(_Fixed(logits), torch.zeros(2000, 1, dtype=torch.int64, device="cuda"), 2, top=7, uniform=u)
+    ends = torch.softmax(answer.top_logprobs.double(), -1).cumsum(-1)
+    clear = ((ends - u.double().unsqueeze(-1)).abs() > 1e-3).all(-1)
+    pick = (ends <= u.double().unsqueeze(-1)).sum(-1, keepdim=True)
+    assert clear.float().mean() > 0.9 and set(pick[clear].flatten().tolist()) == set(range(7))
+    assert torch.equal(answer.tokens[clear], answer.top_tokens.gather(-1, pick.clamp(max=6))[..., 0][clear])
+    assert torch.equal(answer.logprobs[clear], answer.top_logprobs.gather(-1, pick.clamp(max=6))[..., 0][clear])
+
+
+def test_what_is_ruled_out_is_never_taken(built_lib):
+    """Shares that add up to less than the largest number below 1: the last alternative is one that can be taken, not one of those that fill up behind it."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    logits = torch.full((4096, 40), -math.inf, device="cuda")
+    logits[:, 3:20] = torch.randn(4096, 17, generator=g, device="cuda")
+    u = torch.full((4096, 1), 1.0 - 2.0 ** -24, device="cuda")
+    answer = generate(_Fixed(logits), torch.zeros(4096, 1, dtype=torch.int64, device="cuda"), 1, top=30, uniform=u)
+    shares = torch.softmax(answer.top_logprobs[:, 0], -1).cumsum(-1)[:, -1]
+    assert (shares <= u[:, 0]).any() and torch.isfinite(answer.logprobs).all() and (answer.tokens >= 3).all() and (answer.tokens < 20).all()
+    nothing = generate(_Fixed(torch.full((2, 40), -math.inf, device="cuda")), torch.zeros(2, 1, dtype=torch.int64, device="cuda"), 1, top=5, uniform=u[:2])
+    assert nothing.tokens.tolist() == [[0], [0]] and (nothing.logprobs == -math.inf).all()
