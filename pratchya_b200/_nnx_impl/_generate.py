@@ -27,7 +27,7 @@ def generate(model, prompt, steps: int, top: int = 1, uniform: Optional[torch.Te
         raise ValueError(f"generate: uniform {tuple(uniform.shape)} for {prompt.shape[0]} answers of {steps}")
     state, ids, taken = None, prompt, []
     for i in range(steps):
-        logits, state = model.advance(ids, state)
+        logits, state = model.advance(ids, state, last=True)
         scores = token_logprobs(logits[:, -1], top=top)
         pick = torch.zeros_like(scores.top_tokens[:, :1])
         if uniform is not None:

@@ -360,10 +360,10 @@ class PratchyaCausalLM(torch.nn.Module):
         return 0, [(zeros, zeros, wkv) for _ in self.blocks]
 
     @torch.no_grad()
-    def advance(self, input_ids, state=None):
+    def advance(self, input_ids, state=None, last=False):
         """(logits [B, T, V], the state behind the T tokens) of input_ids [B, T] read from `state` on (None: from the beginning): a prompt, or one token at
-        a time.  The norm over a block's heads runs over the T tokens of a call, as the reference's does (_module.py:118-123), so that a text read in pieces
-        has other logits than the same text at once."""
+        a time.  `last`: the logits of the last position alone, [B, 1, V].  The norm over a block's heads runs over the T tokens of a call, as the reference's
+        does (_module.py:118-123), so that a text read in pieces has other logits than the same text at once."""
         bsz, steps = input_ids.shape
         position, layers = self.init_state(bsz) if state is None else state
         t_positions = torch.arange(position, position + steps, device=input_ids.device, dtype=torch.int32)
@@ -371,7 +371,11 @@ class PratchyaCausalLM(torch.nn.Module):
         for blk, (tm_state, cm_state, wkv_state) in zip(self.blocks, layers):
             x, v, tm_state, cm_state, wkv_state = blk(x, v, t_positions, tm_state, cm_state, wkv_state)
             behind.append((tm_state.contiguous(), cm_state.contiguous(), wkv_state))
-        return self.lm_head(self.final_rmsnorm(x)), (position + steps, behind)
+        # the rows of an fp8 Linear's input share scales where they are narrower than a super-group of blocks: lm_head has all of them there, for the same bits
+        if last and (x.shape[2] % (max(1, self.cfg.blksize // 16) * self.cfg.blksize) == 0 or not isinstance(self.lm_head, Linear)):
+            x = x[:, -1:]
+        logits = self.lm_head(self.final_rmsnorm(x))
+        return logits[:, -1:] if last else logits, (position + steps, behind)
 
     def to_int4(self, group: int = 128, zero_points: bool = False):
         """Turns every Linear's weight into 4 bits, in place, and lets go of the dense ones: for a model that answers (`advance`, `score` without gradients).

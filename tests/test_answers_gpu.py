@@ -190,3 +190,30 @@ def test_what_is_ruled_out_is_never_taken(built_lib):
     assert (shares <= u[:, 0]).any() and torch.isfinite(answer.logprobs).all() and (answer.tokens >= 3).all() and (answer.tokens < 20).all()
     nothing = generate(_Fixed(torch.full((2, 40), -math.inf, device="cuda")), torch.zeros(2, 1, dtype=torch.int64, device="cuda"), 1, top=5, uniform=u[:2])
     assert nothing.tokens.tolist() == [[0], [0]] and (nothing.logprobs == -math.inf).all()
+
+
+def test_a_prompt_takes_the_memory_of_one_positions_logits(built_lib):
+    """4096 tokens of a vocabulary of 65536: 1 GB of logits, of which the next token needs a row."""
+    model = PratchyaCausalLM(PratchyaConfig(**{**SMALL, "vocab_size": 65536, "n_layers": 1}), seed=1).to_int4()
+    prompt = torch.randint(0, 65536, (1, 4096), device="cuda")
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    generate(model, prompt, 2, top=3)
+    assert torch.cuda.max_memory_allocated() - before < 1 << 28
+
+
+@pytest.mark.parametrize("hidden,steps", [(256, 9), (1024, 5), (1024, 1)])
+def test_the_last_positions_logits_are_those_of_all(built_lib, hidden, steps):
+    """In fp8 to the bit, also where the rows of lm_head's input share scales; in 4 bits the sums may be taken in another order, 2^-24 of their size at each of some thirty steps."""
+    model = PratchyaCausalLM(PratchyaConfig(**{**SMALL, "hidden_size": hidden}), seed=2)
+    ids = torch.randint(0, 640, (3, steps), device="cuda")
+    for bits in (8, 4):
+        whole, state = model.advance(ids)
+        last, behind = model.advance(ids, last=True)
+        assert last.shape == (3, 1, 640) and behind[0] == steps and all(torch.equal(a, b) for x, y in zip(state[1], behind[1]) for a, b in zip(x, y))
+        if bits == 8:
+            assert torch.equal(last, whole[:, -1:])
+        else:
+            assert float((last - whole[:, -1:]).norm() / last.norm()) <= 1e-6
+        model.to_int4(64, True)
