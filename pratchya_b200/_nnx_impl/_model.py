@@ -364,8 +364,12 @@ class PratchyaCausalLM(torch.nn.Module):
         """(logits [B, T, V], the state behind the T tokens) of input_ids [B, T] read from `state` on (None: from the beginning): a prompt, or one token at
         a time.  `last`: the logits of the last position alone, [B, 1, V].  The norm over a block's heads runs over the T tokens of a call, as the reference's
         does (_module.py:118-123), so that a text read in pieces has other logits than the same text at once."""
+        if input_ids.dim() != 2 or input_ids.shape[1] == 0:
+            raise ValueError(f"advance: input_ids {tuple(input_ids.shape)}, not [B, T] of one token or more")
         bsz, steps = input_ids.shape
         position, layers = self.init_state(bsz) if state is None else state
+        if len(layers) != len(self.blocks) or layers[0][0].shape[0] != bsz:
+            raise ValueError(f"advance: a state of {len(layers)} blocks and {layers[0][0].shape[0] if layers else 0} sequences for {len(self.blocks)} and {bsz}")
         t_positions = torch.arange(position, position + steps, device=input_ids.device, dtype=torch.int32)
         x, v, behind = self.pre_rmsnorm(self.embed(input_ids)), None, []
         for blk, (tm_state, cm_state, wkv_state) in zip(self.blocks, layers):

@@ -217,3 +217,12 @@ def test_the_last_positions_logits_are_those_of_all(built_lib, hidden, steps):
         else:
             assert float((last - whole[:, -1:]).norm() / last.norm()) <= 1e-6
         model.to_int4(64, True)
+
+
+def test_advance_refuses_what_it_cannot_go_on_from(built_lib):
+    model, _ = _model()
+    ids = torch.randint(0, 640, (2, 3), device="cuda")
+    position, layers = model.advance(ids)[1]
+    for bad, state in ((ids[:, :0], None), (ids[0], None), (ids, (position, layers[:1])), (ids, (position, layers + layers[:1])), (ids[:1], (position, layers))):
+        with pytest.raises(ValueError):
+            model.advance(bad, state)
