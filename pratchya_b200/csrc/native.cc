@@ -917,7 +917,6 @@ PyMethodDef methods[] = {
     ENTRY(pb_rms_norm), ENTRY(pb_rms_norm_bwd), ENTRY(pb_rms_norm_bwd_workspace_size), ENTRY(pb_relu2), ENTRY(pb_relu2_bwd),
     ENTRY(pb_wkv_finish), ENTRY(pb_wkv_finish_workspace_size), ENTRY(pb_wkv_finish_bwd), ENTRY(pb_wkv_finish_bwd_workspace_size),
     ENTRY(pb_smoothed_xent), ENTRY(pb_smoothed_xent_bwd),
-    ENTRY(pb_token_logprobs), ENTRY(pb_token_logprobs_bwd), ENTRY(pb_quantize_int4), ENTRY(pb_dequantize_int4), ENTRY(pb_int4_product),
     {"set_error", set_error, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
