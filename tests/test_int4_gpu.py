@@ -346,3 +346,46 @@ def test_no_derivative_is_dropped_without_a_word(built_lib):
             for f in (lambda t: int4_matmul_impl(t, *parts, 32), lambda t: quantize_int4_impl(t, 64)[0], lambda t: dequantize_int4_impl(*parts, (256, 32)) + t.sum()):
                 with pytest.raises(RuntimeError, match="traced"):
                     torch.jit.trace(f, x, check_trace=False)
+
+
+# ---- what x keeps in digits --------------------------------------------------------------------------------------------
+
+def _picked(depth, cols, zero_points):
+    """A weight of zeros, but for one of exactly 1 in each column at k = 5 (and a 7, or 14, at k = 6 that sets the scale to 1)."""
+    w = torch.zeros(depth, cols, device="cuda")
+    w[5], w[6] = 1.0, 14.0 if zero_points else 7.0
+    w[7] = -1.0 if zero_points else 0.0
+    parts = quantize_int4_impl(w, 128, zero_points)
+    assert torch.equal(dequantize_int4_impl(*parts, (depth, cols)), w)
+    return parts
+
+
+@pytest.mark.parametrize("zero_points", [False, True])
+@pytest.mark.parametrize("dtype,rows,depth,cols", [("f32", 1, 128, 16), ("f32", 8, 300, 40), ("bf16", 2, 512, 65536), ("bf16", 6, 128, 16)])
+def test_a_weight_of_one_gives_x_to_the_bit(built_lib, dtype, rows, depth, cols, zero_points):
+    """Alone in its block of 128, whatever its size: f32 in four digits, bf16 in three (two rows and many columns) and as it is."""
+    parts = _picked(depth, cols, zero_points)
+    values = torch.tensor([1.0 + 2.0 ** -23, -math.pi, 3.0e38, 1.0e-30, 16777215.0, 1.0 / 3.0, -1.0e-20, 255.0], device="cuda").to(DTYPES[dtype])
+    for at in range(0, 8, rows):
+        x = torch.zeros(min(rows, 8 - at), depth, device="cuda", dtype=DTYPES[dtype])
+        x[:, 5] = values[at:at + rows]
+        assert (int4_matmul_impl(x, *parts, cols, torch.float32) == x[:, 5:6].float()).all()
+
+
+@pytest.mark.parametrize("zero_points", [False, True])
+@pytest.mark.parametrize("dtype,rows,depth,cols,exact,step", [("f32", 1, 128, 16, 6, 30), ("f32", 8, 300, 40, 6, 30), ("bf16", 2, 512, 65536, 14, 22), ("bf16", 8, 128, 16, 126, 126)])
+def test_small_numbers_beside_a_large_one(built_lib, dtype, rows, depth, cols, exact, step, zero_points):
+    """The large one meets weights of zero, so that what is lost of the small one is all that y is off: nothing from 2^-6 (2^-14) of the large one on, and no more than 2^-30 (2^-22) of it
+    below.  A bf16 x that is taken as it is loses nothing."""
+    parts = _picked(depth, cols, zero_points)
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    for power in range(0, 40):
+        for large in (1.0, 1.99, 3.0e5):
+            x = torch.zeros(rows, depth, device="cuda", dtype=DTYPES[dtype])
+            x[:, 100] = large
+            x[:, 5] = ((torch.rand(rows, generator=g, device="cuda") + 1.0) * 0.5 * large * 2.0 ** -power).to(x.dtype)
+            x[-1, 5] = -x[-1, 5]
+            of = float(x[0, 100])
+            off = (int4_matmul_impl(x, *parts, cols, torch.float32).double() - x[:, 5:6].double()).abs()
+            inside = (x[:, 5].double().abs() >= of * 2.0 ** -exact).unsqueeze(-1)
+            assert (off[inside.expand_as(off)] == 0).all() and (off <= of * 2.0 ** -step).all(), (power, large)

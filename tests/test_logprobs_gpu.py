@@ -475,3 +475,13 @@ def test_gradient_of_masked_logits_under_large_cotangents(built_lib, dtype):
         # what is below the type's normal numbers for a cotangent of 1 has fewer bits there
         fine = one.abs() >= 2.0 ** -100
         assert torch.equal(got[fine], (one.double() * 2.0 ** power).to(z.dtype)[fine]) and torch.isfinite(got).all()
+
+
+def test_gradient_of_a_row_read_by_several_texts(built_lib):
+    z, _ = _case(1, 1003, "f32", 47)
+    shared = z[None].detach().requires_grad_(True)
+    t = torch.tensor([[1], [2], [2]], device="cuda")
+    token_logprobs(shared.expand(3, 1, -1), t).logprobs.sum().backward()
+    want = -3 * torch.softmax(z.double(), -1)[0]
+    want[1] += 1; want[2] += 2
+    assert (shared.grad[0, 0].double() - want).abs().max() <= 3 * 2.0 ** -20
