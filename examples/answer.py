@@ -34,6 +34,7 @@ def main():
         print(f"token {t:6d}  log probability {lp:7.3f}  entropy {h:6.3f}  best {tops}")
     with torch.no_grad():
         text = score(model, torch.cat([prompt, answer.tokens], dim=1), top=1)
+    # read at once, not token by token as above: the norm over a block's heads runs over the tokens of a call, so these are other numbers than the answer's
     print(f"log probability of the whole text {float(text.logprobs[0].sum()):.2f} over {text.logprobs.shape[1]} tokens")
 
 

@@ -20,7 +20,10 @@ class Answer(NamedTuple):
 @torch.no_grad()
 def generate(model, prompt, steps: int, top: int = 1, uniform: Optional[torch.Tensor] = None) -> Answer:
     """`steps` tokens after `prompt` [B, T].  The next token is the best of the `top` alternatives, or, with `uniform` [B, steps] of numbers in [0, 1), the one
-    where the sum of their probabilities (as shares of the alternatives') passes that number."""
+    where the sum of their probabilities (as shares of the alternatives') passes that number.
+
+    The log probabilities are those of a text read token by token behind its prompt.  `score` reads it at once and has others: the norm over a block's heads runs
+    over the tokens of a call (see `advance`).  A ratio of the two is none of one policy's; `advance` over the same pieces gives the same numbers again."""
     if prompt.dim() != 2 or prompt.shape[1] == 0 or steps < 1 or top < 1:
         raise ValueError(f"generate: prompt {tuple(prompt.shape)}, {steps} steps, {top} alternatives")
     if uniform is not None and tuple(uniform.shape) != (prompt.shape[0], steps):
@@ -41,6 +44,7 @@ def generate(model, prompt, steps: int, top: int = 1, uniform: Optional[torch.Te
 
 def score(model, ids, top: int = 0) -> TokenLogprobs:
     """How the model takes a text `ids` [B, T]: of each token but the first its log probability behind the ones before it, with the entropy there and the
-    best alternatives [B, T-1, ..].  Differentiable in the model's parameters where gradients are on."""
+    best alternatives [B, T-1, ..].  Differentiable in the model's parameters where gradients are on.  Not what `generate` found for the same tokens: there they are
+    read one by one."""
     logits, _ = model(ids)
     return token_logprobs(logits[:, :-1], ids[:, 1:], top=top)

@@ -661,7 +661,10 @@ template <typename TX, int DIGITS, int MT, int PER_GROUP, bool ZERO> int launch_
   auto kernel = int4_product_kernel<TX, DIGITS, MT, PER_GROUP, ZERO>;
   uint32_t ctas = 1, per_pass = std::min<uint32_t>(p.rows, 8 * MT / kParts), clusters, bytes;
   const uint32_t sms = sm_count(), force = env_switch("PB_INT4_CTAS", 0), force_sm = env_switch("PB_INT4_PERSM", 0);
-  // x in shared memory: split k over a cluster, and where that is not enough serve fewer rows with a pass.  Few tiles of a long contraction are split, too
+  // x in shared memory: split k over a cluster, and where that is not enough serve fewer rows with a pass.  Few tiles of a long contraction (`few`) are split, too, us, one
+  // CTA | by the rule: one f32 row, 16384 x 256 10.1 | 4.1, 16384 x 2048 10.3 | 6.9, 8192 x 2048 6.2 | 5.5, 8192 x 4096 7.9 | 6.7; 8 bf16 rows, 8192 x 2048 7.3 | 6.5; at the
+  // rule's edge it takes longer, 4096 x 2048 4.1 | 4.4.  So is x where making its digits takes a CTA more than its products (`heavy`): 8 f32 rows, 2048 x 256 6.8 | 4.9,
+  // 2048 x 2048 6.9 | 6.4, 2048 x 4096 7.7 | 7.7; of four rows it takes longer where the contraction is short, 1024 x 2048 3.4 | 4.6.
   while (true) {
     const uint32_t per = (p.kblocks + ctas - 1) / ctas;
     uint32_t room = sms / ctas;      // clusters that are resident at once with a CTA an SM; 33 of four and 15 of eight CTAs on 148 SMs

@@ -9,12 +9,14 @@
 //   dz_j = sum_i g_i [j == t_i] + sum_i h_i [j == top_i] - p_j (sum_i g_i + sum_i h_i + g_entropy (logp_j + entropy))
 // with g the cotangents of the given tokens' log probabilities and h those of the alternatives'.
 //
+// Exponentials are ex2.approx.ftz of a difference times log2 e: within 2^-22, and a probability below 2^-126 is 0, also as the gradient's factor.
+//
 // Floor: HBM.  The forward pass reads the logits once (4 or 2 bytes each), the backward pass once more and writes dz.  What it takes beside that is an
 // exponential per logit (16 a cycle and SM: 73 % of a bf16 logit's time at 6.5 TB/s) and six to seven instructions, so packed f32x2 arithmetic, and for the
 // alternatives no more than a thread's two best vectors while the row goes by.  On one B200, us (and of the measured 6.53 TB/s):
 //   2000 x 65536 bf16     48 (84 %) without alternatives, 55 with five, 68 with 64
 //   1000 x 65536 f32      43.5 (92 %), 60 with 64;  4096 x 65536 f32, forward and gradient 509 (97 %)
-//   one row of 65536 f32, five alternatives: 5.7, a launch and some ten dependent steps of 0.2 to 0.8 each
+//   one row of 65536 f32, five alternatives: 5.5, a launch and some ten dependent steps of 0.2 to 0.8 each
 #include "common.cuh"
 
 #include <cooperative_groups.h>
