@@ -383,7 +383,7 @@ class PratchyaCausalLM(torch.nn.Module):
 
     def to_int4(self, group: int = 128, zero_points: bool = False):
         """Turns every Linear's weight into 4 bits, in place, and lets go of the dense ones: for a model that answers (`advance`, `score` without gradients).
-        Made for a few rows a call: a step of one to eight sequences reads a quarter to a half of what fp8's reads, but the activations are f32 and the weight is read
+        Made for a few rows a call: a step of one to eight sequences reads half of what fp8's does, but the activations are f32 and the weight is read
         again for every eight rows of them, so that from some 16 on a Linear in fp8 is faster (2048 x 8192, us, 4 bits | fp8: 8 rows 10 | 16, 32 rows 25 | 17, 1024 rows
         692 | 35; a prompt of 1024 tokens through 24 layers of 2048: 122 ms | 15.6, a token 8.8 | 19).  Returns the model."""
         for module in list(self.modules()):
