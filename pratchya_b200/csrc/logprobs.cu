@@ -586,7 +586,7 @@ template <typename T> __device__ __forceinline__ uint4 load_anywhere(const T* fr
   const uint32_t* w = reinterpret_cast<const uint32_t*>(at & ~(uintptr_t)3);
   const uint32_t a = __ldg(w), b = __ldg(w + 1), c = __ldg(w + 2), d = __ldg(w + 3);
   if ((at & 3) == 0) return make_uint4(a, b, c, d);
-  const uint32_t e = __ldg(w + 4);      // holds the last one
+  const uint32_t e = __ldg(reinterpret_cast<const uint16_t*>(w + 4));      // the last one, and nothing behind it
   return make_uint4(__funnelshift_r(a, b, 16), __funnelshift_r(b, c, 16), __funnelshift_r(c, d, 16), __funnelshift_r(d, e, 16));
 }
 
