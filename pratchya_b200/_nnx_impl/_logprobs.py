@@ -3,6 +3,7 @@ the kernels of csrc/logprobs.cu.  Stands next to the training loss (pratchya/_nn
 smoothed number for a whole batch."""
 from __future__ import annotations
 
+import operator
 from typing import NamedTuple, Optional
 
 import torch
@@ -61,7 +62,7 @@ def _checked(logits, tokens, top):
         raise TypeError(f"token_logprobs: logits are {logits.dtype}; float32 and bfloat16 are taken")
     if logits.dim() == 0 or logits.shape[-1] == 0:
         raise ValueError(f"token_logprobs: logits {tuple(logits.shape)}")
-    lead, top = logits.shape[:-1], int(top)
+    lead, top = logits.shape[:-1], operator.index(top)
     if not 0 <= top <= min(MAX_TOP, logits.shape[-1]):
         raise ValueError(f"token_logprobs: {top} alternatives of {logits.shape[-1]} (at most {MAX_TOP})")
     if tokens is not None:

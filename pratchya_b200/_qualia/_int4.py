@@ -8,6 +8,8 @@ With A = ceil(N / 16) and B = ceil(K / 128): q uint8 [A, B, 1024], scale bf16 [A
 16 columns and 128 values of k in the order in which the product's matrix instructions take them (include/pratchya_b200.h gives it)."""
 from __future__ import annotations
 
+import operator
+
 import torch
 from torch.autograd import forward_ad
 
@@ -72,7 +74,7 @@ def quantize_int4_impl(w: torch.Tensor, group: int = 128, zero_points: bool = Fa
 
 def dequantize_int4_impl(q, scale, zero, shape, dtype=torch.float32):
     """The values [K, N] that the parts of a weight of that shape stand for.  Not differentiable in the scale."""
-    depth, cols = (int(n) for n in shape)
+    depth, cols = (operator.index(n) for n in shape)
     if dtype not in (torch.float32, torch.bfloat16):
         raise TypeError(f"dequantize_int4_impl: {dtype}; float32 and bfloat16 are built")
     out = _lib.native().dequantize_int4(q, scale, zero, depth, cols, dtype)
@@ -100,10 +102,11 @@ def int4_matmul_impl(x, q, scale, zero, cols: int, dtype=None):
         raise TypeError(f"int4_matmul_impl: x is {x.dtype}; float32 and bfloat16 are taken")
     if dtype not in (None, torch.float32, torch.bfloat16):
         raise TypeError(f"int4_matmul_impl: {dtype}; float32 and bfloat16 are built")
-    parts = _int4_parts(q, scale, zero, x.shape[-1], int(cols), "int4_matmul_impl")
+    cols = operator.index(cols)
+    parts = _int4_parts(q, scale, zero, x.shape[-1], cols, "int4_matmul_impl")
     if x.device != q.device:
         raise RuntimeError(f"int4_matmul_impl: x is on {x.device}, the weight on {q.device}")
-    out = _lib.native().int4_product(x.contiguous(), *parts, int(cols), dtype)
+    out = _lib.native().int4_product(x.contiguous(), *parts, cols, dtype)
     if out is None:
         raise RuntimeError("int4_matmul_impl takes plain CUDA tensors only")
     return out

@@ -389,3 +389,14 @@ def test_small_numbers_beside_a_large_one(built_lib, dtype, rows, depth, cols, e
             off = (int4_matmul_impl(x, *parts, cols, torch.float32).double() - x[:, 5:6].double()).abs()
             inside = (x[:, 5].double().abs() >= of * 2.0 ** -exact).unsqueeze(-1)
             assert (off[inside.expand_as(off)] == 0).all() and (off <= of * 2.0 ** -step).all(), (power, large)
+
+
+def test_a_number_of_columns_is_whole(built_lib):
+    parts = quantize_int4_impl(_weight(256, 32, "f32", 1), 64, True)
+    x = torch.randn(2, 256, device="cuda")
+    for bad in (32.5, 32.0, "32"):
+        with pytest.raises(TypeError):
+            int4_matmul_impl(x, *parts, bad)
+        with pytest.raises(TypeError):
+            dequantize_int4_impl(*parts, (256, bad))
+    assert torch.equal(int4_matmul_impl(x, *parts, torch.tensor(32)), int4_matmul_impl(x, *parts, 32))

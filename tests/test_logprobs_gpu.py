@@ -485,3 +485,11 @@ def test_gradient_of_a_row_read_by_several_texts(built_lib):
     want = -3 * torch.softmax(z.double(), -1)[0]
     want[1] += 1; want[2] += 2
     assert (shared.grad[0, 0].double() - want).abs().max() <= 3 * 2.0 ** -20
+
+
+def test_a_number_of_alternatives_is_whole(built_lib):
+    z, tokens = _case(3, 1000, "f32", 3)
+    for bad in (2.5, 2.0, "2", None):
+        with pytest.raises(TypeError):
+            token_logprobs(z, tokens, bad)
+    assert torch.equal(token_logprobs(z, tokens, torch.tensor(2)).top_tokens, token_logprobs(z, tokens, 2).top_tokens)
