@@ -428,6 +428,15 @@ PB_API int pb_dequantize_int4(const uint8_t* q, const void* scale, const uint8_t
 PB_API int pb_int4_product(const void* x, int x_dtype, int64_t rows, int64_t depth, int64_t stride, const uint8_t* q, const void* scale, const uint8_t* zero, int group,
                     int64_t cols, void* out, int out_dtype, void* stream);
 
+/* The orthogonalised update of weights: for each of `batch` matrices G [rows, cols] (f32 or bf16) X = G / (|G| + eps) in the Frobenius norm, then `steps` (1 to 64) times,
+ * with a, b, c = coefficients[3 k .. 3 k + 2] (host memory),  A = X X^T, X = a X + (b A + c A A) X  (A = X^T X from the right where rows > cols), which
+ * draws the singular values towards 1 (the Newton-Schulz step of the reference's optimizer, pratchya/_nnx_impl/_optimizer.py:11-29).  out is bf16 [batch, rows, cols].
+ * X is kept in 22 bits, the products' operands in fp16 (11), sums in f32.  Coefficients that take a singular value of [0, 1] beyond 4 on the way: PB_ERR_UNSUPPORTED.
+ * A matrix with an infinity or a NaN becomes NaN throughout, one of zeros stays zero (eps > 0).  workspace 256-byte aligned, other arrays as their type is. */
+PB_API size_t pb_orthogonalize_workspace_size(int64_t batch, int64_t rows, int64_t cols);
+PB_API int pb_orthogonalize(const void* update, int dtype, int64_t batch, int64_t rows, int64_t cols, int steps, const float* coefficients, double eps,
+                     void* out, void* workspace, size_t workspace_bytes, void* stream);
+
 /* byte transpose [rows, cols] -> [cols, rows] of an fp8 matrix (weight prepared for the forward GEMM) */
 PB_API int pb_transpose_bytes(const void* src, int64_t rows, int64_t cols, void* dst, void* stream);
 

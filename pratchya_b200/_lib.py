@@ -100,6 +100,8 @@ _SIGNATURES = {
     "pb_quantize_int4": (_int, [_ptr, _int, _i64, _i64, _int, _ptr, _ptr, _ptr, _ptr]),
     "pb_dequantize_int4": (_int, [_ptr, _ptr, _ptr, _i64, _i64, _int, _ptr, _int, _ptr]),
     "pb_int4_product": (_int, [_ptr, _int, _i64, _i64, _i64, _ptr, _ptr, _ptr, _int, _i64, _ptr, _int, _ptr]),
+    "pb_orthogonalize_workspace_size": (_sz, [_i64, _i64, _i64]),
+    "pb_orthogonalize": (_int, [_ptr, _int, _i64, _i64, _i64, _int, _ptr, C.c_double, _ptr, _ptr, _sz, _ptr]),
 }
 # extra exports of the diagnostics build (libpratchya_b200_diag.so): test hooks, not part of the C ABI
 _DIAG_SIGNATURES = {
