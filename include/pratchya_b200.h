@@ -428,6 +428,28 @@ PB_API int pb_dequantize_int4(const uint8_t* q, const void* scale, const uint8_t
 PB_API int pb_int4_product(const void* x, int x_dtype, int64_t rows, int64_t depth, int64_t stride, const uint8_t* q, const void* scale, const uint8_t* zero, int group,
                     int64_t cols, void* out, int out_dtype, void* stream);
 
+/* The token embedding (EmbeddingScaled without its quantization, pratchya/_nnx_impl/_module.py:21-37): out[i] = scale * table[ids[i]] for n tokens and a table [vocab, channels], f32 or bf16
+ * as out is.  An id below zero counts from the table's end; padding_id (from 0 on; none: a negative number) gives a row of zeros, and one beyond the table a row of NaN.  The backward call writes every
+ * row of d_table [vocab, channels]: scale times the sum of the rows of g [n, channels] whose token it is, in f32 and in an order that goes by the ids alone; padding and what lies beyond the table has no part in it.
+ * workspace 256-byte aligned, other arrays as their type is. */
+PB_API int pb_embedding_lookup(const void* table, int dtype, int64_t vocab, int64_t channels, const int64_t* ids, int64_t n, float scale, int64_t padding_id, void* out, void* stream);
+PB_API size_t pb_embedding_lookup_bwd_workspace_size(int64_t n, int64_t vocab, int64_t channels);
+PB_API int pb_embedding_lookup_bwd(const void* g, int dtype, const int64_t* ids, int64_t n, int64_t vocab, int64_t channels, float scale, int64_t padding_id, void* d_table,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
+/* Softmax cross entropy of hidden states against a vocabulary's weight without the logits z = x W: for each position with a target t in [0, vocab)
+ *   loss = lse - (1 - smoothing) z_t - smoothing * mean(z),  lse = log sum exp z,
+ * the loss of pb_smoothed_xent (weight 1) behind a product of bf16 x [depth] and weight with f32 sums.  x's row (o, i) lies at o * stride_outer + i * stride_inner elements; the weight is
+ * bf16 [depth, vocab], or with by_word [vocab, depth], rows `ld` elements apart.  A negative target is none: loss and lse 0, and the position's x reaches nothing; one beyond
+ * the vocabulary has loss NaN and otherwise counts as none.  targets, loss, lse, g [outer * inner].  The backward call takes lse back and writes, from the cotangents g of the losses (each may be null),
+ * dx bf16 [outer * inner, depth] and dweight bf16 in the weight's order, rows without gaps: sums in f32 of dz = g (softmax - (1 - smoothing) onehot - smoothing / vocab) rounded to bf16.
+ * The workspace's size goes by the weight's address and ld: one that is not 16-byte aligned or has ld % 8 != 0 is copied there.  workspace 256-byte aligned, other arrays as their type is. */
+PB_API size_t pb_linear_xent_workspace_size(int64_t rows, int64_t depth, const void* weight, int64_t ld, int by_word, int64_t vocab, int backward);
+PB_API int pb_linear_xent(const void* x, int64_t outer, int64_t inner, int64_t stride_outer, int64_t stride_inner, int64_t depth, const void* weight, int64_t ld, int by_word, int64_t vocab,
+                   const int64_t* targets, float smoothing, float* loss, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+PB_API int pb_linear_xent_bwd(const void* x, int64_t outer, int64_t inner, int64_t stride_outer, int64_t stride_inner, int64_t depth, const void* weight, int64_t ld, int by_word, int64_t vocab,
+                       const int64_t* targets, float smoothing, const float* lse, const float* g, void* dx, void* dweight, void* workspace, size_t workspace_bytes, void* stream);
+
 /* The orthogonalised update of weights: for each of `batch` matrices G [rows, cols] (f32 or bf16) X = G / (|G| + eps) in the Frobenius norm, then `steps` (1 to 64) times,
  * with a, b, c = coefficients[3 k .. 3 k + 2] (host memory),  A = X X^T, X = a X + (b A + c A A) X  (A = X^T X from the right where rows > cols), which
  * draws the singular values towards 1 (the Newton-Schulz step of the reference's optimizer, pratchya/_nnx_impl/_optimizer.py:11-29).  out is bf16 [batch, rows, cols].

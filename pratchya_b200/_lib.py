@@ -100,6 +100,12 @@ _SIGNATURES = {
     "pb_quantize_int4": (_int, [_ptr, _int, _i64, _i64, _int, _ptr, _ptr, _ptr, _ptr]),
     "pb_dequantize_int4": (_int, [_ptr, _ptr, _ptr, _i64, _i64, _int, _ptr, _int, _ptr]),
     "pb_int4_product": (_int, [_ptr, _int, _i64, _i64, _i64, _ptr, _ptr, _ptr, _int, _i64, _ptr, _int, _ptr]),
+    "pb_embedding_lookup": (_int, [_ptr, _int, _i64, _i64, _ptr, _i64, C.c_float, _i64, _ptr, _ptr]),
+    "pb_embedding_lookup_bwd_workspace_size": (_sz, [_i64, _i64, _i64]),
+    "pb_embedding_lookup_bwd": (_int, [_ptr, _int, _ptr, _i64, _i64, _i64, C.c_float, _i64, _ptr, _ptr, _sz, _ptr]),
+    "pb_linear_xent_workspace_size": (_sz, [_i64, _i64, _ptr, _i64, _int, _i64, _int]),
+    "pb_linear_xent": (_int, [_ptr] + [_i64] * 5 + [_ptr, _i64, _int, _i64, _ptr, C.c_float, _ptr, _ptr, _ptr, _sz, _ptr]),
+    "pb_linear_xent_bwd": (_int, [_ptr] + [_i64] * 5 + [_ptr, _i64, _int, _i64, _ptr, C.c_float, _ptr, _ptr, _ptr, _ptr, _ptr, _sz, _ptr]),
     "pb_orthogonalize_workspace_size": (_sz, [_i64, _i64, _i64]),
     "pb_orthogonalize": (_int, [_ptr, _int, _i64, _i64, _i64, _int, _ptr, C.c_double, _ptr, _ptr, _sz, _ptr]),
 }

@@ -1733,22 +1733,25 @@ namespace pb {
 int transposed_status_fetch(unsigned int* out);   // transpose_quantize.cu
 int dense_dot_status_fetch(unsigned int* out);    // dense_dot.cu
 int orthogonalize_status_fetch(unsigned int* out);      // orthogonalize.cu
+int linear_xent_status_fetch(unsigned int* out);  // linear_xent.cu
 }
 
 extern "C" int pb_gemm_check(void* stream) {
   PB_CUDA_TRY(cudaStreamSynchronize(static_cast<cudaStream_t>(stream)));
   // all words are read and cleared before any of them is reported
-  unsigned int gemm = 0, transposed = 0, dots = 0, ortho = 0;
+  unsigned int gemm = 0, transposed = 0, dots = 0, ortho = 0, xent = 0;
   const unsigned int zero = 0;
   PB_CUDA_TRY(cudaMemcpyFromSymbol(&gemm, g_gemm_status, sizeof(gemm)));
   if (gemm != 0) PB_CUDA_TRY(cudaMemcpyToSymbol(g_gemm_status, &zero, sizeof(zero)));
   if (int s = transposed_status_fetch(&transposed)) return s;
   if (int s = dense_dot_status_fetch(&dots)) return s;
   if (int s = orthogonalize_status_fetch(&ortho)) return s;
+  if (int s = linear_xent_status_fetch(&xent)) return s;
   if (gemm != 0) return fail((int)gemm, "a bounded device-side wait in the GEMM kernel ran out");
   if (transposed != 0) return fail((int)transposed, "a bounded device-side wait in the transposed quantizer ran out");
   if (dots != 0) return fail((int)dots, "a bounded device-side wait in the dense-dot kernel ran out");
   if (ortho != 0) return fail((int)ortho, "a bounded device-side wait in a product of the orthogonalised update ran out");
+  if (xent != 0) return fail((int)xent, "a bounded device-side wait in a product of the cross entropy without logits ran out");
   return PB_OK;
 }
 

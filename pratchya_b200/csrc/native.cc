@@ -678,6 +678,16 @@ OP(rows_at_two_strides) {
   END_HANDLE_TH_ERRORS
 }
 
+// strides_of_rows(x) -> (outer, inner, stride_outer, stride_inner) of the rows that an op reads in place, or None
+OP(strides_of_rows) {
+  HANDLE_TH_ERRORS
+  NARGS(1);
+  StridedRows r;
+  if (!THPVariable_Check(args[0]) || !strided_rows(THPVariable_Unpack(args[0]), &r)) return none();
+  return Py_BuildValue("LLLL", (long long)r.outer, (long long)r.inner, (long long)r.stride_outer, (long long)r.stride_inner);
+  END_HANDLE_TH_ERRORS
+}
+
 // a call whose result a trace would hold as a constant: the Python text refuses it
 bool traced() { return torch::jit::tracer::isTracing(); }
 // a tensor that a derivative may be asked for, backward or forward: the Python text refuses it where the op has none
@@ -864,6 +874,28 @@ OP(int4_product) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- the token embedding ----
+// embedding_lookup(table [vocab, channels], ids, scale, padding or -1) -> [..., channels]: embedding_lookup without its derivative
+OP(embedding_lookup) {
+  HANDLE_TH_ERRORS
+  NARGS(4);
+  const at::Tensor *table = plain(args[0]), *ids = plain(args[1]);
+  const double scale = PyFloat_AsDouble(args[2]);
+  if (scale == -1.0 && PyErr_Occurred()) return nullptr;
+  const long long padding = PyLong_AsLongLong(args[3]);
+  if (padding == -1 && PyErr_Occurred()) return nullptr;
+  if (!table || !ids || watched() || traced() || !dense(table->scalar_type()) || table->dim() != 2 || table->numel() == 0 || ids->scalar_type() != at::kLong || ids->device() != table->device())
+    return none();
+  const c10::cuda::CUDAGuard guard(table->device());
+  c10::SmallVector<int64_t, 8> shape(ids->sizes().begin(), ids->sizes().end());
+  shape.push_back(table->size(1));
+  at::Tensor out = fresh(shape, table->scalar_type());
+  RUN(pb_embedding_lookup(table->data_ptr(), code(table->scalar_type()), table->size(0), table->size(1), ids->numel() ? ids->data_ptr<int64_t>() : nullptr, ids->numel(), (float)scale, padding,
+                          out.data_ptr(), current_stream(table->device())));
+  return wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
 // empty(shape, dtype, like) -> a tensor on the device of `like`; empties(like, count) -> a list of them, contiguous, of its shape and type
 OP(empty_on) {
   HANDLE_TH_ERRORS
@@ -917,6 +949,8 @@ PyMethodDef methods[] = {
     ENTRY(pb_rms_norm), ENTRY(pb_rms_norm_bwd), ENTRY(pb_rms_norm_bwd_workspace_size), ENTRY(pb_relu2), ENTRY(pb_relu2_bwd),
     ENTRY(pb_wkv_finish), ENTRY(pb_wkv_finish_workspace_size), ENTRY(pb_wkv_finish_bwd), ENTRY(pb_wkv_finish_bwd_workspace_size),
     ENTRY(pb_smoothed_xent), ENTRY(pb_smoothed_xent_bwd),
+    METHOD("embedding_lookup", embedding_lookup), ENTRY(pb_embedding_lookup_bwd), ENTRY(pb_embedding_lookup_bwd_workspace_size),
+    ENTRY(pb_linear_xent), ENTRY(pb_linear_xent_bwd), ENTRY(pb_linear_xent_workspace_size), METHOD("strides_of_rows", strides_of_rows),
     ENTRY(pb_orthogonalize), ENTRY(pb_orthogonalize_workspace_size),
     {"set_error", set_error, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -299,9 +299,8 @@ extern "C" int pb_orthogonalize(const void* update, int dtype, int64_t batch, in
       const double s = most * i / 1024, s2 = s * s;
       next = std::max(next, std::fabs(s * (a + s2 * (b + s2 * c))));
       gram = std::max(gram, std::fabs(s2 * (b + s2 * c)));
-      if (!std::isfinite(next) || !std::isfinite(gram)) next = gram = INFINITY;
     }
-    if (!(next <= kMostX) || !(gram <= kMostB))
+    if (!std::isfinite(a + b + c) || !(next <= kMostX) || !(gram <= kMostB))
       return fail(PB_ERR_UNSUPPORTED, "pb_orthogonalize: coefficients %g %g %g of step %d take singular values beyond %g", a, b, c, k, (double)kMostX);
     most = next;
   }
