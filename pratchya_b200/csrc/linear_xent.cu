@@ -5,8 +5,11 @@
 // Forward: one product (products.cuh) whose epilogue keeps of each 128 logits of a position a maximum, a sum of exponentials and, with smoothing, a sum,
 // and of all of them the target's; a small kernel joins these.  Exponentials are of differences from the maximum, which are exact where they matter (a fused z log2(e) - m
 // saves an instruction of two logits, but from logits of 10^9 on what rounding m leaves takes every term to 0).
-// Backward: the logits once more, a piece of the vocabulary at a time, left as dz in bf16 (rounded once, as an operand of a bf16 product has to
-// be), and two products of the piece: dx, added up over the pieces in f32, and the piece's part of dW.
+// Backward: the logits once more, a piece of the vocabulary at a time, left as dz / (g (1 - a)) in bf16, and two products of the piece: dx, added up over the pieces in
+// f32, and the piece's part of dW.  An operand of a bf16 product is rounded once; divided so, the target's element, the largest, is p_t / (1 - a) - 1 and next to
+// exact while p_t is small, where g's and a's own bits would round all of a position's gradient one way (2.7e-3 of dx and dW, 1.66e-3 of
+// which is the results' own rounding; now GRADIENT_ERROR).  dx takes g (1 - a) in f32 at its end; for dW the hidden states are multiplied by g over the largest g, exactly 1
+// where all are one.
 //
 // Positions without a target do no work: a first kernel numbers those that have one, a second brings their hidden states together (rows
 // of zeros up to a whole tile behind them), and the products read the number of rows on the device.  So what lies in a padded position, a NaN too, reaches nothing.
@@ -18,6 +21,7 @@ using namespace products;
 
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr int kRowTile = 256;                           // hidden states come in whole tiles of them
+constexpr int kGroup = 8;                                // stages, 512 of k, of an accumulator
 constexpr int kPart = 128;                              // logits of a position that an epilogue thread adds up
 constexpr size_t kMostGradient = (size_t)256 << 20;     // bytes of dz at a time
 
@@ -33,8 +37,8 @@ struct SelectParams {
   int64_t vocab;
   int rows;
   int *count, *place, *origin, *target;      // place[row]: its number or -1; origin, target[number]
-  const float *lse, *g;                      // backward: brought together, too
-  float *lse_out, *g_out;
+  const float *lse, *g;                      // backward: brought together, too, and the g of the largest magnitude
+  float *lse_out, *g_out, *g_most;
   float* loss;                               // forward: of positions without a target 0, beyond the vocabulary NaN; and their lse
   float* lse_none;
 };
@@ -45,7 +49,23 @@ __global__ void __launch_bounds__(1024) select_kernel(const __grid_constant__ Se
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int run = (p.rows + 1023) / 1024, first = min(p.rows, (int)threadIdx.x * run), last = min(p.rows, first + run);
   int mine = 0;
-  for (int i = first; i < last; ++i) mine += p.targets[i] >= 0 && p.targets[i] < p.vocab;
+  float most = 0.0f;
+  for (int i = first; i < last; ++i) {
+    const bool there = p.targets[i] >= 0 && p.targets[i] < p.vocab;
+    mine += there;
+    if (p.g && there) most = fmaxf(most, fabsf(p.g[i]));
+  }
+  if (p.g) {
+    __shared__ float tops[32];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (lane == 0) tops[warp] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < 32; ++w) most = fmaxf(most, tops[w]);
+      *p.g_most = most;
+    }
+  }
   int upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -81,7 +101,9 @@ struct GatherParams {
   int64_t inner, stride_outer, stride_inner;
   const int *count, *place;
   unsigned short* out;
-  unsigned short* dx;      // backward: rows of zeros for positions without a target
+  // backward: the rows times g / g_most, and dx's of zeros for positions without a target
+  unsigned short *scaled, *dx;
+  const float *g, *g_most;
   int rows, depth, ld;
   bool vectors, dx_vectors;
 };
@@ -92,18 +114,36 @@ __global__ void __launch_bounds__(256) gather_kernel(const __grid_constant__ Gat
   if (row >= p.rows) {
     const int count = *p.count, to = count + row - p.rows;
     if (to >= (count + kRowTile - 1) / kRowTile * kRowTile) return;
-    for (int c = lane * 8; c < p.ld; c += 256) *reinterpret_cast<uint4*>(p.out + (int64_t)to * p.ld + c) = make_uint4(0u, 0u, 0u, 0u);
+    for (int c = lane * 8; c < p.ld; c += 256) {
+      *reinterpret_cast<uint4*>(p.out + (int64_t)to * p.ld + c) = make_uint4(0u, 0u, 0u, 0u);
+      if (p.scaled) *reinterpret_cast<uint4*>(p.scaled + (int64_t)to * p.ld + c) = make_uint4(0u, 0u, 0u, 0u);
+    }
     return;
   }
   const int to = p.place[row];
   if (to >= 0) {
     const unsigned short* from = p.x + row / p.inner * p.stride_outer + row % p.inner * p.stride_inner;
     unsigned short* out = p.out + (int64_t)to * p.ld;
+    unsigned short* scaled = p.scaled ? p.scaled + (int64_t)to * p.ld : nullptr;
+    float by = 1.0f;
+    if (scaled) {
+      const float most = *p.g_most, g = p.g[to];
+      by = most == 0.0f ? g : __fdiv_rn(g, most);          // every g is zero, or none is a number
+    }
+    auto times = [&](uint32_t x) { return pack_bf16x2(__uint_as_float(x << 16) * by, __uint_as_float(x & 0xffff0000u) * by); };
     if (p.vectors) {
 #pragma unroll 4
-      for (int c = lane * 8; c < p.depth; c += 256) *reinterpret_cast<uint4*>(out + c) = *reinterpret_cast<const uint4*>(from + c);
+      for (int c = lane * 8; c < p.depth; c += 256) {
+        const uint4 v = *reinterpret_cast<const uint4*>(from + c);
+        *reinterpret_cast<uint4*>(out + c) = v;
+        if (scaled) *reinterpret_cast<uint4*>(scaled + c) = make_uint4(times(v.x), times(v.y), times(v.z), times(v.w));
+      }
     } else {
-      for (int c = lane; c < p.ld; c += 32) out[c] = c < p.depth ? from[c] : (unsigned short)0;
+      for (int c = lane; c < p.ld; c += 32) {
+        const unsigned short v = c < p.depth ? from[c] : (unsigned short)0;
+        out[c] = v;
+        if (scaled) scaled[c] = (unsigned short)times(v);
+      }
     }
   } else if (p.dx) {
     unsigned short* out = p.dx + (int64_t)row * p.depth;
@@ -171,32 +211,30 @@ struct StatsEpilogue {
   }
 };
 
-// dz[row][col], rows of `ld` elements: zeros behind the last position, up to the end of its tile
+// dz / (g by)[row][col], rows of `ld` elements: zeros behind the last position, up to the end of its tile.  up = 1 / by, mean = a / V / by, hit = (1 - a) / by
 struct GradientEpilogue {
-  struct Params { const int* target; const float *lse, *g; __nv_bfloat16* dz; int64_t ld; int first; float hit, mean; };
+  struct Params { const int* target; const float* lse; __nv_bfloat16* dz; int64_t ld; int first; float up, mean, hit; };
   const Params& p;
-  float lse, g;
+  float lse;
   int t;
   __device__ __forceinline__ explicit GradientEpilogue(const Params& e) : p(e) {}
   __device__ __forceinline__ void begin(const Place& at) {
     const bool there = at.row < at.rows;
     t = there ? p.target[at.row] - p.first - at.col : -1;
     lse = there ? -p.lse[at.row] : 0.0f;
-    g = there ? p.g[at.row] : 0.0f;
   }
   __device__ __forceinline__ void chunk(const Place& at, int c, float (&v)[32]) {
-    const float less = -g * p.mean;
     const bool there = at.row < at.rows;
 #pragma unroll
     for (int j = 0; j < 32; j += 2) {
       const float2 d = __fmul2_rn(__fadd2_rn(make_float2(v[j], v[j + 1]), make_float2(lse, lse)), make_float2(kLog2E, kLog2E));
-      const float2 r = __ffma2_rn(make_float2(exp2_approx(d.x), exp2_approx(d.y)), make_float2(g, g), make_float2(less, less));
+      const float2 r = __ffma2_rn(make_float2(exp2_approx(d.x), exp2_approx(d.y)), make_float2(p.up, p.up), make_float2(-p.mean, -p.mean));
       v[j] = there ? r.x : 0.0f; v[j + 1] = there ? r.y : 0.0f;
     }
     if (__any_sync(0xffffffffu, t >= c && t < c + 32)) {
 #pragma unroll
       for (int j = 0; j < 32; ++j)
-        if (t == c + j) v[j] = fmaf(-g, p.hit, v[j]);
+        if (t == c + j) v[j] -= p.hit;
     }
     store_row32<Bf16>(p.dz + (int64_t)at.row * p.ld + at.col + c, v);
   }
@@ -206,11 +244,16 @@ struct GradientEpilogue {
 enum { kOnly, kFirst, kMore, kLast };      // of the products that are added up: a single one to bf16; into acc, onto acc, with acc to bf16
 template <int MODE>
 struct StoreEpilogue {
-  struct Params { __nv_bfloat16* out; float* acc; const int* origin; int64_t ld, ld_acc; int vectors; };      // vectors: bytes that rows begin at a multiple of, 32, 16 or 2
+  // what leaves as bf16 is multiplied by `by` and by scale[row], or scale[0] without origin; vectors: bytes that rows of out begin at a multiple of, 32, 16 or 2
+  struct Params { __nv_bfloat16* out; float* acc; const int* origin; const float* scale; float by; int64_t ld, ld_acc; int vectors; };
   const Params& p;
   int64_t row;
+  float scale;
   __device__ __forceinline__ explicit StoreEpilogue(const Params& e) : p(e) {}
-  __device__ __forceinline__ void begin(const Place& at) { row = at.row < at.rows ? (p.origin ? p.origin[at.row] : at.row) : -1; }
+  __device__ __forceinline__ void begin(const Place& at) {
+    row = at.row < at.rows ? (p.origin ? p.origin[at.row] : at.row) : -1;
+    scale = row < 0 || MODE == kFirst || MODE == kMore ? 0.0f : p.by * p.scale[p.origin ? at.row : 0];
+  }
   __device__ __forceinline__ void chunk(const Place& at, int c, float (&v)[32]) {
     const int col = at.col + c;
     if (MODE != kOnly && row >= 0) {
@@ -223,7 +266,11 @@ struct StoreEpilogue {
         else a[j] = f;
       }
     }
-    if (MODE == kFirst || MODE == kMore) return;
+    if constexpr (MODE == kOnly || MODE == kLast) leave(at, col, v);
+  }
+  __device__ __forceinline__ void leave(const Place& at, int col, float (&v)[32]) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] *= scale;
     __nv_bfloat16* to = p.out + row * p.ld + col;
     if (p.vectors >= 16 && col + 32 <= at.cols) {
       if (row < 0) return;
@@ -292,7 +339,7 @@ struct Plan {
   int64_t cap, ld_x, ld_acc, piece, ld_w, inner_w, outer_w, parts;
   int pieces;
   bool pad;
-  size_t off_place, off_origin, off_target, off_lse, off_g, off_x, off_w, off_terms, off_sums, off_hit, off_dz, off_acc, bytes;
+  size_t off_place, off_origin, off_target, off_lse, off_g, off_x, off_scaled, off_w, off_terms, off_sums, off_hit, off_dz, off_acc, bytes;
 };
 int make_plan(const char* name, int64_t rows, int64_t depth, const Weight& w, int64_t vocab, bool backward, Plan* q) {
   if (rows < 0 || rows > (1 << 24) || depth <= 0 || depth > (1 << 20) || vocab <= 0 || vocab > (1 << 28) || w.ld < (w.by_word ? depth : vocab))
@@ -313,9 +360,10 @@ int make_plan(const char* name, int64_t rows, int64_t depth, const Weight& w, in
   q->off_place = take((size_t)rows * 4); q->off_origin = take((size_t)q->cap * 4); q->off_target = take((size_t)q->cap * 4);
   q->off_x = take((size_t)q->cap * q->ld_x * 2);
   q->off_w = take(q->pad ? (size_t)q->outer_w * q->ld_w * 2 : 0);
-  q->off_lse = q->off_g = q->off_dz = q->off_acc = q->off_terms = q->off_sums = q->off_hit = 0;
+  q->off_lse = q->off_g = q->off_scaled = q->off_dz = q->off_acc = q->off_terms = q->off_sums = q->off_hit = 0;
   if (backward) {
     q->off_lse = take((size_t)q->cap * 4); q->off_g = take((size_t)q->cap * 4);
+    q->off_scaled = take((size_t)q->cap * q->ld_x * 2);
     q->off_dz = take((size_t)q->cap * q->piece * 2);
     q->off_acc = take(q->pieces > 1 ? (size_t)q->cap * q->ld_acc * 4 : 0);
   } else {
@@ -345,15 +393,15 @@ int checks(const char* name, const Positions& x, const Weight& w, int64_t vocab,
 template <typename T> T* part(void* workspace, size_t off) { return reinterpret_cast<T*>(static_cast<unsigned char*>(workspace) + off); }
 
 // numbers the positions, brings their hidden states together and the weight where TMA reads it
-int make_ready(const Positions& x, Weight* w, int64_t vocab, const Plan& q, void* ws, float* loss, float* lse_none, const float* lse, const float* g, void* dx, cudaStream_t st) {
+int make_ready(const Positions& x, Weight* w, int64_t vocab, const Plan& q, void* ws, float* loss, float* lse_none, const float* lse, const float* g, void* dx, bool scaled, cudaStream_t st) {
   const int rows = (int)(x.outer * x.inner);
   const SelectParams sp{x.targets, vocab, rows, part<int>(ws, 0), part<int>(ws, q.off_place), part<int>(ws, q.off_origin), part<int>(ws, q.off_target), lse, g,
-                        part<float>(ws, q.off_lse), part<float>(ws, q.off_g), loss, lse_none};
+                        part<float>(ws, q.off_lse), part<float>(ws, q.off_g), part<float>(ws, 64), loss, lse_none};
   launch_behind(select_kernel, 1, 1024, 0, st, sp);
   PB_LAUNCH_CHECK("select_kernel");
   const bool vectors = x.depth % 8 == 0 && !off_by(x.x, 16) && (x.outer == 1 || x.stride_outer % 8 == 0) && (x.inner == 1 || x.stride_inner % 8 == 0);
   const GatherParams gp{static_cast<const unsigned short*>(x.x), x.inner, x.stride_outer, x.stride_inner, part<int>(ws, 0), part<int>(ws, q.off_place), part<unsigned short>(ws, q.off_x),
-                        static_cast<unsigned short*>(dx), rows, (int)x.depth, (int)q.ld_x, vectors, x.depth % 8 == 0 && !off_by(dx, 16)};
+                        scaled ? part<unsigned short>(ws, q.off_scaled) : nullptr, static_cast<unsigned short*>(dx), part<float>(ws, q.off_g), part<float>(ws, 64), rows, (int)x.depth, (int)q.ld_x, vectors, x.depth % 8 == 0 && !off_by(dx, 16)};
   launch_behind(gather_kernel, (unsigned)((rows + kRowTile + 7) / 8), 256, 0, st, gp);
   PB_LAUNCH_CHECK("gather_kernel");
   if (q.pad) {
@@ -376,14 +424,14 @@ const unsigned short* words(const Weight& w, int64_t first) { return static_cast
 template <class E>
 int logits(const Plan& q, const Weight& w, int64_t first, int64_t n, int64_t depth, void* ws, const typename E::Params& e, cudaStream_t st) {
   Params p{};
-  p.count = part<int>(ws, 0); p.counted = 1; p.rows = (int)q.cap; p.cols = (int)n; p.depth = (int)depth; p.batch = 1; p.bf16 = 1;
+  p.count = part<int>(ws, 0); p.counted = 1; p.rows = (int)q.cap; p.cols = (int)n; p.depth = (int)depth; p.batch = 1; p.bf16 = 1; p.group = kGroup;
   const Operand x{part<void>(ws, q.off_x), false, q.cap, depth, q.ld_x, q.cap * q.ld_x}, words_of{words(w, first), !w.by_word, n, depth, w.ld, w.ld * 8};
   return w.by_word ? launch<2, 256, false, false, E>(x, words_of, p, e, st) : launch<2, 256, false, true, E>(x, words_of, p, e, st);
 }
 template <int MODE>
 int to_hidden(const Plan& q, const Weight& w, int64_t first, int64_t n, int64_t depth, void* ws, const typename StoreEpilogue<MODE>::Params& e, cudaStream_t st) {
   Params p{};
-  p.count = part<int>(ws, 0); p.counted = 1; p.rows = (int)q.cap; p.cols = (int)depth; p.depth = (int)n; p.batch = 1; p.bf16 = 1;
+  p.count = part<int>(ws, 0); p.counted = 1; p.rows = (int)q.cap; p.cols = (int)depth; p.depth = (int)n; p.batch = 1; p.bf16 = 1; p.group = kGroup;
   const Operand dz{part<void>(ws, q.off_dz), false, q.cap, n, q.piece, q.cap * q.piece}, words_of{words(w, first), w.by_word, depth, n, w.ld, w.ld * 8};
   return w.by_word ? launch<2, 256, false, true, StoreEpilogue<MODE>>(dz, words_of, p, e, st) : launch<2, 256, false, false, StoreEpilogue<MODE>>(dz, words_of, p, e, st);
 }
@@ -410,7 +458,7 @@ extern "C" int pb_linear_xent(const void* x, int64_t outer, int64_t inner, int64
   if (!loss || !lse) return fail(PB_ERR_NULL_POINTER, "pb_linear_xent: null argument");
   if (off_by(loss, 4) || off_by(lse, 4)) return fail(PB_ERR_MISALIGNED, "pb_linear_xent: misaligned array");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (int s = make_ready(at, &w, vocab, q, workspace, loss, lse, nullptr, nullptr, nullptr, st)) return s;
+  if (int s = make_ready(at, &w, vocab, q, workspace, loss, lse, nullptr, nullptr, nullptr, false, st)) return s;
   int* target = part<int>(workspace, q.off_target);
   float2* terms = part<float2>(workspace, q.off_terms);
   float *sums = part<float>(workspace, q.off_sums), *hit = part<float>(workspace, q.off_hit);
@@ -440,31 +488,33 @@ extern "C" int pb_linear_xent_bwd(const void* x, int64_t outer, int64_t inner, i
   }
   if (!lse || !g) return fail(PB_ERR_NULL_POINTER, "pb_linear_xent_bwd: null argument");
   if (!dx && !dweight) return PB_OK;
-  if (int s = make_ready(at, &w, vocab, q, workspace, nullptr, nullptr, lse, g, dx, st)) return s;
+  if (int s = make_ready(at, &w, vocab, q, workspace, nullptr, nullptr, lse, g, dx, dweight != nullptr, st)) return s;
   int *origin = part<int>(workspace, q.off_origin), *target = part<int>(workspace, q.off_target);
   __nv_bfloat16 *dz = part<__nv_bfloat16>(workspace, q.off_dz), *d_hidden = static_cast<__nv_bfloat16*>(dx);
   float* acc = part<float>(workspace, q.off_acc);
+  const float* gs = part<float>(workspace, q.off_g);
+  const float by = smoothing <= 0.5f ? 1.0f - smoothing : 1.0f;      // without a target's share to speak of, any
   for (int k = 0; k < q.pieces; ++k) {
     const int64_t first = k * q.piece, n = std::min(q.piece, vocab - first);
     if (int s = logits<GradientEpilogue>(q, w, first, n, depth, workspace,
-                                         {target, part<float>(workspace, q.off_lse), part<float>(workspace, q.off_g), dz, q.piece, (int)first, 1.0f - smoothing, smoothing / (float)vocab}, st))
+                                         {target, part<float>(workspace, q.off_lse), dz, q.piece, (int)first, 1.0f / by, smoothing / (float)vocab / by, (1.0f - smoothing) / by}, st))
       return s;
     if (dx) {
       const int vectors = bytes_of(dx, depth);
-      if (int s = q.pieces == 1       ? to_hidden<kOnly>(q, w, first, n, depth, workspace, {d_hidden, acc, origin, depth, q.ld_acc, vectors}, st)
-                : k == 0              ? to_hidden<kFirst>(q, w, first, n, depth, workspace, {d_hidden, acc, origin, depth, q.ld_acc, vectors}, st)
-                : k < q.pieces - 1    ? to_hidden<kMore>(q, w, first, n, depth, workspace, {d_hidden, acc, origin, depth, q.ld_acc, vectors}, st)
-                                      : to_hidden<kLast>(q, w, first, n, depth, workspace, {d_hidden, acc, origin, depth, q.ld_acc, vectors}, st))
+      if (int s = q.pieces == 1       ? to_hidden<kOnly>(q, w, first, n, depth, workspace, {d_hidden, acc, origin, gs, by, depth, q.ld_acc, vectors}, st)
+                : k == 0              ? to_hidden<kFirst>(q, w, first, n, depth, workspace, {d_hidden, acc, origin, gs, by, depth, q.ld_acc, vectors}, st)
+                : k < q.pieces - 1    ? to_hidden<kMore>(q, w, first, n, depth, workspace, {d_hidden, acc, origin, gs, by, depth, q.ld_acc, vectors}, st)
+                                      : to_hidden<kLast>(q, w, first, n, depth, workspace, {d_hidden, acc, origin, gs, by, depth, q.ld_acc, vectors}, st))
         return s;
     }
     if (dweight) {
       Params p{};
-      p.count = part<int>(workspace, 0); p.counted = 2; p.depth = (int)q.cap; p.batch = 1; p.bf16 = 1;
+      p.count = part<int>(workspace, 0); p.counted = 2; p.depth = (int)q.cap; p.batch = 1; p.bf16 = 1; p.group = kGroup;
       p.rows = (int)(w.by_word ? n : depth); p.cols = (int)(w.by_word ? depth : n);
-      const Operand hidden{part<void>(workspace, q.off_x), true, depth, q.cap, q.ld_x, q.cap * q.ld_x}, gradient{dz, true, n, q.cap, q.piece, q.cap * q.piece};
+      const Operand hidden{part<void>(workspace, q.off_scaled), true, depth, q.cap, q.ld_x, q.cap * q.ld_x}, gradient{dz, true, n, q.cap, q.piece, q.cap * q.piece};
       const int64_t ld_out = w.by_word ? depth : vocab;
       __nv_bfloat16* out = static_cast<__nv_bfloat16*>(dweight) + (w.by_word ? first * depth : first);
-      const StoreEpilogue<kOnly>::Params e{out, nullptr, nullptr, ld_out, 0, bytes_of(out, ld_out)};
+      const StoreEpilogue<kOnly>::Params e{out, nullptr, nullptr, part<float>(workspace, 64), by, ld_out, 0, bytes_of(out, ld_out)};
       if (int s = w.by_word ? launch<2, 256, true, true, StoreEpilogue<kOnly>>(gradient, hidden, p, e, st) : launch<2, 256, true, true, StoreEpilogue<kOnly>>(hidden, gradient, p, e, st)) return s;
     }
   }

@@ -7,7 +7,9 @@
 //             SM, where one CTA's 128 x 256 takes 48: what a tile loads from L2 is the nearest bound beside the tensor core);
 //   CTAS = 1: 128 x 128, for products that have few tiles.
 // Persistent: warp 0 loads, a lane of warp 1 (of the leading CTA) issues tcgen05.mma, eight warps empty one accumulator of TMEM while the
-// other fills, each thread one row and half of the columns, 32 at a time.  Every wait is bounded and reported by pb_gemm_check.
+// other fills, each thread one row and half of the columns.  Every wait is bounded and reported by pb_gemm_check.
+// The tensor core's own additions do not round to nearest: an accumulator takes `group` stages of k, and the sums of a tile's groups are added up in the
+// registers that read them.  2-norm errors of the loss of 64 positions of 2048 against 64 bits: one group 1.4e-6, groups of 512 of k GROUP_ERROR.
 #pragma once
 
 #include <cuda.h>
@@ -50,6 +52,7 @@ struct Params {
   int upper;                // only tiles on and above the diagonal (CTAS * 128 == N)
   int band;                 // tile rows that are walked down before the next column
   int bf16;                 // else fp16
+  int group;                // stages of k that an accumulator takes
   uint32_t polls;
   int withhold;             // diagnostics build: the first stage is never filled
 };
@@ -222,96 +225,123 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   const Tiles tiles(p, rows, F::kRows, N);
   const int items = tiles.per_batch * p.batch, first = blockIdx.x / CTAS, stride = gridDim.x / CTAS;
 
-  if (warp == 0) {
-    if (lane == 0) {
-      uint32_t it = 0;
-      bool ok = true;
-      for (int w = first; w < items && ok; w += stride) {
-        int batch, tm, tn;
-        tiles.at(w, batch, tm, tn);
-        const int m0 = tm * F::kRows + rank * 128, n0 = tn * N + rank * F::kBRows;
-        for (int k = 0; k < steps; ++k, ++it) {
-          const int s = it % F::kStages;
-          if (!bar_wait(empty(s), ((it / F::kStages) & 1) ^ 1, p.polls)) { ok = false; break; }
-          if (p.withhold && it == 0) continue;
-          const uint32_t bar = CTAS == 2 ? in_leader(full(s)) : full(s), a = base + s * F::kStageBytes, b = a + F::kABytes;
-          if (leader) bar_expect(full(s), CTAS * F::kStageBytes);
-          if (A_MN) {
-            load_box<CTAS>(a, &map_a, m0, k * kDepth, batch, bar);
-            load_box<CTAS>(a + 8192, &map_a, m0 + 64, k * kDepth, batch, bar);
-          } else {
-            load_box<CTAS>(a, &map_a, k * kDepth, m0, batch, bar);
-          }
-          if (B_MN) {
+  // registers: 128 x 56 + 256 x 216 of the 384 x 168 that the block has
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0) {
+      if (lane == 0) {
+        uint32_t it = 0;
+        bool ok = true;
+        for (int w = first; w < items && ok; w += stride) {
+          int batch, tm, tn;
+          tiles.at(w, batch, tm, tn);
+          const int m0 = tm * F::kRows + rank * 128, n0 = tn * N + rank * F::kBRows;
+          for (int k = 0; k < steps; ++k, ++it) {
+            const int s = it % F::kStages;
+            if (!bar_wait(empty(s), ((it / F::kStages) & 1) ^ 1, p.polls)) { ok = false; break; }
+            if (p.withhold && it == 0) continue;
+            const uint32_t bar = CTAS == 2 ? in_leader(full(s)) : full(s), a = base + s * F::kStageBytes, b = a + F::kABytes;
+            if (leader) bar_expect(full(s), CTAS * F::kStageBytes);
+            if (A_MN) {
+              load_box<CTAS>(a, &map_a, m0, k * kDepth, batch, bar);
+              load_box<CTAS>(a + 8192, &map_a, m0 + 64, k * kDepth, batch, bar);
+            } else {
+              load_box<CTAS>(a, &map_a, k * kDepth, m0, batch, bar);
+            }
+            if (B_MN) {
 #pragma unroll
-            for (int j = 0; j < F::kBRows / 64; ++j) load_box<CTAS>(b + j * 8192, &map_b, n0 + 64 * j, k * kDepth, batch, bar);
-          } else {
-            load_box<CTAS>(b, &map_b, k * kDepth, n0, batch, bar);
+              for (int j = 0; j < F::kBRows / 64; ++j) load_box<CTAS>(b + j * 8192, &map_b, n0 + 64 * j, k * kDepth, batch, bar);
+            } else {
+              load_box<CTAS>(b, &map_b, k * kDepth, n0, batch, bar);
+            }
+          }
+        }
+        // leave only when every copy that this pair started has landed (bounded)
+        if (leader)
+          for (uint32_t k = it > (uint32_t)F::kStages ? it - F::kStages : 0; k < it; ++k)
+            if (!(p.withhold && k == 0)) (void)bar_wait(full(k % F::kStages), (k / F::kStages) & 1, p.polls);
+      }
+    } else if (warp == 1) {
+      if (lane == 0 && leader) {
+        const uint32_t instr = kInstr<CTAS, N, A_MN, B_MN> | (p.bf16 ? kBf16Operands : 0u);
+        uint32_t it = 0, n = 0;
+        bool ok = true;
+        for (int w = first; w < items && ok; w += stride) {
+          for (int k0 = 0; ok && (k0 == 0 || k0 < steps); k0 += p.group, ++n) {
+            const uint32_t ab = n & 1, d = tmem + ab * N;
+            ok = bar_wait(acc_empty(ab), ((n >> 1) & 1) ^ 1, p.polls);
+            tc_after();
+            const int end = min(steps, k0 + p.group);
+            for (int k = k0; ok && k < end; ++k, ++it) {
+              const int s = it % F::kStages;
+              if (!bar_wait(full(s), (it / F::kStages) & 1, p.polls)) { ok = false; break; }
+              tc_after();
+              const uint64_t a = tile_desc<A_MN>(base + s * F::kStageBytes), b = tile_desc<B_MN>(base + s * F::kStageBytes + F::kABytes);
+#pragma unroll
+              for (int j = 0; j < kDepth / 16; ++j) mma<CTAS>(d, a + (uint64_t)(j * kStep16<A_MN>), b + (uint64_t)(j * kStep16<B_MN>), instr, k > k0 || j > 0);
+              commit_to<CTAS>(empty(s));
+            }
+            if (ok) commit_to<CTAS>(acc_full(ab));
           }
         }
       }
-      // leave only when every copy that this pair started has landed (bounded)
-      if (leader)
-        for (uint32_t k = it > (uint32_t)F::kStages ? it - F::kStages : 0; k < it; ++k)
-          if (!(p.withhold && k == 0)) (void)bar_wait(full(k % F::kStages), (k / F::kStages) & 1, p.polls);
     }
-  } else if (warp == 1) {
-    if (lane == 0 && leader) {
-      const uint32_t instr = kInstr<CTAS, N, A_MN, B_MN> | (p.bf16 ? kBf16Operands : 0u);
-      uint32_t it = 0, n = 0;
-      bool ok = true;
-      for (int w = first; w < items && ok; w += stride, ++n) {
-        const uint32_t ab = n & 1, d = tmem + ab * N;
-        if (!bar_wait(acc_empty(ab), ((n >> 1) & 1) ^ 1, p.polls)) break;
-        tc_after();
-        for (int k = 0; k < steps; ++k, ++it) {
-          const int s = it % F::kStages;
-          if (!bar_wait(full(s), (it / F::kStages) & 1, p.polls)) { ok = false; break; }
-          tc_after();
-          const uint64_t a = tile_desc<A_MN>(base + s * F::kStageBytes), b = tile_desc<B_MN>(base + s * F::kStageBytes + F::kABytes);
-#pragma unroll
-          for (int j = 0; j < kDepth / 16; ++j) mma<CTAS>(d, a + (uint64_t)(j * kStep16<A_MN>), b + (uint64_t)(j * kStep16<B_MN>), instr, k > 0 || j > 0);
-          commit_to<CTAS>(empty(s));
-        }
-        if (ok) commit_to<CTAS>(acc_full(ab));
-      }
-    }
-  } else if (warp >= 4) {
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int quad = warp & 3, half = (warp - 4) >> 2;      // rows 32 quad .., columns kCols half ..
     Epilogue epilogue(e);
     Place at;
     at.rows = rows; at.cols = p.cols; at.lane = lane;
     at.staging = base + F::kStages * F::kStageBytes + (warp - 4) * F::kStaging;
     uint32_t n = 0;
-    for (int w = first; w < items; w += stride, ++n) {
+    bool ok = true;
+    for (int w = first; w < items && ok; w += stride) {
       int tm, tn;
       tiles.at(w, at.batch, tm, tn);
-      const uint32_t ab = n & 1;
       at.row = tm * F::kRows + rank * 128 + quad * 32 + lane;
       at.col = tn * N + half * F::kCols;
       at.beside = tm != tn;
-      if (!__all_sync(0xffffffffu, bar_wait(acc_full(ab), (n >> 1) & 1, p.polls))) break;
-      tc_after();
-      const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + ab * N + half * F::kCols;
-      const uint32_t freed = CTAS == 2 ? in_leader(acc_empty(ab)) : acc_empty(ab);
-      epilogue.begin(at);
-      float v[2][32];
-      ld_acc32(from, v[0]);
+      float acc[F::kCols / 32][32];
+      for (int k0 = 0; k0 == 0 || k0 < steps; k0 += p.group, ++n) {
+        const uint32_t ab = n & 1;
+        ok = __all_sync(0xffffffffu, bar_wait(acc_full(ab), (n >> 1) & 1, p.polls));
+        if (!ok) break;
+        tc_after();
+        const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + ab * N + half * F::kCols;
+        const uint32_t freed = CTAS == 2 ? in_leader(acc_empty(ab)) : acc_empty(ab);
+        if (k0 == 0) {
 #pragma unroll
-      for (int c = 0; c < F::kCols / 32; ++c) {
-        wait_acc32(v[c & 1]);
-        if (c + 1 < F::kCols / 32) {
-          ld_acc32(from + 32 * (c + 1), v[(c + 1) & 1]);
+          for (int c = 0; c < F::kCols / 32; ++c) ld_acc32(from + 32 * c, acc[c]);
+#pragma unroll
+          for (int c = 0; c < F::kCols / 32; ++c) wait_acc32(acc[c]);
         } else {
-          tc_before();
-          __syncwarp();
-          if (lane == 0) arrive_in_cluster(freed);
-        }
-        if (steps == 0)
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[c & 1][j] = 0.0f;       // nothing was added up
-        if (at.col + 32 * c < p.cols) epilogue.chunk(at, 32 * c, v[c & 1]);
+          for (int c = 0; c < F::kCols / 32; ++c) {
+            float v[32];
+            ld_acc32(from + 32 * c, v);
+            wait_acc32(v);
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              const float2 s = __fadd2_rn(make_float2(acc[c][j], acc[c][j + 1]), make_float2(v[j], v[j + 1]));
+              acc[c][j] = s.x; acc[c][j + 1] = s.y;
+            }
+          }
+        }
+        tc_before();
+        __syncwarp();
+        if (lane == 0) arrive_in_cluster(freed);
       }
+      if (!ok) break;
+      if (steps == 0) {             // nothing was added up
+#pragma unroll
+        for (int c = 0; c < F::kCols / 32; ++c)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[c][j] = 0.0f;
+      }
+      epilogue.begin(at);
+#pragma unroll
+      for (int c = 0; c < F::kCols / 32; ++c)
+        if (at.col + 32 * c < p.cols) epilogue.chunk(at, 32 * c, acc[c]);
       epilogue.end(at);
     }
   }
@@ -417,6 +447,7 @@ int launch(const Operand& a, const Operand& b, Params p, const typename Epilogue
   if (items == 0) return PB_OK;
   // a band's rows of A, some 16 MB, stay in L2 while its columns go by
   p.band = (int)std::max<int64_t>(1, (16 << 20) / (F::kRows * 2 * std::max<int64_t>(1, p.depth)));
+  if (p.group == 0) p.group = kMaxIndexed;
   p.polls = kWaitPolls; p.withhold = 0;
 #ifdef PB_DIAGNOSTICS
   p.polls = g_polls.load(); p.withhold = g_withhold.load();
