@@ -160,9 +160,10 @@ __global__ void __launch_bounds__(256) pad_kernel(const unsigned short* from, in
 }
 
 // ---- the epilogues ------------------------------------------------------------------------------------------------
+struct Grouped { static constexpr bool kGrouped = true; static constexpr int kSlots = 1; };
 // terms[part][row] = (m, s): the largest z of a part and the sum of exp(z - m); sums[part][row] of z; hit[row] the target's z
 template <bool MEAN>
-struct StatsEpilogue {
+struct StatsEpilogue : Grouped {
   struct Params { const int* target; float2* terms; float* sums; float* hit; int64_t cap; };
   const Params& p;
   float m, s, sum, hit;
@@ -172,32 +173,32 @@ struct StatsEpilogue {
     m = -INFINITY; s = 0.0f; sum = 0.0f;
     t = at.row < at.rows ? p.target[at.row] - at.col : -1;
   }
-  __device__ __forceinline__ void chunk(const Place& at, int c, float (&v)[32]) {
+  __device__ __forceinline__ void block(const Place& at, int c, float (&v)[kBlock]) {
     const int n = at.cols - at.col - c;
-    if (__any_sync(0xffffffffu, t >= c && t < c + 32)) {
+    if (__any_sync(0xffffffffu, t >= c && t < c + kBlock)) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
+      for (int j = 0; j < kBlock; ++j)
         if (t == c + j) p.hit[at.row] = v[j];
     }
     if (MEAN) {
       float2 a = make_float2(0.0f, 0.0f);
 #pragma unroll
-      for (int j = 0; j < 32; j += 2) a = __fadd2_rn(a, make_float2(v[j], v[j + 1]));      // beyond the vocabulary: zeros
+      for (int j = 0; j < kBlock; j += 2) a = __fadd2_rn(a, make_float2(v[j], v[j + 1]));      // beyond the vocabulary: zeros
       sum += a.x + a.y;
     }
-    if (n < 32) {
+    if (n < kBlock) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
+      for (int j = 0; j < kBlock; ++j)
         if (j >= n) v[j] = -INFINITY;
     }
     float top = v[0];
 #pragma unroll
-    for (int j = 1; j < 32; ++j) top = fmaxf(top, v[j]);
+    for (int j = 1; j < kBlock; ++j) top = fmaxf(top, v[j]);
     if (top > m) { s *= exp2_approx((m - top) * kLog2E); m = top; }
     const float base = m == -INFINITY ? 0.0f : -m;
     float2 a = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int j = 0; j < 32; j += 2) {
+    for (int j = 0; j < kBlock; j += 2) {
       const float2 d = __fmul2_rn(__fadd2_rn(make_float2(v[j], v[j + 1]), make_float2(base, base)), make_float2(kLog2E, kLog2E));
       a = __fadd2_rn(a, make_float2(exp2_approx(d.x), exp2_approx(d.y)));
     }
@@ -209,11 +210,12 @@ struct StatsEpilogue {
     p.terms[to] = make_float2(m, s);
     if (MEAN) p.sums[to] = sum;
   }
+  __device__ __forceinline__ void finish(const Place&) {}
 };
 
 // dz / (g by)[row][col], rows of `ld` elements: zeros behind the last position, up to the end of its tile.  up = 1 / by, mean = a / V / by, hit = (1 - a) / by
-struct GradientEpilogue {
-  struct Params { const int* target; const float* lse; __nv_bfloat16* dz; int64_t ld; int first; float up, mean, hit; };
+struct GradientEpilogue : Grouped {
+  struct Params { CUtensorMap dz; const int* target; const float* lse; int first; float up, mean, hit; };
   const Params& p;
   float lse;
   int t;
@@ -223,69 +225,63 @@ struct GradientEpilogue {
     t = there ? p.target[at.row] - p.first - at.col : -1;
     lse = there ? -p.lse[at.row] : 0.0f;
   }
-  __device__ __forceinline__ void chunk(const Place& at, int c, float (&v)[32]) {
+  __device__ __forceinline__ void block(const Place& at, int c, float (&v)[kBlock]) {
     const bool there = at.row < at.rows;
 #pragma unroll
-    for (int j = 0; j < 32; j += 2) {
+    for (int j = 0; j < kBlock; j += 2) {
       const float2 d = __fmul2_rn(__fadd2_rn(make_float2(v[j], v[j + 1]), make_float2(lse, lse)), make_float2(kLog2E, kLog2E));
       const float2 r = __ffma2_rn(make_float2(exp2_approx(d.x), exp2_approx(d.y)), make_float2(p.up, p.up), make_float2(-p.mean, -p.mean));
       v[j] = there ? r.x : 0.0f; v[j + 1] = there ? r.y : 0.0f;
     }
-    if (__any_sync(0xffffffffu, t >= c && t < c + 32)) {
+    if (__any_sync(0xffffffffu, t >= c && t < c + kBlock)) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
+      for (int j = 0; j < kBlock; ++j)
         if (t == c + j) v[j] -= p.hit;
     }
-    store_row32<Bf16>(p.dz + (int64_t)at.row * p.ld + at.col + c, v);
+    if (at.lane == 0) Slots::wait_read();
+    __syncwarp();
+    Slots::stage<Bf16>(at, 0, v);
+    Slots::hand_over();
+    if (at.lane == 0) { Slots::send(at, 0, &p.dz, at.col + c, at.row, 0); Slots::sent(); }
   }
   __device__ __forceinline__ void end(const Place&) {}
+  __device__ __forceinline__ void finish(const Place& at) { if (at.lane == 0) Slots::wait_sent(); }
 };
 
 enum { kOnly, kFirst, kMore, kLast };      // of the products that are added up: a single one to bf16; into acc, onto acc, with acc to bf16
 template <int MODE>
-struct StoreEpilogue {
-  // what leaves as bf16 is multiplied by `by` and by scale[row], or scale[0] without origin; vectors: bytes that rows of out begin at a multiple of, 32, 16 or 2
-  struct Params { __nv_bfloat16* out; float* acc; const int* origin; const float* scale; float by; int64_t ld, ld_acc; int vectors; };
+struct StoreEpilogue : Grouped {
+  // what leaves as bf16 is multiplied by `by` and by scale[row], or scale[0] without origin; acc: a warp's parts of the tiles, 16 bytes a lane in a row
+  struct Params { __nv_bfloat16* out; float4* acc; const int* origin; const float* scale; float by; int64_t ld; bool vectors; };
   const Params& p;
-  int64_t row;
+  int row;
   float scale;
   __device__ __forceinline__ explicit StoreEpilogue(const Params& e) : p(e) {}
   __device__ __forceinline__ void begin(const Place& at) {
     row = at.row < at.rows ? (p.origin ? p.origin[at.row] : at.row) : -1;
     scale = row < 0 || MODE == kFirst || MODE == kMore ? 0.0f : p.by * p.scale[p.origin ? at.row : 0];
   }
-  __device__ __forceinline__ void chunk(const Place& at, int c, float (&v)[32]) {
-    const int col = at.col + c;
-    if (MODE != kOnly && row >= 0) {
-      float4* a = reinterpret_cast<float4*>(p.acc + (int64_t)at.row * p.ld_acc + col);
+  __device__ __forceinline__ void block(const Place& at, int c, float (&v)[kBlock]) {
+    if constexpr (MODE != kOnly) {
+      float4* a = p.acc + ((int64_t)at.part * (kPart / 4) + c / 4) * 32 + at.lane;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float4 f = MODE == kFirst ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : a[j];
+      for (int j = 0; j < kBlock / 4; ++j) {
+        float4 f = MODE == kFirst ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : a[32 * j];
         f.x += v[4 * j]; f.y += v[4 * j + 1]; f.z += v[4 * j + 2]; f.w += v[4 * j + 3];
         if (MODE == kLast) { v[4 * j] = f.x; v[4 * j + 1] = f.y; v[4 * j + 2] = f.z; v[4 * j + 3] = f.w; }
-        else a[j] = f;
+        else a[32 * j] = f;
       }
     }
-    if constexpr (MODE == kOnly || MODE == kLast) leave(at, col, v);
-  }
-  __device__ __forceinline__ void leave(const Place& at, int col, float (&v)[32]) {
+    if constexpr (MODE == kOnly || MODE == kLast) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] *= scale;
-    __nv_bfloat16* to = p.out + row * p.ld + col;
-    if (p.vectors >= 16 && col + 32 <= at.cols) {
-      if (row < 0) return;
-      if (p.vectors == 32) {
-        store_row32<Bf16>(to, v);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          reinterpret_cast<uint4*>(to)[j] = make_uint4(Bf16::pack(v[8 * j], v[8 * j + 1]), Bf16::pack(v[8 * j + 2], v[8 * j + 3]), Bf16::pack(v[8 * j + 4], v[8 * j + 5]), Bf16::pack(v[8 * j + 6], v[8 * j + 7]));
-      }
-    } else {
-      store_block32<Bf16>(at, row >= 0 ? reinterpret_cast<unsigned short*>(to) : nullptr, at.cols - col, v);
+      for (int j = 0; j < kBlock; ++j) v[j] *= scale;
+      Slots::stage<Bf16>(at, 0, v);
+      __syncwarp();
+      Slots::scatter(at.own, at.lane, reinterpret_cast<unsigned short*>(p.out + at.col + c), p.ld, row, at.cols - at.col - c, p.vectors);
     }
   }
   __device__ __forceinline__ void end(const Place&) {}
+  __device__ __forceinline__ void finish(const Place&) {}
 };
 
 // ---- the parts of a position's logits together ----------------------------------------------------------------------
@@ -336,7 +332,7 @@ struct Weight {
 };
 
 struct Plan {
-  int64_t cap, ld_x, ld_acc, piece, ld_w, inner_w, outer_w, parts;
+  int64_t cap, ld_x, piece, ld_w, inner_w, outer_w, parts;
   int pieces;
   bool pad;
   size_t off_place, off_origin, off_target, off_lse, off_g, off_x, off_scaled, off_w, off_terms, off_sums, off_hit, off_dz, off_acc, bytes;
@@ -346,7 +342,6 @@ int make_plan(const char* name, int64_t rows, int64_t depth, const Weight& w, in
     return fail(PB_ERR_BAD_SHAPE, "%s: rows=%lld depth=%lld vocab=%lld, rows of the weight %lld apart", name, (long long)rows, (long long)depth, (long long)vocab, (long long)w.ld);
   q->cap = (rows + kRowTile - 1) / kRowTile * kRowTile;
   q->ld_x = (depth + 7) / 8 * 8;
-  q->ld_acc = (depth + 31) / 32 * 32;
   q->inner_w = w.by_word ? depth : vocab; q->outer_w = w.by_word ? vocab : depth;
   q->pad = w.ld % 8 != 0 || off_by(w.at, 16);
   q->ld_w = q->pad ? (q->inner_w + 7) / 8 * 8 : w.ld;
@@ -365,7 +360,7 @@ int make_plan(const char* name, int64_t rows, int64_t depth, const Weight& w, in
     q->off_lse = take((size_t)q->cap * 4); q->off_g = take((size_t)q->cap * 4);
     q->off_scaled = take((size_t)q->cap * q->ld_x * 2);
     q->off_dz = take((size_t)q->cap * q->piece * 2);
-    q->off_acc = take(q->pieces > 1 ? (size_t)q->cap * q->ld_acc * 4 : 0);
+    q->off_acc = take(q->pieces > 1 ? (size_t)q->cap * ((depth + 255) / 256 * 256) * 4 : 0);
   } else {
     q->off_terms = take((size_t)q->parts * q->cap * 8); q->off_sums = take((size_t)q->parts * q->cap * 4); q->off_hit = take((size_t)q->cap * 4);
   }
@@ -417,7 +412,7 @@ int make_ready(const Positions& x, Weight* w, int64_t vocab, const Plan& q, void
   return PB_OK;
 }
 
-int bytes_of(const void* p, int64_t ld) { return !off_by(p, 32) && ld % 16 == 0 ? 32 : !off_by(p, 16) && ld % 8 == 0 ? 16 : 2; }
+bool in_vectors(const void* p, int64_t ld) { return !off_by(p, 16) && ld % 8 == 0; }
 
 const unsigned short* words(const Weight& w, int64_t first) { return static_cast<const unsigned short*>(w.at) + (w.by_word ? first * w.ld : first); }
 
@@ -491,20 +486,22 @@ extern "C" int pb_linear_xent_bwd(const void* x, int64_t outer, int64_t inner, i
   if (int s = make_ready(at, &w, vocab, q, workspace, nullptr, nullptr, lse, g, dx, dweight != nullptr, st)) return s;
   int *origin = part<int>(workspace, q.off_origin), *target = part<int>(workspace, q.off_target);
   __nv_bfloat16 *dz = part<__nv_bfloat16>(workspace, q.off_dz), *d_hidden = static_cast<__nv_bfloat16*>(dx);
-  float* acc = part<float>(workspace, q.off_acc);
+  float4* acc = part<float4>(workspace, q.off_acc);
   const float* gs = part<float>(workspace, q.off_g);
   const float by = smoothing <= 0.5f ? 1.0f - smoothing : 1.0f;      // without a target's share to speak of, any
+  CUtensorMap dz_blocks;
+  if (int s = make_map(&dz_blocks, dz, true, q.piece, q.cap, q.piece, 1, q.cap * q.piece, 32)) return s;
   for (int k = 0; k < q.pieces; ++k) {
     const int64_t first = k * q.piece, n = std::min(q.piece, vocab - first);
     if (int s = logits<GradientEpilogue>(q, w, first, n, depth, workspace,
-                                         {target, part<float>(workspace, q.off_lse), dz, q.piece, (int)first, 1.0f / by, smoothing / (float)vocab / by, (1.0f - smoothing) / by}, st))
+                                         {dz_blocks, target, part<float>(workspace, q.off_lse), (int)first, 1.0f / by, smoothing / (float)vocab / by, (1.0f - smoothing) / by}, st))
       return s;
     if (dx) {
-      const int vectors = bytes_of(dx, depth);
-      if (int s = q.pieces == 1       ? to_hidden<kOnly>(q, w, first, n, depth, workspace, {d_hidden, acc, origin, gs, by, depth, q.ld_acc, vectors}, st)
-                : k == 0              ? to_hidden<kFirst>(q, w, first, n, depth, workspace, {d_hidden, acc, origin, gs, by, depth, q.ld_acc, vectors}, st)
-                : k < q.pieces - 1    ? to_hidden<kMore>(q, w, first, n, depth, workspace, {d_hidden, acc, origin, gs, by, depth, q.ld_acc, vectors}, st)
-                                      : to_hidden<kLast>(q, w, first, n, depth, workspace, {d_hidden, acc, origin, gs, by, depth, q.ld_acc, vectors}, st))
+      const bool vectors = in_vectors(dx, depth);
+      if (int s = q.pieces == 1       ? to_hidden<kOnly>(q, w, first, n, depth, workspace, {d_hidden, acc, origin, gs, by, depth, vectors}, st)
+                : k == 0              ? to_hidden<kFirst>(q, w, first, n, depth, workspace, {d_hidden, acc, origin, gs, by, depth, vectors}, st)
+                : k < q.pieces - 1    ? to_hidden<kMore>(q, w, first, n, depth, workspace, {d_hidden, acc, origin, gs, by, depth, vectors}, st)
+                                      : to_hidden<kLast>(q, w, first, n, depth, workspace, {d_hidden, acc, origin, gs, by, depth, vectors}, st))
         return s;
     }
     if (dweight) {
@@ -514,7 +511,7 @@ extern "C" int pb_linear_xent_bwd(const void* x, int64_t outer, int64_t inner, i
       const Operand hidden{part<void>(workspace, q.off_scaled), true, depth, q.cap, q.ld_x, q.cap * q.ld_x}, gradient{dz, true, n, q.cap, q.piece, q.cap * q.piece};
       const int64_t ld_out = w.by_word ? depth : vocab;
       __nv_bfloat16* out = static_cast<__nv_bfloat16*>(dweight) + (w.by_word ? first * depth : first);
-      const StoreEpilogue<kOnly>::Params e{out, nullptr, nullptr, part<float>(workspace, 64), by, ld_out, 0, bytes_of(out, ld_out)};
+      const StoreEpilogue<kOnly>::Params e{out, nullptr, nullptr, part<float>(workspace, 64), by, ld_out, in_vectors(out, ld_out)};
       if (int s = w.by_word ? launch<2, 256, true, true, StoreEpilogue<kOnly>>(gradient, hidden, p, e, st) : launch<2, 256, true, true, StoreEpilogue<kOnly>>(hidden, gradient, p, e, st)) return s;
     }
   }

@@ -11,6 +11,7 @@
 //
 // Three products a step (products.cuh).  A and B are symmetric: only tiles on and above the diagonal are made, and stored to both places.
 #include <cmath>
+#include <utility>
 
 #include "products.cuh"
 
@@ -19,7 +20,7 @@ namespace {
 using namespace products;
 
 constexpr float kScaleX = 0x1p12f, kScaleA = 0x1p10f;
-constexpr int kParts = 64;            // of a matrix, for its sum of squares
+constexpr int kParts = 256;           // of a matrix, for its sum of squares
 constexpr float kMostX = 4.0f, kMostB = 32.0f;      // of the polynomial on [0, 1] and what it makes of that: half of fp16's range at most
 
 // ---- G -> X -------------------------------------------------------------------------------------------------------
@@ -95,7 +96,9 @@ __global__ void __launch_bounds__(256) normalise_kernel(const __grid_constant__ 
   grid_wait();
   __shared__ float factors[3];
   if (threadIdx.x < 32) {
-    double s = p.sums[(int64_t)blockIdx.y * kParts + threadIdx.x] + p.sums[(int64_t)blockIdx.y * kParts + 32 + threadIdx.x];
+    double s = 0.0;
+#pragma unroll
+    for (int k = 0; k < kParts / 32; ++k) s += p.sums[(int64_t)blockIdx.y * kParts + 32 * k + threadIdx.x];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (threadIdx.x == 0) {
@@ -132,103 +135,144 @@ __global__ void __launch_bounds__(256) normalise_kernel(const __grid_constant__ 
 }
 
 // ---- the epilogues ------------------------------------------------------------------------------------------------
-// 32 columns of a symmetric matrix's row, and where the tile is beside the diagonal the same numbers as a column
-__device__ __forceinline__ void store_both(const Place& at, int c, __half* matrix, int64_t ld, const float (&v)[32]) {
-  const int col = at.col + c;
-  if (at.row >= at.rows) return;
-  store_row32<Fp16>(matrix + (int64_t)at.row * ld + col, v);
-  if (at.beside) {
-    __half* to = matrix + (int64_t)col * ld + at.row;
+struct Ungrouped { static constexpr bool kGrouped = false; static constexpr int kSlots = 2; };
+
+// where a symmetric matrix's blocks go: by its rows, and where the tile is beside the diagonal the same numbers by its columns
+struct Symmetric { CUtensorMap rows, columns; };
+__device__ __forceinline__ void store_both(const Place& at, int c, const Symmetric& to, const float (&v)[kBlock]) {
+  Slots::stage<Fp16>(at, 0, v);
+  if (at.beside_diagonal) Slots::stage_transposed(at, 1, v);
+  Slots::hand_over();
+  if (at.lane == 0 && at.row < at.rows) {
+    Slots::send(at, 0, &to.rows, at.col + c, at.row, at.batch);
+    if (at.beside_diagonal) Slots::send(at, 1, &to.columns, at.row, at.col + c, at.batch);
+    Slots::sent();
+  }
+}
+// until the slots can be written to again
+__device__ __forceinline__ void wait_slots(const Place& at) {
+  if (at.lane == 0) Slots::wait_read();
+  __syncwarp();
+}
+// v = of_v * v + by * the lane's row of what a slot holds
+__device__ __forceinline__ void add_rows(const Place& at, int slot, float of_v, float by, float (&v)[kBlock]) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j, to += ld)
-      if (col + j < at.cols) *to = __float2half_rn(v[j]);
+  for (int k = 0; k < Slots::kPieces; ++k) {
+    const uint4 w = Slots::get(Slots::own(at, slot, k));
+    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float2 x = Fp16::open(words[j]), y = make_float2(v[8 * k + 2 * j], v[8 * k + 2 * j + 1]);
+      if (of_v != 1.0f) y = __fmul2_rn(y, make_float2(of_v, of_v));
+      y = __ffma2_rn(x, make_float2(by, by), y);
+      v[8 * k + 2 * j] = y.x; v[8 * k + 2 * j + 1] = y.y;
+    }
   }
 }
 
-struct GramEpilogue {
-  struct Params { __half* a; int64_t ld, plane; };
+struct GramEpilogue : Ungrouped {
+  struct Params { Symmetric a; };
   const Params& p;
   __device__ __forceinline__ explicit GramEpilogue(const Params& e) : p(e) {}
   __device__ __forceinline__ void begin(const Place&) {}
-  __device__ __forceinline__ void chunk(const Place& at, int c, float (&v)[32]) {
+  __device__ __forceinline__ void block(const Place& at, int c, float (&v)[kBlock]) {
+    wait_slots(at);
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] *= kScaleA / (kScaleX * kScaleX);
-    store_both(at, c, p.a + at.batch * p.plane, p.ld, v);
+    for (int j = 0; j < kBlock; ++j) v[j] *= kScaleA / (kScaleX * kScaleX);
+    store_both(at, c, p.a, v);
   }
   __device__ __forceinline__ void end(const Place&) {}
+  __device__ __forceinline__ void finish(const Place& at) { if (at.lane == 0) Slots::wait_sent(); }
 };
 
-__device__ __forceinline__ void load_row32(const __half* at, uint32_t (&w)[16]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint4 v = *reinterpret_cast<const uint4*>(at + 8 * j);
-    w[4 * j] = v.x; w[4 * j + 1] = v.y; w[4 * j + 2] = v.z; w[4 * j + 3] = v.w;
+// Blocks that are read before they are written: asked for a block ahead, as soon as the slots have been read out.  `pending`: on their way.
+struct Reading : Ungrouped {
+  uint32_t phase = 0;
+  bool pending = false;
+  __device__ __forceinline__ bool arrived(const Place& at) {
+    const bool ok = bar_wait(at.bar, phase, at.polls);
+    phase ^= 1; pending = false;
+    return __all_sync(0xffffffffu, ok);
   }
-}
+  __device__ __forceinline__ void finish(const Place& at) {
+    if (pending) (void)arrived(at);
+    if (at.lane == 0) Slots::wait_sent();
+  }
+};
 
-struct SquareEpilogue {
-  struct Params { const __half* a; __half* b; int64_t ld, plane; float of_a, of_square; };
+struct SquareEpilogue : Reading {
+  struct Params { CUtensorMap a; Symmetric b; float of_a, of_square; };
   const Params& p;
   __device__ __forceinline__ explicit SquareEpilogue(const Params& e) : p(e) {}
-  __device__ __forceinline__ void begin(const Place&) {}
-  __device__ __forceinline__ void chunk(const Place& at, int c, float (&v)[32]) {
-    if (at.row < at.rows) {
-      uint32_t w[16];
-      load_row32(p.a + at.batch * p.plane + (int64_t)at.row * p.ld + at.col + c, w);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float2 a = Fp16::open(w[j]);
-        v[2 * j] = fmaf(v[2 * j], p.of_square, a.x * p.of_a);
-        v[2 * j + 1] = fmaf(v[2 * j + 1], p.of_square, a.y * p.of_a);
-      }
+  __device__ __forceinline__ void ask(const Place& at, int c) {
+    if (c >= at.slice || at.col + c >= at.cols) return;
+    pending = true;
+    if (at.lane == 0) {
+      Slots::wait_read();
+      bar_expect(at.bar, kSlotBytes);
+      Slots::ask(at, 0, &p.a, at.col + c, at.row, at.batch);
     }
-    store_both(at, c, p.b + at.batch * p.plane, p.ld, v);
+  }
+  __device__ __forceinline__ void begin(const Place& at) { ask(at, 0); }
+  __device__ __forceinline__ void block(const Place& at, int c, float (&v)[kBlock]) {
+    if (!arrived(at)) return;
+    add_rows(at, 0, p.of_square, p.of_a, v);
+    __syncwarp();
+    store_both(at, c, p.b, v);
+    ask(at, c + kBlock);
   }
   __device__ __forceinline__ void end(const Place&) {}
 };
 
-// LAST: X leaves as bf16
+// LAST: X leaves as bf16, by TMA or, where its rows do not begin at whole 16 bytes, by the lanes
 template <bool LAST>
-struct UpdateEpilogue {
-  struct Params { const __half *hi, *lo; __half *hi_out, *lo_out; __nv_bfloat16* out; int64_t ld, plane, out_ld, out_plane; bool whole; float of_x; };
+struct UpdateEpilogue : Reading {
+  struct Params { CUtensorMap hi, lo, hi_out, lo_out; __nv_bfloat16* out; int64_t out_ld, out_plane; bool whole; float of_x; };
   const Params& p;
   __device__ __forceinline__ explicit UpdateEpilogue(const Params& e) : p(e) {}
-  __device__ __forceinline__ void begin(const Place&) {}
-  __device__ __forceinline__ void chunk(const Place& at, int c, float (&v)[32]) {
-    const bool there = at.row < at.rows;
-    const int64_t from = at.batch * p.plane + (int64_t)at.row * p.ld + at.col + c;
-    if (there) {
-      uint32_t hi[16], lo[16];
-      load_row32(p.hi + from, hi);
-      load_row32(p.lo + from, lo);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float2 h = Fp16::open(hi[j]), l = Fp16::open(lo[j]);
-        v[2 * j] = fmaf(h.x + l.x, p.of_x, v[2 * j] * (1.0f / kScaleA));
-        v[2 * j + 1] = fmaf(h.y + l.y, p.of_x, v[2 * j + 1] * (1.0f / kScaleA));
-      }
+  __device__ __forceinline__ void ask(const Place& at, int c) {
+    if (c >= at.slice || at.col + c >= at.cols) return;
+    pending = true;
+    if (at.lane == 0) {
+      Slots::wait_read();
+      bar_expect(at.bar, 2 * kSlotBytes);
+      Slots::ask(at, 0, &p.hi, at.col + c, at.row, at.batch);
+      Slots::ask(at, 1, &p.lo, at.col + c, at.row, at.batch);
     }
+  }
+  __device__ __forceinline__ void begin(const Place& at) { ask(at, 0); }
+  __device__ __forceinline__ void block(const Place& at, int c, float (&v)[kBlock]) {
+    constexpr float kDown = LAST ? 1.0f / kScaleX : 1.0f;
+    if (!arrived(at)) return;
+    add_rows(at, 1, kDown / kScaleA, kDown * p.of_x, v);
+    add_rows(at, 0, 1.0f, kDown * p.of_x, v);
+    __syncwarp();
     if constexpr (LAST) {
-#pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] *= 1.0f / kScaleX;
-      const int col = at.col + c;
-      __nv_bfloat16* to = p.out + at.batch * p.out_plane + (int64_t)at.row * p.out_ld + col;
-      if (p.whole && col + 32 <= at.cols) {
-        if (there) store_row32<Bf16>(to, v);
+      Slots::stage<Bf16>(at, 0, v);
+      Slots::hand_over();
+      if (p.whole) {
+        if (at.lane == 0 && at.row < at.rows) { Slots::send(at, 0, &p.hi_out, at.col + c, at.row, at.batch); Slots::sent(); }
       } else {
-        store_block32<Bf16>(at, there ? reinterpret_cast<unsigned short*>(to) : nullptr, at.cols - col, v);
+        Slots::scatter(at.own, at.lane, reinterpret_cast<unsigned short*>(p.out + at.batch * p.out_plane + at.col + c), p.out_ld, at.row < at.rows ? at.row : -1, at.cols - at.col - c, false);
+        Slots::hand_over();
       }
-    } else if (there) {
-      uint32_t hi[16], lo[16];
+    } else {
+      Slots::stage<Fp16>(at, 0, v);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        hi[j] = Fp16::pack(v[2 * j], v[2 * j + 1]);
-        const float2 h = Fp16::open(hi[j]);
-        lo[j] = Fp16::pack(v[2 * j] - h.x, v[2 * j + 1] - h.y);
+      for (int j = 0; j < kBlock; j += 2) {
+        const float2 h = Fp16::open(Fp16::pack(v[j], v[j + 1]));
+        const float2 l = __ffma2_rn(h, make_float2(-1.0f, -1.0f), make_float2(v[j], v[j + 1]));
+        v[j] = l.x; v[j + 1] = l.y;
       }
-      st_global_32bytes(p.hi_out + from, hi); st_global_32bytes(p.hi_out + from + 16, hi + 8);
-      st_global_32bytes(p.lo_out + from, lo); st_global_32bytes(p.lo_out + from + 16, lo + 8);
+      Slots::stage<Fp16>(at, 1, v);
+      Slots::hand_over();
+      if (at.lane == 0 && at.row < at.rows) {
+        Slots::send(at, 0, &p.hi_out, at.col + c, at.row, at.batch);
+        Slots::send(at, 1, &p.lo_out, at.col + c, at.row, at.batch);
+        Slots::sent();
+      }
     }
+    ask(at, c + kBlock);
   }
   __device__ __forceinline__ void end(const Place&) {}
 };
@@ -242,7 +286,7 @@ int make_plan(int64_t batch, int64_t rows, int64_t cols, Plan* q) {
   if (batch <= 0 || rows <= 0 || cols <= 0 || rows > (1 << 24) || cols > (1 << 24) || batch > 65535 || rows * cols > (1ll << 36))
     return fail(PB_ERR_BAD_SHAPE, "pb_orthogonalize: batch=%lld rows=%lld cols=%lld", (long long)batch, (long long)rows, (long long)cols);
   q->d = std::min(rows, cols);
-  q->ld = (cols + 31) / 32 * 32; q->ld_a = (q->d + 31) / 32 * 32;
+  q->ld = (cols + 63) / 64 * 64; q->ld_a = (q->d + 63) / 64 * 64;
   q->plane = rows * q->ld; q->plane_a = q->d * q->ld_a;
   size_t at = 0;
   auto take = [&](size_t bytes) { const size_t was = at; at += (bytes + 255) / 256 * 256; return was; };
@@ -329,23 +373,35 @@ extern "C" int pb_orthogonalize(const void* update, int dtype, int64_t batch, in
   PB_LAUNCH_CHECK("normalise_kernel");
 
   const bool tall = rows > cols;
+  // blocks of 32 rows of X's terms, of A and of B for the epilogues, and their transposes
+  CUtensorMap hi_blocks[2], lo_blocks[2], out_blocks{};
+  for (int i = 0; i < 2; ++i) {
+    if (int s = make_map(&hi_blocks[i], hi[i], false, cols, rows, q.ld, batch, q.plane, 32)) return s;
+    if (int s = make_map(&lo_blocks[i], lo[i], false, cols, rows, q.ld, batch, q.plane, 32)) return s;
+  }
+  const bool whole = !off_by(out, 16) && cols % 8 == 0;
+  if (whole)
+    if (int s = make_map(&out_blocks, out, true, cols, rows, cols, batch, n, 32)) return s;
+  Symmetric gram_blocks, poly_blocks;
+  for (auto [blocks, at] : {std::pair{&gram_blocks, gram}, std::pair{&poly_blocks, poly}}) {
+    if (int s = make_map(&blocks->rows, at, false, q.d, q.d, q.ld_a, batch, q.plane_a, 32)) return s;
+    if (int s = make_map(&blocks->columns, at, false, q.d, q.d, q.ld_a, batch, q.plane_a, kBlock, 32)) return s;
+  }
   Params p{};
   p.batch = (int)batch; p.bf16 = 0;
   for (int k = 0; k < steps; ++k) {
     const int now = k & 1;
-    const bool last = k == steps - 1;
     const float a = coefficients[3 * k], b = coefficients[3 * k + 1], c = coefficients[3 * k + 2];
     const Operand x_rows{hi[now], false, rows, cols, q.ld, q.plane}, x_cols{hi[now], true, cols, rows, q.ld, q.plane};      // X by its rows, and by its columns
     p.rows = p.cols = (int)q.d; p.depth = (int)(tall ? rows : cols); p.upper = 1;
-    const GramEpilogue::Params ge{gram, q.ld_a, q.plane_a};
+    const GramEpilogue::Params ge{gram_blocks};
     if (int s = tall ? run<true, true, GramEpilogue>(x_cols, x_cols, p, ge, st) : run<false, false, GramEpilogue>(x_rows, x_rows, p, ge, st)) return s;
     p.depth = (int)q.d;
     const Operand gram_rows{gram, false, q.d, q.d, q.ld_a, q.plane_a}, poly_rows{poly, false, q.d, q.d, q.ld_a, q.plane_a};
-    if (int s = run<false, false, SquareEpilogue>(gram_rows, gram_rows, p, SquareEpilogue::Params{gram, poly, q.ld_a, q.plane_a, b, c / kScaleA}, st)) return s;
+    if (int s = run<false, false, SquareEpilogue>(gram_rows, gram_rows, p, SquareEpilogue::Params{gram_blocks.rows, poly_blocks, b, c / kScaleA}, st)) return s;
     p.rows = (int)rows; p.cols = (int)cols; p.upper = 0;
-    const bool whole = !off_by(out, 32) && cols % 16 == 0;
-    if (int s = last ? run_update<true>(tall, x_rows, x_cols, poly_rows, p, {hi[now], lo[now], nullptr, nullptr, static_cast<__nv_bfloat16*>(out), q.ld, q.plane, cols, n, whole, a}, st)
-                     : run_update<false>(tall, x_rows, x_cols, poly_rows, p, {hi[now], lo[now], hi[now ^ 1], lo[now ^ 1], nullptr, q.ld, q.plane, cols, n, whole, a}, st))
+    if (int s = k == steps - 1 ? run_update<true>(tall, x_rows, x_cols, poly_rows, p, {hi_blocks[now], lo_blocks[now], out_blocks, out_blocks, static_cast<__nv_bfloat16*>(out), cols, n, whole, a}, st)
+                               : run_update<false>(tall, x_rows, x_cols, poly_rows, p, {hi_blocks[now], lo_blocks[now], hi_blocks[now ^ 1], lo_blocks[now ^ 1], nullptr, 0, 0, true, a}, st))
       return s;
   }
   return PB_OK;

@@ -25,21 +25,23 @@ namespace products {
 namespace {
 
 constexpr int kDepth = 64;                        // k per stage: 128 bytes, a swizzled row
-constexpr int kEpilogueWarps = 8;
-constexpr int kThreads = 128 + 32 * kEpilogueWarps;
 constexpr uint32_t kWaitPolls = 1u << 21;         // a poll parks for up to 2 us: about four seconds at most
 
-template <int CTAS, int N>
+constexpr int kEpilogueWarps = 8;
+constexpr int kThreads = 128 + 32 * kEpilogueWarps;
+constexpr int kBlock = 64;                        // columns that an epilogue takes at a time: 128 bytes
+constexpr int kSlotBytes = 32 * kBlock * 2;       // of an epilogue warp's 32 rows of them
+
+// SLOTS: of shared memory for each epilogue warp
+template <int CTAS, int N, int SLOTS>
 struct Form {
   static constexpr int kRows = 128 * CTAS;        // of a tile
   static constexpr int kBRows = N / CTAS;         // of B that a CTA loads
   static constexpr int kABytes = 128 * kDepth * 2, kBBytes = kBRows * kDepth * 2, kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = 6;
-  static constexpr int kPitch = 34;               // 16-bit elements of a staged row: odd in words, so that columns of it meet no bank twice
-  static constexpr int kStaging = 32 * kPitch * 2;                                       // of an epilogue warp: 32 x 32 elements
-  static constexpr int kSmem = 1024 + kStages * kStageBytes + kEpilogueWarps * kStaging;      // 1024: the tiles start on a swizzle atom
+  static constexpr int kStages = SLOTS == 2 ? 5 : 6;
+  static constexpr int kSmem = 1024 + kStages * kStageBytes + kEpilogueWarps * SLOTS * kSlotBytes;      // 1024: the tiles start on a swizzle atom
   static constexpr int kCols = N / 2;             // of an epilogue thread
-  static_assert(kSmem + 512 <= 232448, "an SM's shared memory");
+  static_assert(kSmem + 512 <= 232448 && kCols % kBlock == 0, "an SM's shared memory, whole blocks");
 };
 
 __device__ unsigned int g_status;                 // 0, or PB_ERR_DEVICE_TIMEOUT once a bounded wait ran out
@@ -149,13 +151,109 @@ __device__ __forceinline__ void wait_acc32(float (&r)[32]) {
                :: "memory");
 }
 
+template <int BLOCK>
+__device__ __forceinline__ void ld_acc(uint32_t taddr, float (&r)[BLOCK]) {
+#pragma unroll
+  for (int j = 0; j < BLOCK; j += 32) ld_acc32(taddr + j, *reinterpret_cast<float(*)[32]>(&r[j]));
+}
+template <int BLOCK>
+__device__ __forceinline__ void wait_acc(float (&r)[BLOCK]) {
+#pragma unroll
+  for (int j = 0; j < BLOCK; j += 32) wait_acc32(*reinterpret_cast<float(*)[32]>(&r[j]));
+}
+
 // What an epilogue is told of a thread's part of a tile: its row, its first column, and where they are on the chip.
 struct Place {
   int batch, row, col;      // of D; the columns are col .. col + Form::kCols
   int rows, cols;           // D's extents
-  bool beside;              // with `upper`: the tile is not on the diagonal
+  int slice;                // of columns, Form::kCols
+  bool beside_diagonal;     // with `upper`: the tile is not on the diagonal
   int lane;
-  uint32_t staging;         // this warp's shared memory, Form::kStaging bytes
+  uint32_t slots, own, bar; // this warp's shared memory, the lane's row there (Slots), and a barrier for what is asked for
+  uint32_t polls;
+  int part;                 // a number for this warp's part of the tile, among all of D
+};
+
+// ---- what epilogues share -------------------------------------------------------------------------------------------
+struct Bf16 {
+  static constexpr bool kBf16 = true;
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
+};
+struct Fp16 {
+  static constexpr bool kBf16 = false;
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    uint32_t p;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(hi), "f"(lo));
+    return p;
+  }
+  static __device__ __forceinline__ float2 open(uint32_t p) { return __half22float2(*reinterpret_cast<const __half2*>(&p)); }
+};
+// A warp's blocks of 32 rows x kBlock 16-bit elements between registers, where a lane has a row, and memory: through slots of 4 KB in shared memory, as TMA's 128-byte swizzle lays
+// them (16-byte pieces of a row exchanged by its number, so that neither side meets a bank twice).  TMA moves them: the same by loads and stores of the lanes, 64
+// bytes of eight rows each, took the last product of a step of four 2048 x 8192 updates 282 us for 200, and a single 2048 x 2048 matrix's 31 for UPDATE_US.
+struct Slots {
+  static constexpr int kBytes = 32 * kBlock * 2, kPieces = kBlock / 8;
+  static __device__ __forceinline__ uint32_t own(const Place& at, int slot, int k) { return (at.own + slot * kBytes) ^ (k << 4); }      // the lane's row's k-th piece
+  static __device__ __forceinline__ void put(uint32_t to, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+  }
+  static __device__ __forceinline__ uint4 get(uint32_t from) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(from) : "memory");
+    return v;
+  }
+  template <class T>
+  static __device__ __forceinline__ void stage(const Place& at, int slot, const float (&v)[kBlock]) {
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k)
+      put(own(at, slot, k), T::pack(v[8 * k], v[8 * k + 1]), T::pack(v[8 * k + 2], v[8 * k + 3]), T::pack(v[8 * k + 4], v[8 * k + 5]), T::pack(v[8 * k + 6], v[8 * k + 7]));
+  }
+  // the block's columns as rows of 32, without a swizzle
+  static __device__ __forceinline__ void stage_transposed(const Place& at, int slot, const float (&v)[kBlock]) {
+#pragma unroll
+    for (int j = 0; j < kBlock; ++j)
+      asm volatile("st.shared.b16 [%0], %1;" ::"r"(at.slots + slot * kBytes + j * 64 + at.lane * 2), "h"(__half_as_ushort(__float2half_rn(v[j]))) : "memory");
+  }
+  // Between a warp's accesses to its slots and TMA's: by all lanes.
+  static __device__ __forceinline__ void hand_over() {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+  }
+  // by one lane
+  static __device__ __forceinline__ void send(const Place& at, int slot, const CUtensorMap* map, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(at.slots + slot * kBytes), "r"(x), "r"(y), "r"(z) : "memory");
+  }
+  static __device__ __forceinline__ void sent() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+  static __device__ __forceinline__ void wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }      // until what was sent has left the slots
+  static __device__ __forceinline__ void wait_sent() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+  static __device__ __forceinline__ void ask(const Place& at, int slot, const CUtensorMap* map, int x, int y, int z) { load_box<1>(at.slots + slot * kBytes, map, x, y, z, at.bar); }
+  // A staged block to rows that TMA does not reach: row `to_row` of each lane's (below 0 none), `ld` elements apart from `first` on; n columns are there; vectors: rows begin at whole 16 bytes.
+  static __device__ __noinline__ void scatter(uint32_t own, int lane, unsigned short* first, int64_t ld, int to_row, int n, bool vectors) {
+    const uint32_t base = own - (lane * (kBlock * 2) + ((lane & 7) << 4));
+    if (vectors && n >= kBlock) {
+      const int piece = lane & 7;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + (lane >> 3), to = __shfl_sync(0xffffffffu, to_row, r);
+        const uint4 v = get(base + r * (kBlock * 2) + ((piece ^ (r & 7)) << 4));
+        if (to >= 0) *reinterpret_cast<uint4*>(first + to * ld + 8 * piece) = v;
+      }
+    } else {
+#pragma unroll 2
+      for (int r = 0; r < 32; ++r) {
+        const int row = __shfl_sync(0xffffffffu, to_row, r);
+        unsigned short* to = first + row * ld;
+#pragma unroll
+        for (int c0 = 0; c0 < kBlock; c0 += 32) {
+          const int c = c0 + lane;
+          unsigned short x;
+          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(base + r * (kBlock * 2) + (((c >> 3) ^ (r & 7)) << 4) + 2 * (c & 7)) : "memory");
+          if (row >= 0 && c < n) to[c] = x;
+        }
+      }
+    }
+    __syncwarp();
+  }
 };
 
 struct Tiles {
@@ -181,15 +279,17 @@ struct Tiles {
   }
 };
 
-// Epilogue: constructed from its Params by every thread of the epilogue warps, then for each tile begin(place), chunk<C>(place, c, v) for each 32 columns from
-// place.col + c on (D's own sums, whatever lies outside of it zeros; not called for columns beyond it), and end(place), by whole warps.
+// Epilogue: constructed from its Params by every thread of the epilogue warps, then for each tile, by whole warps, begin(place) before its sums are there, block(place, c, v) for each kBlock columns
+// from place.col + c on (whatever lies outside of D zeros; not called for columns beyond it), and end(place); at last finish(place), in an abort too.  kSlots: 4 KB a warp each.
+// kGrouped: sums of groups of stages are added up in registers, 128 of a thread, and the warps that load and issue hand over some of theirs.
 template <int CTAS, int N, bool A_MN, bool B_MN, class Epilogue>
 __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(kThreads, 1)
 product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Params p,
                const __grid_constant__ typename Epilogue::Params e) {
-  using F = Form<CTAS, N>;
+  constexpr bool GROUPED = Epilogue::kGrouped;
+  using F = Form<CTAS, N, Epilogue::kSlots>;
   extern __shared__ unsigned char product_smem[];
-  __shared__ __align__(8) uint64_t bars[2 * F::kStages + 4];
+  __shared__ __align__(8) uint64_t bars[2 * F::kStages + 4 + kEpilogueWarps];
   __shared__ uint32_t tmem_slot;
   const uint32_t base = (smem_u32(product_smem) + 1023u) & ~1023u;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -202,7 +302,12 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   if (tid == 0) {
     for (int s = 0; s < F::kStages; ++s) { bar_init(full(s), 1); bar_init(empty(s), 1); }
     for (int a = 0; a < 2; ++a) { bar_init(acc_full(a), 1); bar_init(acc_empty(a), CTAS * kEpilogueWarps); }
+    for (int w = 0; w < kEpilogueWarps; ++w) bar_init(smem_u32(&bars[2 * F::kStages + 4 + w]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (tid == 32 * 2) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
   }
   if (warp == 1) {
     if (CTAS == 2) {
@@ -225,9 +330,9 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   const Tiles tiles(p, rows, F::kRows, N);
   const int items = tiles.per_batch * p.batch, first = blockIdx.x / CTAS, stride = gridDim.x / CTAS;
 
-  // registers: 128 x 56 + 256 x 216 of the 384 x 168 that the block has
+  // registers with GROUPED: 128 x 56 + 256 x 216 of the 384 x 168 that the block has
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (GROUPED) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0) {
       if (lane == 0) {
         uint32_t it = 0;
@@ -287,63 +392,81 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    const int quad = warp & 3, half = (warp - 4) >> 2;      // rows 32 quad .., columns kCols half ..
+    if (GROUPED) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int quad = warp & 3, slice = (warp - 4) >> 2;      // rows 32 quad .., columns kCols slice ..
     Epilogue epilogue(e);
     Place at;
-    at.rows = rows; at.cols = p.cols; at.lane = lane;
-    at.staging = base + F::kStages * F::kStageBytes + (warp - 4) * F::kStaging;
+    at.rows = rows; at.cols = p.cols; at.lane = lane; at.slice = F::kCols;
+    at.slots = base + F::kStages * F::kStageBytes + (warp - 4) * Epilogue::kSlots * kSlotBytes;
+    at.own = at.slots + lane * (kBlock * 2) + ((lane & 7) << 4);
+    at.bar = smem_u32(&bars[2 * F::kStages + 4 + warp - 4]);
+    at.polls = p.polls;
     uint32_t n = 0;
     bool ok = true;
     for (int w = first; w < items && ok; w += stride) {
       int tm, tn;
       tiles.at(w, at.batch, tm, tn);
       at.row = tm * F::kRows + rank * 128 + quad * 32 + lane;
-      at.col = tn * N + half * F::kCols;
-      at.beside = tm != tn;
-      float acc[F::kCols / 32][32];
+      at.col = tn * N + slice * F::kCols;
+      at.beside_diagonal = tm != tn;
+      at.part = (w * CTAS + rank) * kEpilogueWarps + warp - 4;
+      epilogue.begin(at);
+      float acc[GROUPED ? F::kCols / kBlock : 1][kBlock];
+      auto from = [&](uint32_t ab, int c) { return tmem + ((uint32_t)(quad * 32) << 16) + ab * N + slice * F::kCols + c; };
+      auto release = [&](uint32_t ab) {
+        tc_before();
+        __syncwarp();
+        if (lane == 0) arrive_in_cluster(CTAS == 2 ? in_leader(acc_empty(ab)) : acc_empty(ab));
+      };
       for (int k0 = 0; k0 == 0 || k0 < steps; k0 += p.group, ++n) {
         const uint32_t ab = n & 1;
         ok = __all_sync(0xffffffffu, bar_wait(acc_full(ab), (n >> 1) & 1, p.polls));
         if (!ok) break;
         tc_after();
-        const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + ab * N + half * F::kCols;
-        const uint32_t freed = CTAS == 2 ? in_leader(acc_empty(ab)) : acc_empty(ab);
-        if (k0 == 0) {
+        if constexpr (!GROUPED) {
 #pragma unroll
-          for (int c = 0; c < F::kCols / 32; ++c) ld_acc32(from + 32 * c, acc[c]);
-#pragma unroll
-          for (int c = 0; c < F::kCols / 32; ++c) wait_acc32(acc[c]);
+          for (int c = 0; c < F::kCols; c += kBlock) {
+            ld_acc(from(ab, c), acc[0]);
+            wait_acc(acc[0]);
+            if (c + kBlock == F::kCols) release(ab);
+            if (at.col + c < p.cols) epilogue.block(at, c, acc[0]);
+          }
         } else {
+          if (k0 == 0) {
 #pragma unroll
-          for (int c = 0; c < F::kCols / 32; ++c) {
-            float v[32];
-            ld_acc32(from + 32 * c, v);
-            wait_acc32(v);
+            for (int c = 0; c < F::kCols / kBlock; ++c) ld_acc(from(ab, c * kBlock), acc[c]);
 #pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              const float2 s = __fadd2_rn(make_float2(acc[c][j], acc[c][j + 1]), make_float2(v[j], v[j + 1]));
-              acc[c][j] = s.x; acc[c][j + 1] = s.y;
+            for (int c = 0; c < F::kCols / kBlock; ++c) wait_acc(acc[c]);
+          } else {
+#pragma unroll
+            for (int c = 0; c < F::kCols / 32; ++c) {
+              float v[32];
+              ld_acc32(from(ab, 32 * c), v);
+              wait_acc32(v);
+              float* sum = acc[32 * c / kBlock] + 32 * c % kBlock;
+#pragma unroll
+              for (int j = 0; j < 32; j += 2) {
+                const float2 s = __fadd2_rn(make_float2(sum[j], sum[j + 1]), make_float2(v[j], v[j + 1]));
+                sum[j] = s.x; sum[j + 1] = s.y;
+              }
             }
           }
+          release(ab);
         }
-        tc_before();
-        __syncwarp();
-        if (lane == 0) arrive_in_cluster(freed);
       }
       if (!ok) break;
-      if (steps == 0) {             // nothing was added up
+      if constexpr (GROUPED) {
 #pragma unroll
-        for (int c = 0; c < F::kCols / 32; ++c)
+        for (int c = 0; c < F::kCols / kBlock; ++c) {
+          if (steps == 0)             // nothing was added up
 #pragma unroll
-          for (int j = 0; j < 32; ++j) acc[c][j] = 0.0f;
+            for (int j = 0; j < kBlock; ++j) acc[c][j] = 0.0f;
+          if (at.col + c * kBlock < p.cols) epilogue.block(at, c * kBlock, acc[c]);
+        }
       }
-      epilogue.begin(at);
-#pragma unroll
-      for (int c = 0; c < F::kCols / 32; ++c)
-        if (at.col + 32 * c < p.cols) epilogue.chunk(at, 32 * c, acc[c]);
       epilogue.end(at);
     }
+    epilogue.finish(at);
   }
   // Neither CTA leaves, or frees TMEM, while the other can still signal its barriers or issue into its TMEM.
   tc_before();
@@ -356,67 +479,20 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   }
 }
 
-// ---- what epilogues share -------------------------------------------------------------------------------------------
-struct Bf16 {
-  static constexpr bool kBf16 = true;
-  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
-};
-struct Fp16 {
-  static constexpr bool kBf16 = false;
-  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
-    uint32_t p;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(hi), "f"(lo));
-    return p;
-  }
-  static __device__ __forceinline__ float2 open(uint32_t p) { return __half22float2(*reinterpret_cast<const __half2*>(&p)); }
-};
-__device__ __forceinline__ void st_global_32bytes(void* at, const uint32_t* v) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-               ::"l"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
-}
-// 32 elements of a row as two whole 32-byte stores
-template <class T>
-__device__ __forceinline__ void store_row32(void* at, const float (&v)[32]) {
-  uint32_t w[16];
-#pragma unroll
-  for (int j = 0; j < 16; ++j) w[j] = T::pack(v[2 * j], v[2 * j + 1]);
-  st_global_32bytes(at, w);
-  st_global_32bytes(static_cast<char*>(at) + 32, w + 8);
-}
-// A warp's 32 x 32 elements to rows that lie anywhere: through shared memory, so that a warp's store is 64 bytes of one row.  row_of(r): where lane r's row begins at these
-// columns, or null.
-template <class T>
-__device__ __forceinline__ void store_block32(const Place& at, unsigned short* row, int n, const float (&v)[32]) {
-  constexpr int kWords = Form<1, 128>::kPitch / 2;
-#pragma unroll
-  for (int j = 0; j < 16; ++j)
-    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at.staging + 4 * (at.lane * kWords + j)), "r"(T::pack(v[2 * j], v[2 * j + 1])) : "memory");
-  __syncwarp();
-  const unsigned long long mine = reinterpret_cast<unsigned long long>(row);
-#pragma unroll 8
-  for (int r = 0; r < 32; ++r) {
-    unsigned short* to = reinterpret_cast<unsigned short*>(__shfl_sync(0xffffffffu, mine, r));
-    unsigned short x;
-    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(at.staging + 4 * r * kWords + 2 * at.lane));
-    if (to && at.lane < n) to[at.lane] = x;
-  }
-  __syncwarp();
-}
-
 // ---- host side --------------------------------------------------------------------------------------------------------
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// `batch` matrices of [outer, inner] 16-bit elements, rows `ld` apart (a multiple of 8), matrices `plane`; boxes of 64 (inner) x box_outer
-inline int make_map(CUtensorMap* map, const void* base, bool bf16, int64_t inner, int64_t outer, int64_t ld, int64_t batch, int64_t plane, int box_outer) {
+// `batch` matrices of [outer, inner] 16-bit elements, rows `ld` apart (a multiple of 8), matrices `plane`; boxes of 64 (inner) x box_outer, swizzled, or of fewer (inner), as they are
+inline int make_map(CUtensorMap* map, const void* base, bool bf16, int64_t inner, int64_t outer, int64_t ld, int64_t batch, int64_t plane, int box_outer, int box_inner = kDepth) {
   EncodeFn encode = reinterpret_cast<EncodeFn>(tensor_map_encoder());
   if (!encode) return fail(PB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
   const cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)outer, (cuuint64_t)batch};
   const cuuint64_t strides[2] = {(cuuint64_t)(ld * 2), (cuuint64_t)(plane * 2)};
-  const cuuint32_t box[3] = {(cuuint32_t)kDepth, (cuuint32_t)box_outer, 1}, step[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_outer, 1}, step[3] = {1, 1, 1};
   const CUresult r = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box, step,
-                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, box_inner == kDepth ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(PB_ERR_CUDA, "cuTensorMapEncodeTiled (products) failed with CUresult %d", (int)r);
   return PB_OK;
 }
@@ -435,7 +511,7 @@ struct Operand {
 
 template <int CTAS, int N, bool A_MN, bool B_MN, class Epilogue>
 int launch(const Operand& a, const Operand& b, Params p, const typename Epilogue::Params& e, cudaStream_t st) {
-  using F = Form<CTAS, N>;
+  using F = Form<CTAS, N, Epilogue::kSlots>;
   CUtensorMap map_a, map_b;
   auto map = [&](CUtensorMap* m, const Operand& o, int box_rows) {
     return o.mn ? make_map(m, o.at, p.bf16, o.rows, o.depth, o.ld, p.batch, o.plane, kDepth) : make_map(m, o.at, p.bf16, o.depth, o.rows, o.ld, p.batch, o.plane, box_rows);
@@ -447,7 +523,7 @@ int launch(const Operand& a, const Operand& b, Params p, const typename Epilogue
   if (items == 0) return PB_OK;
   // a band's rows of A, some 16 MB, stay in L2 while its columns go by
   p.band = (int)std::max<int64_t>(1, (16 << 20) / (F::kRows * 2 * std::max<int64_t>(1, p.depth)));
-  if (p.group == 0) p.group = kMaxIndexed;
+  if (!Epilogue::kGrouped) p.group = kMaxIndexed;
   p.polls = kWaitPolls; p.withhold = 0;
 #ifdef PB_DIAGNOSTICS
   p.polls = g_polls.load(); p.withhold = g_withhold.load();
