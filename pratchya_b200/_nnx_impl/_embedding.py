@@ -6,7 +6,6 @@ import operator
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from ._logprobs import wants_derivative
@@ -21,10 +20,18 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0,
     scale = float(scale)
     if padding_id is not None:
         padding_id = operator.index(padding_id)
-    table, ids, padding = _checked(table, ids, padding_id)
-    if wants_derivative(table):
-        return _EmbeddingFn.apply(table, ids, scale, padding)
-    return _forward(table, ids, scale, padding)
+    derivative = wants_derivative(table)
+    vocab = table.shape[0] if isinstance(table, torch.Tensor) and table.dim() == 2 else 0
+    if padding_id is None or -vocab <= padding_id < vocab:
+        padding = -1 if padding_id is None else padding_id % vocab
+        out = _lib.native().embedding_lookup(table, ids, scale, padding, derivative)
+        if out is not None:
+            return out
+    table, ids, padding = _checked(table, ids, padding_id)          # what has to be converted first, or refused
+    out = _lib.native().embedding_lookup(table, ids, scale, padding, derivative)
+    if out is None:
+        raise RuntimeError("embedding_lookup takes plain CUDA tensors only")
+    return out
 
 
 def _checked(table, ids, padding_id):
@@ -46,31 +53,3 @@ def _checked(table, ids, padding_id):
     if torch.jit.is_tracing():          # a trace would hold the result as a constant
         raise RuntimeError("embedding_lookup cannot be traced")
     return table.contiguous(), ids.contiguous(), -1 if padding_id is None else padding_id % vocab
-
-
-def _forward(table, ids, scale, padding):
-    out = _lib.native().embedding_lookup(table, ids, scale, padding)
-    if out is None:
-        raise RuntimeError("embedding_lookup takes plain CUDA tensors only")
-    return out
-
-
-class _EmbeddingFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, table, ids, scale, padding):
-        ctx.save_for_backward(ids)
-        ctx.scale, ctx.padding, ctx.shape = scale, padding, table.shape
-        return _forward(table, ids, scale, padding)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        (ids,) = ctx.saved_tensors
-        nat, (vocab, channels) = _lib.native(), ctx.shape
-        g = g.contiguous()
-        d = torch.empty(ctx.shape, dtype=g.dtype, device=g.device)
-        with _lib.on_device(g.device):
-            size = nat.pb_embedding_lookup_bwd_workspace_size(ids.numel(), vocab, channels)
-            workspace = torch.empty(max(size, 256), dtype=torch.uint8, device=g.device)
-            nat.pb_embedding_lookup_bwd(g, _lib.PB_F32 if g.dtype is torch.float32 else _lib.PB_BF16, ids, ids.numel(), vocab, channels, ctx.scale, ctx.padding, d, workspace, size)
-        return d, None, None, None

@@ -42,57 +42,78 @@ struct SelectParams {
   float* loss;                               // forward: of positions without a target 0, beyond the vocabulary NaN; and their lse
   float* lse_none;
 };
-// one CTA: a thread takes a run of positions and counts, the runs' sums meet, and it numbers its own in their order
+// One CTA: 8192 positions at a time, a warp's by ballot, the warps' numbers added up.
 __global__ void __launch_bounds__(1024) select_kernel(const __grid_constant__ SelectParams p) {
   grid_wait();
-  __shared__ int sums[32];
+  constexpr int kRounds = 8;
+  __shared__ int sums[kRounds * 32];
+  __shared__ float tops[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int run = (p.rows + 1023) / 1024, first = min(p.rows, (int)threadIdx.x * run), last = min(p.rows, first + run);
-  int mine = 0;
+  int before = 0;
   float most = 0.0f;
-  for (int i = first; i < last; ++i) {
-    const bool there = p.targets[i] >= 0 && p.targets[i] < p.vocab;
-    mine += there;
-    if (p.g && there) most = fmaxf(most, fabsf(p.g[i]));
-  }
-  if (p.g) {
-    __shared__ float tops[32];
+  for (int first = 0; first < p.rows; first += kRounds * 1024) {
+    int64_t t[kRounds];
+    float l[kRounds], g[kRounds];
+    uint32_t there[kRounds];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    if (lane == 0) tops[warp] = most;
+    for (int r = 0; r < kRounds; ++r) {
+      const int i = first + r * 1024 + threadIdx.x;
+      t[r] = i < p.rows ? p.targets[i] : -1;
+      l[r] = p.lse && i < p.rows ? p.lse[i] : 0.0f;
+      g[r] = p.lse && i < p.rows ? p.g[i] : 0.0f;
+    }
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      const bool is = t[r] >= 0 && t[r] < p.vocab;
+      there[r] = __ballot_sync(0xffffffffu, is);
+      if (is) most = fmaxf(most, fabsf(g[r]));
+      if (lane == 0) sums[r * 32 + warp] = __popc(there[r]);
+    }
     __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int w = 1; w < 32; ++w) most = fmaxf(most, tops[w]);
-      *p.g_most = most;
-    }
-  }
-  int upto = mine;
+    if (warp == 0) {
+      int upto = 0;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int below = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += below;
-  }
-  if (lane == 31) sums[warp] = upto;
-  __syncthreads();
-  int before = 0, all = 0;
-  for (int w = 0; w < 32; ++w) {
-    if (w < warp) before += sums[w];
-    all += sums[w];
-  }
-  int at = before + upto - mine;
-  if (threadIdx.x == 0) *p.count = all;
-  for (int i = first; i < last; ++i) {
-    const int64_t t = p.targets[i];
-    const bool there = t >= 0 && t < p.vocab;
-    p.place[i] = there ? at : -1;
-    if (there) {
-      p.origin[at] = i; p.target[at] = (int)t;
-      if (p.lse) { p.lse_out[at] = p.lse[i]; p.g_out[at] = p.g[i]; }
-      ++at;
-    } else if (p.loss) {
-      p.loss[i] = t < 0 ? 0.0f : nanf("");
-      p.lse_none[i] = 0.0f;
+      for (int r = 0; r < kRounds; ++r) {
+        int n = sums[r * 32 + lane], all = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int below = __shfl_up_sync(0xffffffffu, all, o);
+          if (lane >= o) all += below;
+        }
+        sums[r * 32 + lane] = upto + all - n;
+        upto += __shfl_sync(0xffffffffu, all, 31);
+      }
+      if (lane == 0) tops[0] = __int_as_float(upto);
     }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      const int i = first + r * 1024 + threadIdx.x;
+      if (i >= p.rows) break;
+      if (there[r] >> lane & 1) {
+        const int at = before + sums[r * 32 + warp] + __popc(there[r] & ((1u << lane) - 1));
+        p.place[i] = at; p.origin[at] = i; p.target[at] = (int)t[r];
+        if (p.lse) { p.lse_out[at] = l[r]; p.g_out[at] = g[r]; }
+      } else {
+        p.place[i] = -1;
+        if (p.loss) {
+          p.loss[i] = t[r] < 0 ? 0.0f : nanf("");
+          p.lse_none[i] = 0.0f;
+        }
+      }
+    }
+    before += __float_as_int(tops[0]);
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *p.count = before;
+  if (!p.lse) return;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  if (lane == 0) tops[warp] = most;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 32; ++w) most = fmaxf(most, tops[w]);
+    *p.g_most = most;
   }
 }
 
@@ -106,49 +127,62 @@ struct GatherParams {
   const float *g, *g_most;
   int rows, depth, ld;
   bool vectors, dx_vectors;
+  uint32_t items;
+  FastDiv per_row;
 };
-// a warp a row, and kRowTile more for the zeros behind the last
-__global__ void __launch_bounds__(256) gather_kernel(const __grid_constant__ GatherParams p) {
+// A warp takes kGather elements of a row; kRowTile rows more are zeros behind the last.
+constexpr int kGather = 1024;
+__global__ void __launch_bounds__(128) gather_kernel(const __grid_constant__ GatherParams p) {
   grid_wait();
-  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const uint32_t item = blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (item >= p.items) return;
+  const int row = (int)p.per_row.div(item), lane = threadIdx.x & 31;
+  const int c0 = (int)(item - row * p.per_row.d) * kGather, c1 = min(c0 + kGather, p.ld), behind = *p.count + row - p.rows;
+  const int to = row < p.rows ? p.place[row] : behind < (*p.count + kRowTile - 1) / kRowTile * kRowTile ? behind : -1;
+  unsigned short *out = p.out + (int64_t)to * p.ld, *scaled = p.scaled ? p.scaled + (int64_t)to * p.ld : nullptr;
   if (row >= p.rows) {
-    const int count = *p.count, to = count + row - p.rows;
-    if (to >= (count + kRowTile - 1) / kRowTile * kRowTile) return;
-    for (int c = lane * 8; c < p.ld; c += 256) {
-      *reinterpret_cast<uint4*>(p.out + (int64_t)to * p.ld + c) = make_uint4(0u, 0u, 0u, 0u);
-      if (p.scaled) *reinterpret_cast<uint4*>(p.scaled + (int64_t)to * p.ld + c) = make_uint4(0u, 0u, 0u, 0u);
+    if (to < 0) return;
+    for (int c = c0 + lane * 8; c < c1; c += 256) {
+      *reinterpret_cast<uint4*>(out + c) = make_uint4(0u, 0u, 0u, 0u);
+      if (scaled) *reinterpret_cast<uint4*>(scaled + c) = make_uint4(0u, 0u, 0u, 0u);
     }
     return;
   }
-  const int to = p.place[row];
-  if (to >= 0) {
-    const unsigned short* from = p.x + row / p.inner * p.stride_outer + row % p.inner * p.stride_inner;
-    unsigned short* out = p.out + (int64_t)to * p.ld;
-    unsigned short* scaled = p.scaled ? p.scaled + (int64_t)to * p.ld : nullptr;
-    float by = 1.0f;
-    if (scaled) {
-      const float most = *p.g_most, g = p.g[to];
-      by = most == 0.0f ? g : __fdiv_rn(g, most);          // every g is zero, or none is a number
+  if (to < 0) {
+    if (!p.dx) return;
+    unsigned short* none = p.dx + (int64_t)row * p.depth;
+    if (p.dx_vectors) for (int c = c0 + lane * 8; c < min(c1, p.depth); c += 256) *reinterpret_cast<uint4*>(none + c) = make_uint4(0u, 0u, 0u, 0u);
+    else for (int c = c0 + lane; c < min(c1, p.depth); c += 32) none[c] = 0;
+    return;
+  }
+  const unsigned short* from = p.x + row / p.inner * p.stride_outer + row % p.inner * p.stride_inner;
+  float by = 1.0f;
+  if (scaled) {
+    const float most = *p.g_most, g = p.g[to];
+    by = most == 0.0f ? g : __fdiv_rn(g, most);          // every g is zero, or none is a number
+  }
+  auto times = [&](uint32_t x) { return pack_bf16x2(__uint_as_float(x << 16) * by, __uint_as_float(x & 0xffff0000u) * by); };
+  if (p.vectors) {
+    uint4 v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int c = c0 + lane * 8 + 256 * k;
+      v[k] = c < p.depth ? *reinterpret_cast<const uint4*>(from + c) : make_uint4(0u, 0u, 0u, 0u);
     }
-    auto times = [&](uint32_t x) { return pack_bf16x2(__uint_as_float(x << 16) * by, __uint_as_float(x & 0xffff0000u) * by); };
-    if (p.vectors) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int c = c0 + lane * 8 + 256 * k;
+      if (c >= c1) break;
+      *reinterpret_cast<uint4*>(out + c) = v[k];
+      if (scaled) *reinterpret_cast<uint4*>(scaled + c) = make_uint4(times(v[k].x), times(v[k].y), times(v[k].z), times(v[k].w));
+    }
+  } else {
 #pragma unroll 4
-      for (int c = lane * 8; c < p.depth; c += 256) {
-        const uint4 v = *reinterpret_cast<const uint4*>(from + c);
-        *reinterpret_cast<uint4*>(out + c) = v;
-        if (scaled) *reinterpret_cast<uint4*>(scaled + c) = make_uint4(times(v.x), times(v.y), times(v.z), times(v.w));
-      }
-    } else {
-      for (int c = lane; c < p.ld; c += 32) {
-        const unsigned short v = c < p.depth ? from[c] : (unsigned short)0;
-        out[c] = v;
-        if (scaled) scaled[c] = (unsigned short)times(v);
-      }
+    for (int c = c0 + lane; c < c1; c += 32) {
+      const unsigned short v = c < p.depth ? from[c] : (unsigned short)0;
+      out[c] = v;
+      if (scaled) scaled[c] = (unsigned short)times(v);
     }
-  } else if (p.dx) {
-    unsigned short* out = p.dx + (int64_t)row * p.depth;
-    if (p.dx_vectors) for (int c = lane * 8; c < p.depth; c += 256) *reinterpret_cast<uint4*>(out + c) = make_uint4(0u, 0u, 0u, 0u);
-    else for (int c = lane; c < p.depth; c += 32) out[c] = 0;
   }
 }
 
@@ -248,40 +282,34 @@ struct GradientEpilogue : Grouped {
   __device__ __forceinline__ void finish(const Place& at) { if (at.lane == 0) Slots::wait_sent(); }
 };
 
-enum { kOnly, kFirst, kMore, kLast };      // of the products that are added up: a single one to bf16; into acc, onto acc, with acc to bf16
-template <int MODE>
+// D times `by` and scale[row], or scale[0] without origin, as bf16 in rows of `ld`; with origin row r goes to row origin[r].  By TMA where that reaches the rows (`blocks`), else by the lanes.
 struct StoreEpilogue : Grouped {
-  // what leaves as bf16 is multiplied by `by` and by scale[row], or scale[0] without origin; acc: a warp's parts of the tiles, 16 bytes a lane in a row
-  struct Params { __nv_bfloat16* out; float4* acc; const int* origin; const float* scale; float by; int64_t ld; bool vectors; };
+  struct Params { CUtensorMap blocks; __nv_bfloat16* out; const int* origin; const float* scale; float by; int64_t ld; bool vectors; };
   const Params& p;
   int row;
   float scale;
   __device__ __forceinline__ explicit StoreEpilogue(const Params& e) : p(e) {}
   __device__ __forceinline__ void begin(const Place& at) {
     row = at.row < at.rows ? (p.origin ? p.origin[at.row] : at.row) : -1;
-    scale = row < 0 || MODE == kFirst || MODE == kMore ? 0.0f : p.by * p.scale[p.origin ? at.row : 0];
+    scale = row < 0 ? 0.0f : p.by * p.scale[p.origin ? at.row : 0];
   }
   __device__ __forceinline__ void block(const Place& at, int c, float (&v)[kBlock]) {
-    if constexpr (MODE != kOnly) {
-      float4* a = p.acc + ((int64_t)at.part * (kPart / 4) + c / 4) * 32 + at.lane;
 #pragma unroll
-      for (int j = 0; j < kBlock / 4; ++j) {
-        float4 f = MODE == kFirst ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : a[32 * j];
-        f.x += v[4 * j]; f.y += v[4 * j + 1]; f.z += v[4 * j + 2]; f.w += v[4 * j + 3];
-        if (MODE == kLast) { v[4 * j] = f.x; v[4 * j + 1] = f.y; v[4 * j + 2] = f.z; v[4 * j + 3] = f.w; }
-        else a[32 * j] = f;
-      }
-    }
-    if constexpr (MODE == kOnly || MODE == kLast) {
-#pragma unroll
-      for (int j = 0; j < kBlock; ++j) v[j] *= scale;
-      Slots::stage<Bf16>(at, 0, v);
+    for (int j = 0; j < kBlock; ++j) v[j] *= scale;
+    if (!p.origin && p.vectors) {
+      if (at.lane == 0) Slots::wait_read();
       __syncwarp();
-      Slots::scatter(at.own, at.lane, reinterpret_cast<unsigned short*>(p.out + at.col + c), p.ld, row, at.cols - at.col - c, p.vectors);
+      Slots::stage<Bf16>(at, 0, v);
+      Slots::hand_over();
+      if (at.lane == 0 && at.row < at.rows) { Slots::send(at, 0, &p.blocks, at.col + c, at.row, 0); Slots::sent(); }
+      return;
     }
+    Slots::stage<Bf16>(at, 0, v);
+    __syncwarp();
+    Slots::scatter(at.own, at.lane, reinterpret_cast<unsigned short*>(p.out + at.col + c), p.ld, row, at.cols - at.col - c, p.vectors);
   }
   __device__ __forceinline__ void end(const Place&) {}
-  __device__ __forceinline__ void finish(const Place&) {}
+  __device__ __forceinline__ void finish(const Place& at) { if (at.lane == 0) Slots::wait_sent(); }
 };
 
 // ---- the parts of a position's logits together ----------------------------------------------------------------------
@@ -294,7 +322,7 @@ __global__ void __launch_bounds__(1024) join_kernel(const float2* terms, const f
   const int n = *count, row = blockIdx.x * 32 + (threadIdx.x & 31), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (blockIdx.x * 32 >= n) return;
   float m = -INFINITY, s = 0.0f, sum = 0.0f;
-#pragma unroll 4
+#pragma unroll 8
   for (int k = warp; k < parts; k += 32) {      // rows up to cap are there, if not told of
     const float2 t = terms[(int64_t)k * cap + row];
     if (MEAN) sum += sums[(int64_t)k * cap + row];
@@ -333,15 +361,29 @@ struct Weight {
 
 struct Plan {
   int64_t cap, ld_x, piece, ld_w, inner_w, outer_w, parts;
+  int64_t rows;
   int pieces;
   bool pad;
-  size_t off_place, off_origin, off_target, off_lse, off_g, off_x, off_scaled, off_w, off_terms, off_sums, off_hit, off_dz, off_acc, bytes;
+  size_t off_place, off_origin, off_target, off_lse, off_g, off_x, off_scaled, off_w, off_terms, off_sums, off_hit, off_dz, off_parts, bytes;
 };
+template <typename T> T* part(void* workspace, size_t off) { return reinterpret_cast<T*>(static_cast<unsigned char*>(workspace) + off); }
+// Where there is one tile of rows, half of a pair's 256 would be idle: a CTA's 128 x 256.  64 positions of 2048 against 65536 words: FEW_US
+bool few_rows(const Plan& q) { return q.rows <= 128; }
+
+// dx's product of a piece: few tiles of many stages, so they are cut
+Params hidden_params(const Plan& q, int64_t n, int64_t depth, void* ws) {
+  Params p{};
+  p.count = part<int>(ws, 0); p.counted = 1; p.rows = (int)(few_rows(q) ? 128 : q.cap); p.cols = (int)depth; p.depth = (int)n; p.batch = 1; p.bf16 = 1; p.group = kGroup;
+  if (few_rows(q)) cut_stages<1, 256>(&p, (int)(q.piece / kDepth));
+  else cut_stages<2, 256>(&p, (int)(q.piece / kDepth));
+  return p;
+}
 int make_plan(const char* name, int64_t rows, int64_t depth, const Weight& w, int64_t vocab, bool backward, Plan* q) {
   if (rows < 0 || rows > (1 << 24) || depth <= 0 || depth > (1 << 20) || vocab <= 0 || vocab > (1 << 28) || w.ld < (w.by_word ? depth : vocab))
     return fail(PB_ERR_BAD_SHAPE, "%s: rows=%lld depth=%lld vocab=%lld, rows of the weight %lld apart", name, (long long)rows, (long long)depth, (long long)vocab, (long long)w.ld);
+  q->rows = rows;
   q->cap = (rows + kRowTile - 1) / kRowTile * kRowTile;
-  q->ld_x = (depth + 7) / 8 * 8;
+  q->ld_x = (depth + 63) / 64 * 64;      // rows of whole 128-byte lines
   q->inner_w = w.by_word ? depth : vocab; q->outer_w = w.by_word ? vocab : depth;
   q->pad = w.ld % 8 != 0 || off_by(w.at, 16);
   q->ld_w = q->pad ? (q->inner_w + 7) / 8 * 8 : w.ld;
@@ -355,12 +397,13 @@ int make_plan(const char* name, int64_t rows, int64_t depth, const Weight& w, in
   q->off_place = take((size_t)rows * 4); q->off_origin = take((size_t)q->cap * 4); q->off_target = take((size_t)q->cap * 4);
   q->off_x = take((size_t)q->cap * q->ld_x * 2);
   q->off_w = take(q->pad ? (size_t)q->outer_w * q->ld_w * 2 : 0);
-  q->off_lse = q->off_g = q->off_scaled = q->off_dz = q->off_acc = q->off_terms = q->off_sums = q->off_hit = 0;
+  q->off_lse = q->off_g = q->off_scaled = q->off_dz = q->off_parts = q->off_terms = q->off_sums = q->off_hit = 0;
   if (backward) {
     q->off_lse = take((size_t)q->cap * 4); q->off_g = take((size_t)q->cap * 4);
     q->off_scaled = take((size_t)q->cap * q->ld_x * 2);
     q->off_dz = take((size_t)q->cap * q->piece * 2);
-    q->off_acc = take(q->pieces > 1 ? (size_t)q->cap * ((depth + 255) / 256 * 256) * 4 : 0);
+    const Params p = hidden_params(*q, q->piece, depth, nullptr);
+    q->off_parts = take((size_t)(few_rows(*q) ? parts_of<1, 256>(p) : parts_of<2, 256>(p)) * 16);
   } else {
     q->off_terms = take((size_t)q->parts * q->cap * 8); q->off_sums = take((size_t)q->parts * q->cap * 4); q->off_hit = take((size_t)q->cap * 4);
   }
@@ -385,7 +428,6 @@ int checks(const char* name, const Positions& x, const Weight& w, int64_t vocab,
   return PB_OK;
 }
 
-template <typename T> T* part(void* workspace, size_t off) { return reinterpret_cast<T*>(static_cast<unsigned char*>(workspace) + off); }
 
 // numbers the positions, brings their hidden states together and the weight where TMA reads it
 int make_ready(const Positions& x, Weight* w, int64_t vocab, const Plan& q, void* ws, float* loss, float* lse_none, const float* lse, const float* g, void* dx, bool scaled, cudaStream_t st) {
@@ -395,9 +437,11 @@ int make_ready(const Positions& x, Weight* w, int64_t vocab, const Plan& q, void
   launch_behind(select_kernel, 1, 1024, 0, st, sp);
   PB_LAUNCH_CHECK("select_kernel");
   const bool vectors = x.depth % 8 == 0 && !off_by(x.x, 16) && (x.outer == 1 || x.stride_outer % 8 == 0) && (x.inner == 1 || x.stride_inner % 8 == 0);
+  const int64_t per_row = (q.ld_x + kGather - 1) / kGather;
+  if ((rows + kRowTile) * per_row > kMaxIndexed) return fail(PB_ERR_BAD_SHAPE, "pb_linear_xent: %d positions of %lld", rows, (long long)x.depth);
   const GatherParams gp{static_cast<const unsigned short*>(x.x), x.inner, x.stride_outer, x.stride_inner, part<int>(ws, 0), part<int>(ws, q.off_place), part<unsigned short>(ws, q.off_x),
-                        scaled ? part<unsigned short>(ws, q.off_scaled) : nullptr, static_cast<unsigned short*>(dx), part<float>(ws, q.off_g), part<float>(ws, 64), rows, (int)x.depth, (int)q.ld_x, vectors, x.depth % 8 == 0 && !off_by(dx, 16)};
-  launch_behind(gather_kernel, (unsigned)((rows + kRowTile + 7) / 8), 256, 0, st, gp);
+                        scaled ? part<unsigned short>(ws, q.off_scaled) : nullptr, static_cast<unsigned short*>(dx), part<float>(ws, q.off_g), part<float>(ws, 64), rows, (int)x.depth, (int)q.ld_x, vectors, x.depth % 8 == 0 && !off_by(dx, 16), (uint32_t)((rows + kRowTile) * per_row), FastDiv((uint32_t)per_row)};
+  launch_behind(gather_kernel, (gp.items + 3) / 4, 128, 0, st, gp);
   PB_LAUNCH_CHECK("gather_kernel");
   if (q.pad) {
     const unsigned x_blocks = (unsigned)std::min<int64_t>(8, (q.inner_w + 255) / 256), y = (unsigned)std::min<int64_t>(65535, q.outer_w), z = (unsigned)((q.outer_w + 65534) / 65535);
@@ -419,16 +463,18 @@ const unsigned short* words(const Weight& w, int64_t first) { return static_cast
 template <class E>
 int logits(const Plan& q, const Weight& w, int64_t first, int64_t n, int64_t depth, void* ws, const typename E::Params& e, cudaStream_t st) {
   Params p{};
-  p.count = part<int>(ws, 0); p.counted = 1; p.rows = (int)q.cap; p.cols = (int)n; p.depth = (int)depth; p.batch = 1; p.bf16 = 1; p.group = kGroup;
+  p.count = part<int>(ws, 0); p.counted = 1; p.rows = (int)(few_rows(q) ? 128 : q.cap); p.cols = (int)n; p.depth = (int)depth; p.batch = 1; p.bf16 = 1; p.group = kGroup;
   const Operand x{part<void>(ws, q.off_x), false, q.cap, depth, q.ld_x, q.cap * q.ld_x}, words_of{words(w, first), !w.by_word, n, depth, w.ld, w.ld * 8};
+  if (few_rows(q)) return w.by_word ? launch<1, 256, false, false, E>(x, words_of, p, e, st) : launch<1, 256, false, true, E>(x, words_of, p, e, st);
   return w.by_word ? launch<2, 256, false, false, E>(x, words_of, p, e, st) : launch<2, 256, false, true, E>(x, words_of, p, e, st);
 }
-template <int MODE>
-int to_hidden(const Plan& q, const Weight& w, int64_t first, int64_t n, int64_t depth, void* ws, const typename StoreEpilogue<MODE>::Params& e, cudaStream_t st) {
-  Params p{};
-  p.count = part<int>(ws, 0); p.counted = 1; p.rows = (int)q.cap; p.cols = (int)depth; p.depth = (int)n; p.batch = 1; p.bf16 = 1; p.group = kGroup;
+int to_hidden(const Plan& q, const Weight& w, int64_t first, int64_t n, int64_t depth, void* ws, cudaStream_t st) {
+  const Params p = hidden_params(q, n, depth, ws);
   const Operand dz{part<void>(ws, q.off_dz), false, q.cap, n, q.piece, q.cap * q.piece}, words_of{words(w, first), w.by_word, depth, n, w.ld, w.ld * 8};
-  return w.by_word ? launch<2, 256, false, true, StoreEpilogue<MODE>>(dz, words_of, p, e, st) : launch<2, 256, false, false, StoreEpilogue<MODE>>(dz, words_of, p, e, st);
+  using E = PartEpilogue<true>;
+  const E::Params e{part<float4>(ws, q.off_parts), first > 0};
+  if (few_rows(q)) return w.by_word ? launch<1, 256, false, true, E>(dz, words_of, p, e, st) : launch<1, 256, false, false, E>(dz, words_of, p, e, st);
+  return w.by_word ? launch<2, 256, false, true, E>(dz, words_of, p, e, st) : launch<2, 256, false, false, E>(dz, words_of, p, e, st);
 }
 
 }  // namespace
@@ -486,7 +532,6 @@ extern "C" int pb_linear_xent_bwd(const void* x, int64_t outer, int64_t inner, i
   if (int s = make_ready(at, &w, vocab, q, workspace, nullptr, nullptr, lse, g, dx, dweight != nullptr, st)) return s;
   int *origin = part<int>(workspace, q.off_origin), *target = part<int>(workspace, q.off_target);
   __nv_bfloat16 *dz = part<__nv_bfloat16>(workspace, q.off_dz), *d_hidden = static_cast<__nv_bfloat16*>(dx);
-  float4* acc = part<float4>(workspace, q.off_acc);
   const float* gs = part<float>(workspace, q.off_g);
   const float by = smoothing <= 0.5f ? 1.0f - smoothing : 1.0f;      // without a target's share to speak of, any
   CUtensorMap dz_blocks;
@@ -496,14 +541,8 @@ extern "C" int pb_linear_xent_bwd(const void* x, int64_t outer, int64_t inner, i
     if (int s = logits<GradientEpilogue>(q, w, first, n, depth, workspace,
                                          {dz_blocks, target, part<float>(workspace, q.off_lse), (int)first, 1.0f / by, smoothing / (float)vocab / by, (1.0f - smoothing) / by}, st))
       return s;
-    if (dx) {
-      const bool vectors = in_vectors(dx, depth);
-      if (int s = q.pieces == 1       ? to_hidden<kOnly>(q, w, first, n, depth, workspace, {d_hidden, acc, origin, gs, by, depth, vectors}, st)
-                : k == 0              ? to_hidden<kFirst>(q, w, first, n, depth, workspace, {d_hidden, acc, origin, gs, by, depth, vectors}, st)
-                : k < q.pieces - 1    ? to_hidden<kMore>(q, w, first, n, depth, workspace, {d_hidden, acc, origin, gs, by, depth, vectors}, st)
-                                      : to_hidden<kLast>(q, w, first, n, depth, workspace, {d_hidden, acc, origin, gs, by, depth, vectors}, st))
-        return s;
-    }
+    if (dx)
+      if (int s = to_hidden(q, w, first, n, depth, workspace, st)) return s;
     if (dweight) {
       Params p{};
       p.count = part<int>(workspace, 0); p.counted = 2; p.depth = (int)q.cap; p.batch = 1; p.bf16 = 1; p.group = kGroup;
@@ -511,9 +550,17 @@ extern "C" int pb_linear_xent_bwd(const void* x, int64_t outer, int64_t inner, i
       const Operand hidden{part<void>(workspace, q.off_scaled), true, depth, q.cap, q.ld_x, q.cap * q.ld_x}, gradient{dz, true, n, q.cap, q.piece, q.cap * q.piece};
       const int64_t ld_out = w.by_word ? depth : vocab;
       __nv_bfloat16* out = static_cast<__nv_bfloat16*>(dweight) + (w.by_word ? first * depth : first);
-      const StoreEpilogue<kOnly>::Params e{out, nullptr, nullptr, part<float>(workspace, 64), by, ld_out, in_vectors(out, ld_out)};
-      if (int s = w.by_word ? launch<2, 256, true, true, StoreEpilogue<kOnly>>(gradient, hidden, p, e, st) : launch<2, 256, true, true, StoreEpilogue<kOnly>>(hidden, gradient, p, e, st)) return s;
+      StoreEpilogue::Params e{{}, out, nullptr, part<float>(workspace, 64), by, ld_out, in_vectors(out, ld_out)};
+      if (e.vectors)
+        if (int s = make_map(&e.blocks, out, true, p.cols, p.rows, ld_out, 1, (int64_t)p.rows * ld_out, 32)) return s;
+      if (int s = w.by_word ? launch<2, 256, true, true, StoreEpilogue>(gradient, hidden, p, e, st) : launch<2, 256, true, true, StoreEpilogue>(hidden, gradient, p, e, st)) return s;
     }
+  }
+  if (dx) {
+    const StoreEpilogue::Params e{{}, d_hidden, origin, gs, by, depth, in_vectors(dx, depth)};
+    const Params p = hidden_params(q, q.piece, depth, workspace);
+    const float4* parts = part<float4>(workspace, q.off_parts);
+    if (int s = few_rows(q) ? launch_finish<1, 256, StoreEpilogue>(parts, p, e, st) : launch_finish<2, 256, StoreEpilogue>(parts, p, e, st)) return s;
   }
   return PB_OK;
 }

@@ -875,10 +875,62 @@ OP(int4_product) {
 }
 
 // ---- the token embedding ----
-// embedding_lookup(table [vocab, channels], ids, scale, padding or -1) -> [..., channels]: embedding_lookup without its derivative
+int rows_of(const at::Tensor& table, const at::Tensor& ids, double scale, int64_t padding, at::Tensor* out) {
+  c10::SmallVector<int64_t, 8> shape(ids.sizes().begin(), ids.sizes().end());
+  shape.push_back(table.size(1));
+  *out = fresh(shape, table.scalar_type());
+  return without_gil([&] {
+    return pb_embedding_lookup(table.data_ptr(), code(table.scalar_type()), table.size(0), table.size(1), ids.numel() ? ids.data_ptr<int64_t>() : nullptr, ids.numel(), (float)scale, padding,
+                               out->data_ptr(), current_stream(table.device()));
+  });
+}
+
+// The lookup with its derivative, once.
+struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
+  using List = torch::autograd::variable_list;
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& table, const at::Tensor& ids, double scale, int64_t padding) {
+    const c10::cuda::CUDAGuard guard(table.device());
+    at::Tensor out;
+    const int status = rows_of(table, ids, scale, padding, &out);
+    TORCH_CHECK(status == PB_OK, "pratchya_b200 status ", status, ": ", pb_last_error());
+    ctx->save_for_backward({ids});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding"] = padding;
+    ctx->saved_data["vocab"] = table.size(0);
+    ctx->saved_data["channels"] = table.size(1);
+    ctx->saved_data["type"] = table.scalar_type();
+    return out;
+  }
+  static List backward(torch::autograd::AutogradContext* ctx, List g) {
+    const at::Tensor ids = ctx->get_saved_variables()[0];
+    const int64_t vocab = ctx->saved_data["vocab"].toInt(), channels = ctx->saved_data["channels"].toInt();
+    const at::ScalarType type = ctx->saved_data["type"].toScalarType();
+    const bool again = g[0].requires_grad() && at::GradMode::is_enabled();      // a derivative of this one is asked for
+    at::Tensor d;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      const at::Tensor gg = g[0].to(type).contiguous();
+      const c10::cuda::CUDAGuard guard(gg.device());
+      d = fresh({vocab, channels}, type);
+      const size_t bytes = pb_embedding_lookup_bwd_workspace_size(ids.numel(), vocab, channels);
+      at::Tensor ws = fresh({(int64_t)bytes}, at::kByte);
+      const int status = pb_embedding_lookup_bwd(gg.numel() ? gg.data_ptr() : nullptr, code(type), gg.numel() ? ids.data_ptr<int64_t>() : nullptr, ids.numel(), vocab, channels,
+                                                 (float)ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt(), d.data_ptr(), ws.data_ptr(), bytes, current_stream(gg.device()));
+      TORCH_CHECK(status == PB_OK, "pratchya_b200 status ", status, ": ", pb_last_error());
+    }
+    if (again) {
+      d.requires_grad_(true);      // an input of a node that fails when its own derivative is asked for
+      auto refuse = std::make_shared<torch::autograd::DelayedError>("embedding_lookup has no second derivative", 1);
+      d = (*refuse)({std::move(d)})[0];
+    }
+    return {d, at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+// embedding_lookup(table [vocab, channels], ids, scale, padding or -1, derivative) -> [..., channels]; with derivative it is differentiable in the table
 OP(embedding_lookup) {
   HANDLE_TH_ERRORS
-  NARGS(4);
+  NARGS(5);
   const at::Tensor *table = plain(args[0]), *ids = plain(args[1]);
   const double scale = PyFloat_AsDouble(args[2]);
   if (scale == -1.0 && PyErr_Occurred()) return nullptr;
@@ -887,11 +939,9 @@ OP(embedding_lookup) {
   if (!table || !ids || watched() || traced() || !dense(table->scalar_type()) || table->dim() != 2 || table->numel() == 0 || ids->scalar_type() != at::kLong || ids->device() != table->device())
     return none();
   const c10::cuda::CUDAGuard guard(table->device());
-  c10::SmallVector<int64_t, 8> shape(ids->sizes().begin(), ids->sizes().end());
-  shape.push_back(table->size(1));
-  at::Tensor out = fresh(shape, table->scalar_type());
-  RUN(pb_embedding_lookup(table->data_ptr(), code(table->scalar_type()), table->size(0), table->size(1), ids->numel() ? ids->data_ptr<int64_t>() : nullptr, ids->numel(), (float)scale, padding,
-                          out.data_ptr(), current_stream(table->device())));
+  if (PyObject_IsTrue(args[4]) == 1) return wrap(EmbeddingFunction::apply(*table, *ids, scale, (int64_t)padding));
+  at::Tensor out;
+  if (const int status = rows_of(*table, *ids, scale, padding, &out)) return raise_status(status);
   return wrap(out);
   END_HANDLE_TH_ERRORS
 }
@@ -949,7 +999,7 @@ PyMethodDef methods[] = {
     ENTRY(pb_rms_norm), ENTRY(pb_rms_norm_bwd), ENTRY(pb_rms_norm_bwd_workspace_size), ENTRY(pb_relu2), ENTRY(pb_relu2_bwd),
     ENTRY(pb_wkv_finish), ENTRY(pb_wkv_finish_workspace_size), ENTRY(pb_wkv_finish_bwd), ENTRY(pb_wkv_finish_bwd_workspace_size),
     ENTRY(pb_smoothed_xent), ENTRY(pb_smoothed_xent_bwd),
-    METHOD("embedding_lookup", embedding_lookup), ENTRY(pb_embedding_lookup_bwd), ENTRY(pb_embedding_lookup_bwd_workspace_size),
+    METHOD("embedding_lookup", embedding_lookup),
     ENTRY(pb_linear_xent), ENTRY(pb_linear_xent_bwd), ENTRY(pb_linear_xent_workspace_size), METHOD("strides_of_rows", strides_of_rows),
     ENTRY(pb_orthogonalize), ENTRY(pb_orthogonalize_workspace_size),
     {"set_error", set_error, METH_O, nullptr},

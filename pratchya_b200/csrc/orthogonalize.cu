@@ -77,6 +77,18 @@ __global__ void __launch_bounds__(256) square_sums_kernel(const T* g, int64_t n,
   }
 }
 
+// 2^12 / (|G| + eps), of |G|^2 = s, as two powers of two and a rest in [1, 2): each within f32 where the whole may not be.  NaN for an infinity or a NaN anywhere.
+__device__ __forceinline__ void scale_factors(double s, double eps, float* factors) {
+  const double by = (double)kScaleX / (sqrt(s) + eps);
+  int e = 0;
+  const double rest = 2.0 * frexp(by, &e);
+  const bool fine = isfinite(by) && isfinite(s);
+  e -= 1;
+  factors[0] = fine ? (float)rest : nanf("");
+  factors[1] = fine ? ldexpf(1.0f, e / 2) : 1.0f;
+  factors[2] = fine ? ldexpf(1.0f, e - e / 2) : 1.0f;
+}
+
 __device__ __forceinline__ void two_terms(float x, __half& hi, __half& lo) {
   hi = __float2half_rn(x);
   lo = __float2half_rn(x - __half2float(hi));
@@ -102,15 +114,7 @@ __global__ void __launch_bounds__(256) normalise_kernel(const __grid_constant__ 
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (threadIdx.x == 0) {
-      // 2^12 / (|G| + eps) as two powers of two and a rest in [1, 2): each within f32 where the whole may not be
-      const double by = (double)kScaleX / (sqrt(s) + p.eps);
-      int e = 0;
-      const double rest = 2.0 * frexp(by, &e);
-      const bool fine = isfinite(by) && isfinite(s);
-      e -= 1;
-      factors[0] = fine ? (float)rest : nanf("");      // an infinity or a NaN anywhere: nothing else
-      factors[1] = ldexpf(1.0f, e / 2);
-      factors[2] = ldexpf(1.0f, e - e / 2);
+      scale_factors(s, p.eps, factors);
     }
   }
   __syncthreads();
@@ -277,14 +281,315 @@ struct UpdateEpilogue : Reading {
   __device__ __forceinline__ void end(const Place&) {}
 };
 
+// ---- matrices of up to 128 columns (or rows) ----------------------------------------------------------------------
+// All steps in one launch, X never in memory: a cluster of CTAs shares the other direction, 256 of it each; a thread has one of these, 128 numbers of X in f32, and their fp16
+// roundings lie in shared memory as an operand, the same tile as X (rows by k) and as X^T (k by rows).  A step: the cluster's CTAs make their parts of
+// A = X^T X and send each other the rows that they add up (S CTAs 128 / S each); these go to all as fp16; every CTA makes A A, B and its own rows of X B.  The low-rank layers' weights,
+// 2048 x 128: one 127 us by three products a step, NARROW_US so; 120 of them NARROW_ALL.
+// What it is bound by: a step's chain, some CHAIN cycles of barriers of the cluster, tensor core round trips and fp16 rows through shared memory.
+constexpr int kNarrow = 128, kSlab = 256, kMostClusters = 16;
+constexpr int kNarrowSmem = 1024 + kSlab * kNarrow * 2 + 2 * kNarrow * kNarrow * 2 + kNarrow * kNarrow * 4;      // X, A and B, sums from the others
+
+struct NarrowParams {
+  const void* g;
+  __nv_bfloat16* out;
+  int64_t length;           // of the long direction
+  int width, size, steps;   // of the short one; CTAs of a cluster
+  bool tall;                // the long direction is rows
+  bool vectors, out_vectors;
+  double eps;
+  float coefficients[64 * 3];
+  uint32_t polls;
+};
+__device__ __forceinline__ void cluster_barrier() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void async_fence() { asm volatile("fence.proxy.async;" ::: "memory"); }
+__device__ __forceinline__ uint64_t narrow_desc(uint32_t addr, uint32_t next) {      // 128-byte swizzle; K-major (next: unused), or M/N-major with the next 64 rows `next` bytes on
+  return (uint64_t)((addr & 0x3ffffu) >> 4) | ((uint64_t)(next >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// the 16-byte piece of row r at columns 8 k .. of a matrix of `rows` rows by 128 columns: two panels of 64 columns
+__device__ __forceinline__ uint32_t piece_at(uint32_t base, int rows, int r, int k) { return base + (k >> 3) * (rows * 128) + r * 128 + (((k & 7) ^ (r & 7)) << 4); }
+
+template <typename T>
+__global__ void __launch_bounds__(kSlab, 1) narrow_kernel(const __grid_constant__ NarrowParams p) {
+  extern __shared__ unsigned char narrow_smem[];
+  __shared__ __align__(8) uint64_t bar;
+  __shared__ uint32_t tmem_slot;
+  __shared__ double squares[8], of_cluster[kMostClusters];
+  __shared__ float factors[3];
+  const uint32_t base = (smem_u32(narrow_smem) + 1023u) & ~1023u, x_at = base, a_at = x_at + kSlab * kNarrow * 2, b_at = a_at + kNarrow * kNarrow * 2, sums_at = b_at + kNarrow * kNarrow * 2;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, quad = warp & 3, half = warp >> 2;
+  const int rank = (int)(blockIdx.x % p.size), share = kNarrow / p.size;      // rows of A that this CTA adds up
+  if (tid == 0) {
+    bar_init(smem_u32(&bar), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_before();
+  __syncthreads();
+  cluster_barrier();          // the others run, and can be written to
+  tc_after();
+  const uint32_t tmem = *(volatile uint32_t*)&tmem_slot, lanes = tmem + ((uint32_t)(quad * 32) << 16);
+  grid_wait();
+
+  // this thread's numbers
+  const int64_t matrix = (int64_t)(blockIdx.x / p.size) * p.length * p.width, at = (int64_t)rank * kSlab + tid;
+  const T* g = static_cast<const T*>(p.g) + matrix;
+  float x[kNarrow];
+  if (p.tall && p.vectors) {
+    constexpr int kN = Vec<T>::kN;
+#pragma unroll
+    for (int j = 0; j < kNarrow; j += kN) {
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (at < p.length && j < p.width) v = __ldg(reinterpret_cast<const uint4*>(g + at * p.width + j));
+      Vec<T>::open(v, x + j);
+    }
+  } else {
+    const T* from = p.tall ? g + at * p.width : g + at;
+    const int64_t step = p.tall ? 1 : p.length;
+#pragma unroll
+    for (int j = 0; j < kNarrow; ++j) x[j] = at < p.length && j < p.width ? Elem<T>::to_f32(from[j * step]) : 0.0f;
+  }
+  double s = 0.0;
+#pragma unroll
+  for (int j = 0; j < kNarrow; ++j) s = fma((double)x[j], (double)x[j], s);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane == 0) squares[warp] = s;
+  __syncthreads();
+  if (tid < p.size) {
+    for (int w = 1; w < 8; ++w) s = w == 1 ? squares[0] + squares[1] : s + squares[w];
+    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(in_cta(smem_u32(&of_cluster[rank]), tid)), "d"(s) : "memory");
+  }
+  cluster_barrier();
+  if (tid == 0) {
+    s = 0.0;
+    for (int r = 0; r < p.size; ++r) s += of_cluster[r];
+    scale_factors(s, p.eps, factors);
+  }
+  __syncthreads();
+  const float f1 = factors[1], f2 = factors[2], f0 = factors[0];
+#pragma unroll
+  for (int j = 0; j < kNarrow; ++j) x[j] = x[j] * f1 * f2 * f0;
+
+  constexpr uint32_t kSquare = (1u << 4) | ((uint32_t)(kNarrow >> 3) << 17) | ((uint32_t)(128 >> 4) << 24), kTransposed = kSquare | (3u << 15);
+  uint32_t phase = 0;
+  auto products_done = [&] {
+    (void)bar_wait(smem_u32(&bar), phase, p.polls);      // where it runs out, the status says so and the barriers below are still met
+    phase ^= 1;
+    tc_after();
+  };
+  for (int step = 0; step < p.steps; ++step) {
+    const float a = p.coefficients[3 * step], b = p.coefficients[3 * step + 1], c = p.coefficients[3 * step + 2];
+    // X's first terms as an operand
+#pragma unroll
+    for (int k = 0; k < kNarrow / 8; ++k) {
+      const float* v = x + 8 * k;
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(piece_at(x_at, kSlab, tid, k)), "r"(Fp16::pack(v[0], v[1])), "r"(Fp16::pack(v[2], v[3])), "r"(Fp16::pack(v[4], v[5])),
+                   "r"(Fp16::pack(v[6], v[7])) : "memory");
+    }
+    async_fence();
+    tc_before();
+    __syncthreads();
+    if (tid == 0) {          // A = X^T X of this CTA's 256
+      tc_after();
+#pragma unroll 4
+      for (int k = 0; k < kSlab / 16; ++k) {
+        const uint64_t d = narrow_desc(x_at + k * 2048, kSlab * 128);
+        mma<1>(tmem, d, d, kTransposed, k > 0);
+      }
+      commit_to<1>(smem_u32(&bar));
+    }
+    products_done();
+    {                        // row quad * 32 + lane of it, 64 columns, to whom adds that row up; 16-byte pieces of a row exchanged by its number
+      const int row = quad * 32 + lane;
+      const uint32_t to = in_cta(sums_at + ((uint32_t)(rank * share + row % share) * kNarrow) * 4, row / share);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v[32];
+        ld_acc32(lanes + half * 64 + h * 32, v);
+        wait_acc32(v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + (((half * 16 + h * 8 + k) ^ lane) << 4)), "f"(v[4 * k]), "f"(v[4 * k + 1]), "f"(v[4 * k + 2]), "f"(v[4 * k + 3]) : "memory");
+      }
+      tc_before();
+    }
+    cluster_barrier();
+    for (int i = tid; i < share * (kNarrow / 4); i += kSlab) {      // four columns of a row, in the CTAs' order, to all of them
+      const int row = i / (kNarrow / 4), piece = i % (kNarrow / 4), whole = rank * share + row;
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int r = 0; r < p.size; ++r) {
+        float4 w;
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(w.x), "=f"(w.y), "=f"(w.z), "=f"(w.w)
+                     : "r"(sums_at + (uint32_t)(r * share + row) * kNarrow * 4 + ((piece ^ (whole & 31)) << 4)) : "memory");
+        v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+      }
+      constexpr float kDown = kScaleA / (kScaleX * kScaleX);
+      const uint32_t lo = Fp16::pack(v.x * kDown, v.y * kDown), hi = Fp16::pack(v.z * kDown, v.w * kDown), to = piece_at(a_at, kNarrow, whole, piece >> 1) + (piece & 1) * 8;
+      for (int r = 0; r < p.size; ++r) asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(in_cta(to, r)), "r"(lo), "r"(hi) : "memory");
+    }
+    async_fence();
+    cluster_barrier();
+    async_fence();
+    if (tid == 0) {          // A A
+      tc_after();
+#pragma unroll
+      for (int k = 0; k < kNarrow / 16; ++k) {
+        const uint64_t d = narrow_desc(a_at + (k >> 2) * (kNarrow * 128) + (k & 3) * 32, 16);
+        mma<1>(tmem + kNarrow, d, d, kSquare, k > 0);
+      }
+      commit_to<1>(smem_u32(&bar));
+    }
+    products_done();
+    {                        // B = b A + c A A
+      const int row = quad * 32 + lane;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v[32];
+        ld_acc32(lanes + kNarrow + half * 64 + h * 32, v);
+        wait_acc32(v);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int piece = half * 8 + h * 4 + k;
+          const uint4 w = Slots::get(piece_at(a_at, kNarrow, row, piece));
+          const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+          uint32_t to[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = Fp16::open(words[j]);
+            to[j] = Fp16::pack(fmaf(v[8 * k + 2 * j], c / kScaleA, f.x * b), fmaf(v[8 * k + 2 * j + 1], c / kScaleA, f.y * b));
+          }
+          Slots::put(piece_at(b_at, kNarrow, row, piece), to[0], to[1], to[2], to[3]);
+        }
+      }
+    }
+    async_fence();
+    tc_before();
+    __syncthreads();
+    if (tid == 0) {          // X B, 128 of X at a time
+      tc_after();
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int k = 0; k < kNarrow / 16; ++k)
+          mma<1>(tmem + (2 + t) * kNarrow, narrow_desc(x_at + (k >> 2) * (kSlab * 128) + t * (128 * 128) + (k & 3) * 32, 16), narrow_desc(b_at + (k >> 2) * (kNarrow * 128) + (k & 3) * 32, 16), kSquare, k > 0);
+      commit_to<1>(smem_u32(&bar));
+    }
+    products_done();
+#pragma unroll
+    for (int h = 0; h < kNarrow / 32; ++h) {
+      float v[32];
+      ld_acc32(lanes + (2 + half) * kNarrow + h * 32, v);
+      wait_acc32(v);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) x[32 * h + j] = fmaf(x[32 * h + j], a, v[j] * (1.0f / kScaleA));
+    }
+  }
+  if (at < p.length) {
+    __nv_bfloat16* out = p.out + matrix;
+    if (p.tall && p.out_vectors) {
+#pragma unroll
+      for (int j = 0; j < kNarrow; j += 8) {
+        const float* v = x + j;
+        constexpr float kDown = 1.0f / kScaleX;
+        if (j < p.width)
+          *reinterpret_cast<uint4*>(out + at * p.width + j) = make_uint4(pack_bf16x2(v[0] * kDown, v[1] * kDown), pack_bf16x2(v[2] * kDown, v[3] * kDown), pack_bf16x2(v[4] * kDown, v[5] * kDown), pack_bf16x2(v[6] * kDown, v[7] * kDown));
+      }
+    } else {
+      __nv_bfloat16* to = p.tall ? out + at * p.width : out + at;
+      const int64_t by = p.tall ? 1 : p.length;
+#pragma unroll
+      for (int j = 0; j < kNarrow; ++j)
+        if (j < p.width) to[j * by] = __float2bfloat16_rn(x[j] * (1.0f / kScaleX));
+    }
+  }
+  tc_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+// A cluster's CTAs for a matrix; 0: too long, or too wide
+int narrow_size(int64_t rows, int64_t cols) {
+  const int64_t length = std::max(rows, cols), width = std::min(rows, cols);
+  if (width > kNarrow || length > kMostClusters * kSlab) return 0;
+  int size = 1;
+  while (size * kSlab < length) size *= 2;
+  return size;
+}
+
+int run_narrow(const void* update, int dtype, int64_t batch, int64_t rows, int64_t cols, int steps, const float* coefficients, double eps, void* out, cudaStream_t st) {
+  NarrowParams p{};
+  p.g = update; p.out = static_cast<__nv_bfloat16*>(out);
+  p.tall = rows >= cols; p.length = std::max(rows, cols); p.width = (int)std::min(rows, cols); p.size = narrow_size(rows, cols); p.steps = steps; p.eps = eps;
+  p.vectors = !off_by(update, 16) && p.width * (dtype == PB_F32 ? 4 : 2) % 16 == 0;
+  p.out_vectors = !off_by(out, 16) && p.width % 8 == 0;
+  std::copy(coefficients, coefficients + 3 * steps, p.coefficients);
+  p.polls = kWaitPolls;
+#ifdef PB_DIAGNOSTICS
+  p.polls = g_polls.load();
+#endif
+  auto kernel = dtype == PB_F32 ? narrow_kernel<float> : narrow_kernel<__nv_bfloat16>;
+  PB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kNarrowSmem));      // per device
+  if (p.size > 8) PB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3((unsigned)(batch * p.size)); config.blockDim = dim3(kSlab); config.dynamicSmemBytes = kNarrowSmem; config.stream = st;
+  cudaLaunchAttribute how[2];
+  how[0].id = cudaLaunchAttributeClusterDimension;
+  how[0].val.clusterDim.x = (unsigned)p.size; how[0].val.clusterDim.y = how[0].val.clusterDim.z = 1;
+  how[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  how[1].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = how; config.numAttrs = 2;
+  cudaLaunchKernelEx(&config, kernel, p);
+  PB_LAUNCH_CHECK("narrow_kernel");
+  return PB_OK;
+}
+
 // ---- host side ----------------------------------------------------------------------------------------------------
+// Forms of a product's tiles: 256 x 256 and 256 x 128 of a CTA pair, 128 x 128 of a CTA.  A tile's stage of 64 of k is bound by its loads from L2, some 58 bytes a clock into an SM: 563, 413 and 540 cycles, and
+// a tile takes 9000, 6000 and 5000 more until its sums have left.  So the wide pair's is the best wherever its tiles fill the chip, and the others where it
+// would leave half of it idle: A of 2048 x 2048, 36 tiles | 72, FORM_US.
+enum Tile { kPair256, kPair128, kSingle };
+double cost_of(Tile tile, const Params& p) {
+  const int64_t stages = (p.depth + kDepth - 1) / kDepth;
+  auto rounds = [](int64_t tiles, int64_t clusters) { return (tiles + clusters - 1) / clusters; };
+  return tile == kPair256 ? rounds(tiles_of<2, 256>(p), clusters_of<2>()) * (563.0 * stages + 9000) : tile == kPair128 ? rounds(tiles_of<2, 128>(p), clusters_of<2>()) * (413.0 * stages + 6000)
+                          : rounds(tiles_of<1, 128>(p), clusters_of<1>()) * (540.0 * stages + 5000);
+}
+Tile tile_of(const Params& p) {
+  Tile best = kPair256;
+  for (Tile t : {kPair128, kSingle})
+    if (cost_of(t, p) < cost_of(best, p)) best = t;
+  return best;
+}
+template <bool A_MN, bool B_MN, class E>
+int run(const Operand& a, const Operand& b, const Params& p, const typename E::Params& e, cudaStream_t st) {
+  const Tile tile = tile_of(p);
+  return tile == kPair256 ? launch<2, 256, A_MN, B_MN, E>(a, b, p, e, st) : tile == kPair128 ? launch<2, 128, A_MN, B_MN, E>(a, b, p, e, st) : launch<1, 128, A_MN, B_MN, E>(a, b, p, e, st);
+}
+
 struct Plan {
   int64_t d, ld, ld_a, plane, plane_a;
-  size_t off_hi[2], off_lo[2], off_a, off_b, bytes;
+  Params gram;              // A's product; cut where its tiles are few and long
+  size_t off_hi[2], off_lo[2], off_a, off_b, off_parts, bytes;
 };
 int make_plan(int64_t batch, int64_t rows, int64_t cols, Plan* q) {
   if (batch <= 0 || rows <= 0 || cols <= 0 || rows > (1 << 24) || cols > (1 << 24) || batch > 65535 || rows * cols > (1ll << 36))
     return fail(PB_ERR_BAD_SHAPE, "pb_orthogonalize: batch=%lld rows=%lld cols=%lld", (long long)batch, (long long)rows, (long long)cols);
+  if (narrow_size(rows, cols)) {
+    q->bytes = 256;         // never written to
+    return PB_OK;
+  }
   q->d = std::min(rows, cols);
   q->ld = (cols + 63) / 64 * 64; q->ld_a = (q->d + 63) / 64 * 64;
   q->plane = rows * q->ld; q->plane_a = q->d * q->ld_a;
@@ -294,18 +599,17 @@ int make_plan(int64_t batch, int64_t rows, int64_t cols, Plan* q) {
   for (int i = 0; i < 2; ++i) { q->off_hi[i] = take((size_t)batch * q->plane * 2); q->off_lo[i] = take((size_t)batch * q->plane * 2); }
   q->off_a = take((size_t)batch * q->plane_a * 2);
   q->off_b = take((size_t)batch * q->plane_a * 2);
+  q->gram = Params{};
+  Params& p = q->gram;
+  p.batch = (int)batch; p.rows = p.cols = (int)q->d; p.depth = (int)std::max(rows, cols); p.upper = 1;
+  Params cut = p;
+  cut_stages<2, 256>(&cut, (p.depth + kDepth - 1) / kDepth);
+  const int64_t clusters = clusters_of<2>(), tiles = tiles_of<2, 256>(p);
+  const double cut_cost = 563.0 * ((tiles * cut.cuts + clusters - 1) / clusters * (cut.cut + kPartCost) + tiles * cut.cuts / kJoinParts) + 8000;      // and another launch
+  if (cut.cuts > 1 && cut_cost < cost_of(tile_of(p), p)) p = cut;
+  q->off_parts = take(p.cuts ? (size_t)parts_of<2, 256>(p) * 16 : 0);
   q->bytes = at;
   return PB_OK;
-}
-
-// 256 x 256 tiles of a CTA pair, or 128 x 128 ones of a CTA where pairs would leave most SMs without any
-bool small_tiles(int64_t rows, int64_t cols, int64_t batch, bool upper) {
-  const int64_t tm = (rows + 255) / 256, tn = (cols + 255) / 256;
-  return batch * (upper ? tn * (tn + 1) / 2 : tm * tn) * 4 <= sm_count() / 2;
-}
-template <bool A_MN, bool B_MN, class E>
-int run(const Operand& a, const Operand& b, const Params& p, const typename E::Params& e, cudaStream_t st) {
-  return small_tiles(p.rows, p.cols, p.batch, p.upper) ? launch<1, 128, A_MN, B_MN, E>(a, b, p, e, st) : launch<2, 256, A_MN, B_MN, E>(a, b, p, e, st);
 }
 
 template <bool LAST>
@@ -349,6 +653,7 @@ extern "C" int pb_orthogonalize(const void* update, int dtype, int64_t batch, in
     most = next;
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (narrow_size(rows, cols)) return run_narrow(update, dtype, batch, rows, cols, steps, coefficients, eps, out, st);
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   double* sums = reinterpret_cast<double*>(ws);
   __half* hi[2] = {reinterpret_cast<__half*>(ws + q.off_hi[0]), reinterpret_cast<__half*>(ws + q.off_hi[1])};
@@ -393,10 +698,16 @@ extern "C" int pb_orthogonalize(const void* update, int dtype, int64_t batch, in
     const int now = k & 1;
     const float a = coefficients[3 * k], b = coefficients[3 * k + 1], c = coefficients[3 * k + 2];
     const Operand x_rows{hi[now], false, rows, cols, q.ld, q.plane}, x_cols{hi[now], true, cols, rows, q.ld, q.plane};      // X by its rows, and by its columns
-    p.rows = p.cols = (int)q.d; p.depth = (int)(tall ? rows : cols); p.upper = 1;
     const GramEpilogue::Params ge{gram_blocks};
-    if (int s = tall ? run<true, true, GramEpilogue>(x_cols, x_cols, p, ge, st) : run<false, false, GramEpilogue>(x_rows, x_rows, p, ge, st)) return s;
-    p.depth = (int)q.d;
+    if (q.gram.cuts) {
+      float4* parts = reinterpret_cast<float4*>(ws + q.off_parts);
+      const PartEpilogue<false>::Params pe{parts, false};
+      if (int s = tall ? launch<2, 256, true, true, PartEpilogue<false>>(x_cols, x_cols, q.gram, pe, st) : launch<2, 256, false, false, PartEpilogue<false>>(x_rows, x_rows, q.gram, pe, st)) return s;
+      if (int s = launch_finish<2, 256, GramEpilogue>(parts, q.gram, ge, st)) return s;
+    } else if (int s = tall ? run<true, true, GramEpilogue>(x_cols, x_cols, q.gram, ge, st) : run<false, false, GramEpilogue>(x_rows, x_rows, q.gram, ge, st)) {
+      return s;
+    }
+    p.rows = p.cols = p.depth = (int)q.d; p.upper = 1;
     const Operand gram_rows{gram, false, q.d, q.d, q.ld_a, q.plane_a}, poly_rows{poly, false, q.d, q.d, q.ld_a, q.plane_a};
     if (int s = run<false, false, SquareEpilogue>(gram_rows, gram_rows, p, SquareEpilogue::Params{gram_blocks.rows, poly_blocks, b, c / kScaleA}, st)) return s;
     p.rows = (int)rows; p.cols = (int)cols; p.upper = 0;

@@ -38,7 +38,7 @@ struct Form {
   static constexpr int kRows = 128 * CTAS;        // of a tile
   static constexpr int kBRows = N / CTAS;         // of B that a CTA loads
   static constexpr int kABytes = 128 * kDepth * 2, kBBytes = kBRows * kDepth * 2, kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = SLOTS == 2 ? 5 : 6;
+  static constexpr int kStages = kStageBytes > 32768 ? 4 : SLOTS == 2 ? 5 : 6;
   static constexpr int kSmem = 1024 + kStages * kStageBytes + kEpilogueWarps * SLOTS * kSlotBytes;      // 1024: the tiles start on a swizzle atom
   static constexpr int kCols = N / 2;             // of an epilogue thread
   static_assert(kSmem + 512 <= 232448 && kCols % kBlock == 0, "an SM's shared memory, whole blocks");
@@ -55,6 +55,7 @@ struct Params {
   int band;                 // tile rows that are walked down before the next column
   int bf16;                 // else fp16
   int group;                // stages of k that an accumulator takes
+  int cuts, cut;            // 0: whole tiles; else the parts that a tile's stages are cut into, and their length
   uint32_t polls;
   int withhold;             // diagnostics build: the first stage is never filled
 };
@@ -151,6 +152,20 @@ __device__ __forceinline__ void wait_acc32(float (&r)[32]) {
                :: "memory");
 }
 
+__device__ __forceinline__ void ld_acc16(uint32_t taddr, float (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+        "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+      : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void wait_acc16(float (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]),
+                 "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15])
+               :: "memory");
+}
 template <int BLOCK>
 __device__ __forceinline__ void ld_acc(uint32_t taddr, float (&r)[BLOCK]) {
 #pragma unroll
@@ -160,6 +175,13 @@ template <int BLOCK>
 __device__ __forceinline__ void wait_acc(float (&r)[BLOCK]) {
 #pragma unroll
   for (int j = 0; j < BLOCK; j += 32) wait_acc32(*reinterpret_cast<float(*)[32]>(&r[j]));
+}
+
+// by an instruction that no compiler makes without the condition (a volatile load in a conditional expression was made, of a null pointer)
+__device__ __forceinline__ int counted_on_device(const Params& p) {
+  int n = 0;
+  if (p.counted) asm volatile("ld.global.b32 %0, [%1];" : "=r"(n) : "l"(p.count) : "memory");
+  return n;
 }
 
 // What an epilogue is told of a thread's part of a tile: its row, its first column, and where they are on the chip.
@@ -256,26 +278,48 @@ struct Slots {
   }
 };
 
+// Tiles of D, band by band.  upper: those with anything on or above the diagonal, column after column; a tile is `ratio` times as high as wide.
 struct Tiles {
-  int tiles_m, tiles_n, per_batch, band, upper;
-  __device__ __forceinline__ Tiles(const Params& p, int rows, int tile_rows, int tile_cols) {
+  int tiles_m, tiles_n, per_batch, band, upper, ratio;
+  __host__ __device__ __forceinline__ Tiles(const Params& p, int rows, int tile_rows, int tile_cols) {
     tiles_m = (rows + tile_rows - 1) / tile_rows; tiles_n = (p.cols + tile_cols - 1) / tile_cols;
-    per_batch = p.upper ? tiles_n * (tiles_n + 1) / 2 : tiles_m * tiles_n;
-    band = p.band; upper = p.upper;
+    band = p.band; upper = p.upper; ratio = tile_rows > tile_cols ? tile_rows / tile_cols : 1;
+    const int high = tiles_n / ratio;
+    per_batch = upper ? ratio * high * (high + 1) / 2 + tiles_n % ratio * (high + 1) : tiles_m * tiles_n;
   }
   __device__ __forceinline__ void at(int t, int& batch, int& tm, int& tn) const {
     batch = t / per_batch;
     t -= batch * per_batch;
-    if (upper) {            // column after column down to the diagonal
-      tn = (int)((sqrtf(8.0f * (float)t + 1.0f) - 1.0f) * 0.5f);
-      while (tn * (tn + 1) / 2 > t) --tn;
-      while ((tn + 1) * (tn + 2) / 2 <= t) ++tn;
-      tm = t - tn * (tn + 1) / 2;
+    if (upper) {            // `ratio` columns of one tile, as many of two, ...
+      int high = (int)((sqrtf(8.0f * (float)(t / ratio) + 1.0f) - 1.0f) * 0.5f);
+      while (ratio * high * (high + 1) / 2 > t) --high;
+      while (ratio * (high + 1) * (high + 2) / 2 <= t) ++high;
+      t -= ratio * high * (high + 1) / 2;
+      tn = high * ratio + t / (high + 1);
+      tm = t % (high + 1);
       return;
     }
     const int whole = band * tiles_n, b = t / whole, within = t - b * whole, rows = min(band, tiles_m - b * band);
     tn = within / rows;
     tm = b * band + (within - tn * rows);
+  }
+};
+
+// What a cluster works on: tiles in turn, or with p.cuts parts of `cut` stages of them: all tiles' first parts, then all tiles' second ones, ..., so that what is under way
+// at a time reads the same of k.  (Runs of stages of one length for all clusters balance best, but then nothing is read twice from L2: 16384 of k, 8192 x
+// 2048 sums 500 us for CUTS_US.)
+struct Work {
+  int at, items, stride, steps, tiles, cut, part;
+  __device__ __forceinline__ Work(const Params& p, int tiles_, int steps_, int cluster, int clusters)
+      : at(cluster), items(tiles_ * max(1, p.cuts)), stride(clusters), steps(steps_), tiles(tiles_), cut(p.cuts ? p.cut : steps_), part(0) {}
+  // stages [k0, k1) of a tile; none where the last ones are not there
+  __device__ __forceinline__ bool next(int& tile, int& k0, int& k1) {
+    if (at >= items) return false;
+    part = at / tiles;
+    tile = at - part * tiles;
+    k0 = min(steps, part * cut); k1 = min(steps, k0 + cut);
+    at += stride;
+    return true;
   }
 };
 
@@ -324,11 +368,12 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   tc_after();
   const uint32_t tmem = *(volatile uint32_t*)&tmem_slot;
   grid_wait();
-  const int count = p.counted ? *(const volatile int*)p.count : 0;
+  const int count = counted_on_device(p);
   const int rows = p.counted == 1 ? count : p.rows, depth = p.counted == 2 ? count : p.depth;
   const int steps = (depth + kDepth - 1) / kDepth;
   const Tiles tiles(p, rows, F::kRows, N);
-  const int items = tiles.per_batch * p.batch, first = blockIdx.x / CTAS, stride = gridDim.x / CTAS;
+  const int items = tiles.per_batch * p.batch;
+  Work work(p, items, steps, blockIdx.x / CTAS, gridDim.x / CTAS);
 
   // registers with GROUPED: 128 x 56 + 256 x 216 of the 384 x 168 that the block has
   if (warp < 4) {
@@ -337,11 +382,12 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       if (lane == 0) {
         uint32_t it = 0;
         bool ok = true;
-        for (int w = first; w < items && ok; w += stride) {
+        int w, k, k1;
+        while (ok && work.next(w, k, k1)) {
           int batch, tm, tn;
           tiles.at(w, batch, tm, tn);
           const int m0 = tm * F::kRows + rank * 128, n0 = tn * N + rank * F::kBRows;
-          for (int k = 0; k < steps; ++k, ++it) {
+          for (; k < k1; ++k, ++it) {
             const int s = it % F::kStages;
             if (!bar_wait(empty(s), ((it / F::kStages) & 1) ^ 1, p.polls)) { ok = false; break; }
             if (p.withhold && it == 0) continue;
@@ -371,12 +417,13 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         const uint32_t instr = kInstr<CTAS, N, A_MN, B_MN> | (p.bf16 ? kBf16Operands : 0u);
         uint32_t it = 0, n = 0;
         bool ok = true;
-        for (int w = first; w < items && ok; w += stride) {
-          for (int k0 = 0; ok && (k0 == 0 || k0 < steps); k0 += p.group, ++n) {
+        int w, begin, k1;
+        while (ok && work.next(w, begin, k1)) {
+          for (int k0 = begin; ok && (k0 == begin || k0 < k1); k0 += p.group, ++n) {
             const uint32_t ab = n & 1, d = tmem + ab * N;
             ok = bar_wait(acc_empty(ab), ((n >> 1) & 1) ^ 1, p.polls);
             tc_after();
-            const int end = min(steps, k0 + p.group);
+            const int end = k1 - k0 < p.group ? k1 : k0 + p.group;
             for (int k = k0; ok && k < end; ++k, ++it) {
               const int s = it % F::kStages;
               if (!bar_wait(full(s), (it / F::kStages) & 1, p.polls)) { ok = false; break; }
@@ -403,13 +450,14 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     at.polls = p.polls;
     uint32_t n = 0;
     bool ok = true;
-    for (int w = first; w < items && ok; w += stride) {
+    int w, begin, k1;
+    while (ok && work.next(w, begin, k1)) {
       int tm, tn;
       tiles.at(w, at.batch, tm, tn);
       at.row = tm * F::kRows + rank * 128 + quad * 32 + lane;
       at.col = tn * N + slice * F::kCols;
-      at.beside_diagonal = tm != tn;
-      at.part = (w * CTAS + rank) * kEpilogueWarps + warp - 4;
+      at.beside_diagonal = tm != tn / tiles.ratio;
+      at.part = ((work.part * items + w) * CTAS + rank) * kEpilogueWarps + warp - 4;
       epilogue.begin(at);
       float acc[GROUPED ? F::kCols / kBlock : 1][kBlock];
       auto from = [&](uint32_t ab, int c) { return tmem + ((uint32_t)(quad * 32) << 16) + ab * N + slice * F::kCols + c; };
@@ -418,7 +466,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         __syncwarp();
         if (lane == 0) arrive_in_cluster(CTAS == 2 ? in_leader(acc_empty(ab)) : acc_empty(ab));
       };
-      for (int k0 = 0; k0 == 0 || k0 < steps; k0 += p.group, ++n) {
+      for (int k0 = begin; k0 == begin || k0 < k1; k0 += p.group, ++n) {
         const uint32_t ab = n & 1;
         ok = __all_sync(0xffffffffu, bar_wait(acc_full(ab), (n >> 1) & 1, p.polls));
         if (!ok) break;
@@ -428,24 +476,27 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           for (int c = 0; c < F::kCols; c += kBlock) {
             ld_acc(from(ab, c), acc[0]);
             wait_acc(acc[0]);
+            if (begin == k1)          // nothing was added up
+#pragma unroll
+              for (int j = 0; j < kBlock; ++j) acc[0][j] = 0.0f;
             if (c + kBlock == F::kCols) release(ab);
             if (at.col + c < p.cols) epilogue.block(at, c, acc[0]);
           }
         } else {
-          if (k0 == 0) {
+          if (k0 == begin) {
 #pragma unroll
             for (int c = 0; c < F::kCols / kBlock; ++c) ld_acc(from(ab, c * kBlock), acc[c]);
 #pragma unroll
             for (int c = 0; c < F::kCols / kBlock; ++c) wait_acc(acc[c]);
           } else {
 #pragma unroll
-            for (int c = 0; c < F::kCols / 32; ++c) {
-              float v[32];
-              ld_acc32(from(ab, 32 * c), v);
-              wait_acc32(v);
-              float* sum = acc[32 * c / kBlock] + 32 * c % kBlock;
+            for (int c = 0; c < F::kCols / 16; ++c) {
+              float v[16];
+              ld_acc16(from(ab, 16 * c), v);
+              wait_acc16(v);
+              float* sum = acc[16 * c / kBlock] + 16 * c % kBlock;
 #pragma unroll
-              for (int j = 0; j < 32; j += 2) {
+              for (int j = 0; j < 16; j += 2) {
                 const float2 s = __fadd2_rn(make_float2(sum[j], sum[j + 1]), make_float2(v[j], v[j + 1]));
                 sum[j] = s.x; sum[j + 1] = s.y;
               }
@@ -458,7 +509,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       if constexpr (GROUPED) {
 #pragma unroll
         for (int c = 0; c < F::kCols / kBlock; ++c) {
-          if (steps == 0)             // nothing was added up
+          if (begin == k1)            // nothing was added up
 #pragma unroll
             for (int j = 0; j < kBlock; ++j) acc[c][j] = 0.0f;
           if (at.col + c * kBlock < p.cols) epilogue.block(at, c * kBlock, acc[c]);
@@ -477,6 +528,80 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     if (CTAS == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(2 * N)) : "memory");
     else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(2 * N)) : "memory");
   }
+}
+
+// ---- products whose tiles are cut -----------------------------------------------------------------------------------
+// The sums of a part of a tile's stages, 16 bytes a lane in a row; `add`: onto what is there, of a product before.
+template <bool GROUPED>
+struct PartEpilogue {
+  static constexpr bool kGrouped = GROUPED;
+  static constexpr int kSlots = 1;
+  struct Params { float4* parts; bool add; };
+  const Params& p;
+  __device__ __forceinline__ explicit PartEpilogue(const Params& e) : p(e) {}
+  __device__ __forceinline__ void begin(const Place&) {}
+  __device__ __forceinline__ void block(const Place& at, int c, float (&v)[kBlock]) {
+    float4* to = p.parts + ((int64_t)at.part * at.slice + c) * 8 + at.lane;
+#pragma unroll
+    for (int j = 0; j < kBlock / 4; ++j) {
+      float4 f = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+      if (p.add) {
+        const float4 g = to[32 * j];
+        f.x += g.x; f.y += g.y; f.z += g.z; f.w += g.w;
+      }
+      to[32 * j] = f;
+    }
+  }
+  __device__ __forceinline__ void end(const Place&) {}
+  __device__ __forceinline__ void finish(const Place&) {}
+};
+// A tile's parts together, in their order, and its epilogue: a CTA for 128 rows of a tile and one block of each of the epilogue's warps.
+template <int CTAS, int N, class Epilogue>
+__global__ void __launch_bounds__(32 * kEpilogueWarps) finish_kernel(const float4* parts, const __grid_constant__ Params p, const __grid_constant__ typename Epilogue::Params e) {
+  using F = Form<CTAS, N, Epilogue::kSlots>;
+  extern __shared__ unsigned char finish_smem[];
+  __shared__ __align__(8) uint64_t bars[kEpilogueWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = warp & 3, slice = warp >> 2;
+  if (threadIdx.x < kEpilogueWarps) bar_init(smem_u32(&bars[threadIdx.x]), 1);
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  __syncthreads();
+  grid_wait();
+  const int count = counted_on_device(p);
+  const int rows = p.counted == 1 ? count : p.rows;
+  const Tiles tiles(p, rows, F::kRows, N);
+  const int items = tiles.per_batch * p.batch, w = blockIdx.x / CTAS, rank = blockIdx.x % CTAS;
+  if (w >= items) return;
+  Epilogue epilogue(e);
+  Place at;
+  int tm, tn;
+  tiles.at(w, at.batch, tm, tn);
+  at.rows = rows; at.cols = p.cols; at.lane = lane; at.slice = F::kCols; at.polls = p.polls;
+  at.slots = ((smem_u32(finish_smem) + 1023u) & ~1023u) + warp * Epilogue::kSlots * kSlotBytes;
+  at.own = at.slots + lane * (kBlock * 2) + ((lane & 7) << 4);
+  at.bar = smem_u32(&bars[warp]);
+  at.row = tm * F::kRows + rank * 128 + quad * 32 + lane;
+  at.col = tn * N + slice * F::kCols;
+  at.beside_diagonal = tm != tn / tiles.ratio;
+  at.part = 0;
+  epilogue.begin(at);
+  const int c = blockIdx.y * kBlock;
+  if (at.col + c < p.cols) {
+    float v[kBlock];
+#pragma unroll
+    for (int j = 0; j < kBlock; ++j) v[j] = 0.0f;
+#pragma unroll 2
+    for (int k = 0; k < p.cuts; ++k) {
+      const float4* from = parts + (((int64_t)k * items + w) * CTAS + rank) * kEpilogueWarps * (F::kCols * 8) + (warp * F::kCols + c) * 8 + lane;
+#pragma unroll
+      for (int j = 0; j < kBlock / 4; ++j) {
+        const float4 f = from[32 * j];
+        v[4 * j] += f.x; v[4 * j + 1] += f.y; v[4 * j + 2] += f.z; v[4 * j + 3] += f.w;
+      }
+    }
+    epilogue.block(at, c, v);
+  }
+  epilogue.end(at);
+  epilogue.finish(at);
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------------
@@ -509,6 +634,22 @@ struct Operand {
   int64_t rows, depth, ld, plane;
 };
 
+template <int CTAS> int64_t clusters_of() { return sm_count() / CTAS; }
+template <int CTAS, int N>
+int64_t tiles_of(const Params& p) {      // with `counted` rows: at most
+  const int64_t tm = (p.rows + 128 * CTAS - 1) / (128 * CTAS), tn = (p.cols + N - 1) / N, ratio = 128 * CTAS > N ? 128 * CTAS / N : 1, high = tn / ratio;
+  return p.batch * (p.upper ? ratio * high * (high + 1) / 2 + tn % ratio * (high + 1) : tm * tn);
+}
+template <int CTAS, int N>
+void set_common(Params* p) {
+  // a band's rows of A, some 16 MB, stay in L2 while its columns go by
+  p->band = (int)std::min<int64_t>((p->rows + 128 * CTAS - 1) / (128 * CTAS), std::max<int64_t>(1, (16 << 20) / (128 * CTAS * 2 * std::max<int64_t>(1, p->cuts ? (int64_t)p->cut * kDepth : p->depth))));
+  p->polls = kWaitPolls; p->withhold = 0;
+#ifdef PB_DIAGNOSTICS
+  p->polls = g_polls.load(); p->withhold = g_withhold.load();
+#endif
+}
+
 template <int CTAS, int N, bool A_MN, bool B_MN, class Epilogue>
 int launch(const Operand& a, const Operand& b, Params p, const typename Epilogue::Params& e, cudaStream_t st) {
   using F = Form<CTAS, N, Epilogue::kSlots>;
@@ -518,21 +659,47 @@ int launch(const Operand& a, const Operand& b, Params p, const typename Epilogue
   };
   if (int s = map(&map_a, a, 128)) return s;
   if (int s = map(&map_b, b, F::kBRows)) return s;
-  const int64_t tm = (p.rows + F::kRows - 1) / F::kRows, tn = (p.cols + N - 1) / N, items = p.batch * (p.upper ? tn * (tn + 1) / 2 : tm * tn);
+  const int64_t items = tiles_of<CTAS, N>(p);
   if (items > kMaxIndexed / 2) return fail(PB_ERR_BAD_SHAPE, "%lld tiles of a product", (long long)items);
   if (items == 0) return PB_OK;
-  // a band's rows of A, some 16 MB, stay in L2 while its columns go by
-  p.band = (int)std::max<int64_t>(1, (16 << 20) / (F::kRows * 2 * std::max<int64_t>(1, p.depth)));
-  if (!Epilogue::kGrouped) p.group = kMaxIndexed;
-  p.polls = kWaitPolls; p.withhold = 0;
-#ifdef PB_DIAGNOSTICS
-  p.polls = g_polls.load(); p.withhold = g_withhold.load();
-#endif
+  if (!Epilogue::kGrouped) p.group = 1 << 24;      // more stages than there are, and added to one of them within an int
+  set_common<CTAS, N>(&p);
   auto kernel = product_kernel<CTAS, N, A_MN, B_MN, Epilogue>;
   PB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem));      // per device
-  const int64_t clusters = std::min<int64_t>(items, sm_count() / CTAS);
+  const int64_t clusters = std::min<int64_t>(items * std::max(1, p.cuts), clusters_of<CTAS>());
   launch_behind(kernel, (unsigned)(clusters * CTAS), kThreads, F::kSmem, st, map_a, map_b, p, e);
   PB_LAUNCH_CHECK("product_kernel");
+  return PB_OK;
+}
+
+// Cuts a product of few tiles, or of a few more than whole rounds of them, where that pays: a part costs its rounds and, for its accumulators, about kPartCost stages more, and the
+// joining of all parts a stage for every kJoinParts of them.  At most kMostCuts parts of eight stages at least.
+constexpr int kPartCost = 10, kJoinParts = 6, kMostCuts = 32;
+template <int CTAS, int N>
+void cut_stages(Params* p, int stages) {
+  const int64_t tiles = tiles_of<CTAS, N>(*p), clusters = clusters_of<CTAS>();
+  int64_t best = 0;
+  for (int n = 1; n <= kMostCuts && (n == 1 || stages / n >= 8); ++n) {
+    const int64_t cut = (stages + n - 1) / n, cost = (tiles * n + clusters - 1) / clusters * (cut + kPartCost) + tiles * n / kJoinParts;
+    if (n > 1 && cost >= best) continue;
+    best = cost; p->cuts = n; p->cut = (int)cut;
+  }
+  p->cuts = (stages + p->cut - 1) / std::max(1, p->cut);
+}
+// float4s that the parts of a cut product take
+template <int CTAS, int N>
+int64_t parts_of(const Params& p) { return tiles_of<CTAS, N>(p) * p.cuts * CTAS * (128 * N / 4); }
+
+template <int CTAS, int N, class Epilogue>
+int launch_finish(const float4* parts, Params p, const typename Epilogue::Params& e, cudaStream_t st) {
+  const int64_t items = tiles_of<CTAS, N>(p);
+  if (items == 0) return PB_OK;
+  set_common<CTAS, N>(&p);
+  constexpr int kSmem = 1024 + kEpilogueWarps * Epilogue::kSlots * kSlotBytes;
+  auto kernel = finish_kernel<CTAS, N, Epilogue>;
+  PB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+  launch_behind(kernel, dim3((unsigned)(items * CTAS), Form<CTAS, N, Epilogue::kSlots>::kCols / kBlock), 32 * kEpilogueWarps, kSmem, st, parts, p, e);
+  PB_LAUNCH_CHECK("finish_kernel");
   return PB_OK;
 }
 

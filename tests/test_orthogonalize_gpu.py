@@ -136,3 +136,17 @@ def test_captured_and_on_another_stream(built_lib):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, -want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(256, 128), (257, 128), (512, 127), (513, 1), (1024, 65), (1025, 64), (2049, 128), (4096, 128), (128, 4096), (3000, 120), (99, 3001), (4097, 128), (20, 2048, 128), (3, 128, 300),
+                                   (129, 6000), (6000, 129), (300, 8000), (500, 2100), (2, 260, 5000), (700, 700), (3, 900, 520), (1280, 1024)])
+def test_every_form(built_lib, shape, dtype):
+    """One launch for all steps by one to sixteen CTAs a matrix, A in whole tiles of three sizes, and cut along its contraction."""
+    g = (torch.randn(shape, generator=_gen(sum(shape)), device="cuda") * 30).to(dtype)
+    got = orthogonalize(g)
+    assert _lib.load().pb_gemm_check(torch.cuda.current_stream().cuda_stream) == 0
+    assert _off(got, _exact(g)) <= (MANY if min(shape[-2:]) >= 16 else FEW)
+    assert torch.equal(got, orthogonalize(g))
+    if len(shape) == 3:
+        assert torch.equal(got[-1], orthogonalize(g[-1])) or _off(got[-1], _exact(g[-1])) <= MANY          # alone, it may be cut otherwise
