@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(kSlab, 1) narrow_kernel(const __grid_constant_
   __shared__ uint32_t tmem_slot;
   __shared__ double squares[8], of_cluster[kMostClusters];
   __shared__ float factors[3];
-  const uint32_t base = (smem_u32(narrow_smem) + 1023u) & ~1023u, x_at = base, a_at = x_at + kSlab * kNarrow * 2, b_at = a_at + kNarrow * kNarrow * 2, sums_at = b_at + kNarrow * kNarrow * 2;
+  const uint32_t base = (smem_u32(narrow_smem) + 1023u) & ~1023u, x_at = base, a_at = x_at + kSlab * kNarrow * 2, sums_at = a_at + kNarrow * kNarrow * 2, b_at = sums_at + kNarrow * kNarrow * 4;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, quad = warp & 3, half = warp >> 2;
   const int rank = (int)(blockIdx.x % p.size), share = kNarrow / p.size;      // rows of A that this CTA adds up
   if (tid == 0) {
@@ -357,9 +357,15 @@ __global__ void __launch_bounds__(kSlab, 1) narrow_kernel(const __grid_constant_
 #pragma unroll
     for (int j = 0; j < kNarrow; ++j) x[j] = at < p.length && j < p.width ? Elem<T>::to_f32(from[j * step]) : 0.0f;
   }
-  double s = 0.0;
+  float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-  for (int j = 0; j < kNarrow; ++j) s = fma((double)x[j], (double)x[j], s);
+  for (int j = 0; j < kNarrow; ++j) part[j & 3] = fmaf(x[j], x[j], part[j & 3]);
+  double s = (double)((part[0] + part[1]) + (part[2] + part[3]));
+  if (!(s < 0x1p120) || s < 0x1p-60) {          // squares that leave f32, or lose their bits in it
+    s = 0.0;
+#pragma unroll
+    for (int j = 0; j < kNarrow; ++j) s = fma((double)x[j], (double)x[j], s);
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (lane == 0) squares[warp] = s;
@@ -493,23 +499,32 @@ __global__ void __launch_bounds__(kSlab, 1) narrow_kernel(const __grid_constant_
       for (int j = 0; j < 32; ++j) x[32 * h + j] = fmaf(x[32 * h + j], a, v[j] * (1.0f / kScaleA));
     }
   }
-  if (at < p.length) {
-    __nv_bfloat16* out = p.out + matrix;
-    if (p.tall && p.out_vectors) {
+  constexpr float kDown = 1.0f / kScaleX;
+  if (p.tall) {              // the CTA's rows lie together: through shared memory, 16 or two bytes a thread
+    const int here = (int)max((int64_t)0, min((int64_t)kSlab, p.length - (int64_t)rank * kSlab)) * p.width;
+    __nv_bfloat16 *to = p.out + matrix + (int64_t)rank * kSlab * p.width, *from = reinterpret_cast<__nv_bfloat16*>(narrow_smem + (base - smem_u32(narrow_smem)));
+    if (p.out_vectors) {     // where a row's 16-byte pieces are a multiple of eight, they are exchanged by its number, against bank conflicts
+      const int pieces = p.width / 8, turn = pieces % 8 == 0 ? 7 : 0;
 #pragma unroll
-      for (int j = 0; j < kNarrow; j += 8) {
-        const float* v = x + j;
-        constexpr float kDown = 1.0f / kScaleX;
-        if (j < p.width)
-          *reinterpret_cast<uint4*>(out + at * p.width + j) = make_uint4(pack_bf16x2(v[0] * kDown, v[1] * kDown), pack_bf16x2(v[2] * kDown, v[3] * kDown), pack_bf16x2(v[4] * kDown, v[5] * kDown), pack_bf16x2(v[6] * kDown, v[7] * kDown));
+      for (int k = 0; k < kNarrow / 8; ++k) {
+        const float* v = x + 8 * k;
+        if (k < pieces)
+          reinterpret_cast<uint4*>(from)[tid * pieces + (k ^ (tid & turn))] = make_uint4(pack_bf16x2(v[0] * kDown, v[1] * kDown), pack_bf16x2(v[2] * kDown, v[3] * kDown), pack_bf16x2(v[4] * kDown, v[5] * kDown), pack_bf16x2(v[6] * kDown, v[7] * kDown));
       }
+      __syncthreads();
+      for (int i = tid; i < here / 8; i += kSlab) reinterpret_cast<uint4*>(to)[i] = reinterpret_cast<const uint4*>(from)[i ^ (i / pieces & turn)];
     } else {
-      __nv_bfloat16* to = p.tall ? out + at * p.width : out + at;
-      const int64_t by = p.tall ? 1 : p.length;
 #pragma unroll
       for (int j = 0; j < kNarrow; ++j)
-        if (j < p.width) to[j * by] = __float2bfloat16_rn(x[j] * (1.0f / kScaleX));
+        if (j < p.width) from[tid * p.width + j] = __float2bfloat16_rn(x[j] * kDown);
+      __syncthreads();
+      for (int i = tid; i < here; i += kSlab) to[i] = from[i];
     }
+  } else if (at < p.length) {
+    __nv_bfloat16* to = p.out + matrix + at;
+#pragma unroll
+    for (int j = 0; j < kNarrow; ++j)
+      if (j < p.width) to[j * p.length] = __float2bfloat16_rn(x[j] * kDown);
   }
   tc_before();
   __syncthreads();
