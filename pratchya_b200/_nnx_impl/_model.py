@@ -19,9 +19,11 @@ from dataclasses import dataclass
 import torch
 
 from .._qualia import _ops
+from ._embedding import embedding_lookup
 from ._glue import QuantizedMix, can_quantize_mixes, can_quantize_relu2, relu2, relu2_quantized, rms_norm, token_shift_lerp, token_shift_lerp_quantized, wkv_finish, wkv_prepare
 from ._glue import smoothed_cross_entropy as fused_cross_entropy
 from ._int4 import Int4Linear
+from ._linear_xent import linear_cross_entropy
 from ._module import linear_fp8
 from ._nograph import no_graph
 from ._wkv7 import wkv_state_scan
@@ -321,35 +323,49 @@ class PratchyaCausalLM(torch.nn.Module):
         self.lm_head = Linear(cfg.hidden_size, cfg.vocab_size, (cfg.blksize, 1), gen, device)
 
     def embed(self, input_ids):                      # EmbeddingScaled, _module.py:21-37
-        rows = self.embedding[input_ids]             # the rows of a (1,blk)-quantized table quantize as the table does: row-local super-groups
+        rows = embedding_lookup(self.embedding, input_ids)      # the rows of a (1,blk)-quantized table quantize as the table does: row-local super-groups
         return read_param(rows, (1, self.cfg.blksize)) * math.sqrt(self.cfg.hidden_size)
 
-    def forward(self, input_ids, label=None, keep_logits=True):
-        """(logits, loss).  `keep_logits=False` (with labels, fused kernels): the logits are not returned and the loss's
-        backward pass writes their cotangent over them, for a training step that only wants the loss."""
-        cfg = self.cfg
+    def hidden(self, input_ids):
+        """What lm_head is given, [B, T, C]: the blocks' output from a zero state behind the final norm."""
         bsz, steps = input_ids.shape
         dev = input_ids.device
         t_positions = torch.arange(steps, device=dev, dtype=torch.int32)
         x = self.pre_rmsnorm(self.embed(input_ids))
         v = None
-        zeros_c = torch.zeros(bsz, 1, cfg.hidden_size, device=dev)
+        zeros_c = torch.zeros(bsz, 1, self.cfg.hidden_size, device=dev)
         for i, blk in enumerate(self.blocks):
             if i < self.remat and torch.is_grad_enabled():
                 x, v = _RematBlock.apply(blk, t_positions, zeros_c, x, v)
             else:
                 x, v, _, _, _ = blk(x, v, t_positions, zeros_c, zeros_c, None)
-        x = self.final_rmsnorm(x)
-        logits = self.lm_head(x)
+        return self.final_rmsnorm(x)
+
+    def forward(self, input_ids, label=None, keep_logits=True):
+        """(logits, loss).  `keep_logits=False` (with labels, fused kernels): the logits are not returned and the loss's
+        backward pass writes their cotangent over them, for a training step that only wants the loss."""
+        logits = self.lm_head(self.hidden(input_ids))
         loss = None
         if label is not None:
-            if cfg.fused_glue:
+            if self.cfg.fused_glue:
                 loss = fused_cross_entropy(logits, label, reuse_logits=not keep_logits)
                 if not keep_logits:
                     logits = None
             else:
                 loss = smoothed_cross_entropy(logits, label)
         return logits, loss
+
+    def loss_without_logits(self, input_ids, label, alpha: float = 0.1):
+        """The loss of forward(input_ids, label) with lm_head's weight and its input in bf16 where forward has them in fp8, and no logits (8.6 GB and as much again for their
+        cotangent with 32768 tokens and 65536 words): `linear_cross_entropy` of every position but the last of each sequence, their mean."""
+        if not isinstance(self.lm_head, Linear):
+            raise TypeError("loss_without_logits: lm_head's dense weight is gone (to_int4)")
+        bsz, steps = input_ids.shape
+        if steps < 2 or tuple(label.shape) != (bsz, steps):
+            raise ValueError(f"loss_without_logits: input_ids {tuple(input_ids.shape)}, label {tuple(label.shape)}")
+        targets = torch.cat([label[:, 1:], label.new_full((bsz, 1), -1)], dim=1)
+        losses = linear_cross_entropy(self.hidden(input_ids).to(torch.bfloat16), self.lm_head.kernel.to(torch.bfloat16), targets, smoothing=alpha)
+        return losses.sum() / (bsz * (steps - 1))
 
     def init_state(self, batch: int):
         """The zero state of `batch` sequences (`init_state`, _config.py:41-52): (position, [(tm_state, cm_state, wkv_state) of each block])."""

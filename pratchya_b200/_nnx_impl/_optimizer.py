@@ -2,10 +2,10 @@
 parameters (pratchya/_nnx_impl/_optimizer.py:171-205, f32 blend) and the scanned branch for stacked 3-D
 parameters (:108-160, bfloat16 blend per layer), which is the one the model's scanned blocks take.
 
-Only the part that works on QArrayImpl data is here: the blend of gradient and momentum and the
-re-quantization of the new momentum.  What the reference does with `c` afterwards -- sign() for the
-Lion branch (:213), Newton-Schulz for the Muon branch (:208) -- and its schedules and parameter
-tree handling are the optimizer's own logic and stay with the caller.
+The part that works on QArrayImpl data is here, the blend of gradient and momentum and the
+re-quantization of the new momentum, and what follows it for one parameter: sign() for the Lion
+branch (:213), Newton-Schulz for the Muon branch (:208).  The schedules and the parameter tree
+handling are the optimizer's own logic and stay with the caller.
 """
 from __future__ import annotations
 
@@ -17,6 +17,7 @@ import torch
 from .. import _lib
 from .._lib import check
 from .._qualia._qarr import QArrayImpl
+from ._orthogonalize import orthogonalize
 
 
 def momentum_update(g: QArrayImpl, m: QArrayImpl, beta1: float, beta2: float):
@@ -93,3 +94,8 @@ def momentum_update_stacked(g: QArrayImpl, m: QArrayImpl, beta1: float, beta2: f
 def lion_update(c: torch.Tensor, param_f32: torch.Tensor, lr: float, weight_decay: float) -> torch.Tensor:
     """update = -(lr * sign(c) + lr * weight_decay * p), :213-215."""
     return -(lr * torch.sign(c) + lr * weight_decay * param_f32)
+
+
+def muon_update(c: torch.Tensor, param_f32: torch.Tensor, lr: float, weight_decay: float, steps: int = 5) -> torch.Tensor:
+    """update = -(lr * newton_schulz(c) + lr * weight_decay * p), :136-142 and :208-211, for one 2-D parameter or a stack of them; c in f32 or bf16."""
+    return -(lr * orthogonalize(c.detach(), steps=steps).to(param_f32.dtype) + lr * weight_decay * param_f32)

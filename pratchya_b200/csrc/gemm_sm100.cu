@@ -1734,6 +1734,10 @@ int transposed_status_fetch(unsigned int* out);   // transpose_quantize.cu
 int dense_dot_status_fetch(unsigned int* out);    // dense_dot.cu
 int orthogonalize_status_fetch(unsigned int* out);      // orthogonalize.cu
 int linear_xent_status_fetch(unsigned int* out);  // linear_xent.cu
+#ifdef PB_DIAGNOSTICS
+void orthogonalize_control(uint32_t polls, int withhold);
+void linear_xent_control(uint32_t polls, int withhold);
+#endif
 }
 
 extern "C" int pb_gemm_check(void* stream) {
@@ -1764,6 +1768,12 @@ extern "C" PB_API int pb_debug_gemm_profile(unsigned long long* out16, void* str
   unsigned long long zero[16] = {0};
   PB_CUDA_TRY(cudaMemcpyFromSymbol(out16, g_gemm_prof, sizeof(zero)));
   PB_CUDA_TRY(cudaMemcpyToSymbol(g_gemm_prof, zero, sizeof(zero)));
+  return PB_OK;
+}
+// The same for the products of the cross entropy without logits and of the orthogonalised update: poll budget (0: the default), and whether a launch's first stage is left unfilled.
+extern "C" PB_API int pb_debug_product_control(unsigned int polls, int withhold) {
+  orthogonalize_control(polls, withhold);
+  linear_xent_control(polls, withhold);
   return PB_OK;
 }
 // Sets the poll budget of the bounded waits (0 restores the default) and the diagnostic bits of

@@ -480,6 +480,9 @@ int to_hidden(const Plan& q, const Weight& w, int64_t first, int64_t n, int64_t 
 }  // namespace
 
 int linear_xent_status_fetch(unsigned int* out) { return status_fetch(out); }
+#ifdef PB_DIAGNOSTICS
+void linear_xent_control(uint32_t polls, int withhold) { control(polls, withhold); }
+#endif
 }  // namespace pb
 
 using namespace pb;

@@ -301,7 +301,7 @@ struct NarrowParams {
   float coefficients[64 * 3];
   uint32_t polls;
 };
-__device__ __forceinline__ void cluster_barrier() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_sync_all() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t in_cta(uint32_t addr, int rank) {
   uint32_t r;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
@@ -316,14 +316,11 @@ __device__ __forceinline__ uint32_t piece_at(uint32_t base, int rows, int r, int
 
 template <typename T>
 __global__ void __launch_bounds__(kSlab, 1) narrow_kernel(const __grid_constant__ NarrowParams p) {
-  extern __shared__ unsigned char narrow_smem[];
+  extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t bar;
   __shared__ uint32_t tmem_slot;
-  __shared__ double squares[8], of_cluster[kMostClusters];
-  __shared__ float factors[3];
-  const uint32_t base = (smem_u32(narrow_smem) + 1023u) & ~1023u, x_at = base, a_at = x_at + kSlab * kNarrow * 2, sums_at = a_at + kNarrow * kNarrow * 2, b_at = sums_at + kNarrow * kNarrow * 4;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u, x_at = base, a_at = x_at + kSlab * kNarrow * 2, sums_at = a_at + kNarrow * kNarrow * 2, b_at = sums_at + kNarrow * kNarrow * 4;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, quad = warp & 3, half = warp >> 2;
-  const int rank = (int)(blockIdx.x % p.size), share = kNarrow / p.size;      // rows of A that this CTA adds up
   if (tid == 0) {
     bar_init(smem_u32(&bar), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -334,10 +331,13 @@ __global__ void __launch_bounds__(kSlab, 1) narrow_kernel(const __grid_constant_
   }
   tc_before();
   __syncthreads();
-  cluster_barrier();          // the others run, and can be written to
+  cluster_sync_all();          // the others run, and can be written to
   tc_after();
   const uint32_t tmem = *(volatile uint32_t*)&tmem_slot, lanes = tmem + ((uint32_t)(quad * 32) << 16);
   grid_wait();
+  __shared__ double squares[8], of_cluster[kMostClusters];
+  __shared__ float factors[3];
+  const int rank = (int)(blockIdx.x % p.size), share = kNarrow / p.size;      // rows of A that this CTA adds up
 
   // this thread's numbers
   const int64_t matrix = (int64_t)(blockIdx.x / p.size) * p.length * p.width, at = (int64_t)rank * kSlab + tid;
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(kSlab, 1) narrow_kernel(const __grid_constant_
     for (int w = 1; w < 8; ++w) s = w == 1 ? squares[0] + squares[1] : s + squares[w];
     asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(in_cta(smem_u32(&of_cluster[rank]), tid)), "d"(s) : "memory");
   }
-  cluster_barrier();
+  cluster_sync_all();
   if (tid == 0) {
     s = 0.0;
     for (int r = 0; r < p.size; ++r) s += of_cluster[r];
@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(kSlab, 1) narrow_kernel(const __grid_constant_
       }
       tc_before();
     }
-    cluster_barrier();
+    cluster_sync_all();
     for (int i = tid; i < share * (kNarrow / 4); i += kSlab) {      // four columns of a row, in the CTAs' order, to all of them
       const int row = i / (kNarrow / 4), piece = i % (kNarrow / 4), whole = rank * share + row;
       float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(kSlab, 1) narrow_kernel(const __grid_constant_
       for (int r = 0; r < p.size; ++r) asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(in_cta(to, r)), "r"(lo), "r"(hi) : "memory");
     }
     async_fence();
-    cluster_barrier();
+    cluster_sync_all();
     async_fence();
     if (tid == 0) {          // A A
       tc_after();
@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(kSlab, 1) narrow_kernel(const __grid_constant_
   constexpr float kDown = 1.0f / kScaleX;
   if (p.tall) {              // the CTA's rows lie together: through shared memory, 16 or two bytes a thread
     const int here = (int)max((int64_t)0, min((int64_t)kSlab, p.length - (int64_t)rank * kSlab)) * p.width;
-    __nv_bfloat16 *to = p.out + matrix + (int64_t)rank * kSlab * p.width, *from = reinterpret_cast<__nv_bfloat16*>(narrow_smem + (base - smem_u32(narrow_smem)));
+    __nv_bfloat16 *to = p.out + matrix + (int64_t)rank * kSlab * p.width, *from = reinterpret_cast<__nv_bfloat16*>(smem_raw + (base - smem_u32(smem_raw)));
     if (p.out_vectors) {     // where a row's 16-byte pieces are a multiple of eight, they are exchanged by its number, against bank conflicts
       const int pieces = p.width / 8, turn = pieces % 8 == 0 ? 7 : 0;
 #pragma unroll
@@ -635,6 +635,9 @@ int run_update(bool tall, const Operand& x_rows, const Operand& x_cols, const Op
 }  // namespace
 
 int orthogonalize_status_fetch(unsigned int* out) { return status_fetch(out); }
+#ifdef PB_DIAGNOSTICS
+void orthogonalize_control(uint32_t polls, int withhold) { control(polls, withhold); }
+#endif
 }  // namespace pb
 
 using namespace pb;

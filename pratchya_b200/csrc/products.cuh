@@ -625,6 +625,10 @@ inline int make_map(CUtensorMap* map, const void* base, bool bf16, int64_t inner
 #ifdef PB_DIAGNOSTICS
 std::atomic<uint32_t> g_polls{kWaitPolls};
 std::atomic<int> g_withhold{0};
+inline void control(uint32_t polls, int withhold) {
+  g_polls.store(polls ? polls : kWaitPolls);
+  g_withhold.store(withhold);
+}
 #endif
 
 // An operand: `rows` (of D's rows or columns) x depth, its k lying together or (mn) its rows

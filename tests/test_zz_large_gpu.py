@@ -42,3 +42,38 @@ def test_codes_beyond_two_to_the_32(built_lib):
     want = x.double() @ w
     # whole numbers up to a block's scale: a row's error is that of 128 + 3 additions in f32
     assert ((y[:, -16:].double() - want).abs() <= 140 * 2.0 ** -24 * (x.double().abs() @ w.abs())).all()
+
+
+def test_weights_and_tables_beyond_two_to_the_31(built_lib):
+    """140001 words of 16384, 2.3 billion numbers: the losses of the last words, and the weight's gradient there, as if those words' weights were alone at their place among logits that are
+    far below; a table of a billion rows' bytes: its last rows and their gradient."""
+    from pratchya_b200._nnx_impl import embedding_lookup, linear_cross_entropy
+    vocab, depth = 140001, 16384
+    g = torch.Generator(device="cuda").manual_seed(19)
+    w = torch.zeros(vocab, depth, dtype=torch.bfloat16, device="cuda")
+    few = (torch.randn(9, depth, generator=g, device="cuda") / 16).bfloat16()
+    w[-9:] = few
+    assert w.numel() > 2 ** 31
+    x = torch.randn(20, depth, generator=g, device="cuda").bfloat16()
+    t = torch.randint(vocab - 9, vocab, (20,), generator=g, device="cuda")
+    w.requires_grad_(True)
+    loss = linear_cross_entropy(x, w.t(), t)
+    z = x.double() @ few.double().t()
+    lse = torch.logsumexp(torch.cat([z, torch.full((20, 1), 0.0, device="cuda", dtype=torch.float64) + torch.log(torch.tensor(vocab - 9.0, device="cuda", dtype=torch.float64))], 1), 1)
+    want = lse - z.gather(1, (t - vocab + 9)[:, None])[:, 0]
+    assert (loss.double() - want).abs().max() <= 1e-4
+    (d,) = torch.autograd.grad(loss.sum(), w)
+    p = (z - lse[:, None]).exp() - torch.nn.functional.one_hot(t - vocab + 9, 9)
+    exact = p.t() @ x.double()
+    assert (d[-9:].double() - exact).norm() <= 3 * 2.0 ** -8 * exact.norm()
+    rest = (torch.zeros_like(lse) - lse).exp() @ x.double()                # what every other word's row is
+    assert (d[:2].double() - rest).norm() <= 3 * 2.0 ** -8 * 2 ** 0.5 * rest.norm()
+    del w, d
+    table = torch.zeros(2 ** 20 + 3, 2056, dtype=torch.bfloat16, device="cuda").requires_grad_(True)
+    with torch.no_grad():
+        table[-3:] = torch.randn(3, 2056, generator=g, device="cuda").bfloat16()
+    ids = torch.tensor([2 ** 20 + 2, 5, -1, 2 ** 20, -3], device="cuda")
+    rows = embedding_lookup(table, ids)
+    assert torch.equal(rows, table[ids]) and table.numel() > 2 ** 31
+    (d,) = torch.autograd.grad(rows, table, torch.ones_like(rows))
+    assert (d[-1] == 2).all() and (d[-2] == 0).all() and (d[-3] == 2).all() and (d[5] == 1).all() and d.float().sum() == 5 * 2056
