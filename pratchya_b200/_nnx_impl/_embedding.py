@@ -6,9 +6,11 @@ import operator
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from ._logprobs import wants_derivative
+from ._nograph import run
 
 
 def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, padding_id: Optional[int] = None) -> torch.Tensor:
@@ -28,10 +30,7 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0,
         if out is not None:
             return out
     table, ids, padding = _checked(table, ids, padding_id)          # what has to be converted first, or refused
-    out = _lib.native().embedding_lookup(table, ids, scale, padding, derivative)
-    if out is None:
-        raise RuntimeError("embedding_lookup takes plain CUDA tensors only")
-    return out
+    return run(_EmbeddingFn, table, ids, scale, padding) if derivative else _forward(table, ids, scale, padding)
 
 
 def _checked(table, ids, padding_id):
@@ -53,3 +52,33 @@ def _checked(table, ids, padding_id):
     if torch.jit.is_tracing():          # a trace would hold the result as a constant
         raise RuntimeError("embedding_lookup cannot be traced")
     return table.contiguous(), ids.contiguous(), -1 if padding_id is None else padding_id % vocab
+
+
+def _forward(table, ids, scale, padding):
+    out = torch.empty((*ids.shape, table.shape[1]), dtype=table.dtype, device=table.device)
+    _lib.native().pb_embedding_lookup(table, _type(table), *table.shape, ids, ids.numel(), scale, padding, out)
+    return out
+
+
+def _type(x):
+    return _lib.PB_F32 if x.dtype is torch.float32 else _lib.PB_BF16
+
+
+class _EmbeddingFn(torch.autograd.Function):
+    """What the extension's own function does, for calls that a dispatch mode watches."""
+    @staticmethod
+    def forward(ctx, table, ids, scale, padding):
+        ctx.save_for_backward(ids)
+        ctx.scale, ctx.padding, ctx.shape = scale, padding, table.shape
+        return _forward(table, ids, scale, padding)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        (ids,) = ctx.saved_tensors
+        nat, g = _lib.native(), g.contiguous()
+        d = torch.empty(ctx.shape, dtype=g.dtype, device=g.device)
+        size = nat.pb_embedding_lookup_bwd_workspace_size(ids.numel(), *ctx.shape)
+        workspace = torch.empty(max(size, 256), dtype=torch.uint8, device=g.device)
+        nat.pb_embedding_lookup_bwd(g, _type(g), ids, ids.numel(), *ctx.shape, ctx.scale, ctx.padding, d, workspace, size)
+        return d, None, None, None

@@ -9,7 +9,7 @@ import operator
 import torch
 
 from .. import _lib
-from ._nograph import no_graph
+from ._logprobs import wants_derivative
 
 #: a, b, c of the odd polynomial a s + b s^3 + c s^5: steepest at zero of those that keep [0, 1] near 1 in five steps
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
@@ -30,7 +30,7 @@ def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients=COEFFICIENT
         raise ValueError(f"orthogonalize: update {tuple(update.shape)} is no matrix")
     if torch.jit.is_tracing():          # a trace would hold the result as a constant
         raise RuntimeError("orthogonalize cannot be traced")
-    if (torch.is_grad_enabled() and update.requires_grad) or not (torch.is_grad_enabled() or no_graph()):
+    if wants_derivative(update):
         raise RuntimeError("orthogonalize has no derivative: call it under torch.no_grad() or with update.detach()")
     steps, eps = operator.index(steps), float(eps)
     if not 1 <= steps <= 64 or not (eps >= 0.0 and math.isfinite(eps)):

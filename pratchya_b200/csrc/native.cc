@@ -999,7 +999,7 @@ PyMethodDef methods[] = {
     ENTRY(pb_rms_norm), ENTRY(pb_rms_norm_bwd), ENTRY(pb_rms_norm_bwd_workspace_size), ENTRY(pb_relu2), ENTRY(pb_relu2_bwd),
     ENTRY(pb_wkv_finish), ENTRY(pb_wkv_finish_workspace_size), ENTRY(pb_wkv_finish_bwd), ENTRY(pb_wkv_finish_bwd_workspace_size),
     ENTRY(pb_smoothed_xent), ENTRY(pb_smoothed_xent_bwd),
-    METHOD("embedding_lookup", embedding_lookup),
+    METHOD("embedding_lookup", embedding_lookup), ENTRY(pb_embedding_lookup), ENTRY(pb_embedding_lookup_bwd), ENTRY(pb_embedding_lookup_bwd_workspace_size),
     ENTRY(pb_linear_xent), ENTRY(pb_linear_xent_bwd), ENTRY(pb_linear_xent_workspace_size), METHOD("strides_of_rows", strides_of_rows),
     ENTRY(pb_orthogonalize), ENTRY(pb_orthogonalize_workspace_size),
     {"set_error", set_error, METH_O, nullptr},

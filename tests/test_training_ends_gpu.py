@@ -4,9 +4,11 @@ import ctypes as C
 
 import pytest
 import torch
+from torch.autograd import forward_ad
+from torch.utils._python_dispatch import TorchDispatchMode
 
 from pratchya_b200 import _lib
-from pratchya_b200._nnx_impl import linear_cross_entropy, momentum_update_stacked, muon_update, orthogonalize
+from pratchya_b200._nnx_impl import embedding_lookup, linear_cross_entropy, momentum_update_stacked, muon_update, orthogonalize
 from pratchya_b200._nnx_impl._model import PratchyaCausalLM, PratchyaConfig, read_param
 from pratchya_b200._qualia import QArrayImpl
 
@@ -160,3 +162,37 @@ def test_two_calls_at_once(built_lib):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(a, want[i][0]) and torch.equal(b, want[i][1]) for a, b in got[i])
+
+
+def test_no_derivative_is_dropped_without_a_word(built_lib):
+    """Forward-mode differentiation, function transforms and traces are refused by each; a dispatch mode that watches changes nothing."""
+    g = torch.Generator(device="cuda").manual_seed(6)
+    table, ids = torch.randn(50, 64, generator=g, device="cuda"), torch.randint(0, 50, (7,), generator=g, device="cuda")
+    x, w, t = torch.randn(7, 64, generator=g, device="cuda").bfloat16(), torch.randn(64, 30, generator=g, device="cuda").bfloat16(), torch.randint(0, 30, (7,), generator=g, device="cuda")
+    calls = [lambda v: embedding_lookup(v, ids), lambda v: linear_cross_entropy(v, w, t), lambda v: linear_cross_entropy(x, v, t), lambda v: orthogonalize(v)]
+    inputs = [table, x, w, table]
+    for call, v in zip(calls, inputs):
+        with forward_ad.dual_level(), pytest.raises(RuntimeError):
+            call(forward_ad.make_dual(v, torch.ones_like(v)))
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(call, (v,), (torch.ones_like(v),))
+        with torch.no_grad(), pytest.raises(RuntimeError):
+            torch.func.vmap(call)(torch.stack([v, v]))
+        with pytest.raises(RuntimeError):
+            torch.jit.trace(call, (v,), check_trace=False)
+
+    class Watching(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    for call, v in zip(calls, inputs):
+        want = call(v)
+        with Watching():
+            assert torch.equal(call(v), want)
+        if call is calls[3]:
+            continue
+        leaf = v.detach().requires_grad_(True)
+        (d,) = torch.autograd.grad(call(leaf).float().sum(), leaf)
+        with Watching():
+            (again,) = torch.autograd.grad(call(leaf).float().sum(), leaf)
+        assert torch.equal(d, again)
