@@ -8,7 +8,7 @@
 // Backward: the logits once more, a piece of the vocabulary at a time, left as dz / (g (1 - a)) in bf16, and two products of the piece: dx, added up over the pieces in
 // f32, and the piece's part of dW.  An operand of a bf16 product is rounded once; divided so, the target's element, the largest, is p_t / (1 - a) - 1 and next to
 // exact while p_t is small, where g's and a's own bits would round all of a position's gradient one way (2.7e-3 of dx and dW, 1.66e-3 of
-// which is the results' own rounding; now GRADIENT_ERROR).  dx takes g (1 - a) in f32 at its end; for dW the hidden states are multiplied by g over the largest g, exactly 1
+// which is the results' own rounding; now 2.3e-3).  dx takes g (1 - a) in f32 at its end; for dW the hidden states are multiplied by g over the largest g, exactly 1
 // where all are one.
 //
 // Positions without a target do no work: a first kernel numbers those that have one, a second brings their hidden states together (rows
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(128) gather_kernel(const __grid_constant__ Gat
 // a weight whose rows do not lie as TMA wants them, to rows that do
 __global__ void __launch_bounds__(256) pad_kernel(const unsigned short* from, int64_t inner, int64_t ld_from, unsigned short* to, int64_t ld_to) {
   grid_wait();
-  const int64_t row = blockIdx.y + (int64_t)blockIdx.z * 65535;
+  const int64_t row = blockIdx.y;
   for (int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x; c < inner; c += (int64_t)gridDim.x * 256) to[row * ld_to + c] = from[row * ld_from + c];
 }
 
@@ -367,7 +367,8 @@ struct Plan {
   size_t off_place, off_origin, off_target, off_lse, off_g, off_x, off_scaled, off_w, off_terms, off_sums, off_hit, off_dz, off_parts, bytes;
 };
 template <typename T> T* part(void* workspace, size_t off) { return reinterpret_cast<T*>(static_cast<unsigned char*>(workspace) + off); }
-// Where there is one tile of rows, half of a pair's 256 would be idle: a CTA's 128 x 256.  64 positions of 2048 against 65536 words: FEW_US
+// Where there is one tile of rows, half of a pair's 256 would be idle: a CTA's 128 x 256.  The product of 64 positions of 2048 with 65536 words:
+// 62 us by a pair's, 50 so (41 are the weight's bytes).
 bool few_rows(const Plan& q) { return q.rows <= 128; }
 
 // dx's product of a piece: few tiles of many stages, so they are cut

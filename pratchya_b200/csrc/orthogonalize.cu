@@ -285,8 +285,9 @@ struct UpdateEpilogue : Reading {
 // All steps in one launch, X never in memory: a cluster of CTAs shares the other direction, 256 of it each; a thread has one of these, 128 numbers of X in f32, and their fp16
 // roundings lie in shared memory as an operand, the same tile as X (rows by k) and as X^T (k by rows).  A step: the cluster's CTAs make their parts of
 // A = X^T X and send each other the rows that they add up (S CTAs 128 / S each); these go to all as fp16; every CTA makes A A, B and its own rows of X B.  The low-rank layers' weights,
-// 2048 x 128: one 127 us by three products a step, NARROW_US so; 120 of them NARROW_ALL.
-// What it is bound by: a step's chain, some CHAIN cycles of barriers of the cluster, tensor core round trips and fp16 rows through shared memory.
+// 2048 x 128: one 127 us by three products a step, 54 so; 120 of them 917 and 452 (fifteen clusters of eight run at a time).
+// What it is bound by: a step's chain of 17000 cycles, half of them the cluster's sums (16 bytes a clock into an SM, two barriers); the rest are tensor core round trips and fp16 rows
+// through shared memory, with nothing of another matrix beside them.
 constexpr int kNarrow = 128, kSlab = 256, kMostClusters = 16;
 constexpr int kNarrowSmem = 1024 + kSlab * kNarrow * 2 + 2 * kNarrow * kNarrow * 2 + kNarrow * kNarrow * 4;      // X, A and B, sums from the others
 
@@ -573,7 +574,7 @@ int run_narrow(const void* update, int dtype, int64_t batch, int64_t rows, int64
 // ---- host side ----------------------------------------------------------------------------------------------------
 // Forms of a product's tiles: 256 x 256 and 256 x 128 of a CTA pair, 128 x 128 of a CTA.  A tile's stage of 64 of k is bound by its loads from L2, some 58 bytes a clock into an SM: 563, 413 and 540 cycles, and
 // a tile takes 9000, 6000 and 5000 more until its sums have left.  So the wide pair's is the best wherever its tiles fill the chip, and the others where it
-// would leave half of it idle: A of 2048 x 2048, 36 tiles | 72, FORM_US.
+// would leave half of it idle: A of 2048 x 2048, 36 tiles | 72, 22.4 us | 17.3.
 enum Tile { kPair256, kPair128, kSingle };
 double cost_of(Tile tile, const Params& p) {
   const int64_t stages = (p.depth + kDepth - 1) / kDepth;

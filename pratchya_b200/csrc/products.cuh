@@ -5,11 +5,11 @@
 // into 128-byte swizzled tiles and the matrix descriptors say which, so that no operand is ever transposed.  A tile is 128 CTAS x N:
 //   CTAS = 2: a cluster of two CTAs makes 256 x 256; each loads its own 128 rows of A and its own 128 of B (32 KB per 64 of k and
 //             SM, where one CTA's 128 x 256 takes 48: what a tile loads from L2 is the nearest bound beside the tensor core);
-//   CTAS = 1: 128 x 128, for products that have few tiles.
+//   the same pair with 256 x 128, and CTAS = 1 with 128 x 128 or 128 x 256: for products that have few tiles, or few rows.
 // Persistent: warp 0 loads, a lane of warp 1 (of the leading CTA) issues tcgen05.mma, eight warps empty one accumulator of TMEM while the
 // other fills, each thread one row and half of the columns.  Every wait is bounded and reported by pb_gemm_check.
 // The tensor core's own additions do not round to nearest: an accumulator takes `group` stages of k, and the sums of a tile's groups are added up in the
-// registers that read them.  2-norm errors of the loss of 64 positions of 2048 against 64 bits: one group 1.4e-6, groups of 512 of k GROUP_ERROR.
+// registers that read them.  2-norm errors of the loss of 64 positions of 2048 against 64 bits: one group 1.4e-6, groups of 512 of k 2.4e-7.
 #pragma once
 
 #include <cuda.h>
@@ -51,7 +51,7 @@ struct Params {
   int counted;
   int rows, cols, depth;    // extents of D and k; with `counted` the most that count may say
   int batch;
-  int upper;                // only tiles on and above the diagonal (CTAS * 128 == N)
+  int upper;                // only tiles that reach the diagonal or lie above it; where a block is stored once more transposed is the epilogue's affair
   int band;                 // tile rows that are walked down before the next column
   int bf16;                 // else fp16
   int group;                // stages of k that an accumulator takes
@@ -212,7 +212,7 @@ struct Fp16 {
 };
 // A warp's blocks of 32 rows x kBlock 16-bit elements between registers, where a lane has a row, and memory: through slots of 4 KB in shared memory, as TMA's 128-byte swizzle lays
 // them (16-byte pieces of a row exchanged by its number, so that neither side meets a bank twice).  TMA moves them: the same by loads and stores of the lanes, 64
-// bytes of eight rows each, took the last product of a step of four 2048 x 8192 updates 282 us for 200, and a single 2048 x 2048 matrix's 31 for UPDATE_US.
+// bytes of eight rows each, took the last product of a step of four 2048 x 8192 updates 282 us for 222, and a single 2048 x 2048 matrix's 31 for 22.5.
 struct Slots {
   static constexpr int kBytes = 32 * kBlock * 2, kPieces = kBlock / 8;
   static __device__ __forceinline__ uint32_t own(const Place& at, int slot, int k) { return (at.own + slot * kBytes) ^ (k << 4); }      // the lane's row's k-th piece
@@ -307,7 +307,7 @@ struct Tiles {
 
 // What a cluster works on: tiles in turn, or with p.cuts parts of `cut` stages of them: all tiles' first parts, then all tiles' second ones, ..., so that what is under way
 // at a time reads the same of k.  (Runs of stages of one length for all clusters balance best, but then nothing is read twice from L2: 16384 of k, 8192 x
-// 2048 sums 500 us for CUTS_US.)
+// 2048 sums 500 us for 370.)
 struct Work {
   int at, items, stride, steps, tiles, cut, part;
   __device__ __forceinline__ Work(const Params& p, int tiles_, int steps_, int cluster, int clusters)
