@@ -357,7 +357,8 @@ class PratchyaCausalLM(torch.nn.Module):
 
     def loss_without_logits(self, input_ids, label, alpha: float = 0.1):
         """The loss of forward(input_ids, label) with lm_head's weight and its input in bf16 where forward has them in fp8, and no logits (8.6 GB and as much again for their
-        cotangent with 32768 tokens and 65536 words): `linear_cross_entropy` of every position but the last of each sequence, their mean."""
+        cotangent with 32768 tokens and 65536 words): `linear_cross_entropy` of every position but the last of each sequence, their mean; a
+        negative label has loss 0 and counts in it."""
         if not isinstance(self.lm_head, Linear):
             raise TypeError("loss_without_logits: lm_head's dense weight is gone (to_int4)")
         bsz, steps = input_ids.shape

@@ -35,10 +35,12 @@ def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients=COEFFICIENT
     steps, eps = operator.index(steps), float(eps)
     if not 1 <= steps <= 64 or not (eps >= 0.0 and math.isfinite(eps)):
         raise ValueError(f"orthogonalize: {steps} steps (1 to 64), eps {eps}")
-    flat = [float(v) for t in coefficients for v in (t if hasattr(t, "__len__") else (t,))]
-    if len(flat) not in (3, 3 * steps) or len(coefficients) != (3 if not hasattr(coefficients[0], "__len__") else steps):
+    triples = [t for t in coefficients]
+    if not any(hasattr(t, "__len__") for t in triples):
+        triples = [triples] * steps
+    if len(triples) != steps or not all(hasattr(t, "__len__") and len(t) == 3 for t in triples):
         raise ValueError(f"orthogonalize: coefficients are three numbers or {steps} times three")
-    flat = flat * steps if len(flat) == 3 and not hasattr(coefficients[0], "__len__") else flat
+    flat = [float(v) for t in triples for v in t]
     out = torch.empty(update.shape, dtype=torch.bfloat16, device=update.device)
     if update.numel() == 0:
         return out

@@ -196,3 +196,13 @@ def test_no_derivative_is_dropped_without_a_word(built_lib):
         with Watching():
             (again,) = torch.autograd.grad(call(leaf).float().sum(), leaf)
         assert torch.equal(d, again)
+
+
+def test_coefficients_of_another_number_than_three(built_lib):
+    g = torch.randn(40, 300, device="cuda")
+    a, b, c = 3.4445, -4.7750, 2.0315
+    want = orthogonalize(g, steps=2)
+    assert torch.equal(orthogonalize(g, steps=2, coefficients=[a, b, c]), want) and torch.equal(orthogonalize(g, steps=2, coefficients=((a, b, c), [a, b, c])), want)
+    for wrong in ((), (a, b), (a, b, c, a), ((a, b), (c, a, b, c)), ((a, b, c),), ((a, b, c), a, b), ((a, b, c), (a, b, c), (a, b, c))):
+        with pytest.raises(ValueError):
+            orthogonalize(g, steps=2, coefficients=wrong)
