@@ -484,8 +484,9 @@ extern "C" int pb_embedding_lookup(const void* table, int dtype, int64_t vocab, 
   const LookupParams p{table, ids, out, vocab, channels, padding_id, (uint32_t)items, FastDiv((uint32_t)per_row), scale};
   const unsigned grid = (unsigned)((items + 3) / 4);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == PB_F32) launch_behind(vectors ? lookup_kernel<float, true> : lookup_kernel<float, false>, grid, 128, 0, st, p);
-  else launch_behind(vectors ? lookup_kernel<__nv_bfloat16, true> : lookup_kernel<__nv_bfloat16, false>, grid, 128, 0, st, p);
+  auto go = [&](auto kernel) { launch_behind(kernel, grid, 128, 0, st, p); };
+  if (dtype == PB_F32) vectors ? go(lookup_kernel<float, true>) : go(lookup_kernel<float, false>);
+  else vectors ? go(lookup_kernel<__nv_bfloat16, true>) : go(lookup_kernel<__nv_bfloat16, false>);
   PB_LAUNCH_CHECK("lookup_kernel");
   return PB_OK;
 }

@@ -234,3 +234,23 @@ def test_captured_with_an_eager_graph_alive(built_lib):
     for graph, loss, grads in graphs:
         assert torch.equal(loss.detach().flip(0), eager.detach()) and torch.equal(grads[0].flip(0), want[0])
         assert (grads[1].double() - want[1].double()).norm() <= 2.0 ** -8 * want[1].double().norm()      # other sums' order
+
+
+@pytest.mark.parametrize("tied", (False, True))
+@pytest.mark.parametrize("offset", range(9))
+def test_weights_that_are_copied_first_give_the_same_bits(built_lib, tied, offset):
+    """Columns of a wider array, from any element on: what TMA cannot read is moved, and nothing else changes; the last row ends with the array."""
+    g = torch.Generator(device="cuda").manual_seed(70 + offset)
+    inner, outer = 328, 137
+    wide = torch.randn(outer, inner + offset, generator=g, device="cuda").bfloat16()
+    view = wide[:, offset:]
+    weight, whole = (view.t(), view.clone().t()) if tied else (view, view.clone())
+    x = torch.randn(70, weight.shape[0], generator=g, device="cuda").bfloat16()
+    t = torch.randint(0, weight.shape[1], (70,), generator=g, device="cuda")
+    up = torch.rand(70, generator=g, device="cuda")
+    got, want = [], []
+    for w, to in ((weight, got), (whole, want)):
+        a, b = x.clone().requires_grad_(True), w.detach().requires_grad_(True)
+        loss = linear_cross_entropy(a, b, t, smoothing=0.1)
+        to += [loss, *torch.autograd.grad(loss, (a, b), up)]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
