@@ -364,6 +364,8 @@ class PratchyaCausalLM(torch.nn.Module):
         bsz, steps = input_ids.shape
         if steps < 2 or tuple(label.shape) != (bsz, steps):
             raise ValueError(f"loss_without_logits: input_ids {tuple(input_ids.shape)}, label {tuple(label.shape)}")
+        if not (label.is_floating_point() or label.is_complex() or label.dtype is torch.bool):
+            label = label.to(torch.int64)                # an unsigned type has no -1
         targets = torch.cat([label[:, 1:], label.new_full((bsz, 1), -1)], dim=1)
         losses = linear_cross_entropy(self.hidden(input_ids).to(torch.bfloat16), self.lm_head.kernel.to(torch.bfloat16), targets, smoothing=alpha)
         return losses.sum() / (bsz * (steps - 1))
