@@ -77,9 +77,10 @@ __global__ void __launch_bounds__(256) square_sums_kernel(const T* g, int64_t n,
   }
 }
 
-// 2^12 / (|G| + eps), of |G|^2 = s, as two powers of two and a rest in [1, 2): each within f32 where the whole may not be.  NaN for an infinity or a NaN anywhere.
+// 2^12 / (|G| + eps), of |G|^2 = s, as two powers of two and a rest in [1, 2): each within f32 where the whole may not be (2^161 for the least f32 alone).  NaN for an infinity or a NaN
+// anywhere.  Nothing but zeros stays so by any factor that is a number; under a tiny eps the formula's own is none.
 __device__ __forceinline__ void scale_factors(double s, double eps, float* factors) {
-  const double by = (double)kScaleX / (sqrt(s) + eps);
+  const double by = s == 0.0 && eps > 0.0 ? 1.0 : (double)kScaleX / (sqrt(s) + eps);
   int e = 0;
   const double rest = 2.0 * frexp(by, &e);
   const bool fine = isfinite(by) && isfinite(s);

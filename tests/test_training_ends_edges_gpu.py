@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from pratchya_b200._nnx_impl import orthogonalize
 from pratchya_b200._nnx_impl._model import PratchyaCausalLM, PratchyaConfig
 
 pytestmark = pytest.mark.gpu
@@ -33,3 +34,16 @@ def test_labels_that_are_no_whole_numbers(built_lib):
     for label in (ids.float(), ids.bool(), ids.to(torch.complex64)):
         with pytest.raises(TypeError):
             _model().loss_without_logits(ids, label)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(3, 40, 50), (2048, 64), (200, 300), (2, 700, 260)])
+def test_zeros_stay_zeros_under_any_eps(built_lib, shape, dtype):
+    """0 / (0 + eps), beside a matrix that is not zero in a stack; down to the least double."""
+    for eps in (5e-324, 1e-310, 1e-100, 1e-74, 1e-60, 1e-7, 1e300):
+        g = torch.zeros(shape, dtype=dtype, device="cuda")
+        assert torch.equal(orthogonalize(g, eps=eps), torch.zeros(shape, dtype=torch.bfloat16, device="cuda")), eps
+        if len(shape) == 3 and eps < 1e-7:
+            g[0] = torch.randn(shape[1:], generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(dtype)
+            got = orthogonalize(g, eps=eps)
+            assert torch.equal(got[0], orthogonalize(g, eps=0.0)[0]) and not got[1:].any(), eps      # the norm is 40 and more: no eps of these moves a bit of it
