@@ -18,6 +18,7 @@ constexpr int kSortThreads = 512, kSortWarps = kSortThreads / 32;
 constexpr int kWarpKeys = 128, kTile = kWarpKeys * kSortWarps;      // keys a CTA sorts
 constexpr int kMostBits = 9, kBins = 1 << kMostBits;
 constexpr int kRun = 32, kShortRun = 8;      // sorted positions a CTA adds up: the fewer where there are few, that CTAs ask for all of them at once
+constexpr int kFewTiles = 320, kChunk = 256;      // up to kFewTiles a tile adds up the others' counts by itself; else they are summed first, kChunk tiles a CTA
 constexpr int kAlone = 4096, kAloneThreads = 1024, kAloneWarps = kAloneThreads / 32;      // pairs that one CTA sorts
 constexpr int kSumThreads = 128;
 constexpr int kAhead = 8;             // rows of g that a thread asks for at once
@@ -111,6 +112,7 @@ struct SortParams {
   const uint32_t *keys, *order;    // later ones
   uint32_t *keys_out, *order_out;
   uint32_t* counts;                // [tiles][kBins]
+  uint32_t* sums;                  // of many tiles: [chunks + 1][kBins], see scan_kernel
   uint32_t* present;               // the first pass: a bit for each row that a token has
   int64_t vocab, padding;
   uint32_t n, tiles, shift, bits;
@@ -141,6 +143,56 @@ __global__ void __launch_bounds__(kSortThreads) count_kernel(const __grid_consta
   p.counts[(size_t)blockIdx.x * kBins + threadIdx.x] = bins[threadIdx.x];
 }
 
+// the pairs of lower digits than this thread's, of which there are `all`
+__device__ __forceinline__ uint32_t below_digit(uint32_t all) {
+  __shared__ uint32_t sums[kSortWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t upto = all;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t below = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += below;
+  }
+  if (lane == 31) sums[warp] = upto;
+  __syncthreads();
+  uint32_t base = upto - all;
+  for (int w = 0; w < warp; ++w) base += sums[w];
+  return base;
+}
+
+// Counts of many tiles: where each of them reads all others' the work grows with the square of the tokens.  The gradient of 65536 words of 8 channels, us, by every tile | by the
+// kernels here: 2^19 tokens (256 tiles) 187 | 199, 2^20 352 | 322, 2^22 1807 | 961, 2^23 5100 | 1680.
+// A CTA's chunk of tiles: each one's counts become those of the chunk's tiles before it, and the chunk's own go to sums[chunk].
+__global__ void __launch_bounds__(kSortThreads) scan_kernel(const __grid_constant__ SortParams p) {
+  grid_wait();
+  const uint32_t end = min(p.tiles, (blockIdx.x + 1) * kChunk);
+  uint32_t before = 0;
+  for (uint32_t t0 = blockIdx.x * kChunk; t0 < end; t0 += 16) {
+    uint32_t c[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) c[k] = t0 + k < end ? p.counts[(size_t)(t0 + k) * kBins + threadIdx.x] : 0u;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      if (t0 + k < end) p.counts[(size_t)(t0 + k) * kBins + threadIdx.x] = before;
+      before += c[k];
+    }
+  }
+  p.sums[blockIdx.x * kBins + threadIdx.x] = before;
+}
+// One CTA: the same for the chunks, of which the last row is that of a digit's first pair.
+__global__ void __launch_bounds__(kSortThreads) scan_chunks_kernel(const __grid_constant__ SortParams p) {
+  grid_wait();
+  const uint32_t chunks = (p.tiles + kChunk - 1) / kChunk;
+  uint32_t before = 0;
+#pragma unroll 8
+  for (uint32_t k = 0; k < chunks; ++k) {
+    const uint32_t c = p.sums[k * kBins + threadIdx.x];
+    p.sums[k * kBins + threadIdx.x] = before;
+    before += c;
+  }
+  p.sums[chunks * kBins + threadIdx.x] = below_digit(before);
+}
+
 template <int THREADS, int ROWS>
 __device__ __forceinline__ void zero_rows(const ZeroParams& p, uint32_t block) {
   const int64_t first = (int64_t)block * ROWS;
@@ -158,27 +210,23 @@ __global__ void __launch_bounds__(kSortThreads) scatter_kernel(const __grid_cons
   grid_wait();
   if (blockIdx.x >= p.tiles) return zero_rows<kSortThreads, kZeroRows>(p.zero, blockIdx.x - p.tiles);
   __shared__ uint32_t at[kSortWarps][kBins];
-  __shared__ uint32_t sums[kSortWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t bin = threadIdx.x, mask = (1u << p.bits) - 1;
-  uint32_t before = 0, all = 0;
-#pragma unroll 8
-  for (uint32_t t = 0; t < p.tiles; ++t) {
-    const uint32_t c = p.counts[(size_t)t * kBins + bin];
-    all += c;
-    if (t < blockIdx.x) before += c;
-  }
   for (int w = 0; w < kSortWarps; ++w) at[w][bin] = 0;
-  uint32_t upto = all;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t below = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += below;
+  uint32_t base = 0;
+  if (p.sums) {
+    base = p.counts[(size_t)blockIdx.x * kBins + bin] + p.sums[blockIdx.x / kChunk * kBins + bin] + p.sums[(p.tiles + kChunk - 1) / kChunk * kBins + bin];
+    __syncthreads();
+  } else {
+    uint32_t all = 0;
+#pragma unroll 8
+    for (uint32_t t = 0; t < p.tiles; ++t) {
+      const uint32_t c = p.counts[(size_t)t * kBins + bin];
+      all += c;
+      if (t < blockIdx.x) base += c;
+    }
+    base += below_digit(all);
   }
-  if (lane == 31) sums[warp] = upto;
-  __syncthreads();
-  uint32_t base = upto - all + before;
-  for (int w = 0; w < warp; ++w) base += sums[w];
   uint32_t keys[kWarpKeys / 32], digits[kWarpKeys / 32];
   const uint32_t first = blockIdx.x * kTile + warp * kWarpKeys + lane;
 #pragma unroll
@@ -426,7 +474,7 @@ __global__ void __launch_bounds__(kJoin * kJoinThreads) join_kernel(const __grid
 // ---- host side ------------------------------------------------------------------------------------------------------
 struct Plan {
   uint32_t tiles, run, blocks;
-  size_t off_keys[2], off_order[2], off_counts, off_partial, bytes;
+  size_t off_keys[2], off_order[2], off_counts, off_sums, off_partial, bytes;
 };
 int make_plan(int64_t n, int64_t vocab, int64_t channels, Plan* q) {
   if (n < 0 || n > (1 << 28) || vocab <= 0 || vocab > (1 << 30) || channels <= 0 || channels > (1 << 21))
@@ -438,6 +486,7 @@ int make_plan(int64_t n, int64_t vocab, int64_t channels, Plan* q) {
   auto take = [&](size_t bytes) { const size_t was = at; at += (bytes + 255) / 256 * 256; return was; };
   for (int i = 0; i < 2; ++i) { q->off_keys[i] = take((size_t)n * 4); q->off_order[i] = take((size_t)n * 4); }
   q->off_counts = take((size_t)q->tiles * kBins * 4);
+  q->off_sums = take(q->tiles > kFewTiles ? ((size_t)(q->tiles + kChunk - 1) / kChunk + 1) * kBins * 4 : 0);
   q->off_partial = take((size_t)q->blocks * 2 * channels * 4);
   q->bytes = at;
   return PB_OK;
@@ -527,6 +576,7 @@ extern "C" int pb_embedding_lookup_bwd(const void* g, int dtype, const int64_t* 
     PB_CUDA_TRY(cudaMemsetAsync(present, 0, (size_t)words * 4, st));
     SortParams p{};
     p.counts = reinterpret_cast<uint32_t*>(ws + q.off_counts);
+    p.sums = q.tiles > kFewTiles ? reinterpret_cast<uint32_t*>(ws + q.off_sums) : nullptr;
     p.vocab = vocab; p.padding = padding_id; p.n = (uint32_t)n; p.tiles = q.tiles; p.zero = zero;
     for (int k = 0, shift = 0; k < passes; ++k) {
       const int width = ((int)bits - shift + passes - k - 1) / (passes - k);
@@ -537,6 +587,12 @@ extern "C" int pb_embedding_lookup_bwd(const void* g, int dtype, const int64_t* 
       p.shift = (uint32_t)shift; p.bits = (uint32_t)width;
       launch_behind(count_kernel, q.tiles, kSortThreads, 0, st, p);
       PB_LAUNCH_CHECK("embedding count_kernel");
+      if (p.sums) {
+        launch_behind(scan_kernel, (q.tiles + kChunk - 1) / kChunk, kSortThreads, 0, st, p);
+        PB_LAUNCH_CHECK("embedding scan_kernel");
+        launch_behind(scan_chunks_kernel, 1, kSortThreads, 0, st, p);
+        PB_LAUNCH_CHECK("embedding scan_chunks_kernel");
+      }
       launch_behind(scatter_kernel, q.tiles + (k == 0 ? (unsigned)((vocab + kZeroRows - 1) / kZeroRows) : 0u), kSortThreads, 0, st, p);
       PB_LAUNCH_CHECK("embedding scatter_kernel");
       shift += width;

@@ -1,0 +1,52 @@
+"""The embedding's gradient behind the sort by many CTAs (more than 4096 tokens): its passes, its tiles, and what is no token.
+
+A sum of n numbers in f32 goes by blocks of at most 32, then four ways: within (32 + n / 128 + 10) 2^-24 of the sum of magnitudes, or (n - 1) 2^-24 of it where that is less;
+the product with scale and the rounding to the table's type half a step each."""
+import pytest
+import torch
+
+from pratchya_b200._nnx_impl import embedding_lookup
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+TILE = 2048
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _check(vocab, channels, dtype, ids, scale=1.0, padding=None):
+    table = torch.randn(vocab, channels, generator=_gen(vocab), device="cuda").to(dtype).requires_grad_(True)
+    rows = embedding_lookup(table, ids, scale, padding)
+    g = torch.randn(rows.shape, generator=_gen(1), device="cuda").to(dtype)
+    (d,) = torch.autograd.grad(rows, table, g, retain_graph=True)
+    row = torch.where(ids < 0, ids + vocab, ids)
+    use = (row >= 0) & (row < vocab) & (row != (-1 if padding is None else padding % vocab))
+    at, gg = row[use], g[use].double()
+    zeros = torch.zeros(table.shape, dtype=torch.float64, device="cuda")
+    exact, size = zeros.index_add(0, at, gg) * scale, zeros.index_add(0, at, gg.abs()) * abs(scale)
+    n = torch.bincount(at, minlength=vocab).double().unsqueeze(-1)
+    bound = torch.minimum(n, 42 + n / 128) * 2.0 ** -24 * size + (2.0 ** -23 + torch.finfo(dtype).eps / 2) * exact.abs() + 2.0 ** -126 * (size > 0)
+    off = (d.double() - exact).abs()
+    assert d.dtype == dtype and (off <= bound).all(), (off / bound.clamp(min=1e-300)).max().item()
+    assert not d[(n == 0).squeeze(-1)].any()
+    assert torch.equal(torch.autograd.grad(rows, table, g)[0], d)
+    return d
+
+
+@pytest.mark.parametrize("n", [320 * TILE - 1, 320 * TILE, 320 * TILE + 1, 512 * TILE, 512 * TILE + 1, 520 * TILE + 77])
+def test_counts_of_many_tiles(built_lib, n):
+    """Around the number of tiles from which their counts are added up ahead of the pass, and around a chunk of them; one pass to three."""
+    for vocab, channels in ((1, 1), (300, 8), (511, 3), (70000, 4), (300000, 2)):
+        ids = torch.randint(-vocab, vocab, (n,), generator=_gen(n + vocab), device="cuda")
+        _check(vocab, channels, F32, ids)
+        odd = torch.where(torch.rand(n, generator=_gen(2), device="cuda") < 0.2, vocab + 3, ids)
+        _check(vocab, channels, BF16, odd, 0.5, vocab // 2)
+
+
+def test_workspace_of_many_tiles(built_lib):
+    """The sums of the tiles' counts lie in it where they are used."""
+    few, many = (built_lib.pb_embedding_lookup_bwd_workspace_size(n, 1000, 1) for n in (320 * TILE, 320 * TILE + 1))
+    assert many >= few + 3 * 2048
