@@ -11,6 +11,7 @@
 //
 // Three products a step (products.cuh).  A and B are symmetric: only tiles on and above the diagonal are made, and stored to both places.
 #include <cmath>
+#include <mutex>
 #include <utility>
 
 #include "products.cuh"
@@ -536,10 +537,38 @@ __global__ void __launch_bounds__(kSlab, 1) narrow_kernel(const __grid_constant_
   }
 }
 
+// The CTAs that a cluster may have on the current device.  Every GPU that runs the kernel has room for eight; sixteen, an SM each in one GPC, may be more than a part of a GPU has.
+int most_clusters() {
+#ifdef PB_DIAGNOSTICS
+  if (g_withhold.load() & kEightAtMost) return 8;
+#endif
+  static std::mutex mu;
+  static int cached[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 8;
+  std::lock_guard<std::mutex> lock(mu);
+  if (cached[dev] == 0) {
+    auto fits = [](auto kernel) {
+      cudaLaunchConfig_t config{};
+      config.gridDim = dim3(kMostClusters); config.blockDim = dim3(kSlab); config.dynamicSmemBytes = kNarrowSmem;
+      cudaLaunchAttribute size;
+      size.id = cudaLaunchAttributeClusterDimension;
+      size.val.clusterDim.x = kMostClusters; size.val.clusterDim.y = size.val.clusterDim.z = 1;
+      config.attrs = &size; config.numAttrs = 1;
+      int clusters = 0;
+      return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kNarrowSmem) == cudaSuccess &&
+             cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+             cudaOccupancyMaxActiveClusters(&clusters, kernel, &config) == cudaSuccess && clusters > 0;
+    };
+    cached[dev] = fits(narrow_kernel<float>) && fits(narrow_kernel<__nv_bfloat16>) ? kMostClusters : 8;
+    (void)cudaGetLastError();      // where it does not fit, that is no error of the call
+  }
+  return cached[dev];
+}
 // A cluster's CTAs for a matrix; 0: too long, or too wide
 int narrow_size(int64_t rows, int64_t cols) {
   const int64_t length = std::max(rows, cols), width = std::min(rows, cols);
-  if (width > kNarrow || length > kMostClusters * kSlab) return 0;
+  if (width > kNarrow || length > kMostClusters * kSlab || (length > 8 * kSlab && most_clusters() < kMostClusters)) return 0;
   int size = 1;
   while (size * kSlab < length) size *= 2;
   return size;

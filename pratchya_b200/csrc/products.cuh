@@ -625,6 +625,7 @@ inline int make_map(CUtensorMap* map, const void* base, bool bf16, int64_t inner
 #ifdef PB_DIAGNOSTICS
 std::atomic<uint32_t> g_polls{kWaitPolls};
 std::atomic<int> g_withhold{0};
+constexpr int kFirstStage = 1, kEightAtMost = 2;      // of g_withhold: see pb_debug_product_control
 inline void control(uint32_t polls, int withhold) {
   g_polls.store(polls ? polls : kWaitPolls);
   g_withhold.store(withhold);
@@ -650,7 +651,7 @@ void set_common(Params* p) {
   p->band = (int)std::min<int64_t>((p->rows + 128 * CTAS - 1) / (128 * CTAS), std::max<int64_t>(1, (16 << 20) / (128 * CTAS * 2 * std::max<int64_t>(1, p->cuts ? (int64_t)p->cut * kDepth : p->depth))));
   p->polls = kWaitPolls; p->withhold = 0;
 #ifdef PB_DIAGNOSTICS
-  p->polls = g_polls.load(); p->withhold = g_withhold.load();
+  p->polls = g_polls.load(); p->withhold = g_withhold.load() & kFirstStage;
 #endif
 }
 
