@@ -1771,7 +1771,7 @@ extern "C" PB_API int pb_debug_gemm_profile(unsigned long long* out16, void* str
   return PB_OK;
 }
 // The same for the products of the cross entropy without logits and of the orthogonalised update: poll budget (0: the default), and in the bits of `withhold` whether a launch's
-// first stage is left unfilled (1) and whether a cluster has eight CTAs at most, as on a part of a GPU (2).
+// first stage is left unfilled (1), whether a cluster has eight CTAs at most, as on a part of a GPU (2), and whether what an epilogue reads never comes (4).
 extern "C" PB_API int pb_debug_product_control(unsigned int polls, int withhold) {
   orthogonalize_control(polls, withhold);
   linear_xent_control(polls, withhold);

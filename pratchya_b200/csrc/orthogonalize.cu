@@ -191,17 +191,25 @@ struct GramEpilogue : Ungrouped {
   __device__ __forceinline__ void finish(const Place& at) { if (at.lane == 0) Slots::wait_sent(); }
 };
 
-// Blocks that are read before they are written: asked for a block ahead, as soon as the slots have been read out.  `pending`: on their way.
+// Blocks that are read before they are written: asked for a block ahead, as soon as the slots have been read out.  `pending`: on their way.  `lost`: the wait for one ran out; its
+// barrier's phase stays open, so nothing more is asked for, read or written, and the end waits for it once more.
 struct Reading : Ungrouped {
   uint32_t phase = 0;
-  bool pending = false;
+  bool pending = false, lost = false;
   __device__ __forceinline__ bool arrived(const Place& at) {
-    const bool ok = bar_wait(at.bar, phase, at.polls);
+    if (lost) return false;
+    lost = !__all_sync(0xffffffffu, bar_wait(at.bar, phase, at.polls));
+    if (lost) return false;
     phase ^= 1; pending = false;
-    return __all_sync(0xffffffffu, ok);
+    return true;
+  }
+  __device__ __forceinline__ bool asks(const Place& at, int c) {
+    if (lost || c >= at.slice || at.col + c >= at.cols) return false;
+    pending = true;
+    return at.lane == 0 && !at.withheld;
   }
   __device__ __forceinline__ void finish(const Place& at) {
-    if (pending) (void)arrived(at);
+    if (pending) (void)bar_wait(at.bar, phase, at.polls);
     if (at.lane == 0) Slots::wait_sent();
   }
 };
@@ -211,13 +219,10 @@ struct SquareEpilogue : Reading {
   const Params& p;
   __device__ __forceinline__ explicit SquareEpilogue(const Params& e) : p(e) {}
   __device__ __forceinline__ void ask(const Place& at, int c) {
-    if (c >= at.slice || at.col + c >= at.cols) return;
-    pending = true;
-    if (at.lane == 0) {
-      Slots::wait_read();
-      bar_expect(at.bar, kSlotBytes);
-      Slots::ask(at, 0, &p.a, at.col + c, at.row, at.batch);
-    }
+    if (!asks(at, c)) return;
+    Slots::wait_read();
+    bar_expect(at.bar, kSlotBytes);
+    Slots::ask(at, 0, &p.a, at.col + c, at.row, at.batch);
   }
   __device__ __forceinline__ void begin(const Place& at) { ask(at, 0); }
   __device__ __forceinline__ void block(const Place& at, int c, float (&v)[kBlock]) {
@@ -237,14 +242,11 @@ struct UpdateEpilogue : Reading {
   const Params& p;
   __device__ __forceinline__ explicit UpdateEpilogue(const Params& e) : p(e) {}
   __device__ __forceinline__ void ask(const Place& at, int c) {
-    if (c >= at.slice || at.col + c >= at.cols) return;
-    pending = true;
-    if (at.lane == 0) {
-      Slots::wait_read();
-      bar_expect(at.bar, 2 * kSlotBytes);
-      Slots::ask(at, 0, &p.hi, at.col + c, at.row, at.batch);
-      Slots::ask(at, 1, &p.lo, at.col + c, at.row, at.batch);
-    }
+    if (!asks(at, c)) return;
+    Slots::wait_read();
+    bar_expect(at.bar, 2 * kSlotBytes);
+    Slots::ask(at, 0, &p.hi, at.col + c, at.row, at.batch);
+    Slots::ask(at, 1, &p.lo, at.col + c, at.row, at.batch);
   }
   __device__ __forceinline__ void begin(const Place& at) { ask(at, 0); }
   __device__ __forceinline__ void block(const Place& at, int c, float (&v)[kBlock]) {

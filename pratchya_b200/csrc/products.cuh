@@ -44,6 +44,8 @@ struct Form {
   static_assert(kSmem + 512 <= 232448 && kCols % kBlock == 0, "an SM's shared memory, whole blocks");
 };
 
+constexpr int kFirstStage = 1, kEightAtMost = 2, kAsked = 4;      // bits of what the diagnostics build withholds, see pb_debug_product_control
+
 __device__ unsigned int g_status;                 // 0, or PB_ERR_DEVICE_TIMEOUT once a bounded wait ran out
 
 struct Params {
@@ -57,7 +59,7 @@ struct Params {
   int group;                // stages of k that an accumulator takes
   int cuts, cut;            // 0: whole tiles; else the parts that a tile's stages are cut into, and their length
   uint32_t polls;
-  int withhold;             // diagnostics build: the first stage is never filled
+  int withhold;             // diagnostics build: kFirstStage, kAsked
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -193,6 +195,7 @@ struct Place {
   int lane;
   uint32_t slots, own, bar; // this warp's shared memory, the lane's row there (Slots), and a barrier for what is asked for
   uint32_t polls;
+  bool withheld;            // diagnostics build: nothing that is asked for is sent for
   int part;                 // a number for this warp's part of the tile, among all of D
 };
 
@@ -390,7 +393,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           for (; k < k1; ++k, ++it) {
             const int s = it % F::kStages;
             if (!bar_wait(empty(s), ((it / F::kStages) & 1) ^ 1, p.polls)) { ok = false; break; }
-            if (p.withhold && it == 0) continue;
+            if ((p.withhold & kFirstStage) && it == 0) continue;
             const uint32_t bar = CTAS == 2 ? in_leader(full(s)) : full(s), a = base + s * F::kStageBytes, b = a + F::kABytes;
             if (leader) bar_expect(full(s), CTAS * F::kStageBytes);
             if (A_MN) {
@@ -410,7 +413,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         // leave only when every copy that this pair started has landed (bounded)
         if (leader)
           for (uint32_t k = it > (uint32_t)F::kStages ? it - F::kStages : 0; k < it; ++k)
-            if (!(p.withhold && k == 0)) (void)bar_wait(full(k % F::kStages), (k / F::kStages) & 1, p.polls);
+            if (!((p.withhold & kFirstStage) && k == 0)) (void)bar_wait(full(k % F::kStages), (k / F::kStages) & 1, p.polls);
       }
     } else if (warp == 1) {
       if (lane == 0 && leader) {
@@ -447,7 +450,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     at.slots = base + F::kStages * F::kStageBytes + (warp - 4) * Epilogue::kSlots * kSlotBytes;
     at.own = at.slots + lane * (kBlock * 2) + ((lane & 7) << 4);
     at.bar = smem_u32(&bars[2 * F::kStages + 4 + warp - 4]);
-    at.polls = p.polls;
+    at.polls = p.polls; at.withheld = p.withhold & kAsked;
     uint32_t n = 0;
     bool ok = true;
     int w, begin, k1;
@@ -575,7 +578,7 @@ __global__ void __launch_bounds__(32 * kEpilogueWarps) finish_kernel(const float
   Place at;
   int tm, tn;
   tiles.at(w, at.batch, tm, tn);
-  at.rows = rows; at.cols = p.cols; at.lane = lane; at.slice = F::kCols; at.polls = p.polls;
+  at.rows = rows; at.cols = p.cols; at.lane = lane; at.slice = F::kCols; at.polls = p.polls; at.withheld = false;
   at.slots = ((smem_u32(finish_smem) + 1023u) & ~1023u) + warp * Epilogue::kSlots * kSlotBytes;
   at.own = at.slots + lane * (kBlock * 2) + ((lane & 7) << 4);
   at.bar = smem_u32(&bars[warp]);
@@ -625,7 +628,6 @@ inline int make_map(CUtensorMap* map, const void* base, bool bf16, int64_t inner
 #ifdef PB_DIAGNOSTICS
 std::atomic<uint32_t> g_polls{kWaitPolls};
 std::atomic<int> g_withhold{0};
-constexpr int kFirstStage = 1, kEightAtMost = 2;      // of g_withhold: see pb_debug_product_control
 inline void control(uint32_t polls, int withhold) {
   g_polls.store(polls ? polls : kWaitPolls);
   g_withhold.store(withhold);
@@ -651,7 +653,7 @@ void set_common(Params* p) {
   p->band = (int)std::min<int64_t>((p->rows + 128 * CTAS - 1) / (128 * CTAS), std::max<int64_t>(1, (16 << 20) / (128 * CTAS * 2 * std::max<int64_t>(1, p->cuts ? (int64_t)p->cut * kDepth : p->depth))));
   p->polls = kWaitPolls; p->withhold = 0;
 #ifdef PB_DIAGNOSTICS
-  p->polls = g_polls.load(); p->withhold = g_withhold.load() & kFirstStage;
+  p->polls = g_polls.load(); p->withhold = g_withhold.load();
 #endif
 }
 
