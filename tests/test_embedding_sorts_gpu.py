@@ -50,3 +50,30 @@ def test_workspace_of_many_tiles(built_lib):
     """The sums of the tiles' counts lie in it where they are used."""
     few, many = (built_lib.pb_embedding_lookup_bwd_workspace_size(n, 1000, 1) for n in (320 * TILE, 320 * TILE + 1))
     assert many >= few + 3 * 2048
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [4097, 9001])
+@pytest.mark.parametrize("vocab,channels", [(1, 1), (2, 3), (300, 5), (300, 72), (511, 128), (512, 129), (513, 1001), (262143, 4), (262144, 3), (300000, 5), (300000, 8)])
+def test_any_table(built_lib, vocab, channels, n, dtype):
+    """One pass to three, rows in vectors and not, zeros beside the first pass, in tables of no whole tile of them."""
+    ids = torch.randint(-vocab, vocab, (n,), generator=_gen(n + vocab), device="cuda")
+    _check(vocab, channels, dtype, ids, 45.25)
+    _check(vocab, channels, dtype, torch.sort(ids).values)
+    _check(vocab, channels, dtype, torch.full((n,), vocab - 1, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [4097, 9001])
+@pytest.mark.parametrize("vocab,channels", [(1, 3), (300, 72), (700, 5), (65536, 9), (300000, 4)])
+def test_padding_and_ids_outside(built_lib, vocab, channels, n, dtype):
+    """What is padding or beyond the table sorts behind every token, by the same passes, and has no part in any row."""
+    ids = torch.randint(-vocab, vocab, (n,), generator=_gen(n + vocab), device="cuda")
+    chance = torch.rand(n, generator=_gen(3), device="cuda")
+    for padding in sorted({0, vocab // 2, vocab - 1, -1, -vocab}):
+        d = _check(vocab, channels, dtype, torch.where(chance < 0.4, padding, ids), 2.0, padding)
+        assert not d[padding].any()
+    for far in (vocab, -vocab - 1, 1 << 40, -(1 << 62)):
+        _check(vocab, channels, dtype, torch.where(chance < 0.5, far, ids), 1.0, 0)
+    assert not _check(vocab, channels, dtype, torch.full((n,), vocab, device="cuda")).any()                # no token at all
+    assert not _check(vocab, channels, dtype, torch.full((n,), vocab - 1, device="cuda"), 1.0, -1).any()
