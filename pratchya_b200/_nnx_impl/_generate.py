@@ -23,7 +23,9 @@ def generate(model, prompt, steps: int, top: int = 1, uniform: Optional[torch.Te
     where the sum of their probabilities (as shares of the alternatives') passes that number.
 
     The log probabilities are those of a text read token by token behind its prompt.  `score` reads it at once and has others: the norm over a block's heads runs
-    over the tokens of a call (see `advance`).  Importance ratios want both sides from the same of the two."""
+    over the tokens of a call (see `advance`).  Importance ratios want both sides from the same of the two.
+
+    A prompt with a token beyond the vocabulary is not refused: its answer's log probabilities are NaN, and its tokens say nothing."""
     if prompt.dim() != 2 or prompt.shape[1] == 0 or steps < 1 or top < 1:
         raise ValueError(f"generate: prompt {tuple(prompt.shape)}, {steps} steps, {top} alternatives")
     if uniform is not None and tuple(uniform.shape) != (prompt.shape[0], steps):

@@ -323,6 +323,8 @@ class PratchyaCausalLM(torch.nn.Module):
         self.lm_head = Linear(cfg.hidden_size, cfg.vocab_size, (cfg.blksize, 1), gen, device)
 
     def embed(self, input_ids):                      # EmbeddingScaled, _module.py:21-37
+        """The table's rows of input_ids, through their quantization.  A token beyond the vocabulary on either side is not refused, which would wait for the GPU: its row is NaN,
+        and so are all logits of its sequence and the loss of the batch."""
         rows = embedding_lookup(self.embedding, input_ids)      # the rows of a (1,blk)-quantized table quantize as the table does: row-local super-groups
         return read_param(rows, (1, self.cfg.blksize)) * math.sqrt(self.cfg.hidden_size)
 

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from pratchya_b200._nnx_impl import orthogonalize
+from pratchya_b200._nnx_impl import generate, orthogonalize
 from pratchya_b200._nnx_impl._model import PratchyaCausalLM, PratchyaConfig
 
 pytestmark = pytest.mark.gpu
@@ -47,3 +47,43 @@ def test_zeros_stay_zeros_under_any_eps(built_lib, shape, dtype):
             g[0] = torch.randn(shape[1:], generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(dtype)
             got = orthogonalize(g, eps=eps)
             assert torch.equal(got[0], orthogonalize(g, eps=0.0)[0]) and not got[1:].any(), eps      # the norm is 40 and more: no eps of these moves a bit of it
+
+
+def _polynomial(g, eps, steps=5):
+    x = g.double()
+    x = x / (x.norm(dim=(-2, -1), keepdim=True) + eps)
+    tall = x.shape[-2] > x.shape[-1]
+    x = x.mT if tall else x
+    for _ in range(steps):
+        p = x @ x.mT
+        x = 3.4445 * x + (-4.7750 * p + 2.0315 * p @ p) @ x
+    return x.mT if tall else x
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(200, 300), (700, 260), (2, 131, 2000), (129, 6000)])
+def test_updates_of_any_scale_by_products(built_lib, shape, dtype):
+    """As test_orthogonalize_gpu.py has it for one launch, with the errors that it derives: squares beyond f32 on either side, an eps beside the norm and one of 10^4 of it.
+
+    X's numbers have two fp16 terms of 2^12 of them, within 2^-25 where both are subnormal: 2^-37, of m n of them 2^-37 sqrt(m n), which of X's norm 10^-4 is 6e-5 at most here."""
+    for scale in (1e-42, 1e-30, 1e-12, 1.0, 1e15, 1e30, 1e36):
+        g = (torch.randn(shape, generator=torch.Generator(device="cuda").manual_seed(9), device="cuda", dtype=torch.float64) * scale).to(dtype)
+        norm = g.double().norm(dim=(-2, -1)).max().item()
+        for eps in (0.0, norm, 1e4 * norm):
+            got, want = orthogonalize(g, eps=eps), _polynomial(g, eps)
+            if norm == 0.0:                                        # 1e-42 in bf16, by an eps of zero
+                assert got.isnan().all() and want.isnan().all()
+                continue
+            assert ((got.double() - want).norm(dim=(-2, -1)) <= 5e-3 * want.norm(dim=(-2, -1))).all(), (scale, eps)
+
+
+def test_a_token_beyond_the_vocabulary(built_lib):
+    """Its sequence's logits are NaN, with the loss, and those of the others are not: nothing in between takes the NaN for a number."""
+    model, ids = _model(), _ids(640)
+    wrong = ids.clone()
+    wrong[1, 17] = 640
+    with torch.no_grad():
+        logits, loss = model(wrong, ids)
+        assert logits[1].isnan().all() and loss.isnan() and model.loss_without_logits(wrong, ids).isnan()
+        assert not logits[0].isnan().any() and not logits[2].isnan().any()
+        assert generate(model, wrong, 2).logprobs[1].isnan().all()
