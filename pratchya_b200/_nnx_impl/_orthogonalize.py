@@ -21,7 +21,8 @@ def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients=COEFFICIENT
 
     `coefficients`: (a, b, c), or `steps` triples of them; refused where they take a singular value beyond 4.  X is carried with 22 bits from step to step and the products'
     operands have 11, so that the result is within some 3e-3 of the exact polynomial's in the 2-norm (half of that is bf16's own rounding) for updates of
-    any rank.  An update with an infinity or a NaN becomes NaN throughout, one of zeros stays zero (eps > 0; else 0 / 0).  Has no derivative."""
+    any rank (more where the update's norm is 10^-5 of eps and less: X's numbers are held to 2^-37).  An update with an infinity or a NaN becomes NaN throughout, one of zeros
+    stays zero (eps > 0; else 0 / 0).  Has no derivative."""
     if not isinstance(update, torch.Tensor) or not update.is_cuda:
         raise RuntimeError("orthogonalize needs a CUDA tensor: pratchya_b200 has no CPU path")
     if update.dtype not in (torch.float32, torch.bfloat16):
