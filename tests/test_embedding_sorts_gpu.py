@@ -77,3 +77,25 @@ def test_padding_and_ids_outside(built_lib, vocab, channels, n, dtype):
         _check(vocab, channels, dtype, torch.where(chance < 0.5, far, ids), 1.0, 0)
     assert not _check(vocab, channels, dtype, torch.full((n,), vocab, device="cuda")).any()                # no token at all
     assert not _check(vocab, channels, dtype, torch.full((n,), vocab - 1, device="cuda"), 1.0, -1).any()
+
+
+@pytest.mark.parametrize("n", [4097, 9001, 320 * TILE + 5])
+def test_captured(built_lib, n):
+    """Replays with other tokens: nothing of a pass, its counts or its bitmap among them, is left for the next one."""
+    table, g = torch.randn(1000, 8, generator=_gen(1), device="cuda"), torch.randn(n, 8, generator=_gen(2), device="cuda")
+    ids = torch.randint(-1000, 1000, (n,), generator=_gen(3), device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        leaf, graph = table.detach().requires_grad_(True), torch.cuda.CUDAGraph()
+        torch.autograd.grad(embedding_lookup(leaf, ids), leaf, g)
+        with torch.cuda.graph(graph, stream=side):
+            rows = embedding_lookup(leaf, ids, 2.0, 7)
+            (d,) = torch.autograd.grad(rows, leaf, g)
+    torch.cuda.current_stream().wait_stream(side)
+    for most in (1000, 10, 1, 1003):
+        ids.copy_(torch.randint(0, most, (n,), generator=_gen(most), device="cuda"))
+        graph.replay()
+        own = table.detach().requires_grad_(True)
+        want = embedding_lookup(own, ids, 2.0, 7)
+        assert torch.equal(rows.nan_to_num(7.5), want.nan_to_num(7.5)) and torch.equal(d, torch.autograd.grad(want, own, g)[0])

@@ -87,3 +87,29 @@ def test_a_token_beyond_the_vocabulary(built_lib):
         assert logits[1].isnan().all() and loss.isnan() and model.loss_without_logits(wrong, ids).isnan()
         assert not logits[0].isnan().any() and not logits[2].isnan().any()
         assert generate(model, wrong, 2).logprobs[1].isnan().all()
+
+
+def test_more_matrices_than_a_call_of_the_library_takes(built_lib):
+    g = torch.randn(65535 + 70, 3, 2, generator=torch.Generator(device="cuda").manual_seed(4), device="cuda")
+    for update in (g, g.bfloat16(), g.mT):
+        got = orthogonalize(update)
+        assert torch.equal(got[-100:], orthogonalize(update[-100:])) and torch.equal(got[:100], orthogonalize(update[:100]))
+        want = _polynomial(update, 1e-7)
+        # few numbers may all be rounded the worst way: test_orthogonalize_gpu.py derives it
+        assert ((got.double() - want).norm(dim=(1, 2)) <= (7.6 * 2.0 ** -11 * 5.2 + 2.0 ** -8) * want.norm(dim=(1, 2))).all()
+
+
+@pytest.mark.parametrize("shape", [(200, 64), (1500, 128), (2, 4096, 100), (200, 6000), (2, 300, 260)])
+def test_updates_captured(built_lib, shape):
+    """One CTA, clusters of eight and of sixteen, products cut and not."""
+    g = torch.randn(shape, generator=torch.Generator(device="cuda").manual_seed(5), device="cuda")
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            out = orthogonalize(g)
+    torch.cuda.current_stream().wait_stream(side)
+    for k in range(3):
+        g.copy_(torch.randn(shape, generator=torch.Generator(device="cuda").manual_seed(6 + k), device="cuda"))
+        graph.replay()
+        assert torch.equal(out, orthogonalize(g))
