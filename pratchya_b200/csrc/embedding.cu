@@ -3,7 +3,7 @@
 // Both are bound by bytes: rows read and written; g read once and every row of d_table written once, most of them zeros.
 //
 // The gradient goes by sorted tokens and has no float atomics, so that its bits do not depend on the order of threads: (id, position) pairs are sorted by id, stable, with
-// digits of up to nine bits (two passes up to 2^18 words); a block of up to kRun sorted positions is then one CTA's for a slab of columns: runs of one id that
+// digits of up to nine bits (two passes below 2^18 words); a block of up to kRun sorted positions is then one CTA's for a slab of columns: runs of one id that
 // lie in it go to d_table at once, and what of a run crosses its ends leaves as partial sums in f32, which another kernel adds up in their order.  Which rows no
 // token has is a bitmap; they are zeroed by CTAs beside those of the first pass that moves pairs, so that the sort is behind bytes that have to be written anyway.
 // Up to 4096 tokens one CTA sorts in its shared memory, and the zeros are written beside the sums.

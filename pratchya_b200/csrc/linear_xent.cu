@@ -407,7 +407,7 @@ template <typename T> T* part(void* workspace, size_t off) { return reinterpret_
 // 62 us by a pair's, 50 so (41 are the weight's bytes).
 bool few_rows(const Plan& q) { return q.rows <= 128; }
 
-// dx's product of a piece: few tiles of many stages, so they are cut
+// dx's product of a piece: few tiles of many stages, so they are cut, by the most positions that may count; how many do is known on the device alone
 Params hidden_params(const Plan& q, int64_t n, int64_t depth, void* ws) {
   Params p{};
   p.count = part<int>(ws, 0); p.counted = 1; p.rows = (int)(few_rows(q) ? 128 : q.cap); p.cols = (int)depth; p.depth = (int)n; p.batch = 1; p.bf16 = 1; p.group = kGroup;

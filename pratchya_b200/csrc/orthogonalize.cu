@@ -567,7 +567,7 @@ int most_clusters() {
   }
   return cached[dev];
 }
-// A cluster's CTAs for a matrix; 0: too long, or too wide
+// A cluster's CTAs for a matrix; 0: too long, or too wide.  2048 x 128 | 129: 54 | 132 us, 4096 x 128 | 4097 x 128: 59 | 142
 int narrow_size(int64_t rows, int64_t cols) {
   const int64_t length = std::max(rows, cols), width = std::min(rows, cols);
   if (width > kNarrow || length > kMostClusters * kSlab || (length > 8 * kSlab && most_clusters() < kMostClusters)) return 0;
