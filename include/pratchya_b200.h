@@ -454,7 +454,7 @@ PB_API int pb_linear_xent_bwd(const void* x, int64_t outer, int64_t inner, int64
  * with a, b, c = coefficients[3 k .. 3 k + 2] (host memory),  A = X X^T, X = a X + (b A + c A A) X  (A = X^T X from the right where rows > cols), which
  * draws the singular values towards 1 (the Newton-Schulz step of the reference's optimizer, pratchya/_nnx_impl/_optimizer.py:11-29).  out is bf16 [batch, rows, cols].
  * X is kept in 22 bits, the products' operands in fp16 (11), sums in f32.  Coefficients that take a singular value of [0, 1] beyond 4 on the way: PB_ERR_UNSUPPORTED.
- * A matrix with an infinity or a NaN becomes NaN throughout, one of zeros stays zero (eps > 0).  workspace 256-byte aligned, other arrays as their type is. */
+ * A matrix with an infinity or a NaN becomes NaN throughout, one of zeros stays zero (eps > 0).  The workspace's size is the current device's.  workspace 256-byte aligned, other arrays as their type is. */
 PB_API size_t pb_orthogonalize_workspace_size(int64_t batch, int64_t rows, int64_t cols);
 PB_API int pb_orthogonalize(const void* update, int dtype, int64_t batch, int64_t rows, int64_t cols, int steps, const float* coefficients, double eps,
                      void* out, void* workspace, size_t workspace_bytes, void* stream);

@@ -563,7 +563,7 @@ int most_clusters() {
              cudaOccupancyMaxActiveClusters(&clusters, kernel, &config) == cudaSuccess && clusters > 0;
     };
     cached[dev] = fits(narrow_kernel<float>) && fits(narrow_kernel<__nv_bfloat16>) ? kMostClusters : 8;
-    (void)cudaGetLastError();      // where it does not fit, that is no error of the call
+    if (cached[dev] == 8) (void)cudaGetLastError();      // no error of the call
   }
   return cached[dev];
 }
